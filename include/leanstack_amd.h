@@ -328,6 +328,46 @@ int lsk_lm_head_argmax_noalloc_bf16(const void* w_packed, int layout_id, int V, 
                                     float* logits_opt, int logits_mode, long long* out_idx,
                                     void* hip_stream);
 
+/* Device workspace of lsk_constrain_logits (any contents; 0 if the shape is not
+ * supported). */
+size_t lsk_constrain_workspace_bytes(int M, int V);
+
+/* Each request's constraints on its logits, and its greedy token.  For value
+ * v of row m, in fp32 with one rounding per step:
+ *   z = logits[m][v]
+ *   v in the row's history:            z = z > 0 ? z / repetition : z * repetition
+ *   c > 0 times behind the prompt:     z = (z - frequency * c) - presence
+ *   v among the row's bias_ids:        z = z + its value
+ *   v not allowed:                     z = -inf
+ * out[m][v] = z rounded to the logits' type, tokens[m] = the lowest index of the
+ * row's largest out (NaN counts as larger than any number), -1 if every value
+ * is -inf.
+ *   logits        device, fp32 (LSK_LOGITS_FP32) or bf16 (LSK_LOGITS_BF16), row m
+ *                 at logits + m * logits_ld
+ *   history       NULL, or device int32: row m's tokens so far at history + m *
+ *                 history_ld, the first history_lens[m] (NULL: history_len) of
+ *                 history_len (at most 2^20) count; the first prompt_lens[m]
+ *                 (NULL: none) of those are its prompt.  Tokens outside [0, V)
+ *                 count for nothing.
+ *   repetition, frequency, presence   NULL (1, 0, 0), or device fp32 [M]
+ *   bias_ids, bias_values   bias_count (0..1023) entries per row, int32 and fp32,
+ *                 at stride bias_ld; ids outside [0, V) name no value, and of
+ *                 several entries for one value the last counts
+ *   allowed       NULL (all), or device int32 words, row m at allowed + m *
+ *                 allowed_ld: bit v % 32 of word v / 32 set where v is allowed
+ *   out           [M][V] contiguous; may be the logits themselves
+ *   tokens        device int64 [M]
+ *   workspace     lsk_constrain_workspace_bytes(M, V) bytes, 8-byte aligned; calls
+ *                 that share one must be stream-ordered.
+ * The reference has no counterpart (its head is greedy over the raw logits,
+ * src/leanstack/runtime/cutile_logits.py:37-69). */
+int lsk_constrain_logits(const void* logits, int logits_mode, int M, int V, long long logits_ld,
+                         const int* history, long long history_ld, int history_len, const int* history_lens,
+                         const int* prompt_lens, const float* repetition, const float* frequency,
+                         const float* presence, const int* bias_ids, const float* bias_values,
+                         long long bias_ld, int bias_count, const int* allowed, long long allowed_ld,
+                         void* out, long long* tokens, void* workspace, size_t ws_bytes, void* hip_stream);
+
 /* ------------------------------------------------------------------------
  * Stack programs: a whole decode / verify step of projections in ONE launch.
  *

@@ -38,6 +38,9 @@ ERR_WORKSPACE = -4
 
 # Largest M served by the decode/verify kernel (kDecodeMaxM in the library).
 DECODE_MAX_M = 16
+# Longest token history and bias list of constrain_logits (kConstrainMax... in the library).
+CONSTRAIN_MAX_HISTORY = 1 << 20
+CONSTRAIN_MAX_BIAS = 1023
 # Largest activation row stride in elements (kMaxActivationStride).
 MAX_ACTIVATION_STRIDE = (1 << 22) - 8
 
@@ -100,6 +103,13 @@ _SIGNATURES: dict[str, tuple[type | None, list]] = {
     "lsk_lm_head_argmax_noalloc_bf16": (
         _c_int,
         [_c_void, _c_int, _c_int, _c_int, _c_void, _c_int, _c_int, _c_void, _c_int, _c_void, _c_void],
+    ),
+    "lsk_constrain_workspace_bytes": (_c_size, [_c_int, _c_int]),
+    "lsk_constrain_logits": (
+        _c_int,
+        [_c_void, _c_int, _c_int, _c_int, ctypes.c_longlong, _c_void, ctypes.c_longlong, _c_int, _c_void, _c_void, _c_void,
+         _c_void, _c_void, _c_void, _c_void, ctypes.c_longlong, _c_int, _c_void, ctypes.c_longlong, _c_void, _c_void,
+         _c_void, _c_size, _c_void],
     ),
 }
 

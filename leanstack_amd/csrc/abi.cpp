@@ -390,6 +390,61 @@ int lsk_rmsnorm_lm_head_argmax_bf16(const void* w_packed, int layout_id, int V, 
 
 }  // extern "C"
 
+// ------------------------------------------------------------- constrained logits
+
+extern "C" {
+
+size_t lsk_constrain_workspace_bytes(int M, int V) {
+  if (M < 1 || V < 1 || V > (1 << 30)) return 0;
+  return (size_t)M * lsk::constrain_slices(M, V) * sizeof(unsigned long long);
+}
+
+int lsk_constrain_logits(const void* logits, int logits_mode, int M, int V, long long logits_ld, const int* history,
+                         long long history_ld, int history_len, const int* history_lens, const int* prompt_lens,
+                         const float* repetition, const float* frequency, const float* presence, const int* bias_ids,
+                         const float* bias_values, long long bias_ld, int bias_count, const int* allowed,
+                         long long allowed_ld, void* out, long long* tokens, void* workspace, size_t ws_bytes,
+                         void* hip_stream) {
+  lsk::clear_error();
+  if (int st = lsk::check_constrain_args(logits, logits_mode, M, V, logits_ld, history, history_ld, history_len,
+                                         history_lens, prompt_lens, repetition, frequency, presence, bias_ids,
+                                         bias_values, bias_ld, bias_count, allowed, allowed_ld, out, tokens))
+    return st;
+  const size_t need = lsk_constrain_workspace_bytes(M, V);
+  if (workspace == nullptr || ws_bytes < need || !aligned(workspace, 8))
+    return fail(LSK_ERR_WORKSPACE, "constrained logits need a workspace of %zu bytes, 8-byte aligned (got %zu)", need,
+                workspace ? ws_bytes : 0);
+  lsk::ConstrainArgs a;
+  a.logits = logits;
+  a.out = out;
+  a.history = history;
+  a.history_lens = history_lens;
+  a.prompt_lens = prompt_lens;
+  a.repetition = repetition;
+  a.frequency = frequency;
+  a.presence = presence;
+  a.bias_ids = bias_ids;
+  a.bias_values = bias_values;
+  a.allowed = reinterpret_cast<const unsigned*>(allowed);
+  a.keys = static_cast<unsigned long long*>(workspace);
+  a.tokens = tokens;
+  a.logits_ld = (size_t)logits_ld;
+  a.history_ld = (size_t)history_ld;
+  a.bias_ld = (size_t)bias_ld;
+  a.allowed_ld = (size_t)allowed_ld;
+  a.M = M;
+  a.V = V;
+  a.slice = lsk::constrain_slice(M, V);
+  a.slices = lsk::constrain_slices(M, V);
+  a.history_len = history != nullptr ? history_len : 0;
+  a.bias_count = bias_count;
+  hipError_t err = lsk::launch_constrain(a, logits_mode == LSK_LOGITS_BF16, static_cast<hipStream_t>(hip_stream));
+  if (err != hipSuccess) return hip_fail(err, "constrained logits kernel launch");
+  return LSK_OK;
+}
+
+}  // extern "C"
+
 // ----------------------------------------------------------------- stack programs
 
 namespace {

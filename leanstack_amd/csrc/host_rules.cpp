@@ -153,6 +153,43 @@ int check_attention_args(const void* qkv, int n_q, int n_kv, int head_dim, const
   return LSK_OK;
 }
 
+int check_constrain_args(const void* logits, int logits_mode, int M, int V, long long logits_ld, const int* history,
+                         long long history_ld, int history_len, const int* history_lens, const int* prompt_lens,
+                         const float* repetition, const float* frequency, const float* presence, const int* bias_ids,
+                         const float* bias_values, long long bias_ld, int bias_count, const int* allowed,
+                         long long allowed_ld, const void* out, const long long* tokens) {
+  if (logits_mode != LSK_LOGITS_FP32 && logits_mode != LSK_LOGITS_BF16)
+    return fail(LSK_ERR_INVALID, "unknown logits mode %d", logits_mode);
+  if (M < 1 || V < 1 || V > (1 << 30)) return fail(LSK_ERR_INVALID, "M=%d rows of V=%d values", M, V);
+  if ((long long)M * constrain_slices(M, V) > 0xffffffffLL / kConstrainThreads)  // a grid's threads are counted in 32 bits
+    return fail(LSK_ERR_INVALID, "M=%d rows of V=%d values are too many", M, V);
+  if (logits == nullptr || out == nullptr || tokens == nullptr) return fail(LSK_ERR_INVALID, "null device pointer");
+  const uintptr_t item = logits_mode == LSK_LOGITS_FP32 ? 4 : 2;
+  if (!aligned(logits, item) || !aligned(out, item) || !aligned(tokens, 8))
+    return fail(LSK_ERR_INVALID, "logits, out and tokens must be aligned to their values");
+  if (logits_ld < V) return fail(LSK_ERR_INVALID, "logits_ld=%lld must be at least V=%d", logits_ld, V);
+  if (logits == out && logits_ld != V) return fail(LSK_ERR_INVALID, "in place, the logits' rows must be contiguous");
+  if (history != nullptr) {
+    if (history_len < 1 || history_len > kConstrainMaxHistory || history_ld < history_len)
+      return fail(LSK_ERR_INVALID, "history of %d tokens (1..%d) at stride %lld", history_len, kConstrainMaxHistory,
+                  history_ld);
+  } else if (history_lens || prompt_lens || repetition || frequency || presence) {
+    return fail(LSK_ERR_INVALID, "lengths or penalties given without a history");
+  }
+  if (bias_count < 0 || bias_count > kConstrainMaxBias)
+    return fail(LSK_ERR_INVALID, "bias_count=%d must be 0..%d", bias_count, kConstrainMaxBias);
+  if (bias_count > 0 && (bias_ids == nullptr || bias_values == nullptr || bias_ld < bias_count))
+    return fail(LSK_ERR_INVALID, "%d biases need their ids and values at a stride of at least that (%lld)", bias_count,
+                bias_ld);
+  if (allowed != nullptr && allowed_ld < (V + 31) / 32)
+    return fail(LSK_ERR_INVALID, "allowed_ld=%lld must be at least %d words", allowed_ld, (V + 31) / 32);
+  const void* words[] = {history,  history_lens, prompt_lens, repetition, frequency,
+                         presence, bias_ids,     bias_values, allowed};
+  for (const void* p : words)
+    if (!aligned(p, 4)) return fail(LSK_ERR_INVALID, "32-bit arguments must be 4-byte aligned");
+  return LSK_OK;
+}
+
 int check_lm_head(const void* w_packed, int layout_id, int V, int K, const void* x, int M, int ldx,
                   const float* logits_opt, int logits_mode, const long long* out_idx) {
   if (layout_id != LSK_LAYOUT_MFMA16X32)

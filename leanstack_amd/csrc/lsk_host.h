@@ -60,6 +60,29 @@ constexpr int attention_most_chunks(int max_seq_len) {
   return most < kAttnMaxChunks ? most : kAttnMaxChunks;
 }
 
+// Constrained logits (constrain.hip): a row's vocabulary is cut into slices, one
+// workgroup each; a slice's counts are one LDS word per entry.
+constexpr int kConstrainMaxHistory = 1 << 20;
+constexpr int kConstrainMaxBias = 1023;
+constexpr int kConstrainMaxSlice = 16384;
+constexpr int kConstrainThreads = 512;
+
+// Vocabulary entries per slice: the largest that 64 KB of LDS count while the
+// rows alone fill the chip, down to 2048 when there are few (a multiple of 64,
+// so that a slice starts at an aligned value where its row does).
+constexpr int constrain_slice(int M, int V) {
+  const int least = (V + kConstrainMaxSlice - 1) / kConstrainMaxSlice;
+  const int most = (V + 2047) / 2048;
+  const int wanted = (512 + M - 1) / M;
+  const int slices = wanted < least ? least : wanted > most ? most : wanted;
+  const int slice = ((V + slices - 1) / slices + 63) / 64 * 64;
+  return slice < kConstrainMaxSlice ? slice : kConstrainMaxSlice;
+}
+constexpr int constrain_slices(int M, int V) {
+  const int slice = constrain_slice(M, V);
+  return (V + slice - 1) / slice;
+}
+
 // Record `fmt` as this thread's lsk_last_error() message; returns `status`.
 int fail(int status, const char* fmt, ...) __attribute__((format(printf, 2, 3)));
 void clear_error();
@@ -83,6 +106,13 @@ int check_qk_rope_args(const void* qkv, int B, int T, int ld, int n_q, int n_kv,
                        const void* q_norm_weight, const void* k_norm_weight, float eps, const void* cos,
                        const void* sin, long long rope_batch_stride, long long rope_row_stride, const void* q_out,
                        const void* k_out);
+
+// Argument rules of lsk_constrain_logits (all but the workspace's size).
+int check_constrain_args(const void* logits, int logits_mode, int M, int V, long long logits_ld, const int* history,
+                         long long history_ld, int history_len, const int* history_lens, const int* prompt_lens,
+                         const float* repetition, const float* frequency, const float* presence, const int* bias_ids,
+                         const float* bias_values, long long bias_ld, int bias_count, const int* allowed,
+                         long long allowed_ld, const void* out, const long long* tokens);
 
 // Argument rules shared by both decode attention entry points (all but pos
 // and the workspace).

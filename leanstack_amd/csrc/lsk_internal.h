@@ -239,6 +239,25 @@ struct QkRopeArgs {
 };
 hipError_t launch_qk_rope(const QkRopeArgs& a, hipStream_t stream);
 
+// Constrained logits of M rows and the greedy token of each (constrain.hip).
+// Optional pointers are NULL; keys: M * slices words of the workspace.
+struct ConstrainArgs {
+  const void* logits;
+  void* out;
+  const int* history;
+  const int* history_lens;
+  const int* prompt_lens;
+  const float *repetition, *frequency, *presence;
+  const int* bias_ids;
+  const float* bias_values;
+  const unsigned* allowed;
+  unsigned long long* keys;
+  long long* tokens;
+  size_t logits_ld, history_ld, bias_ld, allowed_ld;
+  int M, V, slice, slices, history_len, bias_count;
+};
+hipError_t launch_constrain(const ConstrainArgs& a, bool bf16, hipStream_t stream);
+
 // Number of scoring workgroups (= argmax partials per row) the lm_head
 // kernel uses for V vocab rows (V % 16 == 0): with NB = V / 16 row-blocks,
 // NB if NB <= 512, else (NB - T) / 2 + T with T = 512 + (NB - 512) % 2 (pairs

@@ -603,6 +603,130 @@ def lm_head_argmax_noalloc(hidden: torch.Tensor, weight: PackedWeight, out: torc
     return out
 
 
+def _per_row(t: torch.Tensor | None, m: int, dtype: torch.dtype, what: str) -> None:
+    """Check an optional contiguous [m] argument."""
+    if t is not None and (t.dtype is not dtype or t.shape != (m,) or not t.is_contiguous()):
+        raise ValueError(f"{what} must be a contiguous {dtype} tensor of {m} values, got {t.dtype} {tuple(t.shape)}")
+
+
+def _row_list(t: torch.Tensor, m: int, dtype: torch.dtype, what: str) -> int:
+    """Check an [m, n] argument with contiguous rows; the row stride."""
+    if t.dtype is not dtype or t.dim() != 2 or t.shape[0] != m or (t.shape[1] > 1 and t.stride(1) != 1):
+        raise ValueError(f"{what} must be a {dtype} tensor of {m} contiguous rows, got {t.dtype} {tuple(t.shape)} with "
+                         f"strides {t.stride()}")
+    if m > 1 and t.stride(0) < t.shape[1]:
+        raise ValueError(f"{what} must not repeat or interleave its rows (stride {t.stride(0)} of {t.shape[1]} values)")
+    return t.stride(0) if m > 1 else t.shape[1]
+
+
+def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether the address ranges of two tensors meet."""
+    def last(t):
+        return t.data_ptr() + (sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1) * t.element_size()
+    return a.data_ptr() < last(b) and b.data_ptr() < last(a)
+
+
+def constrain_logits(logits: torch.Tensor, *, history: torch.Tensor | None = None,
+                     history_lens: torch.Tensor | None = None, prompt_lens: torch.Tensor | None = None,
+                     repetition: torch.Tensor | None = None, frequency: torch.Tensor | None = None,
+                     presence: torch.Tensor | None = None, bias_ids: torch.Tensor | None = None,
+                     bias_values: torch.Tensor | None = None, allowed: torch.Tensor | None = None,
+                     out: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """Each request's constraints on its row of logits [M, V] (float32 or
+    bfloat16), and its greedy token: (out [M, V] in the logits' type, int64 [M]).
+
+    In this order, in fp32: tokens of the row's history are divided (if positive)
+    or multiplied (if not) by `repetition`; those said c > 0 times behind the
+    prompt lose `frequency` * c and `presence`; `bias_values` are added at
+    `bias_ids`; values not `allowed` become -inf.  The token is the lowest index
+    of the row's largest value (NaN counts as the largest), -1 where all are -inf.
+
+    history: int32 [M, L], of which the first history_lens[m] tokens count (all
+    without history_lens) and the first prompt_lens[m] are the prompt (none without
+    prompt_lens); tokens outside [0, V) count for nothing.  repetition, frequency,
+    presence: float32 [M] (1, 0, 0 without).  bias_ids / bias_values: int32 /
+    float32 [M, n], n up to 1023, the last of several entries for one token counts,
+    ids outside [0, V) for none.  allowed: int32 [M, ceil(V / 32)], bit v % 32 of
+    word v // 32 set where v is allowed.  Lengths and lists are read on the device,
+    so a captured call follows what they hold at each replay.  out: a contiguous
+    [M, V] tensor of the logits' type, or the (contiguous) logits themselves."""
+    if logits.dtype is torch.float32:
+        mode = _lib.LOGITS_FP32
+    elif logits.dtype is torch.bfloat16:
+        mode = _lib.LOGITS_BF16
+    else:
+        raise ValueError(f"logits must be float32 or bfloat16, got {logits.dtype}")
+    if logits.dim() != 2 or logits.shape[1] < 1:
+        raise ValueError(f"logits must be [M, V], got {tuple(logits.shape)}")
+    m, v = logits.shape
+    named = [(history, "history"), (history_lens, "history_lens"), (prompt_lens, "prompt_lens"),
+             (repetition, "repetition"), (frequency, "frequency"), (presence, "presence"), (bias_ids, "bias_ids"),
+             (bias_values, "bias_values"), (allowed, "allowed"), (out, "out")]
+    dev = _one_device(logits, *named)
+    history_ld = history_len = bias_ld = bias_count = allowed_ld = 0
+    if history is not None:
+        history_ld = _row_list(history, m, torch.int32, "history")
+        history_len = history.shape[1]
+        if history_len > _lib.CONSTRAIN_MAX_HISTORY:
+            raise ValueError(f"history holds {history_len} tokens per row, at most {_lib.CONSTRAIN_MAX_HISTORY}")
+        _per_row(history_lens, m, torch.int32, "history_lens")
+        _per_row(prompt_lens, m, torch.int32, "prompt_lens")
+        for t, what in named[3:6]:
+            _per_row(t, m, torch.float32, what)
+    elif any(t is not None for t, _ in named[1:6]):
+        raise ValueError("lengths or penalties given without a history")
+    if bias_ids is not None and bias_values is not None:
+        bias_ld = _row_list(bias_ids, m, torch.int32, "bias_ids")
+        bias_count = bias_ids.shape[1]
+        if _row_list(bias_values, m, torch.float32, "bias_values") != bias_ld or bias_values.shape != bias_ids.shape:
+            raise ValueError(f"bias_ids and bias_values must have the same shape and strides, got {tuple(bias_ids.shape)} "
+                             f"/ {tuple(bias_values.shape)}")
+        if bias_count > _lib.CONSTRAIN_MAX_BIAS:
+            raise ValueError(f"{bias_count} biases per row, at most {_lib.CONSTRAIN_MAX_BIAS}")
+    elif bias_ids is not None or bias_values is not None:
+        raise ValueError("bias_ids and bias_values go together")
+    if allowed is not None:
+        allowed_ld = _row_list(allowed, m, torch.int32, "allowed")
+        if allowed.shape[1] != (v + 31) // 32:
+            raise ValueError(f"allowed must hold {(v + 31) // 32} words per row, got {allowed.shape[1]}")
+    src = logits
+    if (v > 1 and logits.stride(1) != 1) or (m > 1 and logits.stride(0) < v):
+        src = logits.contiguous()
+    if out is None:
+        out = torch.empty((m, v), device=logits.device, dtype=logits.dtype)
+    else:
+        if out.dtype is not logits.dtype or out.shape != logits.shape or not out.is_contiguous():
+            raise ValueError(f"out must be a contiguous {logits.dtype} tensor of {m} x {v} values")
+        if src is logits and m and out.data_ptr() != logits.data_ptr() and _overlap(out, logits):
+            raise ValueError("out must be the logits themselves or not overlap them")
+        if src is logits and out.data_ptr() == logits.data_ptr() and not logits.is_contiguous():
+            raise ValueError("in place, the logits must be contiguous")
+    _require_device(logits, "logits")
+    tokens = torch.empty((m,), device=logits.device, dtype=torch.long)
+    if m == 0:
+        return out, tokens
+    nbytes = _constrain_workspace_bytes(m, v)
+    workspace = torch.empty(nbytes, device=logits.device, dtype=torch.uint8)
+    with _on(dev):
+        status = _lib.load().lsk_constrain_logits(
+            src.data_ptr(), mode, m, v, src.stride(0) if m > 1 else v, _ptr(history) if history_len else None, history_ld,
+            history_len, _ptr(history_lens) if history_len else None, _ptr(prompt_lens) if history_len else None,
+            *((_ptr(repetition), _ptr(frequency), _ptr(presence)) if history_len else (None, None, None)),
+            _ptr(bias_ids), _ptr(bias_values), bias_ld, bias_count, _ptr(allowed), allowed_ld, out.data_ptr(),
+            tokens.data_ptr(), workspace.data_ptr(), nbytes, stream_handle())
+    _lib.check(status, "lsk_constrain_logits")
+    return out, tokens
+
+
+@functools.lru_cache(maxsize=1024)
+def _constrain_workspace_bytes(m: int, v: int) -> int:
+    return _lib.load().lsk_constrain_workspace_bytes(m, v)
+
+
+def _ptr(t: torch.Tensor | None) -> int | None:
+    return None if t is None else t.data_ptr()
+
+
 class StackStep:
     """A prepared stack program: many projections at the same M in one
     persistent launch (lsk_stack_prepare / lsk_stack_run).
