@@ -328,6 +328,43 @@ int lsk_lm_head_argmax_noalloc_bf16(const void* w_packed, int layout_id, int V, 
                                     float* logits_opt, int logits_mode, long long* out_idx,
                                     void* hip_stream);
 
+/* Device workspace of lsk_lora_add_bf16 for these sizes (any contents; 0: none). */
+size_t lsk_lora_workspace_bytes(int M, int N, int K, int rank_tiles, int count);
+
+/* Low-rank adapters of many requests beside a shared projection: for row m with
+ * a = index[m] in [0, count),
+ *   z[m] = y[m] + scale[a] * (x[m] . A_a^T) . B_a^T,
+ * and z[m] = y[m] for any other index; out[m] = z[m] (LSK_EPI_NONE), or
+ * SiLU(gate) * up of it (LSK_EPI_SILU_MUL; y in the column order of a gate_up
+ * weight's packed rows, 16 gate columns, their 16 up columns, ..., as
+ * lsk_linear_bf16 gives it when the gate_up tiles are passed as
+ * LSK_LAYOUT_MFMA16X32; out has N/2 columns).  fp32 sums, one rounding to bf16.
+ *   y, x       device bf16 [M][N] and [M][K] at strides ldy, ldx (multiples of 8,
+ *              at most 2^22 - 8), 16-byte aligned; N % 16 == 0 (% 32 for
+ *              LSK_EPI_SILU_MUL), K % 32 == 0
+ *   a_tiles    device bf16, per adapter A_a [16 * rank_tiles][K] in
+ *              LSK_LAYOUT_MFMA16X32
+ *   b_tiles    device bf16, per adapter B_a [N][16 * rank_tiles], columns
+ *              32j..32j+31 of the output in rank_tiles tiles of 1 KB: the 16
+ *              bytes at 16*l of tile (j, t) hold B_a[n0][16t + 4(l/16) + e], e =
+ *              0..3, then the same of n1, with c = l % 16 and n0 = 32j + 8(c/4) +
+ *              c%4, n1 = n0 + 4 (LSK_EPI_SILU_MUL: n0 = 16j + c, the gate row,
+ *              and n1 = N/2 + n0, its up row); rows past N are zero
+ *   scale, ranks   device fp32 / int32 [count]; of A_a's rows and B_a's columns the
+ *              first ranks[a] count
+ *   rank_tiles 1, 2, 3, 4, 6 or 8 (rank 16 to 128)
+ *   index      device int32 [M]
+ *   out        [M][N] (or [M][N/2]) contiguous, 16-byte aligned; may be y itself
+ *              (LSK_EPI_NONE, contiguous rows)
+ *   workspace  lsk_lora_workspace_bytes(...) bytes, 16-byte aligned; calls that
+ *              share one must be stream-ordered.
+ * The reference has no adapters; the shared projections are those of
+ * src/leanstack/runtime/qwen_explicit.py:748, :819, :828-830. */
+int lsk_lora_add_bf16(const void* y, int M, int N, int ldy, const void* x, int K, int ldx,
+                      const void* a_tiles, const void* b_tiles, const float* scale, const int* ranks,
+                      int count, int rank_tiles, const int* index, int epilogue, void* out,
+                      void* workspace, size_t ws_bytes, void* hip_stream);
+
 /* Device workspace of lsk_constrain_logits (any contents; 0 if the shape is not
  * supported). */
 size_t lsk_constrain_workspace_bytes(int M, int V);

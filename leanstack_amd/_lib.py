@@ -104,6 +104,12 @@ _SIGNATURES: dict[str, tuple[type | None, list]] = {
         _c_int,
         [_c_void, _c_int, _c_int, _c_int, _c_void, _c_int, _c_int, _c_void, _c_int, _c_void, _c_void],
     ),
+    "lsk_lora_workspace_bytes": (_c_size, [_c_int] * 5),
+    "lsk_lora_add_bf16": (
+        _c_int,
+        [_c_void, _c_int, _c_int, _c_int, _c_void, _c_int, _c_int, _c_void, _c_void, _c_void, _c_void, _c_int, _c_int,
+         _c_void, _c_int, _c_void, _c_void, _c_size, _c_void],
+    ),
     "lsk_constrain_workspace_bytes": (_c_size, [_c_int, _c_int]),
     "lsk_constrain_logits": (
         _c_int,

@@ -390,6 +390,56 @@ int lsk_rmsnorm_lm_head_argmax_bf16(const void* w_packed, int layout_id, int V, 
 
 }  // extern "C"
 
+// ------------------------------------------------------------- low-rank adapters
+
+extern "C" {
+
+size_t lsk_lora_workspace_bytes(int M, int N, int K, int rank_tiles, int count) {
+  if (M < 1 || N < 1 || K < lsk::kTileK || count < 1 || !lsk::adapter_rank_supported(rank_tiles)) return 0;
+  return (size_t)lsk::adapter_workspace_bytes(lsk::adapter_plan(M, N, K, rank_tiles, count), rank_tiles);
+}
+
+int lsk_lora_add_bf16(const void* y, int M, int N, int ldy, const void* x, int K, int ldx, const void* a_tiles,
+                      const void* b_tiles, const float* scale, const int* ranks, int count, int rank_tiles,
+                      const int* index, int epilogue, void* out, void* workspace, size_t ws_bytes, void* hip_stream) {
+  lsk::clear_error();
+  if (int st = lsk::check_lora_args(y, M, N, ldy, x, K, ldx, a_tiles, b_tiles, scale, ranks, count, rank_tiles, index,
+                                    epilogue, out))
+    return st;
+  const lsk::AdapterPlan p = lsk::adapter_plan(M, N, K, rank_tiles, count);
+  const size_t need = (size_t)lsk::adapter_workspace_bytes(p, rank_tiles);
+  if (need > 0 && (workspace == nullptr || ws_bytes < need || !aligned(workspace, 16)))
+    return fail(LSK_ERR_WORKSPACE, "the adapters need a workspace of %zu bytes, 16-byte aligned (got %zu)", need,
+                workspace ? ws_bytes : 0);
+  lsk::AdapterArgs a;
+  a.y = static_cast<const __bf16*>(y);
+  a.x = static_cast<const __bf16*>(x);
+  a.a_tiles = static_cast<const __bf16*>(a_tiles);
+  a.b_tiles = static_cast<const __bf16*>(b_tiles);
+  a.scale = scale;
+  a.ranks = ranks;
+  a.index = index;
+  a.out = static_cast<__bf16*>(out);
+  a.h = static_cast<float*>(workspace);
+  a.a_stride = (size_t)rank_tiles * 16 * K;
+  a.b_stride = (size_t)((N + 31) / 32) * rank_tiles * 512;
+  a.M = M;
+  a.N = N;
+  a.K = K;
+  a.ldx = ldx;
+  a.ldy = ldy;
+  a.count = count;
+  a.tiles = p.tiles;
+  a.slots = p.slots;
+  a.ranges = p.ranges;
+  a.splits = p.splits;
+  hipError_t err = lsk::launch_adapters(a, rank_tiles, epilogue == LSK_EPI_SILU_MUL, static_cast<hipStream_t>(hip_stream));
+  if (err != hipSuccess) return hip_fail(err, "adapter kernel launch");
+  return LSK_OK;
+}
+
+}  // extern "C"
+
 // ------------------------------------------------------------- constrained logits
 
 extern "C" {

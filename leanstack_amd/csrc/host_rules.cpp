@@ -190,6 +190,37 @@ int check_constrain_args(const void* logits, int logits_mode, int M, int V, long
   return LSK_OK;
 }
 
+int check_lora_args(const void* y, int M, int N, int ldy, const void* x, int K, int ldx, const void* a_tiles,
+                    const void* b_tiles, const float* scale, const int* ranks, int count, int rank_tiles,
+                    const int* index, int epilogue, const void* out) {
+  if (epilogue != LSK_EPI_NONE && epilogue != LSK_EPI_SILU_MUL)
+    return fail(LSK_ERR_INVALID, "epilogue %d: the adapters take none or SiLU*up", epilogue);
+  if (int st = check_shape(epilogue == LSK_EPI_SILU_MUL ? LSK_LAYOUT_MFMA16X32_GATEUP : LSK_LAYOUT_MFMA16X32, N, K))
+    return st;
+  if (M < 1 || count < 1) return fail(LSK_ERR_INVALID, "M=%d rows and %d adapters must be positive", M, count);
+  if (!adapter_rank_supported(rank_tiles))
+    return fail(LSK_ERR_INVALID, "rank_tiles=%d: the rank must be 16, 32, 48, 64, 96 or 128", rank_tiles);
+  if (N > kMaxActivationStride || K > kMaxActivationStride)
+    return fail(LSK_ERR_INVALID, "N=%d and K=%d must be at most %d", N, K, kMaxActivationStride);
+  const AdapterPlan p = adapter_plan(M, N, K, rank_tiles, count);
+  const long long groups = (long long)p.tiles * p.slots;
+  if (groups * (p.ranges > p.splits ? p.ranges : p.splits) > 0xffffffffLL / kAdapterThreads)
+    return fail(LSK_ERR_INVALID, "M=%d rows are too many", M);  // a grid's threads are counted in 32 bits
+  if (ldx < K || ldx % 8 != 0 || ldx > kMaxActivationStride)
+    return fail(LSK_ERR_INVALID, "ldx=%d must be a multiple of 8, K=%d..%d", ldx, K, kMaxActivationStride);
+  if (ldy < N || ldy % 8 != 0 || ldy > kMaxActivationStride)
+    return fail(LSK_ERR_INVALID, "ldy=%d must be a multiple of 8, N=%d..%d", ldy, N, kMaxActivationStride);
+  const void* wide[] = {y, x, a_tiles, b_tiles, out};
+  for (const void* q : wide)
+    if (q == nullptr || !aligned(q, 16)) return fail(LSK_ERR_INVALID, "y, x, the tiles and out must be 16-byte aligned device pointers");
+  const void* words[] = {scale, ranks, index};
+  for (const void* q : words)
+    if (q == nullptr || !aligned(q, 4)) return fail(LSK_ERR_INVALID, "scale, ranks and index must be 4-byte aligned device pointers");
+  if (out == y && (epilogue != LSK_EPI_NONE || ldy != N))
+    return fail(LSK_ERR_INVALID, "in place, y's rows must be contiguous and the epilogue none");
+  return LSK_OK;
+}
+
 int check_lm_head(const void* w_packed, int layout_id, int V, int K, const void* x, int M, int ldx,
                   const float* logits_opt, int logits_mode, const long long* out_idx) {
   if (layout_id != LSK_LAYOUT_MFMA16X32)

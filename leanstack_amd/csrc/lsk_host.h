@@ -83,6 +83,49 @@ constexpr int constrain_slices(int M, int V) {
   return (V + slice - 1) / slice;
 }
 
+// Low-rank adapters (adapters.hip): 16 rows of x, an adapter that they name
+// (slot) and a range of output columns per workgroup.
+constexpr int kAdapterThreads = 512;
+
+// 16-row tiles of the adapters' rank that the kernels are built for.
+constexpr bool adapter_rank_supported(int rank_tiles) {
+  return rank_tiles >= 1 && rank_tiles <= 8 && rank_tiles != 5 && rank_tiles != 7;
+}
+
+// How a call runs: slots per 16 rows, ranges of output columns per slot, and K
+// ranges of the first of two launches (0: one launch).
+struct AdapterPlan {
+  int tiles, slots, ranges, splits;
+};
+constexpr AdapterPlan adapter_plan(int M, int N, int K, int rank_tiles, int count) {
+  AdapterPlan p = {(M - 1) / 16 + 1, count < 16 ? count : 16, 1, 0};
+  // Groups that are likely to have work: rows of a decode batch each name an
+  // adapter of their own, neighbouring rows of prompts the same.
+  const int busy = p.tiles * (M <= 128 ? p.slots : 1);
+  const int blocks = (N + 31) / 32;
+  const int wanted = (512 + busy - 1) / busy;
+  const int most = (blocks + 7) / 8;  // a block for each wave
+  p.ranges = wanted < 1 ? 1 : wanted > most ? most : wanted;
+  // Bytes of A that the one-launch form reads per workgroup, from L2.
+  const long long again = (long long)K * rank_tiles * 32;
+  if (p.ranges > 1 && again > 256 * 1024) {
+    const int ktiles = K / kTileK;
+    const int split = (512 + busy - 1) / busy;
+    const int least = (ktiles + 7) / 8;
+    p.splits = split < 1 ? 1 : split > least ? least : split;
+    if (p.splits > 16) p.splits = 16;
+  }
+  return p;
+}
+constexpr unsigned long long adapter_workspace_bytes(const AdapterPlan& p, int rank_tiles) {
+  return (unsigned long long)p.splits * (unsigned long long)p.tiles * (unsigned long long)rank_tiles * 1024;
+}
+
+// Argument rules of lsk_lora_add_bf16 (all but the workspace's size).
+int check_lora_args(const void* y, int M, int N, int ldy, const void* x, int K, int ldx, const void* a_tiles,
+                    const void* b_tiles, const float* scale, const int* ranks, int count, int rank_tiles,
+                    const int* index, int epilogue, const void* out);
+
 // Record `fmt` as this thread's lsk_last_error() message; returns `status`.
 int fail(int status, const char* fmt, ...) __attribute__((format(printf, 2, 3)));
 void clear_error();

@@ -258,6 +258,20 @@ struct ConstrainArgs {
 };
 hipError_t launch_constrain(const ConstrainArgs& a, bool bf16, hipStream_t stream);
 
+// Low-rank adapters added to M projected rows (adapters.hip).  Tiles as in
+// leanstack_amd.h; strides in elements per adapter; h: the partials of the first
+// of two launches (splits > 0).
+struct AdapterArgs {
+  const __bf16 *y, *x, *a_tiles, *b_tiles;
+  const float* scale;
+  const int *ranks, *index;
+  __bf16* out;
+  float* h;
+  size_t a_stride, b_stride;
+  int M, N, K, ldx, ldy, count, tiles, slots, ranges, splits;
+};
+hipError_t launch_adapters(const AdapterArgs& a, int rank_tiles, bool silu, hipStream_t stream);
+
 // Number of scoring workgroups (= argmax partials per row) the lm_head
 // kernel uses for V vocab rows (V % 16 == 0): with NB = V / 16 row-blocks,
 // NB if NB <= 512, else (NB - T) / 2 + T with T = 512 + (NB - 512) % 2 (pairs

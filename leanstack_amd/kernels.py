@@ -16,6 +16,7 @@ import functools
 import torch
 
 from . import _lib
+from .adapters import AdapterStore
 from .layout import PackedWeight
 
 
@@ -63,7 +64,7 @@ def _rows(x: torch.Tensor, k: int, what: str) -> tuple[torch.Tensor, int, int]:
     x2 = x.reshape(-1, k)
     if (x2.stride(-1) != 1 or (x2.shape[0] > 1 and (x2.stride(0) % 8 or x2.stride(0) > _lib.MAX_ACTIVATION_STRIDE))
             or x2.data_ptr() % 16):
-        x2 = x2.contiguous()
+        x2 = x2.clone(memory_format=torch.contiguous_format)  # (contiguous() keeps a misaligned start)
     ld = x2.stride(0) if x2.shape[0] > 1 else k
     return x2, x2.shape[0], ld
 
@@ -601,6 +602,82 @@ def lm_head_argmax_noalloc(hidden: torch.Tensor, weight: PackedWeight, out: torc
             logits_out.data_ptr() if logits_out is not None else None, logits_mode, out.data_ptr(), stream_handle())
     _lib.check(status, "lsk_lm_head_argmax_noalloc_bf16")
     return out
+
+
+@functools.lru_cache(maxsize=4096)
+def _lora_workspace_bytes(m: int, n: int, k: int, rank_tiles: int, count: int) -> int:
+    return _lib.load().lsk_lora_workspace_bytes(m, n, k, rank_tiles, count)
+
+
+def lora_add(y: torch.Tensor, x: torch.Tensor, store: AdapterStore, index: torch.Tensor, *,
+             epilogue: int = _lib.EPI_NONE, out: torch.Tensor | None = None) -> torch.Tensor:
+    """The rows' own low-rank adapters added to what a shared projection gave:
+    z = y + scale (x . A^T) . B^T of adapter index[m] of `store` (a row whose
+    index is outside [0, store.count) keeps y), in fp32, rounded once.
+
+    y: [..., N] bfloat16, x: [..., K] bfloat16, the projection's input; index: int32,
+    one per row, read on the device.  epilogue EPI_NONE returns z; EPI_SILU_MUL
+    (a gate_up store) returns SiLU(gate) * up of z, y being in the column order of
+    the gate_up weight's packed rows (lora_linear makes it).  out: contiguous
+    [..., N] (or N/2), and with EPI_NONE it may be y itself."""
+    if not isinstance(store, AdapterStore):
+        raise ValueError("store must be an AdapterStore")
+    silu = epilogue == _lib.EPI_SILU_MUL
+    if silu != store.gate_up or epilogue not in (_lib.EPI_NONE, _lib.EPI_SILU_MUL):
+        raise ValueError(f"epilogue {epilogue}: a gate_up store takes EPI_SILU_MUL, any other EPI_NONE")
+    n, k = store.n, store.k
+    y2, m, ldy = _rows(y, n, "y")
+    x2, xm, ldx = _rows(x, k, "x")
+    if xm != m:
+        raise ValueError(f"x has {xm} rows, y has {m}")
+    if index.dtype is not torch.int32 or index.numel() != m or not index.is_contiguous():
+        raise ValueError(f"index must be a contiguous int32 tensor of {m} values, got {index.dtype} {tuple(index.shape)}")
+    n_out = n // 2 if silu else n
+    if out is not None:
+        _check_out(out, m, n_out, torch.bfloat16)
+        if out.data_ptr() % 16:
+            raise ValueError("out must be 16-byte aligned")
+        if _overlap(out, x2) or (_overlap(out, y2) and (silu or out.data_ptr() != y2.data_ptr() or not y2.is_contiguous())):
+            raise ValueError("out must be y itself (contiguous, EPI_NONE) or overlap neither y nor x")
+    _require_device(y, "y")
+    dev = _one_device(y, (x, "x"), (store.a_tiles, "store"), (index, "index"), (out, "out"))
+    if out is None:
+        out = y.new_empty((*y.shape[:-1], n_out))
+    if m == 0:
+        return out
+    nbytes = _lora_workspace_bytes(m, n, k, store.rank_tiles, store.count)
+    workspace = y.new_empty((nbytes // 2,)) if nbytes else None
+    with _on(dev):
+        status = _lib.load().lsk_lora_add_bf16(
+            y2.data_ptr(), m, n, ldy, x2.data_ptr(), k, ldx, store.a_tiles.data_ptr(), store.b_tiles.data_ptr(),
+            store.scales.data_ptr(), store.ranks.data_ptr(), store.count, store.rank_tiles, index.data_ptr(), epilogue,
+            out.data_ptr(), _ptr(workspace), nbytes, stream_handle())
+    _lib.check(status, "lsk_lora_add_bf16")
+    return out
+
+
+def lora_linear(x: torch.Tensor, weight: PackedWeight, store: AdapterStore, index: torch.Tensor, *,
+                epilogue: int = _lib.EPI_NONE, residual: torch.Tensor | None = None,
+                out: torch.Tensor | None = None, workspace: torch.Tensor | None | str = "auto") -> torch.Tensor:
+    """linear() with the rows' own adapters: the shared projection (its residual
+    included) rounded to bf16 as linear() gives it, the adapters added by
+    lora_add; EPI_SILU_MUL takes SiLU(gate) * up after the adapters."""
+    if not isinstance(weight, PackedWeight):
+        raise ValueError("weight must be a PackedWeight (pack it with leanstack_amd.layout / leanserve)")
+    if not isinstance(store, AdapterStore) or (store.n, store.k) != weight.shape:
+        raise ValueError(f"the store's adapters must be of the weight's shape {weight.shape}")
+    if store.gate_up != (weight.layout == _lib.LAYOUT_MFMA16X32_GATEUP) or store.gate_up != (epilogue == _lib.EPI_SILU_MUL):
+        raise ValueError("a gate_up weight takes a gate_up store and EPI_SILU_MUL, and no other does")
+    if out is not None and (out.data_ptr() % 16 or _overlap(out, x)):
+        raise ValueError("out must be 16-byte aligned and not overlap x")
+    if epilogue == _lib.EPI_SILU_MUL:
+        # the same tiles read as a plain weight give both halves, before SiLU, in packed order
+        if residual is not None:
+            raise ValueError("EPI_SILU_MUL takes no residual")
+        both = PackedWeight(weight.data, weight.n, weight.k, _lib.LAYOUT_MFMA16X32)
+        return lora_add(linear(x, both, workspace=workspace), x, store, index, epilogue=epilogue, out=out)
+    y = linear(x, weight, epilogue=epilogue, residual=residual, out=out, workspace=workspace)
+    return lora_add(y, x, store, index, out=y)
 
 
 def _per_row(t: torch.Tensor | None, m: int, dtype: torch.dtype, what: str) -> None:
