@@ -328,6 +328,41 @@ int lsk_lm_head_argmax_noalloc_bf16(const void* w_packed, int layout_id, int V, 
                                     float* logits_opt, int logits_mode, long long* out_idx,
                                     void* hip_stream);
 
+/* Device workspace of lsk_prefix_attention_bf16 (any contents; 0: none). */
+size_t lsk_prefix_attention_workspace_bytes(int B, int T, int n_q, int n_kv, int P, int S);
+
+/* Attention of a batch of requests that share a prefix: query token t of request
+ * b attends all P prefix rows and the first lens[b] - (T - 1 - t) of the request's
+ * own rows (its T new tokens' keys and values are the last of lens[b]; a request
+ * of lens 0 attends the prefix alone),
+ *   out[b][t][h][d] = softmax(scale * q K^T) V,  q head h reading kv head
+ * h / (n_q / n_kv); scores, maxima and sums in fp32, the weights of V rounded to bf16 and normalised by
+ * the sum of the rounded ones, bf16 output.  A query that sees no row gives
+ * zeros; one whose rows all score -inf gives NaN.
+ *   q            device bf16, [d] at q + b * q_batch_stride + h * q_head_stride +
+ *                t * q_token_stride (elements; multiples of 8)
+ *   prefix_k, prefix_v   device bf16, row i of kv head j at j *
+ *                prefix_head_stride + i * prefix_row_stride (>= d)
+ *   k, v         device bf16, row i of request b, kv head j at b * batch_stride +
+ *                j * head_stride + i * row_stride; S rows are there, of which
+ *                lens[b] (device int32 [B], taken within 0..S) are written.  Rows
+ *                behind them are not read.
+ *   out          [B][T][n_q * d] contiguous
+ *   workspace    lsk_prefix_attention_workspace_bytes(...) bytes, 16-byte aligned;
+ *                calls that share one must be stream-ordered.
+ * d must be 128; pointers 16-byte aligned; a kv head's rows must span less than
+ * 2^31 bytes.  Results do not depend on timing: every sum has a fixed order.
+ * Takes the place of F.scaled_dot_product_attention over a cache of every
+ * request's whole context (src/leanstack/runtime/qwen_explicit.py:894-912,
+ * :1000-1039). */
+int lsk_prefix_attention_bf16(const void* q, long long q_batch_stride, long long q_head_stride,
+                              long long q_token_stride, int B, int T, int n_q, int n_kv, int head_dim,
+                              const void* prefix_k, const void* prefix_v, long long prefix_head_stride,
+                              int prefix_row_stride, int P, const void* k, const void* v,
+                              long long batch_stride, long long head_stride, int row_stride, int S,
+                              const int* lens, float scale, void* out, void* workspace, size_t ws_bytes,
+                              void* hip_stream);
+
 /* Device workspace of lsk_lora_add_bf16 for these sizes (any contents; 0: none). */
 size_t lsk_lora_workspace_bytes(int M, int N, int K, int rank_tiles, int count);
 

@@ -390,6 +390,70 @@ int lsk_rmsnorm_lm_head_argmax_bf16(const void* w_packed, int layout_id, int V, 
 
 }  // extern "C"
 
+// ------------------------------------------------------------- attention over a shared prefix
+
+extern "C" {
+
+size_t lsk_prefix_attention_workspace_bytes(int B, int T, int n_q, int n_kv, int P, int S) {
+  if (B < 1 || T < 1 || n_kv < 1 || n_q < n_kv || n_q % n_kv != 0 || P < 0 || S < 0) return 0;
+  return (size_t)lsk::prefix_workspace_bytes(lsk::prefix_plan(B, T, n_q, n_kv, P, S), B, T, n_q);
+}
+
+int lsk_prefix_attention_bf16(const void* q, long long q_batch_stride, long long q_head_stride,
+                              long long q_token_stride, int B, int T, int n_q, int n_kv, int head_dim,
+                              const void* prefix_k, const void* prefix_v, long long prefix_head_stride,
+                              int prefix_row_stride, int P, const void* k, const void* v, long long batch_stride,
+                              long long head_stride, int row_stride, int S, const int* lens, float scale, void* out,
+                              void* workspace, size_t ws_bytes, void* hip_stream) {
+  lsk::clear_error();
+  if (int st = lsk::check_prefix_args(q, q_batch_stride, q_head_stride, q_token_stride, B, T, n_q, n_kv, head_dim,
+                                      prefix_k, prefix_v, prefix_head_stride, prefix_row_stride, P, k, v, batch_stride,
+                                      head_stride, row_stride, S, lens, scale, out))
+    return st;
+  const lsk::PrefixPlan p = lsk::prefix_plan(B, T, n_q, n_kv, P, S);
+  const size_t need = (size_t)lsk::prefix_workspace_bytes(p, B, T, n_q);
+  if (need > 0 && (workspace == nullptr || ws_bytes < need || !aligned(workspace, 16)))
+    return fail(LSK_ERR_WORKSPACE, "the attention needs a workspace of %zu bytes, 16-byte aligned (got %zu)", need,
+                workspace ? ws_bytes : 0);
+  lsk::PrefixArgs a;
+  a.q = static_cast<const __bf16*>(q);
+  a.pk = static_cast<const __bf16*>(prefix_k);
+  a.pv = static_cast<const __bf16*>(prefix_v);
+  a.k = static_cast<const __bf16*>(k);
+  a.v = static_cast<const __bf16*>(v);
+  a.lens = lens;
+  a.out = static_cast<__bf16*>(out);
+  a.rows = (size_t)B * T * n_q;
+  a.part_o = static_cast<float*>(workspace);
+  a.part_ml = need > 0 ? a.part_o + (size_t)(p.prefix_parts + p.own_parts) * a.rows * lsk::kAttnHeadDim : nullptr;
+  a.q_b = (size_t)q_batch_stride;
+  a.q_h = (size_t)q_head_stride;
+  a.q_t = (size_t)q_token_stride;
+  a.p_h = (size_t)prefix_head_stride;
+  a.k_b = (size_t)batch_stride;
+  a.k_h = (size_t)head_stride;
+  a.p_row = prefix_row_stride;
+  a.k_row = row_stride;
+  a.B = B;
+  a.T = T;
+  a.G = n_q / n_kv;
+  a.n_q = n_q;
+  a.n_kv = n_kv;
+  a.P = P;
+  a.S = S;
+  a.prefix_items = n_kv * p.prefix_tiles * p.prefix_parts;
+  a.prefix_parts = p.prefix_parts;
+  a.prefix_chunk = p.prefix_chunk;
+  a.own_tiles = p.own_tiles;
+  a.own_chunk = p.own_chunk;
+  a.scale = scale;
+  hipError_t err = lsk::launch_prefix_attention(a, p, static_cast<hipStream_t>(hip_stream));
+  if (err != hipSuccess) return hip_fail(err, "prefix attention kernel launch");
+  return LSK_OK;
+}
+
+}  // extern "C"
+
 // ------------------------------------------------------------- low-rank adapters
 
 extern "C" {

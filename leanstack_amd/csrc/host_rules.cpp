@@ -190,6 +190,43 @@ int check_constrain_args(const void* logits, int logits_mode, int M, int V, long
   return LSK_OK;
 }
 
+int check_prefix_args(const void* q, long long q_batch, long long q_head, long long q_token, int B, int T, int n_q,
+                      int n_kv, int head_dim, const void* prefix_k, const void* prefix_v, long long prefix_head,
+                      int prefix_row, int P, const void* k, const void* v, long long batch, long long head, int row,
+                      int S, const int* lens, float scale, const void* out) {
+  if (head_dim != kAttnHeadDim)
+    return fail(LSK_ERR_INVALID, "head_dim=%d: the attention kernel is built for %d", head_dim, kAttnHeadDim);
+  if (n_kv < 1 || n_q < n_kv || n_q % n_kv != 0)
+    return fail(LSK_ERR_INVALID, "n_q=%d must be a multiple of n_kv=%d", n_q, n_kv);
+  if (B < 1 || T < 1 || P < 0 || S < 0) return fail(LSK_ERR_INVALID, "B=%d, T=%d, P=%d, S=%d rows", B, T, P, S);
+  // Query rows and grids are counted in 32 bits, key rows addressed with 31.
+  const long long most = 0xffffffffLL / kPrefixThreads;
+  if ((long long)B * T > most || (long long)B * T * n_q > most)
+    return fail(LSK_ERR_INVALID, "B=%d, T=%d, n_q=%d: too many query rows", B, T, n_q);
+  const PrefixPlan p = prefix_plan(B, T, n_q, n_kv, P, S);
+  const long long prefix_items = (long long)n_kv * p.prefix_tiles * p.prefix_parts;
+  const long long own_items = (long long)n_kv * B * p.own_tiles;
+  if (own_items > most || prefix_items > most || prefix_items + own_items * (p.joint ? 1 : p.own_parts) > most)
+    return fail(LSK_ERR_INVALID, "B=%d, T=%d, n_q=%d over %d + %d rows: too many items", B, T, n_q, P, S);
+  if (prefix_row < head_dim || row < head_dim || prefix_row % 8 != 0 || row % 8 != 0)
+    return fail(LSK_ERR_INVALID, "row strides %d, %d must be multiples of 8, at least %d", prefix_row, row, head_dim);
+  if ((long long)P * prefix_row >= (1LL << 30) || (long long)S * row >= (1LL << 30))
+    return fail(LSK_ERR_INVALID, "%d and %d rows at strides %d and %d: a head's rows must stay below 2^31 bytes", P, S,
+                prefix_row, row);
+  const long long strides[] = {q_batch, q_head, q_token, prefix_head, batch, head};
+  for (long long s : strides)
+    if (s < 0 || s % 8 != 0) return fail(LSK_ERR_INVALID, "strides must be multiples of 8, not negative (%lld)", s);
+  if (q == nullptr || lens == nullptr || out == nullptr || (P > 0 && (prefix_k == nullptr || prefix_v == nullptr)) ||
+      (S > 0 && (k == nullptr || v == nullptr)))
+    return fail(LSK_ERR_INVALID, "null device pointer");
+  const void* wide[] = {q, prefix_k, prefix_v, k, v, out};
+  for (const void* w : wide)
+    if (!aligned(w, 16)) return fail(LSK_ERR_INVALID, "q, the keys and values and out must be 16-byte aligned");
+  if (!aligned(lens, 4)) return fail(LSK_ERR_INVALID, "lens must be 4-byte aligned");
+  if (!std::isfinite(scale)) return fail(LSK_ERR_INVALID, "scale must be finite");
+  return LSK_OK;
+}
+
 int check_lora_args(const void* y, int M, int N, int ldy, const void* x, int K, int ldx, const void* a_tiles,
                     const void* b_tiles, const float* scale, const int* ranks, int count, int rank_tiles,
                     const int* index, int epilogue, const void* out) {

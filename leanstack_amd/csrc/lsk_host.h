@@ -60,6 +60,52 @@ constexpr int attention_most_chunks(int max_seq_len) {
   return most < kAttnMaxChunks ? most : kAttnMaxChunks;
 }
 
+// Attention over a shared prefix (prefix_attention.hip).
+constexpr int kPrefixThreads = 256;
+
+// How a call runs.  joint: one launch, an item per 32 query rows of one request
+// and kv head.  Else prefix_parts ranges of prefix_chunk prefix rows per kv head and
+// prefix_tiles of 32 (shared: 128) query rows, and own_parts ranges of own_chunk own rows per kv
+// head, request and own_tiles of 32 query rows.
+struct PrefixPlan {
+  bool joint, shared;
+  int prefix_tiles, prefix_chunk, prefix_parts, own_tiles, own_chunk, own_parts;
+};
+constexpr int ceil_div(long long a, long long b) { return (int)((a + b - 1) / b); }
+constexpr PrefixPlan prefix_plan(int B, int T, int n_q, int n_kv, int P, int S) {
+  PrefixPlan p = {false, false, 0, 128, 0, ceil_div((long long)T * (n_q / n_kv), 32), 128, 0};
+  const long long rows = (long long)B * T * (n_q / n_kv);
+  if ((long long)P + S <= 512) {
+    p.joint = true;
+    return p;
+  }
+  p.shared = rows > 64;
+  if (P > 0) {
+    const int tile = p.shared ? 128 : 32, unit = p.shared ? 32 : 128, least = p.shared ? 256 : 128;
+    p.prefix_tiles = ceil_div(rows, tile);
+    const int wanted = ceil_div(512, (long long)n_kv * p.prefix_tiles);
+    const int chunk = ceil_div(ceil_div(P, wanted), unit) * unit;
+    p.prefix_chunk = chunk < least ? least : chunk;
+    p.prefix_parts = ceil_div(P, p.prefix_chunk);
+  }
+  if (S > 0) {
+    const int chunk = ceil_div(ceil_div(S, 64), 128) * 128;
+    p.own_chunk = chunk < 256 ? 256 : chunk;
+    p.own_parts = ceil_div(S, p.own_chunk);
+  }
+  return p;
+}
+// fp32 (m, l) and O of every query row and part.
+constexpr unsigned long long prefix_workspace_bytes(const PrefixPlan& p, int B, int T, int n_q) {
+  return (unsigned long long)(p.prefix_parts + p.own_parts) * B * T * n_q * (kAttnHeadDim + 2) * 4ull;
+}
+
+// Argument rules of lsk_prefix_attention_bf16 (all but the workspace's size).
+int check_prefix_args(const void* q, long long q_batch, long long q_head, long long q_token, int B, int T, int n_q,
+                      int n_kv, int head_dim, const void* prefix_k, const void* prefix_v, long long prefix_head,
+                      int prefix_row, int P, const void* k, const void* v, long long batch, long long head, int row,
+                      int S, const int* lens, float scale, const void* out);
+
 // Constrained logits (constrain.hip): a row's vocabulary is cut into slices, one
 // workgroup each; a slice's counts are one LDS word per entry.
 constexpr int kConstrainMaxHistory = 1 << 20;

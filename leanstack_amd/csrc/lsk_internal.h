@@ -135,6 +135,34 @@ __device__ __forceinline__ void wave_lds_order() {
   __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
 
+typedef unsigned int lds_load_words_t __attribute__((ext_vector_type(4)));
+
+__device__ __forceinline__ lds_load_words_t buffer_words(const void* base, size_t bytes) {
+  const unsigned long long p = reinterpret_cast<unsigned long long>(base);
+  return lds_load_words_t{(unsigned)p, (unsigned)(p >> 32) & 0xffffu, (unsigned)(bytes < 0x7fffffffu ? bytes : 0x7fffffffu),
+                 0x00020000u};
+}
+
+// 1 KB of global memory straight into LDS: lane l's 16 bytes at voff + soff
+// land at lds + 16 l.  In assembly, with no result register, so that the
+// compiler neither counts it nor waits for it before unrelated LDS reads (one
+// ring in one LDS array would otherwise be drained before every read); each
+// use waits for its own data (wait_steps).  m0, the LDS address of such a load,
+// is written here and named as clobbered.
+template <bool STREAM>
+__device__ __forceinline__ void dma_1k(lds_load_words_t rsrc, unsigned voff, unsigned soff, unsigned lds) {
+  soff = __builtin_amdgcn_readfirstlane(soff);  // wave-uniform; says so to the compiler
+  lds = __builtin_amdgcn_readfirstlane(lds);
+  if constexpr (STREAM)
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen nt lds" ::"s"(lds), "v"(voff),
+                 "s"(rsrc), "s"(soff)
+                 : "m0", "memory");
+  else
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(lds), "v"(voff),
+                 "s"(rsrc), "s"(soff)
+                 : "m0", "memory");
+}
+
 // One projection of a stack program, as the kernel reads it (64 bytes).
 struct StackDesc {
   const bf16x8_t* w;
@@ -257,6 +285,22 @@ struct ConstrainArgs {
   int M, V, slice, slices, history_len, bias_count;
 };
 hipError_t launch_constrain(const ConstrainArgs& a, bool bf16, hipStream_t stream);
+
+// Attention of T query tokens of B requests over P shared and up to S own rows
+// (prefix_attention.hip).  Strides in elements; part_ml / part_o: (m, l) and O of
+// every part and query row (rows = B T n_q), m in base 2.
+struct PrefixArgs {
+  const __bf16 *q, *pk, *pv, *k, *v;
+  const int* lens;
+  __bf16* out;
+  float *part_ml, *part_o;
+  size_t q_b, q_h, q_t, p_h, k_b, k_h, rows;
+  int p_row, k_row;
+  int B, T, G, n_q, n_kv, P, S;
+  int prefix_items, prefix_parts, prefix_chunk, own_tiles, own_chunk;
+  float scale;
+};
+hipError_t launch_prefix_attention(const PrefixArgs& a, const PrefixPlan& plan, hipStream_t stream);
 
 // Low-rank adapters added to M projected rows (adapters.hip).  Tiles as in
 // leanstack_amd.h; strides in elements per adapter; h: the partials of the first

@@ -1,0 +1,628 @@
+// Attention of a batch of requests that share a prefix, for gfx950: T query
+// tokens of each request over P prefix rows, held once, and over the rows that
+// the request has cached since (causal within them).
+//
+//   out = sum_i e^(s_i - m) v_i / sum_i e^(s_i - m),  s = scale q . k,
+// over the prefix rows and the request's own visible rows.  The prefix is read
+// once for many requests' heads instead of once per request, which is what
+// makes a long one cheap.
+//
+// Work is cut into items: 32 (or 4 x 32) query rows of one kv head over a
+// range of key rows.  Query rows of a prefix item are those of any requests (row
+// (b T + t) G + g of the kv head); an own item's are one request's.  A wave
+// holds 32 query rows and takes 32 key rows a step:
+//   S^T = K Q^T on v_mfma_f32_32x32x16_bf16, so that a lane holds 16 scores of
+//     one query row, and the other 16 are in the other half-wave;
+//   the running maximum m and sum l of the softmax, in base 2, in fp32.  m is
+//     raised only where a step exceeds it by 2^8 (weights up to 2^8 are as exact
+//     as weights up to 1, and the sums, rescaled on a raise, stay in range);
+//   O^T += V^T P^T on the same MFMA.  The scores' lanes are those of the B operand
+//     if the 16 key rows of a product are taken in the order that the lanes hold
+//     them in, so P needs no transposition; V^T comes from LDS by
+//     ds_read_b64_tr_b16.
+// P is rounded to bf16, at most 2^-9 of each weight, and l sums the rounded
+// weights: the result is exactly that of slightly other weights, whose errors
+// average out over the rows (the output's own rounding is as large).
+//
+// K and V rows go to LDS by DMA, their 16-byte chunks permuted by row so that
+// neither the reads of K (one row per lane) nor of V (four rows per 16 lanes)
+// meet in a bank.  Rows past the last visible one are that row again, so what
+// lies behind the written rows is never read.
+//
+// Items whose 4 waves share query rows (own rows; few prefix rows) split the
+// key rows, each wave with a slot of its own and no barrier: the next step's K is
+// on its way while P V is multiplied, the next V during the next scores.  Items
+// of 128 query rows share each step's rows among the waves through a ring.
+//
+// An item leaves (m, l, O) in fp32 in the workspace and a second launch adds a
+// row's items up; a short context runs in one launch, each request's items
+// reading the prefix and its own rows.
+
+#include <hip/hip_runtime.h>
+
+#include "lsk_internal.h"
+
+namespace lsk {
+namespace {
+
+typedef float f32x2_t __attribute__((ext_vector_type(2)));
+typedef float f32x4_t __attribute__((ext_vector_type(4)));
+typedef float f32x16_t __attribute__((ext_vector_type(16)));
+typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x4_t __attribute__((ext_vector_type(4)));
+
+constexpr int D = kAttnHeadDim;
+constexpr int kThreads = kPrefixThreads;
+constexpr int kWaves = kThreads / 64;
+static_assert(kWaves == 4, "four waves' slots, and four waves to a shared item");
+constexpr int kStep = 32;                  // key rows, and query rows of a wave
+constexpr int kHalfSlot = kStep * D * 2;   // bytes of a step's K, or V
+constexpr int kSlot = 2 * kHalfSlot;
+constexpr int kSlots = 4;                  // one per wave, or a ring of steps
+constexpr float kRaise = 8.f;
+
+__device__ __forceinline__ float neg_inf() { return -__builtin_huge_valf(); }
+
+// Both halves' values of a lane pair 32 apart, in both lanes.  (The compiler takes
+// a swap of a value with itself for two equal results: it is given a copy that it
+// does not know to be one.)
+struct Halves {
+  float low, high;
+};
+__device__ __forceinline__ Halves both_halves(float v) {
+  const unsigned a = __builtin_bit_cast(unsigned, v);
+  unsigned b = a;
+  asm("" : "+v"(b));
+  const auto r = __builtin_amdgcn_permlane32_swap(a, b, false, false);
+  return {__builtin_bit_cast(float, (unsigned)r[0]), __builtin_bit_cast(float, (unsigned)r[1])};
+}
+__device__ __forceinline__ float other_half_max(float v) {
+  const Halves h = both_halves(v);
+  return fmaxf(h.low, h.high);
+}
+__device__ __forceinline__ float other_half_sum(float v) {
+  const Halves h = both_halves(v);
+  return h.low + h.high;
+}
+
+// Rows that request b has cached, and those of them that its query t sees.
+__device__ __forceinline__ int own_written(const PrefixArgs& a, int b) { return min(max(a.lens[b], 0), a.S); }
+__device__ __forceinline__ int own_visible(const PrefixArgs& a, int b, int t) {
+  return max(own_written(a, b) - (a.T - 1 - t), 0);
+}
+
+// Key rows [begin, end) of one kv head.
+struct Rows {
+  const __bf16 *k, *v;
+  int stride;  // elements from a row to the next
+  int begin, end;
+};
+
+// A wave's softmax state for its 32 query rows: lane (h, c) holds row c, of O the
+// dims 32 db + 8 (i / 4) + 4 h + i % 4, of l the share of the lane's scores.
+struct State {
+  float m, l;
+  f32x16_t o[4];
+};
+
+// Addresses of a lane in a step's rows, the same for every step.
+struct Lane {
+  unsigned k_at[4], v_at[2];  // DMA: byte offsets from the step's first row, K loads 0..3 and V loads 0..1
+  unsigned k_read;            // LDS: row c, chunk h
+  unsigned v_read;            // LDS: transposing read of 4 rows x 16 dims per 16 lanes
+};
+
+// Chunk (16 bytes) `ch` of row r is at position ch ^ (r % 16) for K and
+// ch ^ 2 (r % 8) for V.
+__device__ __forceinline__ Lane lane_addresses(int stride) {
+  const int lane = threadIdx.x & 63;
+  Lane a;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {  // load i: rows 4 i + lane / 16
+    const int r = 4 * i + (lane >> 4);
+    a.k_at[i] = (unsigned)(r * stride * 2 + (((lane & 15) ^ r) << 4));
+  }
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int r = 4 * i + (lane >> 4);
+    a.v_at[i] = (unsigned)(r * stride * 2 + (((lane & 15) ^ (2 * r)) << 4));
+  }
+  const int c = lane & 31, h = lane >> 5;
+  a.k_read = (unsigned)(c * 256 + ((h ^ (c & 15)) << 4));
+  const int i = lane & 15, q = lane >> 4;
+  const int r = 4 * (q >> 1) + (i >> 2);
+  a.v_read = (unsigned)(r * 256 + (((2 * (q & 1) + ((i & 3) >> 1)) ^ (2 * r)) << 4) + ((i & 1) << 3));
+  return a;
+}
+
+// DMA loads [first, first + N) of the 8 (1 KB, 4 rows each) of a step's K or V: all
+// of them, or a wave's two of four waves'.  Rows from `end` on are row end - 1.
+template <bool IS_V, int N>
+__device__ __forceinline__ void load_half(lds_load_words_t buf, const Lane& a, int stride, int row0, int end, int first,
+                                          unsigned lds) {
+  const int lane = threadIdx.x & 63;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const int u = first + i;
+    if (row0 + kStep <= end) {
+      // the chunk order repeats every 16 rows (K) or 8 (V)
+      if constexpr (IS_V)
+        dma_1k<false>(buf, a.v_at[i & 1], (unsigned)(row0 + 4 * (u & ~1)) * (unsigned)(stride * 2), lds + u * 1024);
+      else
+        dma_1k<false>(buf, a.k_at[i & 3], (unsigned)(row0 + 4 * (u & ~3)) * (unsigned)(stride * 2), lds + u * 1024);
+    } else {
+      const int r = 4 * u + (lane >> 4);
+      const int chunk = (lane & 15) ^ (IS_V ? 2 * (r & 7) : (r & 15));
+      const unsigned at = (unsigned)min(row0 + r, end - 1) * (unsigned)(stride * 2) + (unsigned)(chunk << 4);
+      dma_1k<false>(buf, at, 0, lds + u * 1024);
+    }
+  }
+}
+
+typedef __attribute__((address_space(3))) const unsigned char lds_byte_t;
+
+// S^T = K Q^T of a step.
+__device__ __forceinline__ f32x16_t step_scores(lds_byte_t* k, const Lane& a, const bf16x8_t (&qf)[8]) {
+  f32x16_t s = {};
+#pragma unroll
+  for (int ks = 0; ks < 8; ++ks) {
+    const auto* at = reinterpret_cast<__attribute__((address_space(3))) const bf16x8_t*>(k + (a.k_read ^ (unsigned)(ks << 5)));
+    s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*at, qf[ks], s, 0, 0, 0);
+  }
+  return s;
+}
+
+// V^T of rows 16 s .. + 15 (in the lanes' order: slot e of half h is row
+// 16 s + 8 (e / 4) + 4 h + e % 4), dims 32 db .. + 31.
+__device__ __forceinline__ bf16x8_t v_operand(lds_byte_t* v, const Lane& a, int s, int db) {
+  typedef __attribute__((address_space(3))) bf16x4_t lds_bf16x4_t;
+  auto* at = (lds_bf16x4_t*)(v + (a.v_read ^ (unsigned)(db << 6)) + s * 16 * 256);
+  const bf16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4bf16(at);
+  const bf16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4bf16(at + 8 * 256 / 8);
+  return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+}
+
+// The step's weights P (bf16, the B operands of its two products), and m, l, O
+// brought to the new maximum.  limit: key rows that the lane's query row sees, in
+// rows of the step (from 32 on: all).
+template <bool MASK>
+__device__ __forceinline__ void step_weights(f32x16_t s, float c2, int limit, State& st, bf16x8_t (&p)[2]) {
+  const int h = (threadIdx.x & 63) >> 5;
+  if constexpr (MASK) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+      if (8 * (i / 4) + 4 * h + i % 4 >= limit) s[i] = neg_inf();
+  }
+  float mx = s[0];
+#pragma unroll
+  for (int i = 1; i < 16; ++i) mx = fmaxf(mx, s[i]);
+  mx = other_half_max(mx) * c2;
+  if (MASK && limit <= 0) mx = neg_inf();  // (-inf times a scale of zero)
+  const bool raise = mx > st.m + kRaise;
+  if (__ballot(raise)) {  // (a query row's maximum goes by its own scores alone)
+    const float f = raise ? __builtin_amdgcn_exp2f(st.m - mx) : 1.f;
+    st.m = raise ? mx : st.m;
+    st.l *= f;
+#pragma unroll
+    for (int db = 0; db < 4; ++db)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) st.o[db][i] *= f;
+  }
+  const float m = st.m == neg_inf() ? 0.f : st.m;
+  const bf16x2_t ones = {static_cast<__bf16>(1.f), static_cast<__bf16>(1.f)};
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], c2, -m));
+    if (MASK && 8 * (i / 4) + 4 * h + i % 4 >= limit) e = 0.f;
+    p[i / 8][i % 8] = static_cast<__bf16>(e);
+  }
+#pragma unroll
+  for (int i = 0; i < 16; i += 2)
+    st.l = __builtin_amdgcn_fdot2_f32_bf16(bf16x2_t{p[i / 8][i % 8], p[i / 8][i % 8 + 1]}, ones, st.l, false);
+}
+
+__device__ __forceinline__ void step_accumulate(lds_byte_t* v, const Lane& a, const bf16x8_t (&p)[2], State& st) {
+#pragma unroll
+  for (int s = 0; s < 2; ++s)
+#pragma unroll
+    for (int db = 0; db < 4; ++db)
+      st.o[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v_operand(v, a, s, db), p[s], st.o[db], 0, 0, 0);
+}
+
+// V of a step's rows that not every query row sees: a weight of zero does not take
+// an infinity or a NaN out of a product.  Rows from `end` on, which stand in for
+// rows past the last, become zero; so do the infinite and NaN values of the rows
+// from `all` to `end` (write_item adds them to the query rows that see them).
+// Returns whether there were any.
+__device__ __forceinline__ bool mask_values(unsigned char* v, int all, int end) {
+  typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+  const int lane = threadIdx.x & 63;
+  bool found = false;
+#pragma unroll
+  for (int i = 0; i < kHalfSlot / 1024; ++i) {
+    const int r = 4 * i + (lane >> 4);
+    u32x4* at = reinterpret_cast<u32x4*>(v + i * 1024 + lane * 16);
+    if (r >= end) {
+      *at = u32x4{0u, 0u, 0u, 0u};
+    } else if (r >= all) {
+      u32x4 w = *at;
+      bool here = false;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const bool low = (w[e] & 0x00007f80u) == 0x00007f80u, high = (w[e] & 0x7f800000u) == 0x7f800000u;
+        w[e] &= (low ? 0xffff0000u : 0xffffffffu) & (high ? 0x0000ffffu : 0xffffffffu);
+        here |= low | high;
+      }
+      if (here) *at = w;
+      found |= here;
+    }
+  }
+  wave_lds_order();
+  return __ballot(found) != 0;
+}
+
+// vmcnt(8): all but the 8 loads last issued have landed; and what the wave read
+// from LDS before is in registers, so its slot may be written.
+__device__ __forceinline__ void wait_half() { asm volatile("s_waitcnt vmcnt(8) lgkmcnt(0)" ::: "memory"); }
+__device__ __forceinline__ void wait_reads() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
+__device__ __forceinline__ void wait_all() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory"); }
+
+__device__ __forceinline__ lds_load_words_t row_words(const __bf16* p, int stride, int end) {
+  return buffer_words(p, ((size_t)(end - 1) * stride + D) * 2);
+}
+
+// Rows of `src`, the steps w, w + 4, .. for wave w, in the wave's own slot.  limit:
+// key rows that the lane's query row sees; `least`, the least of them (CAUSAL).
+// Returns whether mask_values took values out.
+template <bool CAUSAL>
+__device__ __forceinline__ bool attend_split(const Rows& src, const bf16x8_t (&qf)[8], float c2, int limit,
+                                             int least, unsigned char* slots, State& st) {
+  const int wave = threadIdx.x >> 6;
+  int row0 = src.begin + wave * kStep;
+  if (row0 >= src.end) return false;
+  bool special = false;
+  const Lane a = lane_addresses(src.stride);
+  const lds_load_words_t kb = row_words(src.k, src.stride, src.end), vb = row_words(src.v, src.stride, src.end);
+  auto* slot = (lds_byte_t*)(slots + wave * kSlot);
+  const unsigned at = (unsigned)(size_t)slot;
+  wait_all();  // (loads counted by the compiler are not among those counted here)
+  load_half<false, 8>(kb, a, src.stride, row0, src.end, 0, at);
+  load_half<true, 8>(vb, a, src.stride, row0, src.end, 0, at + kHalfSlot);
+  while (true) {
+    const int next = row0 + kWaves * kStep;
+    const bool more = next < src.end;
+    wait_half();  // K is here
+    const f32x16_t s = step_scores(slot, a, qf);
+    wait_reads();
+    if (more) load_half<false, 8>(kb, a, src.stride, next, src.end, 0, at);
+    bf16x8_t p[2];
+    const bool full = row0 + kStep <= (CAUSAL ? min(least, src.end) : src.end);
+    if (full)
+      step_weights<false>(s, c2, kStep, st, p);
+    else
+      step_weights<true>(s, c2, min(limit, src.end) - row0, st, p);
+    if (more)
+      wait_half();  // V is here
+    else
+      wait_all();
+    if (!full)
+      special |= mask_values(slots + wave * kSlot + kHalfSlot, (CAUSAL ? least : src.end) - row0, src.end - row0);
+    step_accumulate(slot + kHalfSlot, a, p, st);
+    if (!more) break;
+    wait_reads();
+    load_half<true, 8>(vb, a, src.stride, next, src.end, 0, at + kHalfSlot);
+    row0 = next;
+  }
+  wait_all();
+  return special;
+}
+
+// Rows of `src` for four waves with query rows of their own: steps through a
+// ring of kSlots, two K and two V loads of each by each wave.
+__device__ __forceinline__ void attend_shared(const Rows& src, const bf16x8_t (&qf)[8], float c2, unsigned char* slots,
+                                              State& st) {
+  const int wave = threadIdx.x >> 6;
+  Lane a = lane_addresses(src.stride);
+  if (wave & 1) a.k_at[0] = a.k_at[2], a.k_at[1] = a.k_at[3];  // loads 2 wave and 2 wave + 1
+  const lds_load_words_t kb = row_words(src.k, src.stride, src.end), vb = row_words(src.v, src.stride, src.end);
+  const int steps = (src.end - src.begin + kStep - 1) / kStep;
+  auto* ring = (lds_byte_t*)slots;
+  auto load = [&](int i) {
+    // (past the last step the last one again, into a slot that is not read: the
+    // count of loads in flight stays the same)
+    const int row0 = src.begin + min(i, steps - 1) * kStep;
+    const unsigned at = (unsigned)(size_t)ring + (unsigned)(i % kSlots) * kSlot;
+    load_half<false, 2>(kb, a, src.stride, row0, src.end, 2 * wave, at);
+    load_half<true, 2>(vb, a, src.stride, row0, src.end, 2 * wave, at + kHalfSlot);
+  };
+  wait_all();
+#pragma unroll
+  for (int i = 0; i < kSlots - 1; ++i) load(i);
+  for (int i = 0; i < steps; ++i) {
+    // Steps up to i have landed here (two of 4 loads each are behind it), and with
+    // the barrier everywhere; every wave is done with step i - 1, whose slot the
+    // next load takes.
+    asm volatile("s_waitcnt vmcnt(8) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    load(i + kSlots - 1);
+    auto* slot = ring + (i % kSlots) * kSlot;
+    const int row0 = src.begin + i * kStep;
+    const f32x16_t s = step_scores(slot, a, qf);
+    bf16x8_t p[2];
+    const bool full = row0 + kStep <= src.end;
+    if (full)
+      step_weights<false>(s, c2, kStep, st, p);
+    else
+      step_weights<true>(s, c2, src.end - row0, st, p);
+    // (every wave clears the same rows before it reads them)
+    if (!full) mask_values(slots + (i % kSlots) * kSlot + kHalfSlot, src.end - row0, src.end - row0);
+    step_accumulate(slot + kHalfSlot, a, p, st);
+  }
+  wait_all();
+}
+
+// Query row r of kv head j: request, token and q head.
+struct Query {
+  int b, t, h;
+};
+
+// What the 4 waves leave, to rows of the output or of the workspace.
+//   SPLIT: the waves hold the same 32 query rows over different key rows, added
+//   here; else 32 rows each.
+// find(i): query row i of the item, or b = -1 behind the last one.  add(q, d, l, o): what
+// mask_values took out of dims d .. d + 3 for query row q, whose weights sum to l.
+template <bool SPLIT, bool DIRECT, typename Find, typename Add>
+__device__ __forceinline__ void write_item(const PrefixArgs& a, const State& st, unsigned char* slots, float (*ms)[32],
+                                           float (*ls)[32], int part, Find find, Add add) {
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int c = lane & 31, h = lane >> 5;
+  const float l = other_half_sum(st.l);
+  __syncthreads();  // the slots' last reads and loads are done in every wave
+  // O to LDS as rows of 512 bytes, chunk ch of row c at ch ^ c.
+  unsigned char* mine = slots + wave * kSlot + c * 512;
+#pragma unroll
+  for (int db = 0; db < 4; ++db)
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const int ch = 8 * db + 2 * q + h;
+      *reinterpret_cast<f32x4_t*>(mine + ((ch ^ c) << 4)) =
+          f32x4_t{st.o[db][4 * q], st.o[db][4 * q + 1], st.o[db][4 * q + 2], st.o[db][4 * q + 3]};
+    }
+  if (h == 0) {
+    ms[wave][c] = st.m;
+    ls[wave][c] = l;
+  }
+  __syncthreads();
+  constexpr int kPasses = SPLIT ? 1 : 4;
+  constexpr int kFrom = SPLIT ? kWaves : 1;
+#pragma unroll
+  for (int pass = 0; pass < kPasses; ++pass) {
+    const int r = SPLIT ? tid >> 3 : pass * 8 + (lane >> 3);  // of the wave's 32
+    const Query q = find(SPLIT ? r : wave * 32 + r);
+    if (q.b < 0) continue;
+    float w[kFrom], m = neg_inf(), sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < kFrom; ++i) m = fmaxf(m, ms[SPLIT ? i : wave][r]);
+#pragma unroll
+    for (int i = 0; i < kFrom; ++i) {
+      const float mi = ms[SPLIT ? i : wave][r];
+      w[i] = mi == m ? 1.f : __builtin_amdgcn_exp2f(mi - m);
+      sum += w[i] * ls[SPLIT ? i : wave][r];
+    }
+    const size_t row = ((size_t)q.b * a.T + q.t) * a.n_q + q.h;
+    const size_t slot_row = (size_t)part * a.rows + row;
+    // (no row at all: zero; rows that all score -inf: 0 / 0)
+    const bool none = a.P == 0 && own_visible(a, q.b, q.t) == 0;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int ch = (lane & 7) + 8 * k;
+      f32x4_t o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int i = 0; i < kFrom; ++i)
+        o += w[i] * *reinterpret_cast<const f32x4_t*>(slots + (SPLIT ? i : wave) * kSlot + r * 512 + ((ch ^ r) << 4));
+      add(q, 4 * ch, sum, o);
+      if constexpr (DIRECT) {
+        bf16x4_t v;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = static_cast<__bf16>(none ? 0.f : o[e] / sum);
+        *reinterpret_cast<bf16x4_t*>(a.out + row * D + 4 * ch) = v;
+      } else {
+        *reinterpret_cast<f32x4_t*>(a.part_o + slot_row * D + 4 * ch) = o;
+      }
+    }
+    if (!DIRECT && (lane & 7) == 0) *reinterpret_cast<f32x2_t*>(a.part_ml + slot_row * 2) = f32x2_t{m, sum};
+  }
+}
+
+// B operands of a wave's 32 query rows, the sign of the scale in them.
+__device__ __forceinline__ void load_q(const PrefixArgs& a, const Query& q, bf16x8_t (&qf)[8]) {
+  const int h = (threadIdx.x & 63) >> 5;
+  const __bf16* at = a.q + (size_t)q.b * a.q_b + (size_t)q.h * a.q_h + (size_t)q.t * a.q_t + 8 * h;
+  typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+  const unsigned flip = a.scale < 0.f ? 0x80008000u : 0u;
+#pragma unroll
+  for (int ks = 0; ks < 8; ++ks) {
+    u32x4 w = *reinterpret_cast<const u32x4*>(at + 16 * ks);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) w[e] ^= flip;
+    qf[ks] = __builtin_bit_cast(bf16x8_t, w);
+  }
+}
+
+__device__ __forceinline__ State empty_state() {
+  State st;
+  st.m = neg_inf();
+  st.l = 0.f;
+#pragma unroll
+  for (int db = 0; db < 4; ++db) st.o[db] = f32x16_t{};
+  return st;
+}
+
+// One request's query rows r0 .. r0 + 31 of kv head j over its own rows [begin, end),
+// with JOINT over the prefix in front of them.
+template <bool CAUSAL, bool JOINT>
+__device__ __forceinline__ void own_item(const PrefixArgs& a, int j, int b, int r0, int begin, int end, int part,
+                                         unsigned char* slots, float (*ms)[32], float (*ls)[32]) {
+  const int c = threadIdx.x & 31;
+  const int rows = a.T * a.G;
+  auto find = [&](int i) {
+    const int r = r0 + i;
+    return r < rows ? Query{b, r / a.G, j * a.G + r % a.G} : Query{-1, 0, 0};
+  };
+  const Query mine = find(min(c, rows - 1 - r0));
+  bf16x8_t qf[8];
+  load_q(a, mine, qf);
+  State st = empty_state();
+  const float c2 = fabsf(a.scale) * 1.44269504088896341f;
+  if (JOINT && a.P > 0) {
+    const Rows src = {a.pk + (size_t)j * a.p_h, a.pv + (size_t)j * a.p_h, a.p_row, 0, a.P};
+    attend_split<false>(src, qf, c2, a.P, a.P, slots, st);
+  }
+  // The rows that the item's first query row sees all of them see, and none is read
+  // that its last one does not.
+  const int least = own_visible(a, b, r0 / a.G);
+  const int stop = min(end, own_visible(a, b, min(r0 + 31, rows - 1) / a.G));
+  const size_t base = (size_t)b * a.k_b + (size_t)j * a.k_h;
+  bool special = false;
+  if (begin < stop) {
+    const Rows src = {a.k + base, a.v + base, a.k_row, begin, stop};
+    special = attend_split<CAUSAL>(src, qf, c2, own_visible(a, b, mine.t), least, slots, st);
+  }
+  if constexpr (CAUSAL) {
+    // Infinite and NaN values of rows that only some query rows see: to those.
+    const bool any = __syncthreads_or(special);
+    const int first = max(begin, least);
+    write_item<true, JOINT>(a, st, slots, ms, ls, part, find, [&](const Query& q, int d, float sum, f32x4_t& o) {
+      if (!any) return;
+      for (int i = first; i < min(stop, own_visible(a, b, q.t)); ++i) {
+        const bf16x4_t v = *reinterpret_cast<const bf16x4_t*>(a.v + base + (size_t)i * a.k_row + d);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float f = static_cast<float>(v[e]);
+          if (!(fabsf(f) < __builtin_huge_valf())) o[e] += sum != 0.f ? f : f * 0.f;  // (of no weight: NaN)
+        }
+      }
+    });
+  } else {
+    write_item<true, JOINT>(a, st, slots, ms, ls, part, find, [](const Query&, int, float, f32x4_t&) {});
+  }
+}
+
+// Query rows r0 .. r0 + (SHARED ? 127 : 31) of kv head j over prefix rows [begin, end).
+template <bool SHARED>
+__device__ __forceinline__ void prefix_item(const PrefixArgs& a, int j, int r0, int begin, int end, int part,
+                                            unsigned char* slots, float (*ms)[32], float (*ls)[32]) {
+  const int rows = a.B * a.T * a.G;
+  auto find = [&](int i) {
+    const int r = r0 + i;
+    if (r >= rows) return Query{-1, 0, 0};
+    const int bt = r / a.G;
+    return Query{bt / a.T, bt % a.T, j * a.G + r % a.G};
+  };
+  const int i = (SHARED ? (threadIdx.x >> 6) * 32 : 0) + (threadIdx.x & 31);
+  bf16x8_t qf[8];
+  load_q(a, find(min(i, rows - 1 - r0)), qf);
+  State st = empty_state();
+  const float c2 = fabsf(a.scale) * 1.44269504088896341f;
+  const Rows src = {a.pk + (size_t)j * a.p_h, a.pv + (size_t)j * a.p_h, a.p_row, begin, end};
+  if constexpr (SHARED)
+    attend_shared(src, qf, c2, slots, st);
+  else
+    attend_split<false>(src, qf, c2, end, end, slots, st);
+  write_item<!SHARED, false>(a, st, slots, ms, ls, part, find, [](const Query&, int, float, f32x4_t&) {});
+}
+
+// Grid: prefix items (kv head fastest: with 8 of them each XCD's L2 holds one
+// head's rows; then key ranges, then query rows), then own items (kv head,
+// request, query rows, key ranges).
+template <bool SHARED, bool CAUSAL>
+__global__ __launch_bounds__(kThreads, 2) void prefix_attention_kernel(PrefixArgs a) {
+  __shared__ __align__(1024) unsigned char slots[kSlots * kSlot];
+  __shared__ float ms[kWaves][32], ls[kWaves][32];
+  int id = blockIdx.x;
+  if (id < a.prefix_items) {
+    const int j = id % a.n_kv;
+    id /= a.n_kv;
+    const int part = id % a.prefix_parts;
+    const int tile = id / a.prefix_parts;
+    const int begin = part * a.prefix_chunk;
+    prefix_item<SHARED>(a, j, tile * (SHARED ? 128 : 32), begin, min(begin + a.prefix_chunk, a.P), part, slots, ms, ls);
+    return;
+  }
+  id -= a.prefix_items;
+  const int j = id % a.n_kv;
+  id /= a.n_kv;
+  const int b = id % a.B;
+  id /= a.B;
+  const int tile = id % a.own_tiles;
+  const int part = id / a.own_tiles;
+  const int begin = part * a.own_chunk;
+  if (begin >= own_written(a, b)) return;  // (the second launch knows this, too)
+  own_item<CAUSAL, false>(a, j, b, tile * 32, begin, begin + a.own_chunk, a.prefix_parts + part, slots, ms, ls);
+}
+
+// Short contexts, one launch.  Grid: (kv head, request, query rows), the head fastest.
+template <bool CAUSAL>
+__global__ __launch_bounds__(kThreads, 2) void joint_attention_kernel(PrefixArgs a) {
+  __shared__ __align__(1024) unsigned char slots[kSlots * kSlot];
+  __shared__ float ms[kWaves][32], ls[kWaves][32];
+  int id = blockIdx.x;
+  const int j = id % a.n_kv;
+  id /= a.n_kv;
+  const int b = id % a.B;
+  own_item<CAUSAL, true>(a, j, b, id / a.B * 32, 0, a.S, 0, slots, ms, ls);
+}
+
+// Adds a row's items up: 32 lanes per row, 4 dims each, in the order of the key rows.
+__global__ __launch_bounds__(kThreads) void combine_kernel(PrefixArgs a) {
+  const size_t row = (size_t)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5);
+  if (row >= a.rows) return;
+  const int d = 4 * (threadIdx.x & 31);
+  const int bt = (int)(row / a.n_q);
+  const int b = bt / a.T;
+  const int parts = a.prefix_parts + (own_written(a, b) + a.own_chunk - 1) / a.own_chunk;
+  float m = neg_inf(), l = 0.f;
+  f32x4_t o = {0.f, 0.f, 0.f, 0.f};
+  for (int p = 0; p < parts; ++p) {
+    const size_t at = (size_t)p * a.rows + row;
+    const f32x2_t ml = *reinterpret_cast<const f32x2_t*>(a.part_ml + at * 2);
+    const f32x4_t v = *reinterpret_cast<const f32x4_t*>(a.part_o + at * D + d);
+    const float top = fmaxf(m, ml[0]);
+    const float was = m == top ? 1.f : __builtin_amdgcn_exp2f(m - top);
+    const float now = ml[0] == top ? 1.f : __builtin_amdgcn_exp2f(ml[0] - top);
+    l = l * was + ml[1] * now;
+    o = o * was + v * now;
+    m = top;
+  }
+  const bool none = a.P == 0 && own_visible(a, b, bt % a.T) == 0;
+  bf16x4_t v;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) v[e] = static_cast<__bf16>(none ? 0.f : o[e] / l);
+  *reinterpret_cast<bf16x4_t*>(a.out + row * D + d) = v;
+}
+
+template <bool CAUSAL>
+hipError_t launch(const PrefixArgs& a, const PrefixPlan& plan, hipStream_t stream) {
+  const unsigned own = (unsigned)a.n_kv * a.B * a.own_tiles;
+  if (plan.joint) {
+    launch_kernel(joint_attention_kernel<CAUSAL>, dim3(own), dim3(kThreads), 0, stream, a);
+    return hipGetLastError();
+  }
+  const dim3 items((unsigned)a.prefix_items + own * plan.own_parts);
+  if (plan.shared)
+    launch_kernel(prefix_attention_kernel<true, CAUSAL>, items, dim3(kThreads), 0, stream, a);
+  else
+    launch_kernel(prefix_attention_kernel<false, CAUSAL>, items, dim3(kThreads), 0, stream, a);
+  hipError_t err = hipGetLastError();
+  if (err != hipSuccess) return err;
+  launch_kernel(combine_kernel, dim3((unsigned)((a.rows + kThreads / 32 - 1) / (kThreads / 32))), dim3(kThreads), 0,
+                stream, a);
+  return hipGetLastError();
+}
+
+}  // namespace
+
+hipError_t launch_prefix_attention(const PrefixArgs& a, const PrefixPlan& plan, hipStream_t stream) {
+  return a.T > 1 ? launch<true>(a, plan, stream) : launch<false>(a, plan, stream);
+}
+
+}  // namespace lsk

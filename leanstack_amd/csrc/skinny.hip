@@ -57,32 +57,6 @@ __device__ __forceinline__ f32x4_t mfma16(bf16x8_t a, bf16x8_t b, f32x4_t c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
 }
 
-__device__ __forceinline__ u32x4_t buffer_words(const void* base, size_t bytes) {
-  const unsigned long long p = reinterpret_cast<unsigned long long>(base);
-  return u32x4_t{(unsigned)p, (unsigned)(p >> 32) & 0xffffu, (unsigned)(bytes < 0x7fffffffu ? bytes : 0x7fffffffu),
-                 kRawBufferDword3};
-}
-
-// 1 KB of global memory straight into LDS: lane l's 16 bytes at voff + soff
-// land at lds + 16 l.  In assembly, with no result register, so that the
-// compiler neither counts it nor waits for it before unrelated LDS reads (one
-// ring in one LDS array would otherwise be drained before every read); each
-// use waits for its own data (wait_steps).  m0, the LDS address of such a load,
-// is written here and named as clobbered.
-template <bool STREAM>
-__device__ __forceinline__ void dma_1k(u32x4_t rsrc, unsigned voff, unsigned soff, unsigned lds) {
-  soff = __builtin_amdgcn_readfirstlane(soff);  // wave-uniform; says so to the compiler
-  lds = __builtin_amdgcn_readfirstlane(lds);
-  if constexpr (STREAM)
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen nt lds" ::"s"(lds), "v"(voff),
-                 "s"(rsrc), "s"(soff)
-                 : "m0", "memory");
-  else
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(lds), "v"(voff),
-                 "s"(rsrc), "s"(soff)
-                 : "m0", "memory");
-}
-
 // Wait until at most `steps` (0..D-1, wave-uniform) steps of NL loads are in
 // flight.
 template <int NL, int D>

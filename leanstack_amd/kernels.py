@@ -492,6 +492,88 @@ def _gqa_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: flo
     return out
 
 
+def _key_rows(k: torch.Tensor, v: torch.Tensor, what: str) -> tuple[int, ...]:
+    """Strides of key and value rows [..., heads, rows, d] that the attention
+    kernel reads in place (never copied: they are a cache's): a leading one per
+    axis but the last.  Axes of one entry, and empty tensors, take any."""
+    d = k.shape[-1]
+    if k.dtype is not torch.bfloat16 or v.dtype is not torch.bfloat16 or k.shape != v.shape:
+        raise ValueError(f"{what} must be bfloat16 tensors of one shape, got {k.dtype} {tuple(k.shape)} / {v.dtype} "
+                         f"{tuple(v.shape)}")
+    if k.numel() == 0:
+        return (0,) * (k.dim() - 2) + (d,)
+    strides = [s if n > 1 else 0 for n, s in zip(k.shape[:-1], k.stride())]
+    if strides != [s if n > 1 else 0 for n, s in zip(v.shape[:-1], v.stride())] or k.stride(-1) != 1 or v.stride(-1) != 1 \
+            or any(s % 8 for s in strides) or k.data_ptr() % 16 or v.data_ptr() % 16 or 0 < strides[-1] < d:
+        raise ValueError(f"{what} must have equal strides, multiples of 8, rows of unit stride and 16-byte alignment, got "
+                         f"strides {k.stride()} / {v.stride()}")
+    if k.shape[-2] > 1 and strides[-1] == 0:
+        raise ValueError(f"{what}: the rows must not repeat (stride 0)")
+    strides[-1] = strides[-1] or d
+    return tuple(strides)
+
+
+@functools.lru_cache(maxsize=4096)
+def _prefix_workspace_bytes(b: int, t: int, n_q: int, n_kv: int, prefix: int, rows: int) -> int:
+    return _lib.load().lsk_prefix_attention_workspace_bytes(b, t, n_q, n_kv, prefix, rows)
+
+
+def shared_prefix_attention(q: torch.Tensor, prefix_k: torch.Tensor, prefix_v: torch.Tensor, k: torch.Tensor,
+                            v: torch.Tensor, lens: torch.Tensor, scale: float, *,
+                            out: torch.Tensor | None = None) -> torch.Tensor:
+    """softmax(q k^T * scale) v of T query tokens of each of B requests over a
+    prefix that they share and the rows that each has cached since -> [B, T, n_q * d].
+
+    q: [B, n_q, T, d].  prefix_k / prefix_v: [n_kv, P, d], read once for all requests
+    (the written part of an ArenaKVCache layer, for one).  k / v: [B, n_kv, S, d],
+    and lens, int32 [B] on the device: how many of a request's S rows are written,
+    its T new tokens' rows the last of them (lengths outside 0..S are taken at the
+    ends).  Query t sees the prefix and the first lens - (T - 1 - t) own rows.  Rows
+    behind the written ones are not read; a query that sees no row gives zeros.
+    bfloat16, d = 128, q heads in groups of n_q / n_kv.  Caches are read in place at
+    any strides that are multiples of 8; lens is read on the device, so a captured
+    call follows it.  out: a contiguous [B, T, n_q * d] tensor."""
+    if q.dim() != 4 or prefix_k.dim() != 3 or k.dim() != 4:
+        raise ValueError(f"q, prefix_k / prefix_v and k / v must be [B, n_q, T, d], [n_kv, P, d] and [B, n_kv, S, d], got "
+                         f"{tuple(q.shape)}, {tuple(prefix_k.shape)} and {tuple(k.shape)}")
+    b, n_q, t, d = q.shape
+    n_kv, prefix, rows = prefix_k.shape[0], prefix_k.shape[1], k.shape[2]
+    if q.dtype is not torch.bfloat16:
+        raise ValueError(f"q must be bfloat16, got {q.dtype}")
+    if d != 128 or n_kv < 1 or n_q < 1 or n_q % n_kv or prefix_k.shape[2] != d or tuple(k.shape) != (b, n_kv, rows, d):
+        raise ValueError(f"q {tuple(q.shape)}, prefix {tuple(prefix_k.shape)} and own rows {tuple(k.shape)} do not fit "
+                         f"together (d = 128, n_q a multiple of n_kv)")
+    prefix_strides = _key_rows(prefix_k, prefix_v, "prefix_k / prefix_v")
+    strides = _key_rows(k, v, "k / v")
+    _per_row(lens, b, torch.int32, "lens")
+    if out is not None:
+        if tuple(out.shape) != (b, t, n_q * d) or out.dtype is not torch.bfloat16 or not out.is_contiguous() \
+                or out.data_ptr() % 16:
+            raise ValueError(f"out must be a contiguous, 16-byte aligned bfloat16 [{b}, {t}, {n_q * d}] tensor, got "
+                             f"{out.dtype} {tuple(out.shape)}")
+        if any(_overlap(out, x) for x in (q, prefix_k, prefix_v, k, v) if x.numel()):
+            raise ValueError("out must not overlap the inputs")
+    _require_device(q, "q")
+    dev = _one_device(q, (prefix_k, "prefix_k"), (prefix_v, "prefix_v"), (k, "k"), (v, "v"), (lens, "lens"), (out, "out"))
+    if out is None:
+        out = q.new_empty((b, t, n_q * d))
+    if b * t == 0:
+        return out
+    if q.stride(3) != 1 or any(s % 8 for s in q.stride()[:3]) or q.data_ptr() % 16:
+        q = q.clone(memory_format=torch.contiguous_format)
+    nbytes = _prefix_workspace_bytes(b, t, n_q, n_kv, prefix, rows)
+    workspace = q.new_empty((nbytes // 2,)) if nbytes else None
+    q_strides = q.stride()
+    with _on(dev):
+        status = _lib.load().lsk_prefix_attention_bf16(
+            q.data_ptr(), q_strides[0], q_strides[1], q_strides[2], b, t, n_q, n_kv, d, prefix_k.data_ptr(),
+            prefix_v.data_ptr(), prefix_strides[0], prefix_strides[1], prefix, k.data_ptr(), v.data_ptr(), strides[0],
+            strides[1], strides[2], rows, lens.data_ptr(), float(scale), out.data_ptr(), _ptr(workspace), nbytes,
+            stream_handle())
+    _lib.check(status, "lsk_prefix_attention_bf16")
+    return out
+
+
 class LmHeadWorkspace:
     """Device workspace of the greedy head, sized once per (M, V, K): a status
     word and the per-workgroup argmax partials.  Zero-filled here; every call
