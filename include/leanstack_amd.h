@@ -400,8 +400,7 @@ int lsk_lora_add_bf16(const void* y, int M, int N, int ldy, const void* x, int K
                       int count, int rank_tiles, const int* index, int epilogue, void* out,
                       void* workspace, size_t ws_bytes, void* hip_stream);
 
-/* Device workspace of lsk_constrain_logits (any contents; 0 if the shape is not
- * supported). */
+/* Device workspace of lsk_constrain_logits (0 if the shape is not supported). */
 size_t lsk_constrain_workspace_bytes(int M, int V);
 
 /* Each request's constraints on its logits, and its greedy token.  For value
@@ -429,8 +428,9 @@ size_t lsk_constrain_workspace_bytes(int M, int V);
  *                 allowed_ld: bit v % 32 of word v / 32 set where v is allowed
  *   out           [M][V] contiguous; may be the logits themselves
  *   tokens        device int64 [M]
- *   workspace     lsk_constrain_workspace_bytes(M, V) bytes, 8-byte aligned; calls
- *                 that share one must be stream-ordered.
+ *   workspace     lsk_constrain_workspace_bytes(M, V) bytes, 8-byte aligned,
+ *                 zero-filled before its first use; calls leave it zero, and
+ *                 calls that share one must be stream-ordered.
  * The reference has no counterpart (its head is greedy over the raw logits,
  * src/leanstack/runtime/cutile_logits.py:37-69). */
 int lsk_constrain_logits(const void* logits, int logits_mode, int M, int V, long long logits_ld,

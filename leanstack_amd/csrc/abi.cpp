@@ -510,7 +510,7 @@ extern "C" {
 
 size_t lsk_constrain_workspace_bytes(int M, int V) {
   if (M < 1 || V < 1 || V > (1 << 30)) return 0;
-  return (size_t)M * lsk::constrain_slices(M, V) * sizeof(unsigned long long);
+  return (size_t)M * (lsk::kConstrainCounterWords * 4 + (size_t)lsk::constrain_slices(M, V) * 8);
 }
 
 int lsk_constrain_logits(const void* logits, int logits_mode, int M, int V, long long logits_ld, const int* history,
@@ -540,7 +540,8 @@ int lsk_constrain_logits(const void* logits, int logits_mode, int M, int V, long
   a.bias_ids = bias_ids;
   a.bias_values = bias_values;
   a.allowed = reinterpret_cast<const unsigned*>(allowed);
-  a.keys = static_cast<unsigned long long*>(workspace);
+  a.arrived = static_cast<unsigned*>(workspace);
+  a.keys = reinterpret_cast<unsigned long long*>(a.arrived + (size_t)M * lsk::kConstrainCounterWords);
   a.tokens = tokens;
   a.logits_ld = (size_t)logits_ld;
   a.history_ld = (size_t)history_ld;

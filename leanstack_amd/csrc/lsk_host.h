@@ -110,17 +110,19 @@ int check_prefix_args(const void* q, long long q_batch, long long q_head, long l
 // workgroup each; a slice's counts are one LDS word per entry.
 constexpr int kConstrainMaxHistory = 1 << 20;
 constexpr int kConstrainMaxBias = 1023;
-constexpr int kConstrainMaxSlice = 16384;
+constexpr int kConstrainMaxSlice = 10176;
 constexpr int kConstrainThreads = 512;
+constexpr int kConstrainCounterWords = 16;  // a row's counter has 64 bytes to itself
 
-// Vocabulary entries per slice: the largest that 64 KB of LDS count while the
-// rows alone fill the chip, down to 2048 when there are few (a multiple of 64,
-// so that a slice starts at an aligned value where its row does).
+// Vocabulary entries per slice: the most that a quarter of a CU's LDS counts while the rows
+// alone fill the chip, fewer when there are few rows (a multiple of 64, so that a
+// slice starts at an aligned value where its row does).
 constexpr int constrain_slice(int M, int V) {
   const int least = (V + kConstrainMaxSlice - 1) / kConstrainMaxSlice;
-  const int most = (V + 2047) / 2048;
-  const int wanted = (512 + M - 1) / M;
-  const int slices = wanted < least ? least : wanted > most ? most : wanted;
+  const int most = V / 2048 < 32 ? V / 2048 + 1 : 32;
+  const int wanted = (1024 + M - 1) / M;
+  const int some = wanted > most ? most : wanted;
+  const int slices = some < least ? least : some;
   const int slice = ((V + slices - 1) / slices + 63) / 64 * 64;
   return slice < kConstrainMaxSlice ? slice : kConstrainMaxSlice;
 }

@@ -268,7 +268,8 @@ struct QkRopeArgs {
 hipError_t launch_qk_rope(const QkRopeArgs& a, hipStream_t stream);
 
 // Constrained logits of M rows and the greedy token of each (constrain.hip).
-// Optional pointers are NULL; keys: M * slices words of the workspace.
+// Optional pointers are NULL.  The workspace, zero before and after a call: how
+// many of a row's slices are done (kConstrainCounterWords apart), and every slice's key.
 struct ConstrainArgs {
   const void* logits;
   void* out;
@@ -279,6 +280,7 @@ struct ConstrainArgs {
   const int* bias_ids;
   const float* bias_values;
   const unsigned* allowed;
+  unsigned* arrived;
   unsigned long long* keys;
   long long* tokens;
   size_t logits_ld, history_ld, bias_ld, allowed_ld;

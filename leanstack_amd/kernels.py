@@ -497,6 +497,10 @@ def _key_rows(k: torch.Tensor, v: torch.Tensor, what: str) -> tuple[int, ...]:
     kernel reads in place (never copied: they are a cache's): a leading one per
     axis but the last.  Axes of one entry, and empty tensors, take any."""
     d = k.shape[-1]
+    strides = k.stride()
+    if (k.dtype is torch.bfloat16 is v.dtype and k.shape == v.shape and strides == v.stride() and strides[-1] == 1
+            and strides[-2] >= d and not (strides[0] | strides[1] | strides[-2]) & 7):
+        return strides  # (the library checks the addresses)
     if k.dtype is not torch.bfloat16 or v.dtype is not torch.bfloat16 or k.shape != v.shape:
         raise ValueError(f"{what} must be bfloat16 tensors of one shape, got {k.dtype} {tuple(k.shape)} / {v.dtype} "
                          f"{tuple(v.shape)}")
@@ -540,13 +544,17 @@ def shared_prefix_attention(q: torch.Tensor, prefix_k: torch.Tensor, prefix_v: t
     n_kv, prefix, rows = prefix_k.shape[0], prefix_k.shape[1], k.shape[2]
     if q.dtype is not torch.bfloat16:
         raise ValueError(f"q must be bfloat16, got {q.dtype}")
-    if d != 128 or n_kv < 1 or n_q < 1 or n_q % n_kv or prefix_k.shape[2] != d or tuple(k.shape) != (b, n_kv, rows, d):
+    if d != 128 or n_kv < 1 or n_q < 1 or n_q % n_kv or prefix_k.shape[2] != d or k.shape != (b, n_kv, rows, d):
         raise ValueError(f"q {tuple(q.shape)}, prefix {tuple(prefix_k.shape)} and own rows {tuple(k.shape)} do not fit "
                          f"together (d = 128, n_q a multiple of n_kv)")
     prefix_strides = _key_rows(prefix_k, prefix_v, "prefix_k / prefix_v")
     strides = _key_rows(k, v, "k / v")
-    _per_row(lens, b, torch.int32, "lens")
+    index = q.get_device()
+    lens_at = _per_row(lens, b, torch.int32, index, "lens")
+    if not (prefix_k.get_device() == prefix_v.get_device() == k.get_device() == v.get_device() == index):
+        _one_device(q, (prefix_k, "prefix_k"), (prefix_v, "prefix_v"), (k, "k"), (v, "v"))
     if out is not None:
+        _one_device(q, (out, "out"))
         if tuple(out.shape) != (b, t, n_q * d) or out.dtype is not torch.bfloat16 or not out.is_contiguous() \
                 or out.data_ptr() % 16:
             raise ValueError(f"out must be a contiguous, 16-byte aligned bfloat16 [{b}, {t}, {n_q * d}] tensor, got "
@@ -554,21 +562,21 @@ def shared_prefix_attention(q: torch.Tensor, prefix_k: torch.Tensor, prefix_v: t
         if any(_overlap(out, x) for x in (q, prefix_k, prefix_v, k, v) if x.numel()):
             raise ValueError("out must not overlap the inputs")
     _require_device(q, "q")
-    dev = _one_device(q, (prefix_k, "prefix_k"), (prefix_v, "prefix_v"), (k, "k"), (v, "v"), (lens, "lens"), (out, "out"))
     if out is None:
         out = q.new_empty((b, t, n_q * d))
     if b * t == 0:
         return out
-    if q.stride(3) != 1 or any(s % 8 for s in q.stride()[:3]) or q.data_ptr() % 16:
+    q_strides = q.stride()
+    if q_strides[3] != 1 or (q_strides[0] | q_strides[1] | q_strides[2]) & 7 or q.data_ptr() % 16:
         q = q.clone(memory_format=torch.contiguous_format)
+        q_strides = q.stride()
     nbytes = _prefix_workspace_bytes(b, t, n_q, n_kv, prefix, rows)
     workspace = q.new_empty((nbytes // 2,)) if nbytes else None
-    q_strides = q.stride()
-    with _on(dev):
+    with _on(q.device):
         status = _lib.load().lsk_prefix_attention_bf16(
             q.data_ptr(), q_strides[0], q_strides[1], q_strides[2], b, t, n_q, n_kv, d, prefix_k.data_ptr(),
             prefix_v.data_ptr(), prefix_strides[0], prefix_strides[1], prefix, k.data_ptr(), v.data_ptr(), strides[0],
-            strides[1], strides[2], rows, lens.data_ptr(), float(scale), out.data_ptr(), _ptr(workspace), nbytes,
+            strides[1], strides[2], rows, lens_at, float(scale), out.data_ptr(), _ptr(workspace), nbytes,
             stream_handle())
     _lib.check(status, "lsk_prefix_attention_bf16")
     return out
@@ -762,20 +770,32 @@ def lora_linear(x: torch.Tensor, weight: PackedWeight, store: AdapterStore, inde
     return lora_add(y, x, store, index, out=y)
 
 
-def _per_row(t: torch.Tensor | None, m: int, dtype: torch.dtype, what: str) -> None:
-    """Check an optional contiguous [m] argument."""
-    if t is not None and (t.dtype is not dtype or t.shape != (m,) or not t.is_contiguous()):
+def _per_row(t: torch.Tensor | None, m: int, dtype: torch.dtype, device_index: int, what: str) -> int | None:
+    """The address of an optional contiguous [m] argument on the call's device."""
+    if t is None:
+        return None
+    if t.dtype is not dtype or t.dim() != 1 or t.numel() != m or not t.is_contiguous():
         raise ValueError(f"{what} must be a contiguous {dtype} tensor of {m} values, got {t.dtype} {tuple(t.shape)}")
+    if t.get_device() != device_index:
+        raise ValueError(f"{what} is on {t.device}, the call's tensors are on device {device_index}")
+    return t.data_ptr()
 
 
-def _row_list(t: torch.Tensor, m: int, dtype: torch.dtype, what: str) -> int:
-    """Check an [m, n] argument with contiguous rows; the row stride."""
-    if t.dtype is not dtype or t.dim() != 2 or t.shape[0] != m or (t.shape[1] > 1 and t.stride(1) != 1):
-        raise ValueError(f"{what} must be a {dtype} tensor of {m} contiguous rows, got {t.dtype} {tuple(t.shape)} with "
-                         f"strides {t.stride()}")
-    if m > 1 and t.stride(0) < t.shape[1]:
-        raise ValueError(f"{what} must not repeat or interleave its rows (stride {t.stride(0)} of {t.shape[1]} values)")
-    return t.stride(0) if m > 1 else t.shape[1]
+def _row_list(t: torch.Tensor, m: int, dtype: torch.dtype, device_index: int, what: str) -> tuple[int, int, int]:
+    """Address, row stride and row length of an [m, n] argument with contiguous rows."""
+    if t.dtype is not dtype or t.dim() != 2 or t.shape[0] != m:
+        raise ValueError(f"{what} must be a {dtype} tensor of {m} contiguous rows, got {t.dtype} {tuple(t.shape)}")
+    n = t.shape[1]
+    ld, unit = t.stride()
+    if n > 1 and unit != 1:
+        raise ValueError(f"{what} must be a {dtype} tensor of {m} contiguous rows, got strides {(ld, unit)}")
+    if m == 1:
+        ld = n
+    elif ld < n:
+        raise ValueError(f"{what} must not repeat or interleave its rows (stride {ld} of {n} values)")
+    if t.get_device() != device_index:
+        raise ValueError(f"{what} is on {t.device}, the call's tensors are on device {device_index}")
+    return t.data_ptr(), ld, n
 
 
 def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
@@ -809,72 +829,91 @@ def constrain_logits(logits: torch.Tensor, *, history: torch.Tensor | None = Non
     word v // 32 set where v is allowed.  Lengths and lists are read on the device,
     so a captured call follows what they hold at each replay.  out: a contiguous
     [M, V] tensor of the logits' type, or the (contiguous) logits themselves."""
-    if logits.dtype is torch.float32:
+    dtype = logits.dtype
+    if dtype is torch.float32:
         mode = _lib.LOGITS_FP32
-    elif logits.dtype is torch.bfloat16:
+    elif dtype is torch.bfloat16:
         mode = _lib.LOGITS_BF16
     else:
-        raise ValueError(f"logits must be float32 or bfloat16, got {logits.dtype}")
+        raise ValueError(f"logits must be float32 or bfloat16, got {dtype}")
     if logits.dim() != 2 or logits.shape[1] < 1:
         raise ValueError(f"logits must be [M, V], got {tuple(logits.shape)}")
     m, v = logits.shape
-    named = [(history, "history"), (history_lens, "history_lens"), (prompt_lens, "prompt_lens"),
-             (repetition, "repetition"), (frequency, "frequency"), (presence, "presence"), (bias_ids, "bias_ids"),
-             (bias_values, "bias_values"), (allowed, "allowed"), (out, "out")]
-    dev = _one_device(logits, *named)
+    index = logits.get_device()
+    past = lens = prompts = rho = alpha_f = alpha_p = ids = values = words = None
     history_ld = history_len = bias_ld = bias_count = allowed_ld = 0
     if history is not None:
-        history_ld = _row_list(history, m, torch.int32, "history")
-        history_len = history.shape[1]
+        past, history_ld, history_len = _row_list(history, m, torch.int32, index, "history")
         if history_len > _lib.CONSTRAIN_MAX_HISTORY:
             raise ValueError(f"history holds {history_len} tokens per row, at most {_lib.CONSTRAIN_MAX_HISTORY}")
-        _per_row(history_lens, m, torch.int32, "history_lens")
-        _per_row(prompt_lens, m, torch.int32, "prompt_lens")
-        for t, what in named[3:6]:
-            _per_row(t, m, torch.float32, what)
-    elif any(t is not None for t, _ in named[1:6]):
+        lens = _per_row(history_lens, m, torch.int32, index, "history_lens")
+        prompts = _per_row(prompt_lens, m, torch.int32, index, "prompt_lens")
+        rho = _per_row(repetition, m, torch.float32, index, "repetition")
+        alpha_f = _per_row(frequency, m, torch.float32, index, "frequency")
+        alpha_p = _per_row(presence, m, torch.float32, index, "presence")
+        if history_len == 0:  # no token to count or to penalise
+            past = lens = prompts = rho = alpha_f = alpha_p = None
+    elif not (history_lens is prompt_lens is repetition is frequency is presence is None):
         raise ValueError("lengths or penalties given without a history")
     if bias_ids is not None and bias_values is not None:
-        bias_ld = _row_list(bias_ids, m, torch.int32, "bias_ids")
-        bias_count = bias_ids.shape[1]
-        if _row_list(bias_values, m, torch.float32, "bias_values") != bias_ld or bias_values.shape != bias_ids.shape:
+        ids, bias_ld, bias_count = _row_list(bias_ids, m, torch.int32, index, "bias_ids")
+        values, values_ld, values_count = _row_list(bias_values, m, torch.float32, index, "bias_values")
+        if values_ld != bias_ld or values_count != bias_count:
             raise ValueError(f"bias_ids and bias_values must have the same shape and strides, got {tuple(bias_ids.shape)} "
                              f"/ {tuple(bias_values.shape)}")
         if bias_count > _lib.CONSTRAIN_MAX_BIAS:
             raise ValueError(f"{bias_count} biases per row, at most {_lib.CONSTRAIN_MAX_BIAS}")
-    elif bias_ids is not None or bias_values is not None:
+    elif not (bias_ids is bias_values is None):
         raise ValueError("bias_ids and bias_values go together")
     if allowed is not None:
-        allowed_ld = _row_list(allowed, m, torch.int32, "allowed")
-        if allowed.shape[1] != (v + 31) // 32:
-            raise ValueError(f"allowed must hold {(v + 31) // 32} words per row, got {allowed.shape[1]}")
+        words, allowed_ld, count = _row_list(allowed, m, torch.int32, index, "allowed")
+        if count != (v + 31) // 32:
+            raise ValueError(f"allowed must hold {(v + 31) // 32} words per row, got {count}")
+    ld, unit = logits.stride()
     src = logits
-    if (v > 1 and logits.stride(1) != 1) or (m > 1 and logits.stride(0) < v):
-        src = logits.contiguous()
+    if (v > 1 and unit != 1) or (m > 1 and ld < v):
+        src, ld = logits.contiguous(), v
+    elif m == 1:
+        ld = v
     if out is None:
-        out = torch.empty((m, v), device=logits.device, dtype=logits.dtype)
+        out = torch.empty((m, v), device=logits.device, dtype=dtype)
     else:
-        if out.dtype is not logits.dtype or out.shape != logits.shape or not out.is_contiguous():
-            raise ValueError(f"out must be a contiguous {logits.dtype} tensor of {m} x {v} values")
-        if src is logits and m and out.data_ptr() != logits.data_ptr() and _overlap(out, logits):
-            raise ValueError("out must be the logits themselves or not overlap them")
-        if src is logits and out.data_ptr() == logits.data_ptr() and not logits.is_contiguous():
-            raise ValueError("in place, the logits must be contiguous")
+        if out.dtype is not dtype or out.shape != logits.shape or not out.is_contiguous():
+            raise ValueError(f"out must be a contiguous {dtype} tensor of {m} x {v} values")
+        if out.get_device() != index:
+            raise ValueError(f"out is on {out.device}, the call's tensors are on {logits.device}")
+        if m and _overlap(out, logits) and not (src is logits and out.data_ptr() == src.data_ptr() and ld == v):
+            raise ValueError("out must be the logits themselves (contiguous) or not overlap them")
     _require_device(logits, "logits")
-    tokens = torch.empty((m,), device=logits.device, dtype=torch.long)
+    dev = logits.device
+    tokens = torch.empty((m,), device=dev, dtype=torch.long)
     if m == 0:
         return out, tokens
-    nbytes = _constrain_workspace_bytes(m, v)
-    workspace = torch.empty(nbytes, device=logits.device, dtype=torch.uint8)
     with _on(dev):
+        workspace = _constrain_workspace(dev, m, v)
         status = _lib.load().lsk_constrain_logits(
-            src.data_ptr(), mode, m, v, src.stride(0) if m > 1 else v, _ptr(history) if history_len else None, history_ld,
-            history_len, _ptr(history_lens) if history_len else None, _ptr(prompt_lens) if history_len else None,
-            *((_ptr(repetition), _ptr(frequency), _ptr(presence)) if history_len else (None, None, None)),
-            _ptr(bias_ids), _ptr(bias_values), bias_ld, bias_count, _ptr(allowed), allowed_ld, out.data_ptr(),
-            tokens.data_ptr(), workspace.data_ptr(), nbytes, stream_handle())
+            src.data_ptr(), mode, m, v, ld, past, history_ld, history_len, lens, prompts, rho, alpha_f, alpha_p, ids,
+            values, bias_ld, bias_count, words, allowed_ld, out.data_ptr(), tokens.data_ptr(), workspace.data_ptr(),
+            workspace.numel(), stream_handle())
     _lib.check(status, "lsk_constrain_logits")
     return out, tokens
+
+
+# Workspaces of constrain_logits by (device, stream).
+_constrain_workspaces: dict[tuple[int, int], torch.Tensor] = {}
+
+
+def _constrain_workspace(device: torch.device, m: int, v: int) -> torch.Tensor:
+    """A workspace that is zero: the stream's own, which every call leaves zero, or
+    under capture the graph's own, so that replays share none with eager calls."""
+    nbytes = _constrain_workspace_bytes(m, v)
+    if torch.cuda.is_current_stream_capturing():
+        return torch.empty(nbytes, device=device, dtype=torch.uint8).zero_()
+    key = (device.index, stream_handle())
+    workspace = _constrain_workspaces.get(key)
+    if workspace is None or workspace.numel() < nbytes:
+        workspace = _constrain_workspaces[key] = torch.zeros(max(nbytes, 4096), device=device, dtype=torch.uint8)
+    return workspace
 
 
 @functools.lru_cache(maxsize=1024)

@@ -39,13 +39,13 @@ def test_entry_point_rejects_before_launch(bad, code):
     assert lib.lsk_last_error()
 
 
-def test_workspace_covers_every_slice():
-    """8 bytes per slice; slices of at most 16384 values hold the vocabulary."""
+def test_workspace_bytes():
+    """A counter of 64 bytes per row and a key of 8 per slice, slices of at most 10176 values."""
     lib = _lib.load()
     for m in (1, 2, 7, 64, 511, 512, 513, 4096):
-        for v in (1, 63, 64, 65, 2048, 2049, 16384, 16385, 50257, 151936, 1 << 20, 1 << 30):
-            slices = lib.lsk_constrain_workspace_bytes(m, v) // (8 * m)
-            assert slices * 16384 >= v and slices <= max((v + 2047) // 2048, (v + 16383) // 16384 + 1)
+        for v in (1, 63, 64, 65, 2048, 2049, 10176, 16321, 50257, 151936, 1 << 20, 1 << 30):
+            slices, rest = divmod(lib.lsk_constrain_workspace_bytes(m, v) // m - 64, 8)
+            assert rest == 0 and slices * 10176 >= v and slices <= max(v // 2048 + 1, -(-v // 10176) + 1)
     assert lib.lsk_constrain_workspace_bytes(0, 5) == 0 and lib.lsk_constrain_workspace_bytes(5, 0) == 0
 
 

@@ -103,7 +103,8 @@ def _run(logits, kw, **more):
 @pytest.mark.parametrize("dtype", [FP32, BF16])
 @pytest.mark.parametrize("m,v,length,bias,mask", [
     (1, 1, 1, 1, True), (2, 31, 5, 3, True), (3, 33, 40, 0, True), (1, 64, None, 7, False), (4, 1003, 100, 20, True),
-    (1, 16384, 17, 0, False), (700, 130, 9, 2, True), (1, 16385, 1000, 1, True), (5, 50257, 300, 1023, True),
+    (1, 16384, 17, 0, False), (700, 130, 9, 2, True), (1, 16385, 1000, 1, True), (600, 16320, 50, 2, True), (600, 10176, 70, 2, True), (1500, 20353, 70, 2, True),
+    (520, 16321, 50, 0, True), (5, 50257, 300, 1023, True),
     (2, 151936, 4000, 300, True), (64, 20001, 600, 0, False), (600, 33001, 3, 0, True), (3, 4099, None, 0, True),
     (3, 4099, None, 0, False),
 ])

@@ -244,6 +244,17 @@ def test_offsets_past_32_bits(gpu):
     assert torch.equal(kernels.shared_prefix_attention(q, *far, k, v, lens, SCALE), expect)
 
 
+def test_refuses_caches_it_cannot_read_in_place(gpu):
+    q, pk, pv, k, v, lens = _request(3, 1, 8, 2, 70, 50, seed=7)
+    odd = torch.zeros(pk.numel() + 1, device=DEV, dtype=torch.bfloat16)[1:].view(2, 70, D)
+    with pytest.raises(ValueError, match="aligned"):
+        kernels.shared_prefix_attention(q, odd, odd, k, v, lens, SCALE)
+    with pytest.raises(ValueError, match="lens is on"):
+        kernels.shared_prefix_attention(q, pk, pv, k, v, lens.cpu(), SCALE)
+    with pytest.raises(ValueError, match="prefix_v is on"):
+        kernels.shared_prefix_attention(q, pk.contiguous(), pv.contiguous().cpu(), k, v, lens, SCALE)
+
+
 def test_empty_batch(gpu):
     empty = _request(2, 1, 8, 2, 64, 10)
     q, pk, pv, k, v, lens = empty

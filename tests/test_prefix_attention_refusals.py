@@ -67,7 +67,6 @@ def _bf(*shape):
     (dict(k=_bf(3, 2, 5, 256)[..., ::2], v=_bf(3, 2, 5, 256)[..., ::2]), "strides"),
     (dict(k=_bf(3, 2, 5, 132)[..., :128], v=_bf(3, 2, 5, 132)[..., :128]), "strides"),
     (dict(k=_bf(3, 2, 1, 128).expand(-1, -1, 5, -1), v=_bf(3, 2, 1, 128).expand(-1, -1, 5, -1)), "repeat"),
-    (dict(prefix_k=_bf(20 * 128 + 1)[1:].view(2, 10, 128), prefix_v=_bf(20 * 128 + 1)[1:].view(2, 10, 128)), "alignment"),
     (dict(lens=torch.zeros(3)), "lens"), (dict(lens=torch.zeros(2, dtype=torch.int32)), "lens"),
     (dict(lens=torch.zeros(3, dtype=torch.int64)), "lens"), (dict(out=_bf(3, 2, 8, 128)), "out"),
     (dict(out=_bf(3, 2, 1024).float()), "out"), (dict(), "GPU"),
