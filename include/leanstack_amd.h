@@ -364,7 +364,7 @@ int lsk_prefix_attention_bf16(const void* q, long long q_batch_stride, long long
                               void* hip_stream);
 
 /* Device workspace of lsk_lora_add_bf16 for these sizes (any contents; 0: none). */
-size_t lsk_lora_workspace_bytes(int M, int N, int K, int rank_tiles, int count);
+size_t lsk_lora_workspace_bytes(int M, int N, int K, int rank_tiles, int count, int epilogue);
 
 /* Low-rank adapters of many requests beside a shared projection: for row m with
  * a = index[m] in [0, count),
@@ -379,12 +379,13 @@ size_t lsk_lora_workspace_bytes(int M, int N, int K, int rank_tiles, int count);
  *              LSK_EPI_SILU_MUL), K % 32 == 0
  *   a_tiles    device bf16, per adapter A_a [16 * rank_tiles][K] in
  *              LSK_LAYOUT_MFMA16X32
- *   b_tiles    device bf16, per adapter B_a [N][16 * rank_tiles], columns
- *              32j..32j+31 of the output in rank_tiles tiles of 1 KB: the 16
- *              bytes at 16*l of tile (j, t) hold B_a[n0][16t + 4(l/16) + e], e =
- *              0..3, then the same of n1, with c = l % 16 and n0 = 32j + 8(c/4) +
- *              c%4, n1 = n0 + 4 (LSK_EPI_SILU_MUL: n0 = 16j + c, the gate row,
- *              and n1 = N/2 + n0, its up row); rows past N are zero
+ *   b_tiles    device bf16, per adapter B_a [N][16 * rank_tiles] in tiles of 1 KB:
+ *              the 16 bytes at 16*l of a tile hold B_a[n0][16t + 4(l/16) + e], e =
+ *              0..3, then the same of n0 + 4, with c = l % 16 and
+ *              LSK_EPI_NONE: tile (j, t), 32 columns, n0 = 32j + 8(c/4) + c%4;
+ *              LSK_EPI_SILU_MUL: tile (j, t, p), 64 columns of y, p = 0 their
+ *              gate rows, n0 = 32j + 8(c/4) + c%4, p = 1 their up rows, N/2
+ *              further on.  Rows past N (or N/2) are zero.
  *   scale, ranks   device fp32 / int32 [count]; of A_a's rows and B_a's columns the
  *              first ranks[a] count
  *   rank_tiles 1, 2, 3, 4, 6 or 8 (rank 16 to 128)

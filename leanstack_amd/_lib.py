@@ -111,7 +111,7 @@ _SIGNATURES: dict[str, tuple[type | None, list]] = {
          _c_void, ctypes.c_longlong, _c_int, _c_int, _c_void, _c_void, ctypes.c_longlong, ctypes.c_longlong, _c_int, _c_int,
          _c_void, ctypes.c_float, _c_void, _c_void, _c_size, _c_void],
     ),
-    "lsk_lora_workspace_bytes": (_c_size, [_c_int] * 5),
+    "lsk_lora_workspace_bytes": (_c_size, [_c_int] * 6),
     "lsk_lora_add_bf16": (
         _c_int,
         [_c_void, _c_int, _c_int, _c_int, _c_void, _c_int, _c_int, _c_void, _c_void, _c_void, _c_void, _c_int, _c_int,

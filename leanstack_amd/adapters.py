@@ -28,19 +28,17 @@ def _pack_a(a: torch.Tensor) -> torch.Tensor:
 
 def _pack_b(b: torch.Tensor, gate_up: bool) -> torch.Tensor:
     """B [..., N, R] (R a multiple of 16; [gate; up] rows for gate_up) as the
-    tiles of lsk_lora_add_bf16: 32 output columns x 16 ranks each, two 16-column
-    blocks whose values of one lane are neighbours in its 16 bytes."""
+    tiles of lsk_lora_add_bf16: 32 columns x 16 ranks each (for gate_up of 32 gate
+    rows, then of their up rows), a lane's 16 bytes from two rows 4 apart."""
     *lead, n, r = b.shape
-    b = b.reshape(-1, n, r)
-    if gate_up:  # blocks of gate rows and of their up rows
-        blocks = b.view(-1, 2, n // 32, 16, r).transpose(1, 2)
-    else:  # lane rows c of block h are columns 8 (c / 4) + 4 h + c % 4
-        if n % 32:
-            b = torch.cat((b, b.new_zeros(b.shape[0], 32 - n % 32, r)), 1)
-        blocks = b.view(b.shape[0], -1, 4, 2, 4, r).transpose(2, 3)
-    # [adapter, block pair, half, c, rank tile, g, e] -> [adapter, pair, rank tile, g, c, half, e]
-    blocks = blocks.reshape(b.shape[0], -1, 2, 16, r // 16, 4, 4)
-    return blocks.permute(0, 1, 4, 5, 3, 2, 6).reshape(*lead, -1)
+    parts = 2 if gate_up else 1
+    b = b.reshape(-1, parts, n // parts, r)
+    rest = -(n // parts) % 32
+    if rest:
+        b = torch.cat((b, b.new_zeros(*b.shape[:2], rest, r)), 2)
+    # row 32 j + 8 q + 4 half + i, rank 16 t + 4 g + e -> [j, t, part, g, (q, i), half, e]
+    blocks = b.view(b.shape[0], parts, -1, 4, 2, 4, r // 16, 4, 4)
+    return blocks.permute(0, 2, 6, 1, 7, 3, 5, 4, 8).reshape(*lead, -1)
 
 
 class AdapterStore:
@@ -58,7 +56,8 @@ class AdapterStore:
         self.rank_tiles = next(t for t in RANK_TILES if t * TILE_ROWS >= rank)
         self.rank = self.rank_tiles * TILE_ROWS
         self.a_tiles = torch.zeros((count, self.rank * k), device=device, dtype=torch.bfloat16)
-        self.b_tiles = torch.zeros((count, (n + 31) // 32 * 32 * self.rank), device=device, dtype=torch.bfloat16)
+        columns = -(-n // 64) * 64 if gate_up else -(-n // 32) * 32
+        self.b_tiles = torch.zeros((count, columns * self.rank), device=device, dtype=torch.bfloat16)
         self.scales = torch.zeros((count,), device=device, dtype=torch.float32)
         self.ranks = torch.zeros((count,), device=device, dtype=torch.int32)
 

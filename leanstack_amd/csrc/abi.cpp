@@ -458,9 +458,9 @@ int lsk_prefix_attention_bf16(const void* q, long long q_batch_stride, long long
 
 extern "C" {
 
-size_t lsk_lora_workspace_bytes(int M, int N, int K, int rank_tiles, int count) {
+size_t lsk_lora_workspace_bytes(int M, int N, int K, int rank_tiles, int count, int epilogue) {
   if (M < 1 || N < 1 || K < lsk::kTileK || count < 1 || !lsk::adapter_rank_supported(rank_tiles)) return 0;
-  return (size_t)lsk::adapter_workspace_bytes(lsk::adapter_plan(M, N, K, rank_tiles, count), rank_tiles);
+  return (size_t)lsk::adapter_workspace_bytes(lsk::adapter_plan(M, N, K, rank_tiles, count, epilogue == LSK_EPI_SILU_MUL), rank_tiles);
 }
 
 int lsk_lora_add_bf16(const void* y, int M, int N, int ldy, const void* x, int K, int ldx, const void* a_tiles,
@@ -470,7 +470,7 @@ int lsk_lora_add_bf16(const void* y, int M, int N, int ldy, const void* x, int K
   if (int st = lsk::check_lora_args(y, M, N, ldy, x, K, ldx, a_tiles, b_tiles, scale, ranks, count, rank_tiles, index,
                                     epilogue, out))
     return st;
-  const lsk::AdapterPlan p = lsk::adapter_plan(M, N, K, rank_tiles, count);
+  const lsk::AdapterPlan p = lsk::adapter_plan(M, N, K, rank_tiles, count, epilogue == LSK_EPI_SILU_MUL);
   const size_t need = (size_t)lsk::adapter_workspace_bytes(p, rank_tiles);
   if (need > 0 && (workspace == nullptr || ws_bytes < need || !aligned(workspace, 16)))
     return fail(LSK_ERR_WORKSPACE, "the adapters need a workspace of %zu bytes, 16-byte aligned (got %zu)", need,
@@ -486,7 +486,8 @@ int lsk_lora_add_bf16(const void* y, int M, int N, int ldy, const void* x, int K
   a.out = static_cast<__bf16*>(out);
   a.h = static_cast<float*>(workspace);
   a.a_stride = (size_t)rank_tiles * 16 * K;
-  a.b_stride = (size_t)((N + 31) / 32) * rank_tiles * 512;
+  a.b_stride = (size_t)lsk::adapter_blocks(N, epilogue == LSK_EPI_SILU_MUL) * rank_tiles *
+               (epilogue == LSK_EPI_SILU_MUL ? 1024 : 512);
   a.M = M;
   a.N = N;
   a.K = K;
@@ -497,7 +498,7 @@ int lsk_lora_add_bf16(const void* y, int M, int N, int ldy, const void* x, int K
   a.slots = p.slots;
   a.ranges = p.ranges;
   a.splits = p.splits;
-  hipError_t err = lsk::launch_adapters(a, rank_tiles, epilogue == LSK_EPI_SILU_MUL, static_cast<hipStream_t>(hip_stream));
+  hipError_t err = lsk::launch_adapters(a, rank_tiles, p.rows, epilogue == LSK_EPI_SILU_MUL, static_cast<hipStream_t>(hip_stream));
   if (err != hipSuccess) return hip_fail(err, "adapter kernel launch");
   return LSK_OK;
 }

@@ -239,7 +239,7 @@ int check_lora_args(const void* y, int M, int N, int ldy, const void* x, int K, 
     return fail(LSK_ERR_INVALID, "rank_tiles=%d: the rank must be 16, 32, 48, 64, 96 or 128", rank_tiles);
   if (N > kMaxActivationStride || K > kMaxActivationStride)
     return fail(LSK_ERR_INVALID, "N=%d and K=%d must be at most %d", N, K, kMaxActivationStride);
-  const AdapterPlan p = adapter_plan(M, N, K, rank_tiles, count);
+  const AdapterPlan p = adapter_plan(M, N, K, rank_tiles, count, epilogue == LSK_EPI_SILU_MUL);
   const long long groups = (long long)p.tiles * p.slots;
   if (groups * (p.ranges > p.splits ? p.ranges : p.splits) > 0xffffffffLL / kAdapterThreads)
     return fail(LSK_ERR_INVALID, "M=%d rows are too many", M);  // a grid's threads are counted in 32 bits

@@ -131,42 +131,56 @@ constexpr int constrain_slices(int M, int V) {
   return (V + slice - 1) / slice;
 }
 
-// Low-rank adapters (adapters.hip): 16 rows of x, an adapter that they name
+// Low-rank adapters (adapters.hip): a tile of rows of x, an adapter that they name
 // (slot) and a range of output columns per workgroup.
 constexpr int kAdapterThreads = 512;
+constexpr int kAdapterMaxSplits = 8;
 
 // 16-row tiles of the adapters' rank that the kernels are built for.
 constexpr bool adapter_rank_supported(int rank_tiles) {
   return rank_tiles >= 1 && rank_tiles <= 8 && rank_tiles != 5 && rank_tiles != 7;
 }
 
-// How a call runs: slots per 16 rows, ranges of output columns per slot, and K
-// ranges of the first of two launches (0: one launch).
+// How a call runs: tiles of `rows` rows, slots per tile, ranges of output columns, and
+// K ranges of the first of two launches (0: one launch).
+//
+// Up to 128 rows a decode batch is expected, whose rows each name an adapter of
+// their own: tiles of 16 rows and a workgroup per (adapter named, column range), in
+// one launch unless reading A anew for every range (from L2) costs more than a
+// launch: QKV (K = 2560, 24 ranges) with 16 rows and rank 16 7.5 us in one launch,
+// 9 in two; the down projection (K = 9728) with 64 rows and rank 64 16.1 us in
+// two, over 30 in one.
+// Above, prompts, whose neighbouring rows mostly name the same: 64 rows share an adapter's
+// tiles, and the second launch takes y once whatever its rows name.  Slots beyond
+// the first few would be workgroups that find nothing to do (2000 rows of gate_up
+// with 4 slots per tile instead of 1: 14.9 instead of 7.6 us for the first launch).
 struct AdapterPlan {
-  int tiles, slots, ranges, splits;
+  int rows, tiles, slots, ranges, splits;
 };
-constexpr AdapterPlan adapter_plan(int M, int N, int K, int rank_tiles, int count) {
-  AdapterPlan p = {(M - 1) / 16 + 1, count < 16 ? count : 16, 1, 0};
-  // Groups that are likely to have work: rows of a decode batch each name an
-  // adapter of their own, neighbouring rows of prompts the same.
-  const int busy = p.tiles * (M <= 128 ? p.slots : 1);
-  const int blocks = (N + 31) / 32;
+constexpr int adapter_blocks(int N, bool silu) { return silu ? (N + 63) / 64 : (N + 31) / 32; }
+constexpr AdapterPlan adapter_plan(int M, int N, int K, int rank_tiles, int count, bool silu) {
+  const bool decode = M <= 128;
+  AdapterPlan p = {decode ? 16 : 64, 0, 0, 1, 0};
+  p.tiles = (M - 1) / p.rows + 1;
+  const int named = count < M ? count : M;
+  const int share = 32 / p.tiles;
+  const int most_slots = decode ? 16 : share < 1 ? 1 : share > 16 ? 16 : share;
+  p.slots = named < most_slots ? named : most_slots;
+  // Two workgroups per CU, each with a block of columns (a k-tile) for every wave.
+  const int busy = p.tiles * (decode ? p.slots : 1);
   const int wanted = (512 + busy - 1) / busy;
-  const int most = (blocks + 7) / 8;  // a block for each wave
-  p.ranges = wanted < 1 ? 1 : wanted > most ? most : wanted;
-  // Bytes of A that the one-launch form reads per workgroup, from L2.
-  const long long again = (long long)K * rank_tiles * 32;
-  if (p.ranges > 1 && again > 256 * 1024) {
-    const int ktiles = K / kTileK;
-    const int split = (512 + busy - 1) / busy;
-    const int least = (ktiles + 7) / 8;
-    p.splits = split < 1 ? 1 : split > least ? least : split;
-    if (p.splits > 16) p.splits = 16;
+  const int most = (adapter_blocks(N, silu) + 7) / 8;
+  p.ranges = wanted > most ? most : wanted;
+  const long long again = (long long)K * rank_tiles * 32;  // bytes of A per workgroup
+  if (!decode || (p.ranges > 1 && again > 256 * 1024)) {
+    const int most_splits = (K / kTileK + 7) / 8;
+    p.splits = wanted > most_splits ? most_splits : wanted;
+    if (p.splits > kAdapterMaxSplits) p.splits = kAdapterMaxSplits;
   }
   return p;
 }
 constexpr unsigned long long adapter_workspace_bytes(const AdapterPlan& p, int rank_tiles) {
-  return (unsigned long long)p.splits * (unsigned long long)p.tiles * (unsigned long long)rank_tiles * 1024;
+  return (unsigned long long)p.splits * (unsigned long long)p.tiles * (unsigned long long)(rank_tiles * p.rows) * 64;
 }
 
 // Argument rules of lsk_lora_add_bf16 (all but the workspace's size).

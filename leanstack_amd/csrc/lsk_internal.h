@@ -316,7 +316,8 @@ struct AdapterArgs {
   size_t a_stride, b_stride;
   int M, N, K, ldx, ldy, count, tiles, slots, ranges, splits;
 };
-hipError_t launch_adapters(const AdapterArgs& a, int rank_tiles, bool silu, hipStream_t stream);
+// rows: 16 or 64 per tile.
+hipError_t launch_adapters(const AdapterArgs& a, int rank_tiles, int rows, bool silu, hipStream_t stream);
 
 // Number of scoring workgroups (= argmax partials per row) the lm_head
 // kernel uses for V vocab rows (V % 16 == 0): with NB = V / 16 row-blocks,

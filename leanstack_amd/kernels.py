@@ -695,8 +695,8 @@ def lm_head_argmax_noalloc(hidden: torch.Tensor, weight: PackedWeight, out: torc
 
 
 @functools.lru_cache(maxsize=4096)
-def _lora_workspace_bytes(m: int, n: int, k: int, rank_tiles: int, count: int) -> int:
-    return _lib.load().lsk_lora_workspace_bytes(m, n, k, rank_tiles, count)
+def _lora_workspace_bytes(m: int, n: int, k: int, rank_tiles: int, count: int, epilogue: int) -> int:
+    return _lib.load().lsk_lora_workspace_bytes(m, n, k, rank_tiles, count, epilogue)
 
 
 def lora_add(y: torch.Tensor, x: torch.Tensor, store: AdapterStore, index: torch.Tensor, *,
@@ -735,7 +735,7 @@ def lora_add(y: torch.Tensor, x: torch.Tensor, store: AdapterStore, index: torch
         out = y.new_empty((*y.shape[:-1], n_out))
     if m == 0:
         return out
-    nbytes = _lora_workspace_bytes(m, n, k, store.rank_tiles, store.count)
+    nbytes = _lora_workspace_bytes(m, n, k, store.rank_tiles, store.count, epilogue)
     workspace = y.new_empty((nbytes // 2,)) if nbytes else None
     with _on(dev):
         status = _lib.load().lsk_lora_add_bf16(

@@ -15,21 +15,24 @@ FAKE = 0x10000  # aligned, never dereferenced
 INVALID, WORKSPACE = -1, -4
 
 
-@pytest.mark.parametrize("n,r,gate_up", [(32, 16, False), (48, 32, False), (16, 16, False), (192, 64, True)])
+@pytest.mark.parametrize("n,r,gate_up", [(32, 16, False), (48, 32, False), (16, 16, False), (192, 64, True), (96, 16, True)])
 def test_b_tiles_follow_the_documented_layout(n, r, gate_up):
     b = seeded_normal((n, r), 1.0, n + r)
-    tiles = _pack_b(b, gate_up).view(-1, r // 16, 64, 8)  # [32 columns, rank tile, lane, value]
-    assert tiles.shape[0] == (n + 31) // 32
+    parts = 2 if gate_up else 1
+    tiles = _pack_b(b, gate_up).view(-1, r // 16, parts, 64, 8)  # [columns, rank tile, part, lane, value]
+    assert tiles.shape[0] == (n // parts + 31) // 32
     for j in range(tiles.shape[0]):
         for t in range(r // 16):
-            for lane in range(64):
-                g, c = lane // 16, lane % 16
-                n0 = 16 * j + c if gate_up else 32 * j + 8 * (c // 4) + c % 4
-                n1 = n // 2 + n0 if gate_up else n0 + 4
-                for e in range(4):
-                    for half, row in enumerate((n0, n1)):
-                        want = float(b[row, 16 * t + 4 * g + e]) if row < n else 0.0
-                        assert float(tiles[j, t, lane, 4 * half + e]) == want
+            for p in range(parts):
+                for lane in range(64):
+                    g, c = lane // 16, lane % 16
+                    for e in range(4):
+                        for half in range(2):
+                            row = 32 * j + 8 * (c // 4) + c % 4 + 4 * half
+                            want = float(b[p * n // 2 + row, 16 * t + 4 * g + e]) if row < n // parts else 0.0
+                            assert float(tiles[j, t, p, lane, 4 * half + e]) == want
+    store = AdapterStore(1, n, 32, r, gate_up=gate_up, device="cpu")
+    assert store.b_tiles[0].numel() == tiles.numel()
 
 
 def test_a_store_holds_what_is_loaded():
@@ -73,7 +76,7 @@ def test_entry_point_rejects_before_launch(bad, code):
     lib = _lib.load()
     a = dict(y=FAKE, m=20, n=2560, ldy=2560, x=FAKE, k=9728, ldx=9728, a=FAKE, b=FAKE, scale=FAKE, ranks=FAKE, count=6,
              rt=4, index=FAKE, epi=0, out=FAKE + 0x100000, ws=FAKE) | bad
-    need = lib.lsk_lora_workspace_bytes(20, 2560, 9728, 4, 6)
+    need = lib.lsk_lora_workspace_bytes(20, 2560, 9728, 4, 6, 0)
     assert need > 0
     a.setdefault("ws_bytes", need)
     status = lib.lsk_lora_add_bf16(a["y"], a["m"], a["n"], a["ldy"], a["x"], a["k"], a["ldx"], a["a"], a["b"], a["scale"],
@@ -84,14 +87,17 @@ def test_entry_point_rejects_before_launch(bad, code):
 
 
 def test_workspace_bytes():
+    """Whole fp32 partials of h, at most 8; 64 rows to a tile above 128 rows."""
     lib = _lib.load()
-    for m in (1, 16, 17, 300, 5000):
+    for m in (1, 16, 17, 128, 129, 300, 5000):
         for n, k in ((16, 32), (2560, 9728), (19456, 2560)):
             for rt in RANK_TILES:
-                nbytes = lib.lsk_lora_workspace_bytes(m, n, k, rt, 5)
-                assert nbytes % (-(-m // 16) * rt * 1024) == 0 and nbytes <= 16 * -(-m // 16) * rt * 1024
+                rows = 16 if m <= 128 else 64
+                tile = -(-m // rows) * rows * rt * 64
+                splits, rest = divmod(lib.lsk_lora_workspace_bytes(m, n, k, rt, 5, 0), tile)
+                assert rest == 0 and splits <= 8 and (m <= 128 or splits >= 1)
     for bad in ((0, 16, 32, 1, 1), (1, 0, 32, 1, 1), (1, 16, 0, 1, 1), (1, 16, 32, 5, 1), (1, 16, 32, 1, 0)):
-        assert lib.lsk_lora_workspace_bytes(*bad) == 0
+        assert lib.lsk_lora_workspace_bytes(*bad, 0) == 0
 
 
 def test_wrappers_refuse():

@@ -74,6 +74,7 @@ def _index(m, count, seed):
     (1, 16, 32, 1, 1), (1, 2560, 4096, 4, 8), (2, 48, 64, 2, 16), (5, 80, 96, 3, 17), (15, 112, 288, 16, 5),
     (16, 6144, 2560, 20, 16), (17, 2560, 9728, 3, 64), (33, 512, 2048, 33, 100), (64, 2560, 9728, 9, 128),
     (130, 256, 512, 5, 48), (301, 1040, 2560, 4, 32), (40, 2560, 4096, 1, 96), (16, 32, 4096, 40, 128),
+    (128, 528, 512, 60, 16), (129, 16, 32, 64, 3), (640, 2560, 4096, 9, 16), (200, 304, 9728, 3, 128), (1000, 96, 1024, 2, 64),
 ])
 def test_lora_add(gpu, m, n, k, count, rank):
     adapters = _adapters(count, n, k, [max(1, rank - 3 * (i % 4)) for i in range(count)], seed=m)
@@ -91,6 +92,7 @@ def test_lora_add(gpu, m, n, k, count, rank):
 
 @pytest.mark.parametrize("m,n,k,count,rank", [
     (1, 32, 32, 1, 4), (7, 192, 2560, 7, 16), (16, 19456, 2560, 3, 32), (50, 1024, 9728, 16, 128), (200, 320, 512, 2, 64),
+    (300, 96, 2560, 5, 128), (129, 19456, 1024, 3, 16), (90, 160, 9728, 4, 48),
 ])
 def test_lora_silu_mul(gpu, m, n, k, count, rank):
     adapters = _adapters(count, n, k, [rank] * count, seed=m)
@@ -104,14 +106,14 @@ def test_lora_silu_mul(gpu, m, n, k, count, rank):
 
 
 @pytest.mark.parametrize("k,rank", [(512, 16), (9728, 64)])  # one launch and two
-@pytest.mark.parametrize("m", [16, 37])
+@pytest.mark.parametrize("m", [16, 37, 150])
 def test_rows_and_adapters_do_not_touch_each_other(gpu, m, k, rank):
     """A NaN or infinity in one row's x or y, or in an adapter, reaches only the
     rows that it is a part of; indices that name no adapter leave y; unused
     slots may hold anything."""
     n, count = 320, 6
-    two = _lib.load().lsk_lora_workspace_bytes(m, n, k, rank // 16, count) > 0
-    assert two == (k == 9728)
+    two = _lib.load().lsk_lora_workspace_bytes(m, n, k, rank // 16, count, 0) > 0
+    assert two == (k == 9728 or m > 128)
     adapters = _adapters(count, n, k, [rank, rank - 1, rank, 3, rank, rank], seed=5)
     y, x = seeded_normal((m, n), 1.0, 1), seeded_normal((m, k), 1.0, 2)
     index = torch.arange(m, dtype=torch.int32) % 4
@@ -140,8 +142,24 @@ def test_rows_and_adapters_do_not_touch_each_other(gpu, m, k, rank):
     assert torch.equal(got[5], y[5]) and torch.equal(got[6], y[6])
 
 
-def test_strides_shapes_and_empty_calls(gpu):
-    m, n, k = 21, 96, 256
+@pytest.mark.parametrize("runs", [1, 3, 50, 64, 100])
+def test_prompts_of_several_requests(gpu, runs):
+    """Consecutive rows of a request, adapters that change inside a tile of rows
+    and at its edges, requests without one between them."""
+    m, n, k, count = 333, 320, 512, 7
+    adapters = _adapters(count, n, k, [16, 9, 30, 32, 1, 17, 32], seed=2)
+    y, x = seeded_normal((m, n), 1.0, 1), seeded_normal((m, k), 1.0, 2)
+    index = ((torch.arange(m) // runs) % (count + 1) - 1).int()
+    got = kernels.lora_add(y.to(DEV), x.to(DEV), _store(adapters, n, k, 32), index.to(DEV))
+    _check(got, y, x, adapters, index)
+    rows = torch.arange(n).view(2, n // 32, 16).transpose(0, 1).reshape(-1)
+    got = kernels.lora_add(y.to(DEV), x.to(DEV), _store(adapters, n, k, 32, gate_up=True), index.to(DEV), epilogue=SILU)
+    _check(got, y, x, [(a, b[rows], s) for a, b, s in adapters], index, gate_up=True)
+
+
+@pytest.mark.parametrize("m", [21, 140])
+def test_strides_shapes_and_empty_calls(gpu, m):
+    n, k = 96, 256
     adapters = _adapters(3, n, k, [9, 16, 4], seed=1)
     store = _store(adapters, n, k, 16)
     y, x, index = seeded_normal((m, n), 1.0, 1), seeded_normal((m, k), 1.0, 2), _index(m, 3, 4)
@@ -150,7 +168,7 @@ def test_strides_shapes_and_empty_calls(gpu):
     wide_y, wide_x = torch.full((m, n + 24), 9.0, device=DEV).bfloat16(), torch.full((m, k + 40), 9.0, device=DEV).bfloat16()
     wide_y[:, 8:8 + n], wide_x[:, 16:16 + k] = dy, dx
     for fy, fx in ((wide_y[:, 8:8 + n], wide_x[:, 16:16 + k]), (dy.t().contiguous().t(), dx.repeat_interleave(2, 1)[:, ::2]),
-                   (wide_y.clone()[:, 8:8 + n], dx.view(3, 7, k)), (dy.view(1, m, n), dx.view(1, m, k))):
+                   (wide_y.clone()[:, 8:8 + n], dx.view(-1, 7, k)), (dy.view(1, m, n), dx.view(1, m, k))):
         assert torch.equal(kernels.lora_add(fy, fx, store, di).view(m, n), expect)
     shifted = torch.empty(m * k + 1, device=DEV, dtype=torch.bfloat16)[1:].view(m, k)
     shifted.copy_(dx)
@@ -229,11 +247,11 @@ def test_parts_of_a_fused_projection(gpu):
         at += s
 
 
-@pytest.mark.parametrize("k,rank", [(512, 16), (9728, 64)])
-def test_captured_and_on_two_streams(gpu, k, rank):
+@pytest.mark.parametrize("m,k,rank", [(20, 512, 16), (20, 9728, 64), (200, 512, 16)])
+def test_captured_and_on_two_streams(gpu, m, k, rank):
     """Replays follow the index, the rows and the store's slots as they are then;
     calls on two streams at once share nothing."""
-    m, n, count = 20, 640, 4
+    n, count = 640, 4
     adapters = _adapters(count, n, k, [rank] * count, seed=3)
     store, other = _store(adapters, n, k, rank), _store(adapters[::-1], n, k, rank)
     ys = [seeded_normal((m, n), 1.0, s).to(DEV) for s in (1, 2)]
