@@ -208,8 +208,11 @@ int check_prefix_args(const void* q, long long q_batch, long long q_head, long l
   const long long own_items = (long long)n_kv * B * p.own_tiles;
   if (own_items > most || prefix_items > most || prefix_items + own_items * (p.joint ? 1 : p.own_parts) > most)
     return fail(LSK_ERR_INVALID, "B=%d, T=%d, n_q=%d over %d + %d rows: too many items", B, T, n_q, P, S);
-  if (prefix_row < head_dim || row < head_dim || prefix_row % 8 != 0 || row % 8 != 0)
-    return fail(LSK_ERR_INVALID, "row strides %d, %d must be multiples of 8, at least %d", prefix_row, row, head_dim);
+  // (a few steps past the last row are addressed, out of range: their offsets must not wrap)
+  if (prefix_row < head_dim || row < head_dim || prefix_row % 8 != 0 || row % 8 != 0 ||
+      prefix_row > kMaxActivationStride || row > kMaxActivationStride)
+    return fail(LSK_ERR_INVALID, "row strides %d, %d must be multiples of 8, %d..%d", prefix_row, row, head_dim,
+                kMaxActivationStride);
   if ((long long)P * prefix_row >= (1LL << 30) || (long long)S * row >= (1LL << 30))
     return fail(LSK_ERR_INVALID, "%d and %d rows at strides %d and %d: a head's rows must stay below 2^31 bytes", P, S,
                 prefix_row, row);

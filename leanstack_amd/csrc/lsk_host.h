@@ -61,35 +61,62 @@ constexpr int attention_most_chunks(int max_seq_len) {
 }
 
 // Attention over a shared prefix (prefix_attention.hip).
-constexpr int kPrefixThreads = 256;
+constexpr int kPrefixThreads = 512;     // the most of a workgroup
+constexpr int kPrefixSharedRows = 128;  // query rows of an item whose waves share key rows
 
 // How a call runs.  joint: one launch, an item per 32 query rows of one request
 // and kv head.  Else prefix_parts ranges of prefix_chunk prefix rows per kv head and
-// prefix_tiles of 32 (shared: 128) query rows, and own_parts ranges of own_chunk own rows per kv
-// head, request and own_tiles of 32 query rows.
+// prefix_tiles of 32 (shared: 128) query rows, and own_parts ranges of own_chunk own
+// rows per kv head, request and own_tiles of 32 query rows.
 struct PrefixPlan {
   bool joint, shared;
   int prefix_tiles, prefix_chunk, prefix_parts, own_tiles, own_chunk, own_parts;
 };
 constexpr int ceil_div(long long a, long long b) { return (int)((a + b - 1) / b); }
+
+// Measured with 32 q and 8 kv heads, B x T tokens, P + S rows:
+// - One launch while the rows are few and its items, one per CU, run at once:
+//   12x1 500+128 8.5 us in one, 9.7 in two; 1x1 900+64 10.0 in one, 9.1 in two; with
+//   three rounds of items (81x1 187+9) 17.4 in one, 14.8 in two.
+// - Waves that share query rows read the prefix rows once per 32 of them, waves that
+//   share key rows once per 128, and have a barrier per step and fewer items: up to 192
+//   query rows per kv head the first are faster (32x1 4096+1024 19.6 against 24.3 us; 8x5
+//   12000+64 22.5 against 30.5), with 256 the second (64x1 8191+1088 47 against 55).
+// - A part more costs every query row 520 bytes written and read, so items are as many as
+//   the chip runs of them at once and no more: two per CU of items that share key
+//   rows, one of those that do not and are bound by memory (8x1 9000+128 14.9 us,
+//   17.6 with two), and half a CU's worth of own items.
+// - Of the 512 places of shared items the prefix gets its share of all key rows to be
+//   read, so that it does not finish long before the own rows do, whose reads bound
+//   them: 64x1 8191+1088 47 us with 7 parts, 52 with 16; 48x4 16000+320, where the prefix
+//   is most of the work, 82 us with 10 parts, 88 with 5.
+constexpr int kPrefixJointRows = 768;
+constexpr int kPrefixJointItems = 256;
+constexpr int kPrefixSplitRows = 192;
 constexpr PrefixPlan prefix_plan(int B, int T, int n_q, int n_kv, int P, int S) {
   PrefixPlan p = {false, false, 0, 128, 0, ceil_div((long long)T * (n_q / n_kv), 32), 128, 0};
   const long long rows = (long long)B * T * (n_q / n_kv);
-  if ((long long)P + S <= 512) {
+  const long long own_items = (long long)n_kv * B * p.own_tiles;
+  if ((long long)P + S <= kPrefixJointRows && own_items <= kPrefixJointItems) {
     p.joint = true;
     return p;
   }
-  p.shared = rows > 64;
+  p.shared = rows > kPrefixSplitRows;
   if (P > 0) {
-    const int tile = p.shared ? 128 : 32, unit = p.shared ? 32 : 128, least = p.shared ? 256 : 128;
-    p.prefix_tiles = ceil_div(rows, tile);
-    const int wanted = ceil_div(512, (long long)n_kv * p.prefix_tiles);
-    const int chunk = ceil_div(ceil_div(P, wanted), unit) * unit;
+    const int unit = p.shared ? 32 : 128, least = p.shared ? 384 : 256;  // rows of a chunk
+    p.prefix_tiles = ceil_div(rows, p.shared ? kPrefixSharedRows : 32);
+    const long long items = (long long)n_kv * p.prefix_tiles;
+    const long long prefix = (long long)p.prefix_tiles * P, own = (long long)B * S;
+    const long long most = (p.shared ? 512 : 256) / items;
+    const long long share = p.shared ? ceil_div(512 * prefix, (prefix + own) * items) : most;
+    const long long wanted = share < most ? share : most;
+    const int chunk = ceil_div(ceil_div(P, wanted > 1 ? wanted : 1), unit) * unit;
     p.prefix_chunk = chunk < least ? least : chunk;
     p.prefix_parts = ceil_div(P, p.prefix_chunk);
   }
   if (S > 0) {
-    const int chunk = ceil_div(ceil_div(S, 64), 128) * 128;
+    const long long wanted = own_items < 512 ? 512 / own_items : 1;
+    const int chunk = ceil_div(ceil_div(S, wanted), 128) * 128;
     p.own_chunk = chunk < 256 ? 256 : chunk;
     p.own_parts = ceil_div(S, p.own_chunk);
   }

@@ -26,19 +26,32 @@
 //
 // K and V rows go to LDS by DMA, their 16-byte chunks permuted by row so that
 // neither the reads of K (one row per lane) nor of V (four rows per 16 lanes)
-// meet in a bank.  Rows past the last visible one are that row again, so what
-// lies behind the written rows is never read.
+// meet in a bank.  Rows past the last visible one are out of the buffers' range
+// and come as zeros: what lies behind the written rows is never read.
 //
-// Items whose 4 waves share query rows (own rows; few prefix rows) split the
-// key rows, each wave with a slot of its own and no barrier: the next step's K is
-// on its way while P V is multiplied, the next V during the next scores.  Items
-// of 128 query rows share each step's rows among the waves through a ring.
+// Items whose waves share query rows (own rows; a prefix with few query rows) split
+// the key rows, each wave with a slot of its own and no barrier: the next step's K
+// is on its way while P V is multiplied, the next V during the next scores.  Items
+// of 128 query rows share each step's rows among the waves through a ring of slots.
 //
 // An item leaves (m, l, O) in fp32 in the workspace and a second launch adds a
 // row's items up; a short context runs in one launch, each request's items
 // reading the prefix and its own rows.
+//
+// What it measured (32 q, 8 kv heads; B requests of T tokens, P + S rows; the kernels in
+// a graph):
+//   1x5 300+64      9.2 us, one launch: latency (the bytes are 0.3 us)
+//   12x1 1024+512  10.6 us, of it 4 the second launch
+//   64x1 8191+1088  47 us: 166 MB, 4.2 TB/s in the first launch (a copy reaches 4.8)
+//   48x4 16000+320  82 us: 51 GFLOP, 740 TFLOP/s in the first launch (a large matrix
+//     product reaches 1214).  A step of a wave is 512 cycles of MFMA, some 500 of the
+//     softmax's VALU and 128 of a CU's LDS: two waves per SIMD overlap them in part.
+//     Tried and no faster: 8 waves with 256 query rows (74 us for 68), pairs of steps,
+//     half the waves a barrier behind the others, scores ahead of the weights.
 
 #include <hip/hip_runtime.h>
+
+#include <type_traits>
 
 #include "lsk_internal.h"
 
@@ -52,14 +65,13 @@ typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x4_t __attribute__((ext_vector_type(4)));
 
 constexpr int D = kAttnHeadDim;
-constexpr int kThreads = kPrefixThreads;
-constexpr int kWaves = kThreads / 64;
-static_assert(kWaves == 4, "four waves' slots, and four waves to a shared item");
 constexpr int kStep = 32;                  // key rows, and query rows of a wave
 constexpr int kHalfSlot = kStep * D * 2;   // bytes of a step's K, or V
 constexpr int kSlot = 2 * kHalfSlot;
-constexpr int kSlots = 4;                  // one per wave, or a ring of steps
 constexpr float kRaise = 8.f;
+constexpr int kJointWaves = 8;             // of an item of a short context
+constexpr int kWaves = 4;                  // of another item
+static_assert(kPrefixSharedRows == 32 * kWaves, "query rows of an item whose waves have some of their own");
 
 __device__ __forceinline__ float neg_inf() { return -__builtin_huge_valf(); }
 
@@ -135,41 +147,59 @@ __device__ __forceinline__ Lane lane_addresses(int stride) {
   return a;
 }
 
-// DMA loads [first, first + N) of the 8 (1 KB, 4 rows each) of a step's K or V: all
-// of them, or a wave's two of four waves'.  Rows from `end` on are row end - 1.
-template <bool IS_V, int N>
-__device__ __forceinline__ void load_half(lds_load_words_t buf, const Lane& a, int stride, int row0, int end, int first,
-                                          unsigned lds) {
-  const int lane = threadIdx.x & 63;
+// K and V rows up to `end` from 16 (K) or 8 (V) row boundaries of a step on: each load
+// of a step is then the lane's offset, the step's and a buffer.  Rows from `end` on
+// are out of range: zeros to LDS, and no memory access.
+struct Buffers {
+  lds_load_words_t k[2], v[4];
+};
+__device__ __forceinline__ lds_load_words_t rows_from(const __bf16* p, int stride, int end, int first) {
+  const long long bytes = ((long long)(end - 1 - first) * stride + D) * 2;
+  lds_load_words_t w = buffer_words(p + (size_t)first * stride, end > first ? (size_t)bytes : 0);
 #pragma unroll
-  for (int i = 0; i < N; ++i) {
-    const int u = first + i;
-    if (row0 + kStep <= end) {
-      // the chunk order repeats every 16 rows (K) or 8 (V)
-      if constexpr (IS_V)
-        dma_1k<false>(buf, a.v_at[i & 1], (unsigned)(row0 + 4 * (u & ~1)) * (unsigned)(stride * 2), lds + u * 1024);
-      else
-        dma_1k<false>(buf, a.k_at[i & 3], (unsigned)(row0 + 4 * (u & ~3)) * (unsigned)(stride * 2), lds + u * 1024);
-    } else {
-      const int r = 4 * u + (lane >> 4);
-      const int chunk = (lane & 15) ^ (IS_V ? 2 * (r & 7) : (r & 15));
-      const unsigned at = (unsigned)min(row0 + r, end - 1) * (unsigned)(stride * 2) + (unsigned)(chunk << 4);
-      dma_1k<false>(buf, at, 0, lds + u * 1024);
-    }
-  }
+  for (int i = 0; i < 4; ++i) w[i] = __builtin_amdgcn_readfirstlane(w[i]);  // wave-uniform; says so to the compiler
+  return w;
+}
+__device__ __forceinline__ Buffers row_buffers(const Rows& src) {
+  Buffers b;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) b.k[i] = rows_from(src.k, src.stride, src.end, 16 * i);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) b.v[i] = rows_from(src.v, src.stride, src.end, 8 * i);
+  return b;
+}
+
+// A step's K, V to LDS (8 loads of 1 KB, 4 rows each); `off`: byte offset of its first row.
+__device__ __forceinline__ void load_k(const Buffers& b, const Lane& a, unsigned off, unsigned lds) {
+#pragma unroll
+  for (int u = 0; u < 8; ++u) dma_1k<false>(b.k[u >> 2], a.k_at[u & 3] + off, 0, lds + u * 1024);
+}
+__device__ __forceinline__ void load_v(const Buffers& b, const Lane& a, unsigned off, unsigned lds) {
+#pragma unroll
+  for (int u = 0; u < 8; ++u) dma_1k<false>(b.v[u >> 1], a.v_at[u & 1] + off, 0, lds + u * 1024);
 }
 
 typedef __attribute__((address_space(3))) const unsigned char lds_byte_t;
 
-// S^T = K Q^T of a step.
-__device__ __forceinline__ f32x16_t step_scores(lds_byte_t* k, const Lane& a, const bf16x8_t (&qf)[8]) {
-  f32x16_t s = {};
+__device__ __forceinline__ bf16x8_t k_operand(lds_byte_t* k, const Lane& a, int ks) {
+  return *reinterpret_cast<__attribute__((address_space(3))) const bf16x8_t*>(k + (a.k_read ^ (unsigned)(ks << 5)));
+}
+
+// S^T = K Q^T of N steps of key rows.  A product waits twice its time for the one that it
+// adds to: N products by turns, of one step two half sums.
+template <int N>
+__device__ __forceinline__ void step_scores(lds_byte_t* k, const Lane& a, const bf16x8_t (&qf)[8], f32x16_t (&s)[N]) {
+  constexpr int kChains = N > 1 ? N : 2;
+  f32x16_t c[kChains] = {};
 #pragma unroll
-  for (int ks = 0; ks < 8; ++ks) {
-    const auto* at = reinterpret_cast<__attribute__((address_space(3))) const bf16x8_t*>(k + (a.k_read ^ (unsigned)(ks << 5)));
-    s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*at, qf[ks], s, 0, 0, 0);
-  }
-  return s;
+  for (int ks = 0; ks < 8; ++ks)
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      const int chain = N > 1 ? n : ks & 1;
+      c[chain] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k_operand(k + n * kHalfSlot, a, ks), qf[ks], c[chain], 0, 0, 0);
+    }
+#pragma unroll
+  for (int n = 0; n < N; ++n) s[n] = N > 1 ? c[n] : c[0] + c[1];
 }
 
 // V^T of rows 16 s .. + 15 (in the lanes' order: slot e of half h is row
@@ -182,20 +212,23 @@ __device__ __forceinline__ bf16x8_t v_operand(lds_byte_t* v, const Lane& a, int 
   return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
 }
 
-// The step's weights P (bf16, the B operands of its two products), and m, l, O
+// The weights P of N steps (bf16, the B operands of two products each), and m, l, O
 // brought to the new maximum.  limit: key rows that the lane's query row sees, in
-// rows of the step (from 32 on: all).
-template <bool MASK>
-__device__ __forceinline__ void step_weights(f32x16_t s, float c2, int limit, State& st, bf16x8_t (&p)[2]) {
+// rows of the steps.
+template <int N, bool MASK>
+__device__ __forceinline__ void step_weights(f32x16_t (&s)[N], float c2, int limit, State& st, bf16x8_t (&p)[2 * N]) {
   const int h = (threadIdx.x & 63) >> 5;
+  auto seen = [&](int n, int i) { return 32 * n + 8 * (i / 4) + 4 * h + i % 4 < limit; };
   if constexpr (MASK) {
 #pragma unroll
-    for (int i = 0; i < 16; ++i)
-      if (8 * (i / 4) + 4 * h + i % 4 >= limit) s[i] = neg_inf();
-  }
-  float mx = s[0];
+    for (int n = 0; n < N; ++n)
 #pragma unroll
-  for (int i = 1; i < 16; ++i) mx = fmaxf(mx, s[i]);
+      for (int i = 0; i < 16; ++i)
+        if (!seen(n, i)) s[n][i] = neg_inf();
+  }
+  float mx = s[0][0];
+#pragma unroll
+  for (int i = 1; i < 16 * N; ++i) mx = fmaxf(mx, s[i / 16][i % 16]);
   mx = other_half_max(mx) * c2;
   if (MASK && limit <= 0) mx = neg_inf();  // (-inf times a scale of zero)
   const bool raise = mx > st.m + kRaise;
@@ -211,29 +244,33 @@ __device__ __forceinline__ void step_weights(f32x16_t s, float c2, int limit, St
   const float m = st.m == neg_inf() ? 0.f : st.m;
   const bf16x2_t ones = {static_cast<__bf16>(1.f), static_cast<__bf16>(1.f)};
 #pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], c2, -m));
-    if (MASK && 8 * (i / 4) + 4 * h + i % 4 >= limit) e = 0.f;
-    p[i / 8][i % 8] = static_cast<__bf16>(e);
-  }
+  for (int n = 0; n < N; ++n) {
 #pragma unroll
-  for (int i = 0; i < 16; i += 2)
-    st.l = __builtin_amdgcn_fdot2_f32_bf16(bf16x2_t{p[i / 8][i % 8], p[i / 8][i % 8 + 1]}, ones, st.l, false);
+    for (int i = 0; i < 16; ++i) {
+      float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[n][i], c2, -m));
+      if (MASK && !seen(n, i)) e = 0.f;
+      p[2 * n + i / 8][i % 8] = static_cast<__bf16>(e);
+    }
+#pragma unroll
+    for (int i = 0; i < 16; i += 2)
+      st.l = __builtin_amdgcn_fdot2_f32_bf16(bf16x2_t{p[2 * n + i / 8][i % 8], p[2 * n + i / 8][i % 8 + 1]}, ones, st.l,
+                                             false);
+  }
 }
 
-__device__ __forceinline__ void step_accumulate(lds_byte_t* v, const Lane& a, const bf16x8_t (&p)[2], State& st) {
+template <int N>
+__device__ __forceinline__ void step_accumulate(lds_byte_t* v, const Lane& a, const bf16x8_t (&p)[N], State& st) {
 #pragma unroll
-  for (int s = 0; s < 2; ++s)
+  for (int s = 0; s < N; ++s)
 #pragma unroll
     for (int db = 0; db < 4; ++db)
       st.o[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v_operand(v, a, s, db), p[s], st.o[db], 0, 0, 0);
 }
 
-// V of a step's rows that not every query row sees: a weight of zero does not take
-// an infinity or a NaN out of a product.  Rows from `end` on, which stand in for
-// rows past the last, become zero; so do the infinite and NaN values of the rows
-// from `all` to `end` (write_item adds them to the query rows that see them).
-// Returns whether there were any.
+// V of a step's rows that only some query rows see (from `all` to `end`): a weight
+// of zero does not take an infinity or a NaN out of a product, so those become
+// zero, and write_item adds them to the query rows that see them.  Returns whether there
+// were any.
 __device__ __forceinline__ bool mask_values(unsigned char* v, int all, int end) {
   typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
   const int lane = threadIdx.x & 63;
@@ -242,9 +279,7 @@ __device__ __forceinline__ bool mask_values(unsigned char* v, int all, int end) 
   for (int i = 0; i < kHalfSlot / 1024; ++i) {
     const int r = 4 * i + (lane >> 4);
     u32x4* at = reinterpret_cast<u32x4*>(v + i * 1024 + lane * 16);
-    if (r >= end) {
-      *at = u32x4{0u, 0u, 0u, 0u};
-    } else if (r >= all) {
+    if (r >= all && r < end) {
       u32x4 w = *at;
       bool here = false;
 #pragma unroll
@@ -267,96 +302,94 @@ __device__ __forceinline__ void wait_half() { asm volatile("s_waitcnt vmcnt(8) l
 __device__ __forceinline__ void wait_reads() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
 __device__ __forceinline__ void wait_all() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory"); }
 
-__device__ __forceinline__ lds_load_words_t row_words(const __bf16* p, int stride, int end) {
-  return buffer_words(p, ((size_t)(end - 1) * stride + D) * 2);
-}
-
-// Rows of `src`, the steps w, w + 4, .. for wave w, in the wave's own slot.  limit:
-// key rows that the lane's query row sees; `least`, the least of them (CAUSAL).
-// Returns whether mask_values took values out.
-template <bool CAUSAL>
+// Rows of `src`, the steps w, w + NW, .. for wave w of NW, counted from the `first`-th
+// wave on, in the wave's own slot.  limit: key rows that the lane's query row sees;
+// `least`, the least of them (CAUSAL).  Returns whether mask_values took values out.
+template <int NW, bool CAUSAL>
 __device__ __forceinline__ bool attend_split(const Rows& src, const bf16x8_t (&qf)[8], float c2, int limit,
-                                             int least, unsigned char* slots, State& st) {
-  const int wave = threadIdx.x >> 6;
-  int row0 = src.begin + wave * kStep;
+                                             int least, int first, unsigned char* slots, State& st) {
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);  // (uniform: so are the branches on it)
+  int row0 = src.begin + ((wave - first) & (NW - 1)) * kStep;
   if (row0 >= src.end) return false;
   bool special = false;
   const Lane a = lane_addresses(src.stride);
-  const lds_load_words_t kb = row_words(src.k, src.stride, src.end), vb = row_words(src.v, src.stride, src.end);
+  const Buffers buf = row_buffers(src);
   auto* slot = (lds_byte_t*)(slots + wave * kSlot);
   const unsigned at = (unsigned)(size_t)slot;
+  unsigned off = (unsigned)row0 * (unsigned)(src.stride * 2);
   wait_all();  // (loads counted by the compiler are not among those counted here)
-  load_half<false, 8>(kb, a, src.stride, row0, src.end, 0, at);
-  load_half<true, 8>(vb, a, src.stride, row0, src.end, 0, at + kHalfSlot);
-  while (true) {
-    const int next = row0 + kWaves * kStep;
-    const bool more = next < src.end;
+  load_k(buf, a, off, at);
+  load_v(buf, a, off, at + kHalfSlot);
+  auto step = [&](auto masked) __attribute__((always_inline)) {
+    constexpr bool kMask = decltype(masked)::value;
     wait_half();  // K is here
-    const f32x16_t s = step_scores(slot, a, qf);
+    f32x16_t s[1];
+    step_scores<1>(slot, a, qf, s);
     wait_reads();
-    if (more) load_half<false, 8>(kb, a, src.stride, next, src.end, 0, at);
+    off += (unsigned)(NW * kStep) * (unsigned)(src.stride * 2);
+    load_k(buf, a, off, at);
     bf16x8_t p[2];
-    const bool full = row0 + kStep <= (CAUSAL ? min(least, src.end) : src.end);
-    if (full)
-      step_weights<false>(s, c2, kStep, st, p);
-    else
-      step_weights<true>(s, c2, min(limit, src.end) - row0, st, p);
-    if (more)
-      wait_half();  // V is here
-    else
-      wait_all();
-    if (!full)
-      special |= mask_values(slots + wave * kSlot + kHalfSlot, (CAUSAL ? least : src.end) - row0, src.end - row0);
-    step_accumulate(slot + kHalfSlot, a, p, st);
-    if (!more) break;
+    step_weights<1, kMask>(s, c2, min(limit, src.end) - row0, st, p);
+    wait_half();  // V is here
+    if constexpr (kMask && CAUSAL)
+      special |= mask_values(slots + wave * kSlot + kHalfSlot, least - row0, src.end - row0);
+    step_accumulate<2>(slot + kHalfSlot, a, p, st);
     wait_reads();
-    load_half<true, 8>(vb, a, src.stride, next, src.end, 0, at + kHalfSlot);
-    row0 = next;
-  }
+    load_v(buf, a, off, at + kHalfSlot);
+    row0 += NW * kStep;
+  };
+  const int full = CAUSAL ? min(least, src.end) : src.end;
+  while (row0 + kStep <= full) step(std::false_type{});
+  while (row0 < src.end) step(std::true_type{});
   wait_all();
   return special;
 }
 
-// Rows of `src` for four waves with query rows of their own: steps through a
-// ring of kSlots, two K and two V loads of each by each wave.
+// Rows of `src` for four waves with query rows of their own: steps through a ring of
+// four slots, two K and two V loads of each step by each wave.
 __device__ __forceinline__ void attend_shared(const Rows& src, const bf16x8_t (&qf)[8], float c2, unsigned char* slots,
                                               State& st) {
-  const int wave = threadIdx.x >> 6;
-  Lane a = lane_addresses(src.stride);
-  if (wave & 1) a.k_at[0] = a.k_at[2], a.k_at[1] = a.k_at[3];  // loads 2 wave and 2 wave + 1
-  const lds_load_words_t kb = row_words(src.k, src.stride, src.end), vb = row_words(src.v, src.stride, src.end);
-  const int steps = (src.end - src.begin + kStep - 1) / kStep;
+  constexpr int kRing = kWaves * kSlot;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const Lane a = lane_addresses(src.stride);
+  // rows 8 wave .. + 7 of a step
+  const lds_load_words_t kb = rows_from(src.k, src.stride, src.end, 16 * (wave >> 1));
+  const lds_load_words_t vb = rows_from(src.v, src.stride, src.end, 8 * wave);
+  const unsigned k0 = wave & 1 ? a.k_at[2] : a.k_at[0], k1 = wave & 1 ? a.k_at[3] : a.k_at[1];
   auto* ring = (lds_byte_t*)slots;
-  auto load = [&](int i) {
-    // (past the last step the last one again, into a slot that is not read: the
-    // count of loads in flight stays the same)
-    const int row0 = src.begin + min(i, steps - 1) * kStep;
-    const unsigned at = (unsigned)(size_t)ring + (unsigned)(i % kSlots) * kSlot;
-    load_half<false, 2>(kb, a, src.stride, row0, src.end, 2 * wave, at);
-    load_half<true, 2>(vb, a, src.stride, row0, src.end, 2 * wave, at + kHalfSlot);
+  const unsigned at = (unsigned)(size_t)ring + 2048u * wave;
+  unsigned off = (unsigned)src.begin * (unsigned)(src.stride * 2);
+  unsigned to = 0;  // slot of the next load
+  auto load = [&]() __attribute__((always_inline)) {
+    // (past the last row: zeros, so that the count of loads in flight stays the same)
+    dma_1k<false>(kb, k0 + off, 0, at + to);
+    dma_1k<false>(kb, k1 + off, 0, at + to + 1024);
+    dma_1k<false>(vb, a.v_at[0] + off, 0, at + to + kHalfSlot);
+    dma_1k<false>(vb, a.v_at[1] + off, 0, at + to + kHalfSlot + 1024);
+    off += (unsigned)kStep * (unsigned)(src.stride * 2);
+    to = (to + kSlot) & (kRing - 1);
   };
   wait_all();
 #pragma unroll
-  for (int i = 0; i < kSlots - 1; ++i) load(i);
-  for (int i = 0; i < steps; ++i) {
-    // Steps up to i have landed here (two of 4 loads each are behind it), and with
-    // the barrier everywhere; every wave is done with step i - 1, whose slot the
-    // next load takes.
+  for (int i = 0; i < kWaves - 1; ++i) load();
+  unsigned from = 0;
+  int row0 = src.begin;
+  auto step = [&](auto masked) __attribute__((always_inline)) {
+    // Steps up to this one have landed here (two of 4 loads each are behind it), and
+    // with the barrier everywhere; every wave is done with the step before it, whose
+    // slot the next load takes.
     asm volatile("s_waitcnt vmcnt(8) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-    load(i + kSlots - 1);
-    auto* slot = ring + (i % kSlots) * kSlot;
-    const int row0 = src.begin + i * kStep;
-    const f32x16_t s = step_scores(slot, a, qf);
+    load();
+    f32x16_t s[1];
+    step_scores<1>(ring + from, a, qf, s);
     bf16x8_t p[2];
-    const bool full = row0 + kStep <= src.end;
-    if (full)
-      step_weights<false>(s, c2, kStep, st, p);
-    else
-      step_weights<true>(s, c2, src.end - row0, st, p);
-    // (every wave clears the same rows before it reads them)
-    if (!full) mask_values(slots + (i % kSlots) * kSlot + kHalfSlot, src.end - row0, src.end - row0);
-    step_accumulate(slot + kHalfSlot, a, p, st);
-  }
+    step_weights<1, decltype(masked)::value>(s, c2, src.end - row0, st, p);
+    step_accumulate<2>(ring + from + kHalfSlot, a, p, st);
+    from = (from + kSlot) & (kRing - 1);
+    row0 += kStep;
+  };
+  while (row0 + kStep <= src.end) step(std::false_type{});
+  if (row0 < src.end) step(std::true_type{});
   wait_all();
 }
 
@@ -365,12 +398,12 @@ struct Query {
   int b, t, h;
 };
 
-// What the 4 waves leave, to rows of the output or of the workspace.
+// What the NW waves leave, to rows of the output or of the workspace.
 //   SPLIT: the waves hold the same 32 query rows over different key rows, added
 //   here; else 32 rows each.
 // find(i): query row i of the item, or b = -1 behind the last one.  add(q, d, l, o): what
 // mask_values took out of dims d .. d + 3 for query row q, whose weights sum to l.
-template <bool SPLIT, bool DIRECT, typename Find, typename Add>
+template <int NW, bool SPLIT, bool DIRECT, typename Find, typename Add>
 __device__ __forceinline__ void write_item(const PrefixArgs& a, const State& st, unsigned char* slots, float (*ms)[32],
                                            float (*ls)[32], int part, Find find, Add add) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -379,24 +412,27 @@ __device__ __forceinline__ void write_item(const PrefixArgs& a, const State& st,
   __syncthreads();  // the slots' last reads and loads are done in every wave
   // O to LDS as rows of 512 bytes, chunk ch of row c at ch ^ c.
   unsigned char* mine = slots + wave * kSlot + c * 512;
+  if (find(SPLIT ? c : wave * 32 + c).b >= 0) {
 #pragma unroll
-  for (int db = 0; db < 4; ++db)
+    for (int db = 0; db < 4; ++db)
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      const int ch = 8 * db + 2 * q + h;
-      *reinterpret_cast<f32x4_t*>(mine + ((ch ^ c) << 4)) =
-          f32x4_t{st.o[db][4 * q], st.o[db][4 * q + 1], st.o[db][4 * q + 2], st.o[db][4 * q + 3]};
+      for (int q = 0; q < 4; ++q) {
+        const int ch = 8 * db + 2 * q + h;
+        *reinterpret_cast<f32x4_t*>(mine + ((ch ^ c) << 4)) =
+            f32x4_t{st.o[db][4 * q], st.o[db][4 * q + 1], st.o[db][4 * q + 2], st.o[db][4 * q + 3]};
+      }
+    if (h == 0) {
+      ms[wave][c] = st.m;
+      ls[wave][c] = l;
     }
-  if (h == 0) {
-    ms[wave][c] = st.m;
-    ls[wave][c] = l;
   }
   __syncthreads();
+  constexpr int kLanes = SPLIT ? 2 * NW : 8;  // to a query row
   constexpr int kPasses = SPLIT ? 1 : 4;
-  constexpr int kFrom = SPLIT ? kWaves : 1;
+  constexpr int kFrom = SPLIT ? NW : 1;
 #pragma unroll
   for (int pass = 0; pass < kPasses; ++pass) {
-    const int r = SPLIT ? tid >> 3 : pass * 8 + (lane >> 3);  // of the wave's 32
+    const int r = SPLIT ? tid / kLanes : pass * 8 + (lane >> 3);  // of the wave's 32
     const Query q = find(SPLIT ? r : wave * 32 + r);
     if (q.b < 0) continue;
     float w[kFrom], m = neg_inf(), sum = 0.f;
@@ -413,8 +449,8 @@ __device__ __forceinline__ void write_item(const PrefixArgs& a, const State& st,
     // (no row at all: zero; rows that all score -inf: 0 / 0)
     const bool none = a.P == 0 && own_visible(a, q.b, q.t) == 0;
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const int ch = (lane & 7) + 8 * k;
+    for (int k = 0; k < 32 / kLanes; ++k) {
+      const int ch = (lane & (kLanes - 1)) + kLanes * k;
       f32x4_t o = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int i = 0; i < kFrom; ++i)
@@ -429,7 +465,7 @@ __device__ __forceinline__ void write_item(const PrefixArgs& a, const State& st,
         *reinterpret_cast<f32x4_t*>(a.part_o + slot_row * D + 4 * ch) = o;
       }
     }
-    if (!DIRECT && (lane & 7) == 0) *reinterpret_cast<f32x2_t*>(a.part_ml + slot_row * 2) = f32x2_t{m, sum};
+    if (!DIRECT && (lane & (kLanes - 1)) == 0) *reinterpret_cast<f32x2_t*>(a.part_ml + slot_row * 2) = f32x2_t{m, sum};
   }
 }
 
@@ -459,41 +495,46 @@ __device__ __forceinline__ State empty_state() {
 
 // One request's query rows r0 .. r0 + 31 of kv head j over its own rows [begin, end),
 // with JOINT over the prefix in front of them.
-template <bool CAUSAL, bool JOINT>
+template <int NW, bool CAUSAL, bool JOINT>
 __device__ __forceinline__ void own_item(const PrefixArgs& a, int j, int b, int r0, int begin, int end, int part,
                                          unsigned char* slots, float (*ms)[32], float (*ls)[32]) {
   const int c = threadIdx.x & 31;
   const int rows = a.T * a.G;
-  auto find = [&](int i) {
+  auto find = [&](int i) __attribute__((always_inline)) {
     const int r = r0 + i;
     return r < rows ? Query{b, r / a.G, j * a.G + r % a.G} : Query{-1, 0, 0};
   };
   const Query mine = find(min(c, rows - 1 - r0));
   bf16x8_t qf[8];
   load_q(a, mine, qf);
+  const int written = __builtin_amdgcn_readfirstlane(own_written(a, b));
+  if (!JOINT && begin >= written) return;  // (the second launch knows this, too)
   State st = empty_state();
   const float c2 = fabsf(a.scale) * 1.44269504088896341f;
   if (JOINT && a.P > 0) {
     const Rows src = {a.pk + (size_t)j * a.p_h, a.pv + (size_t)j * a.p_h, a.p_row, 0, a.P};
-    attend_split<false>(src, qf, c2, a.P, a.P, slots, st);
+    attend_split<NW, false>(src, qf, c2, a.P, a.P, 0, slots, st);
   }
   // The rows that the item's first query row sees all of them see, and none is read
   // that its last one does not.
-  const int least = own_visible(a, b, r0 / a.G);
-  const int stop = min(end, own_visible(a, b, min(r0 + 31, rows - 1) / a.G));
+  const int least = max(written - (a.T - 1 - r0 / a.G), 0);
+  const int stop = min(end, max(written - (a.T - 1 - min(r0 + 31, rows - 1) / a.G), 0));
   const size_t base = (size_t)b * a.k_b + (size_t)j * a.k_h;
   bool special = false;
   if (begin < stop) {
     const Rows src = {a.k + base, a.v + base, a.k_row, begin, stop};
-    special = attend_split<CAUSAL>(src, qf, c2, own_visible(a, b, mine.t), least, slots, st);
+    // (the waves that had one step less of the prefix come first)
+    special = attend_split<NW, CAUSAL>(src, qf, c2, max(written - (a.T - 1 - mine.t), 0), least,
+                                       JOINT ? (a.P + kStep - 1) / kStep : 0, slots, st);
   }
   if constexpr (CAUSAL) {
     // Infinite and NaN values of rows that only some query rows see: to those.
     const bool any = __syncthreads_or(special);
     const int first = max(begin, least);
-    write_item<true, JOINT>(a, st, slots, ms, ls, part, find, [&](const Query& q, int d, float sum, f32x4_t& o) {
+    write_item<NW, true, JOINT>(a, st, slots, ms, ls, part, find,
+                                [&](const Query& q, int d, float sum, f32x4_t& o) __attribute__((always_inline)) {
       if (!any) return;
-      for (int i = first; i < min(stop, own_visible(a, b, q.t)); ++i) {
+      for (int i = first; i < min(stop, written - (a.T - 1 - q.t)); ++i) {
         const bf16x4_t v = *reinterpret_cast<const bf16x4_t*>(a.v + base + (size_t)i * a.k_row + d);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
@@ -503,7 +544,7 @@ __device__ __forceinline__ void own_item(const PrefixArgs& a, int j, int b, int 
       }
     });
   } else {
-    write_item<true, JOINT>(a, st, slots, ms, ls, part, find, [](const Query&, int, float, f32x4_t&) {});
+    write_item<NW, true, JOINT>(a, st, slots, ms, ls, part, find, [](const Query&, int, float, f32x4_t&) {});
   }
 }
 
@@ -512,7 +553,7 @@ template <bool SHARED>
 __device__ __forceinline__ void prefix_item(const PrefixArgs& a, int j, int r0, int begin, int end, int part,
                                             unsigned char* slots, float (*ms)[32], float (*ls)[32]) {
   const int rows = a.B * a.T * a.G;
-  auto find = [&](int i) {
+  auto find = [&](int i) __attribute__((always_inline)) {
     const int r = r0 + i;
     if (r >= rows) return Query{-1, 0, 0};
     const int bt = r / a.G;
@@ -527,16 +568,16 @@ __device__ __forceinline__ void prefix_item(const PrefixArgs& a, int j, int r0, 
   if constexpr (SHARED)
     attend_shared(src, qf, c2, slots, st);
   else
-    attend_split<false>(src, qf, c2, end, end, slots, st);
-  write_item<!SHARED, false>(a, st, slots, ms, ls, part, find, [](const Query&, int, float, f32x4_t&) {});
+    attend_split<kWaves, false>(src, qf, c2, end, end, 0, slots, st);
+  write_item<kWaves, !SHARED, false>(a, st, slots, ms, ls, part, find, [](const Query&, int, float, f32x4_t&) {});
 }
 
 // Grid: prefix items (kv head fastest: with 8 of them each XCD's L2 holds one
 // head's rows; then key ranges, then query rows), then own items (kv head,
 // request, query rows, key ranges).
 template <bool SHARED, bool CAUSAL>
-__global__ __launch_bounds__(kThreads, 2) void prefix_attention_kernel(PrefixArgs a) {
-  __shared__ __align__(1024) unsigned char slots[kSlots * kSlot];
+__global__ __launch_bounds__(64 * kWaves, 2) void prefix_attention_kernel(PrefixArgs a) {
+  __shared__ __align__(1024) unsigned char slots[kWaves * kSlot];
   __shared__ float ms[kWaves][32], ls[kWaves][32];
   int id = blockIdx.x;
   if (id < a.prefix_items) {
@@ -545,7 +586,8 @@ __global__ __launch_bounds__(kThreads, 2) void prefix_attention_kernel(PrefixArg
     const int part = id % a.prefix_parts;
     const int tile = id / a.prefix_parts;
     const int begin = part * a.prefix_chunk;
-    prefix_item<SHARED>(a, j, tile * (SHARED ? 128 : 32), begin, min(begin + a.prefix_chunk, a.P), part, slots, ms, ls);
+    prefix_item<SHARED>(a, j, tile * (SHARED ? kPrefixSharedRows : 32), begin, min(begin + a.prefix_chunk, a.P), part,
+                            slots, ms, ls);
     return;
   }
   id -= a.prefix_items;
@@ -556,43 +598,70 @@ __global__ __launch_bounds__(kThreads, 2) void prefix_attention_kernel(PrefixArg
   const int tile = id % a.own_tiles;
   const int part = id / a.own_tiles;
   const int begin = part * a.own_chunk;
-  if (begin >= own_written(a, b)) return;  // (the second launch knows this, too)
-  own_item<CAUSAL, false>(a, j, b, tile * 32, begin, begin + a.own_chunk, a.prefix_parts + part, slots, ms, ls);
+  own_item<kWaves, CAUSAL, false>(a, j, b, tile * 32, begin, begin + a.own_chunk, a.prefix_parts + part, slots, ms, ls);
 }
 
 // Short contexts, one launch.  Grid: (kv head, request, query rows), the head fastest.
 template <bool CAUSAL>
-__global__ __launch_bounds__(kThreads, 2) void joint_attention_kernel(PrefixArgs a) {
-  __shared__ __align__(1024) unsigned char slots[kSlots * kSlot];
-  __shared__ float ms[kWaves][32], ls[kWaves][32];
+__global__ __launch_bounds__(64 * kJointWaves, 2) void joint_attention_kernel(PrefixArgs a) {
+  __shared__ __align__(1024) unsigned char slots[kJointWaves * kSlot];
+  __shared__ float ms[kJointWaves][32], ls[kJointWaves][32];
   int id = blockIdx.x;
   const int j = id % a.n_kv;
   id /= a.n_kv;
   const int b = id % a.B;
-  own_item<CAUSAL, true>(a, j, b, id / a.B * 32, 0, a.S, 0, slots, ms, ls);
+  own_item<kJointWaves, CAUSAL, true>(a, j, b, id / a.B * 32, 0, a.S, 0, slots, ms, ls);
 }
 
-// Adds a row's items up: 32 lanes per row, 4 dims each, in the order of the key rows.
-__global__ __launch_bounds__(kThreads) void combine_kernel(PrefixArgs a) {
-  const size_t row = (size_t)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5);
-  if (row >= a.rows) return;
-  const int d = 4 * (threadIdx.x & 31);
+// Adds a row's items up: kGroups times 32 lanes per row, 4 dims each, group g the items
+// g, g + kGroups, .., kPartsAhead of them on their way at a time (past the last the last
+// again, unused); then the groups, in their order.
+constexpr int kCombineThreads = 256;
+constexpr int kGroups = 4;
+constexpr int kCombineRows = kCombineThreads / (32 * kGroups);
+constexpr int kPartsAhead = 4;
+__global__ __launch_bounds__(kCombineThreads) void combine_kernel(PrefixArgs a) {
+  __shared__ float gm[kCombineRows][kGroups], gl[kCombineRows][kGroups];
+  __shared__ f32x4_t go[kCombineRows][kGroups][32];
+  const int g = (threadIdx.x >> 5) % kGroups, mine = threadIdx.x / (32 * kGroups), lane = threadIdx.x & 31;
+  const size_t want = (size_t)blockIdx.x * kCombineRows + mine;
+  const size_t row = want < (size_t)a.rows ? want : a.rows - 1;
+  const int d = 4 * lane;
   const int bt = (int)(row / a.n_q);
   const int b = bt / a.T;
   const int parts = a.prefix_parts + (own_written(a, b) + a.own_chunk - 1) / a.own_chunk;
   float m = neg_inf(), l = 0.f;
   f32x4_t o = {0.f, 0.f, 0.f, 0.f};
-  for (int p = 0; p < parts; ++p) {
-    const size_t at = (size_t)p * a.rows + row;
-    const f32x2_t ml = *reinterpret_cast<const f32x2_t*>(a.part_ml + at * 2);
-    const f32x4_t v = *reinterpret_cast<const f32x4_t*>(a.part_o + at * D + d);
-    const float top = fmaxf(m, ml[0]);
+  auto join = [&](float pm, float pl, f32x4_t po) __attribute__((always_inline)) {
+    const float top = fmaxf(m, pm);
     const float was = m == top ? 1.f : __builtin_amdgcn_exp2f(m - top);
-    const float now = ml[0] == top ? 1.f : __builtin_amdgcn_exp2f(ml[0] - top);
-    l = l * was + ml[1] * now;
-    o = o * was + v * now;
+    const float now = pm == top ? 1.f : __builtin_amdgcn_exp2f(pm - top);
+    l = l * was + pl * now;
+    o = o * was + po * now;
     m = top;
+  };
+  for (int first = g; first < parts; first += kGroups * kPartsAhead) {
+    f32x2_t ml[kPartsAhead];
+    f32x4_t v[kPartsAhead];
+#pragma unroll
+    for (int i = 0; i < kPartsAhead; ++i) {
+      const size_t at = (size_t)min(first + i * kGroups, parts - 1) * a.rows + row;
+      ml[i] = *reinterpret_cast<const f32x2_t*>(a.part_ml + at * 2);
+      v[i] = *reinterpret_cast<const f32x4_t*>(a.part_o + at * D + d);
+    }
+#pragma unroll
+    for (int i = 0; i < kPartsAhead; ++i)
+      if (first + i * kGroups < parts) join(ml[i][0], ml[i][1], v[i]);
   }
+  if (lane == 0) {
+    gm[mine][g] = m;
+    gl[mine][g] = l;
+  }
+  go[mine][g][lane] = o;
+  __syncthreads();
+  if (g != 0 || want >= (size_t)a.rows) return;
+#pragma unroll
+  for (int i = 1; i < kGroups; ++i) join(gm[mine][i], gl[mine][i], go[mine][i][lane]);
   const bool none = a.P == 0 && own_visible(a, b, bt % a.T) == 0;
   bf16x4_t v;
 #pragma unroll
@@ -604,18 +673,17 @@ template <bool CAUSAL>
 hipError_t launch(const PrefixArgs& a, const PrefixPlan& plan, hipStream_t stream) {
   const unsigned own = (unsigned)a.n_kv * a.B * a.own_tiles;
   if (plan.joint) {
-    launch_kernel(joint_attention_kernel<CAUSAL>, dim3(own), dim3(kThreads), 0, stream, a);
+    launch_kernel(joint_attention_kernel<CAUSAL>, dim3(own), dim3(64 * kJointWaves), 0, stream, a);
     return hipGetLastError();
   }
   const dim3 items((unsigned)a.prefix_items + own * plan.own_parts);
   if (plan.shared)
-    launch_kernel(prefix_attention_kernel<true, CAUSAL>, items, dim3(kThreads), 0, stream, a);
+    launch_kernel(prefix_attention_kernel<true, CAUSAL>, items, dim3(64 * kWaves), 0, stream, a);
   else
-    launch_kernel(prefix_attention_kernel<false, CAUSAL>, items, dim3(kThreads), 0, stream, a);
+    launch_kernel(prefix_attention_kernel<false, CAUSAL>, items, dim3(64 * kWaves), 0, stream, a);
   hipError_t err = hipGetLastError();
   if (err != hipSuccess) return err;
-  launch_kernel(combine_kernel, dim3((unsigned)((a.rows + kThreads / 32 - 1) / (kThreads / 32))), dim3(kThreads), 0,
-                stream, a);
+  launch_kernel(combine_kernel, dim3((unsigned)((a.rows + kCombineRows - 1) / kCombineRows)), dim3(kCombineThreads), 0, stream, a);
   return hipGetLastError();
 }
 

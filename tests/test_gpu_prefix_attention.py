@@ -92,6 +92,7 @@ CASES = [
     # 128 query rows to an item
     (40, 1, 32, 8, 600, 70), (9, 8, 32, 8, 1025, 130), (130, 1, 8, 8, 2000, 5), (5, 33, 12, 4, 515, 600),
     (33, 1, 16, 2, 513, 0), (20, 16, 4, 1, 0, 600), (65, 1, 3, 3, 511, 2),
+    (70, 1, 32, 8, 1000, 70), (49, 1, 4, 1, 2000, 300), (200, 1, 8, 8, 1537, 0), (33, 7, 4, 4, 801, 40), (97, 2, 8, 4, 31, 900),
 ]
 
 
@@ -149,7 +150,7 @@ def test_queries_that_see_no_row_give_zeros(gpu, case):
     assert not bool(kernels.shared_prefix_attention(*far, SCALE).any())
 
 
-@pytest.mark.parametrize("prefix,b", [(100, 2), (1000, 2), (1000, 40)])
+@pytest.mark.parametrize("prefix,b", [(100, 2), (1000, 2), (1000, 40), (1000, 60)])
 @pytest.mark.parametrize("t", [1, 6])
 def test_infinities_and_nan(gpu, prefix, b, t):
     """Where they are seen they act as in torch's softmax and product; a query that
@@ -174,7 +175,7 @@ def test_infinities_and_nan(gpu, prefix, b, t):
         assert bool((heads[t - 2, 4:, 6].isfinite()).all())
         others = [i for i in range(D) if i not in (5, 6)]
         assert torch.equal(heads[t - 2:, 4:][..., others], old[t - 2:, 4:][..., others])
-    # the prefix's last row: an infinity beside its copies that fill the step up
+    # the prefix's last row: an infinity, and what fills the step up behind it
     pv[1, prefix - 1, 9], pk[1, prefix - 2, 0] = -math.inf, 0.0
     got = kernels.shared_prefix_attention(q, pk, pv, k, v, lens, SCALE).view(b, t, 8, D)
     assert bool((got[:, :, 4:, 9] == -math.inf).all())
@@ -185,8 +186,8 @@ def test_infinities_and_nan(gpu, prefix, b, t):
 
 
 def test_last_own_row_infinite(gpu):
-    """The rows past a request's last are stood in for by that row, whose infinity stays one."""
-    for case in ((3, 1, 8, 2, 64, 45), (3, 1, 8, 2, 900, 45), (40, 1, 8, 2, 900, 45)):
+    """What stands for the rows past a request's last does not make a NaN of its infinity."""
+    for case in ((3, 1, 8, 2, 64, 45), (3, 1, 8, 2, 900, 45), (40, 1, 8, 2, 900, 45), (50, 1, 8, 2, 900, 45)):
         q, pk, pv, k, v, lens = _request(*case, seed=6)
         lens.fill_(37)
         k[:, :, :37], v[:, :, :37] = 0.1, 0.5
@@ -196,7 +197,7 @@ def test_last_own_row_infinite(gpu):
         assert bool(got[..., [i for i in range(D) if i != 2]].isfinite().all())
 
 
-@pytest.mark.parametrize("case", [(3, 2, 8, 2, 70, 50), (3, 2, 8, 2, 700, 300), (40, 1, 8, 2, 700, 300)])
+@pytest.mark.parametrize("case", [(3, 2, 8, 2, 70, 50), (3, 2, 8, 2, 700, 300), (40, 1, 8, 2, 700, 300), (60, 1, 8, 2, 700, 300)])
 def test_strides(gpu, case):
     """Caches with rows of all heads together, a layer of an ArenaKVCache, one
     request's rows for all, q before its transposition, a given output."""
@@ -262,7 +263,7 @@ def test_empty_batch(gpu):
     assert kernels.shared_prefix_attention(q[:, :, :0], pk, pv, k, v, lens, SCALE).shape == (2, 0, 8 * D)
 
 
-@pytest.mark.parametrize("case", [(3, 1, 32, 8, 200, 100), (3, 4, 32, 8, 700, 300), (40, 1, 32, 8, 700, 300)])
+@pytest.mark.parametrize("case", [(3, 1, 32, 8, 200, 100), (3, 4, 32, 8, 700, 300), (40, 1, 32, 8, 700, 300), (60, 1, 32, 8, 700, 300)])
 def test_captured_and_on_two_streams(gpu, case):
     """Replays follow lens and the rows as they are then; a batch grows row by
     row; calls on two streams and two graphs share nothing."""

@@ -19,6 +19,7 @@ INVALID, WORKSPACE = -1, -4
     (dict(t=0), INVALID), (dict(p=-1), INVALID), (dict(s=-1), INVALID), (dict(b=1 << 20, t=1 << 10), INVALID),
     (dict(b=1 << 19, s=1 << 20), INVALID), (dict(p_row=120), INVALID), (dict(p_row=132), INVALID), (dict(row=64), INVALID),
     (dict(row=132), INVALID), (dict(p=1 << 23), INVALID), (dict(s=1 << 23), INVALID), (dict(p=1 << 20, p_row=1024), INVALID),
+    (dict(p_row=1 << 22), INVALID), (dict(row=1 << 22), INVALID),
     (dict(q_b=-8), INVALID), (dict(q_h=4), INVALID), (dict(q_t=12), INVALID), (dict(p_head=-8), INVALID),
     (dict(batch=4), INVALID), (dict(head=2), INVALID), (dict(q=0), INVALID), (dict(q=FAKE + 8), INVALID), (dict(pk=0), INVALID),
     (dict(pv=FAKE + 8), INVALID), (dict(k=0), INVALID), (dict(v=FAKE + 2), INVALID), (dict(lens=None), INVALID),
