@@ -24,6 +24,14 @@
 // the workspace; the second adds the partials in order.  adapter_plan chooses,
 // and the rows of a group: 64 share an adapter's tiles among four times the
 // rows, 16 keep a small batch's groups small.
+//
+// Bound by bytes for many rows or adapters, by the chain x, A, h, B, z for few:
+//   1 row, o (2560 x 4096), rank 8                        5.0 us
+//   16 rows, QKV (6144 x 2560), 16 of rank 16             7.5 us (4.1 MB)
+//   64 rows, down (2560 x 9728), 32 of rank 64           15.5 us (52 MB, most of
+//     them A, which the first launch reads in 10.3)
+//   2000 rows, gate_up (19456 x 2560), 8 of rank 32        44 us (135 MB: the first
+//     launch 7.6, the second 36.3 for 117 MB, 3.2 TB/s; a copy reaches 4.8)
 
 #include <hip/hip_runtime.h>
 

