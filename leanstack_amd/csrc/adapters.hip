@@ -26,8 +26,8 @@
 // rows, 16 keep a small batch's groups small.
 //
 // Bound by bytes for many rows or adapters, by the chain x, A, h, B, z for few:
-//   1 row, o (2560 x 4096), rank 8                        5.0 us
-//   16 rows, QKV (6144 x 2560), 16 of rank 16             7.5 us (4.1 MB)
+//   1 row, o (2560 x 4096), rank 8                        5.1 us
+//   16 rows, QKV (6144 x 2560), 24 of rank 16             6.3 us (4.1 MB)
 //   64 rows, down (2560 x 9728), 32 of rank 64           15.5 us (52 MB, most of
 //     them A, which the first launch reads in 10.3)
 //   2000 rows, gate_up (19456 x 2560), 8 of rank 32        44 us (135 MB: the first
@@ -48,6 +48,7 @@ typedef unsigned int u32x2_t __attribute__((ext_vector_type(2)));
 
 constexpr int kWaves = 8;
 constexpr int kThreads = kWaves * 64;
+constexpr int kXcds = 8;
 constexpr unsigned kRawBufferDword3 = 0x00020000u;
 // A buffer offset past every row: the load returns zero without a memory access.
 constexpr unsigned kOutOfRange = 0x80000000u;
@@ -280,17 +281,32 @@ __device__ __forceinline__ float half_of(const bf16x8_t& y, int half, int i) { r
 // Blocks [first, last) of share i of n.
 __device__ __forceinline__ int share_begin(int total, int i, int n) { return (int)((long long)total * i / n); }
 
+// Whether the column ranges of a group, which all read its A, go to one XCD's L2 (workgroups
+// go to the XCDs by turns): of up to 16 rows in one launch, with a slot or more for each
+// XCD.  16 rows with 16 adapters, o, rank 16: 9.0 -> 6.3 us, rank 32 12.3 -> 7.7,
+// gate_up, rank 16 9.3 -> 7.9.  Several tiles leave XCDs idle where rows name few
+// adapters (100 rows, gate_up: 17.5 -> 21.2).
+__host__ __device__ inline bool by_xcd(const AdapterArgs& a, bool two) {
+  return !two && a.tiles == 1 && a.slots >= kXcds;
+}
+
 // A decode batch: 16 rows and one of the adapters that they name.  Grid: (tile,
-// slot, column range), the range fastest.
+// slot, column range), the range fastest, or with by_xcd the slot's last three bits.
 template <int RT, bool SILU, bool TWO>
 __global__ __launch_bounds__(kThreads) void adapter_group_kernel(AdapterArgs a) {
   constexpr int CB = 1;
   __shared__ f32x4_t part[TWO ? 1 : kWaves][RT][64];
   __shared__ bf16x8_t hs[RT][64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  int id = blockIdx.x;
-  const int range = id % a.ranges;
-  id /= a.ranges;
+  int id = blockIdx.x, range;
+  if (by_xcd(a, TWO)) {
+    range = id / kXcds % a.ranges;
+    id = id / kXcds / a.ranges * kXcds + id % kXcds;
+    if (id >= a.slots) return;
+  } else {
+    range = id % a.ranges;
+    id /= a.ranges;
+  }
   const int tile = id / a.slots, slot = id % a.slots;
   const int m0 = tile * 16;
   const Group grp = find_group<CB>(a, m0, slot);
@@ -460,7 +476,8 @@ hipError_t launch_silu(const AdapterArgs& a, int rows, hipStream_t stream) {
   const unsigned tiles = (unsigned)a.tiles, groups = tiles * a.slots;
   const dim3 block(kThreads);
   if (rows == 16 && a.splits == 0) {
-    launch_kernel(adapter_group_kernel<RT, SILU, false>, dim3(groups * a.ranges), block, 0, stream, a);
+    const unsigned whole = by_xcd(a, false) ? (groups + kXcds - 1) / kXcds * kXcds : groups;
+    launch_kernel(adapter_group_kernel<RT, SILU, false>, dim3(whole * a.ranges), block, 0, stream, a);
     return hipGetLastError();
   }
   if (rows == 16)

@@ -174,9 +174,11 @@ constexpr bool adapter_rank_supported(int rank_tiles) {
 // Up to 128 rows a decode batch is expected, whose rows each name an adapter of
 // their own: tiles of 16 rows and a workgroup per (adapter named, column range), in
 // one launch unless reading A anew for every range (from L2) costs more than a
-// launch: QKV (K = 2560, 24 ranges) with 16 rows and rank 16 7.5 us in one launch,
-// 9 in two; the down projection (K = 9728) with 64 rows and rank 64 16.1 us in
-// two, over 30 in one.
+// launch.  In one and in two launches, us:
+//   1 tile (its ranges share an L2): QKV (K = 2560) 16 rows, rank 16 6.7, 8.6; o (4096), rank 32 7.7, 8.5;
+//     1 row 6.7, 6.8; QKV, rank 64 14.3, 11.2
+//   several: QKV, 64 rows, rank 16 9.8, 10.2; rank 32 12.8, 11.7; o, rank 16 11.3, 10.1;
+//     rank 32 15.8, 11.1
 // Above, prompts, whose neighbouring rows mostly name the same: 64 rows share an adapter's
 // tiles, and the second launch takes y once whatever its rows name.  Slots beyond
 // the first few would be workgroups that find nothing to do (2000 rows of gate_up
@@ -199,7 +201,7 @@ constexpr AdapterPlan adapter_plan(int M, int N, int K, int rank_tiles, int coun
   const int most = (adapter_blocks(N, silu) + 7) / 8;
   p.ranges = wanted > most ? most : wanted;
   const long long again = (long long)K * rank_tiles * 32;  // bytes of A per workgroup
-  if (!decode || (p.ranges > 1 && again > 256 * 1024)) {
+  if (!decode || (p.ranges > 1 && again > (p.tiles == 1 ? 256 : 96) * 1024)) {
     const int most_splits = (K / kTileK + 7) / 8;
     p.splits = wanted > most_splits ? most_splits : wanted;
     if (p.splits > kAdapterMaxSplits) p.splits = kAdapterMaxSplits;
