@@ -5,10 +5,13 @@ eager ones."""
 
 from __future__ import annotations
 
+from concurrent.futures import ThreadPoolExecutor
+
 import pytest
 import torch
 
 from leanstack_amd import _lib, kernels
+from leanstack_amd.adapters import AdapterStore
 from leanstack_amd.kv_cache import ArenaKVCache
 from leanstack_amd.layout import PackedWeight
 from tests import test_gpu_adapters as adapters_of
@@ -192,3 +195,32 @@ def test_captured_steps_are_the_eager_ones(gpu, b, prefix):
         for x, y in zip(req.parts(), eager.parts()):
             assert torch.equal(x.nan_to_num(7.0) if x.is_floating_point() else x,
                                y.nan_to_num(7.0) if y.is_floating_point() else y)
+
+
+@pytest.mark.parametrize("default", ["cpu", "cuda:0"])
+def test_default_device_and_threads(gpu, default):
+    """A default device changes nothing, and threads with streams of their own do
+    not meet."""
+    model = Model(300)
+    tokens = torch.arange(12, device=DEV)[:, None] * 17 % VOCAB
+    values, token = _step(model, Requests(12, 40), tokens)
+    req = Requests(12, 40)
+    with torch.device(default):
+        store = AdapterStore(COUNT, *SHAPES["o"], RANK, device=DEV)
+        for slot, (a, b, s) in enumerate(model.adapters[0]["o"]):
+            store.load(slot, a, b, s)
+        assert torch.equal(store.a_tiles, model.stores[0]["o"].a_tiles)
+        assert torch.equal(store.b_tiles, model.stores[0]["o"].b_tiles)
+        got = _step(model, req, tokens)
+    assert torch.equal(got[0], values) and torch.equal(got[1], token)
+    torch.cuda.synchronize()
+
+    def work(_):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            results = [_step(model, Requests(12, 40), tokens) for _ in range(4)]
+            torch.cuda.current_stream().synchronize()
+        return results
+
+    with ThreadPoolExecutor(3) as pool:
+        for results in pool.map(work, range(3)):
+            assert all(torch.equal(v, values) and torch.equal(t, token) for v, t in results)
