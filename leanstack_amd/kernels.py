@@ -34,6 +34,11 @@ def _on(device: torch.device):
     return _NO_SWITCH if torch._C._cuda_getDevice() == device.index else torch.cuda.device(device)
 
 
+def _on_index(index: int):
+    """_on() for a device's index."""
+    return _NO_SWITCH if torch._C._cuda_getDevice() == index else torch.cuda.device(index)
+
+
 def _require_device(t: torch.Tensor, what: str) -> None:
     if not t.is_cuda:
         raise ValueError(f"{what} must be a GPU tensor, got device {t.device}")
@@ -572,12 +577,12 @@ def shared_prefix_attention(q: torch.Tensor, prefix_k: torch.Tensor, prefix_v: t
         q_strides = q.stride()
     nbytes = _prefix_workspace_bytes(b, t, n_q, n_kv, prefix, rows)
     workspace = q.new_empty((nbytes // 2,)) if nbytes else None
-    with _on(q.device):
+    with _on_index(index):
         status = _lib.load().lsk_prefix_attention_bf16(
             q.data_ptr(), q_strides[0], q_strides[1], q_strides[2], b, t, n_q, n_kv, d, prefix_k.data_ptr(),
             prefix_v.data_ptr(), prefix_strides[0], prefix_strides[1], prefix, k.data_ptr(), v.data_ptr(), strides[0],
             strides[1], strides[2], rows, lens_at, float(scale), out.data_ptr(), _ptr(workspace), nbytes,
-            stream_handle())
+            torch._C._cuda_getCurrentRawStream(index))
     _lib.check(status, "lsk_prefix_attention_bf16")
     return out
 
@@ -730,18 +735,21 @@ def lora_add(y: torch.Tensor, x: torch.Tensor, store: AdapterStore, index: torch
         if _overlap(out, x2) or (_overlap(out, y2) and (silu or out.data_ptr() != y2.data_ptr() or not y2.is_contiguous())):
             raise ValueError("out must be y itself (contiguous, EPI_NONE) or overlap neither y nor x")
     _require_device(y, "y")
-    dev = _one_device(y, (x, "x"), (store.a_tiles, "store"), (index, "index"), (out, "out"))
+    at = y.get_device()
+    if not (x.get_device() == store.a_tiles.get_device() == index.get_device() == at) or \
+            (out is not None and out.get_device() != at):
+        _one_device(y, (x, "x"), (store.a_tiles, "store"), (index, "index"), (out, "out"))
     if out is None:
         out = y.new_empty((*y.shape[:-1], n_out))
     if m == 0:
         return out
     nbytes = _lora_workspace_bytes(m, n, k, store.rank_tiles, store.count, epilogue)
     workspace = y.new_empty((nbytes // 2,)) if nbytes else None
-    with _on(dev):
+    with _on_index(at):
         status = _lib.load().lsk_lora_add_bf16(
             y2.data_ptr(), m, n, ldy, x2.data_ptr(), k, ldx, store.a_tiles.data_ptr(), store.b_tiles.data_ptr(),
             store.scales.data_ptr(), store.ranks.data_ptr(), store.count, store.rank_tiles, index.data_ptr(), epilogue,
-            out.data_ptr(), _ptr(workspace), nbytes, stream_handle())
+            out.data_ptr(), _ptr(workspace), nbytes, torch._C._cuda_getCurrentRawStream(at))
     _lib.check(status, "lsk_lora_add_bf16")
     return out
 
@@ -885,16 +893,16 @@ def constrain_logits(logits: torch.Tensor, *, history: torch.Tensor | None = Non
         if m and _overlap(out, logits) and not (src is logits and out.data_ptr() == src.data_ptr() and ld == v):
             raise ValueError("out must be the logits themselves (contiguous) or not overlap them")
     _require_device(logits, "logits")
-    dev = logits.device
     tokens = logits.new_empty((m,), dtype=torch.long)
     if m == 0:
         return out, tokens
-    with _on(dev):
-        workspace = _constrain_workspace(dev, m, v)
+    with _on_index(index):
+        stream = torch._C._cuda_getCurrentRawStream(index)
+        workspace = _constrain_workspace(logits, stream, m, v)
         status = _lib.load().lsk_constrain_logits(
             src.data_ptr(), mode, m, v, ld, past, history_ld, history_len, lens, prompts, rho, alpha_f, alpha_p, ids,
             values, bias_ld, bias_count, words, allowed_ld, out.data_ptr(), tokens.data_ptr(), workspace.data_ptr(),
-            workspace.numel(), stream_handle())
+            workspace.numel(), stream)
     _lib.check(status, "lsk_constrain_logits")
     return out, tokens
 
@@ -903,16 +911,17 @@ def constrain_logits(logits: torch.Tensor, *, history: torch.Tensor | None = Non
 _constrain_workspaces: dict[tuple[int, int], torch.Tensor] = {}
 
 
-def _constrain_workspace(device: torch.device, m: int, v: int) -> torch.Tensor:
-    """A workspace that is zero: the stream's own, which every call leaves zero, or
-    under capture the graph's own, so that replays share none with eager calls."""
+def _constrain_workspace(logits: torch.Tensor, stream: int, m: int, v: int) -> torch.Tensor:
+    """A workspace that is zero: the current stream's own, which every call leaves zero,
+    or under capture the graph's own, so that replays share none with eager calls."""
     nbytes = _constrain_workspace_bytes(m, v)
     if torch.cuda.is_current_stream_capturing():
-        return torch.empty(nbytes, device=device, dtype=torch.uint8).zero_()
-    key = (device.index, stream_handle())
+        return logits.new_empty((nbytes,), dtype=torch.uint8).zero_()
+    key = (logits.get_device(), stream)
     workspace = _constrain_workspaces.get(key)
     if workspace is None or workspace.numel() < nbytes:
-        workspace = _constrain_workspaces[key] = torch.zeros(max(nbytes, 4096), device=device, dtype=torch.uint8)
+        workspace = logits.new_empty((max(nbytes, 4096),), dtype=torch.uint8).zero_()
+        _constrain_workspaces[key] = workspace
     return workspace
 
 
