@@ -187,6 +187,24 @@ struct AdapterPlan {
   int rows, tiles, slots, ranges, splits;
 };
 constexpr int adapter_blocks(int N, bool silu) { return silu ? (N + 63) / 64 : (N + 31) / 32; }
+// Column ranges of `tiles` 64-row tiles in the second launch.  A workgroup takes some 4 us
+// until y streams, then about 13 bytes a nanosecond (a CU's share of 3.3 TB/s), a
+// block per wave at a time; a CU runs one, so a few workgroups more than CUs would
+// cost a whole round: gate_up, rank 32, with one round and with two: 512 rows 13.2, 20.5
+// us, 1024 rows 18.2, 23.9; o, 2000 rows 9.5, 12.0.
+constexpr int adapter_rows_ranges(int tiles, int N, bool silu) {
+  const int blocks = adapter_blocks(N, silu), most = (blocks + 7) / 8;
+  const long long pass_ns = 8 * 64 * (silu ? 192 : 128) / 13;
+  int best = 1;
+  long long least = 0;
+  for (int r = 1; r <= most; ++r) {
+    const long long rounds = ((long long)tiles * r + 255) / 256, passes = ((blocks + r - 1) / r + 7) / 8;
+    const long long cost = rounds * (4000 + passes * pass_ns);
+    if (r == 1 || cost <= least) best = r, least = cost;
+    if (rounds > 4) break;
+  }
+  return best;
+}
 constexpr AdapterPlan adapter_plan(int M, int N, int K, int rank_tiles, int count, bool silu) {
   const bool decode = M <= 128;
   AdapterPlan p = {decode ? 16 : 64, 0, 0, 1, 0};
@@ -199,7 +217,7 @@ constexpr AdapterPlan adapter_plan(int M, int N, int K, int rank_tiles, int coun
   const int busy = p.tiles * (decode ? p.slots : 1);
   const int wanted = (512 + busy - 1) / busy;
   const int most = (adapter_blocks(N, silu) + 7) / 8;
-  p.ranges = wanted > most ? most : wanted;
+  p.ranges = !decode ? adapter_rows_ranges(p.tiles, N, silu) : wanted > most ? most : wanted;
   const long long again = (long long)K * rank_tiles * 32;  // bytes of A per workgroup
   if (!decode || (p.ranges > 1 && again > (p.tiles == 1 ? 256 : 96) * 1024)) {
     const int most_splits = (K / kTileK + 7) / 8;
