@@ -88,11 +88,14 @@ constexpr int ceil_div(long long a, long long b) { return (int)((a + b - 1) / b)
 //   17.6 with two), and half a CU's worth of own items.
 // - Of the 512 places of shared items the prefix gets its share of all key rows to be
 //   read, so that it does not finish long before the own rows do, whose reads bound
-//   them: 64x1 8191+1088 47 us with 7 parts, 52 with 16; 48x4 16000+320, where the prefix
-//   is most of the work, 82 us with 10 parts, 88 with 5.
+//   them: 64x1 8191+1088 47 us with 7 parts, 48 with 12, 52 with 16; 48x4 16000+320, where it
+//   is most of the work, 82 us with 10 parts, 88 with 5.  But not fewer than 192: how
+//   many of the S rows are written only the device knows (64x1 8191+4096 of which 100
+//   29 us, with the share alone 87; the same with 1088 of 1088 61, 59).
 constexpr int kPrefixJointRows = 768;
 constexpr int kPrefixJointItems = 256;
 constexpr int kPrefixSplitRows = 192;
+constexpr int kPrefixLeastPlaces = 192;
 constexpr PrefixPlan prefix_plan(int B, int T, int n_q, int n_kv, int P, int S) {
   PrefixPlan p = {false, false, 0, 128, 0, ceil_div((long long)T * (n_q / n_kv), 32), 128, 0};
   const long long rows = (long long)B * T * (n_q / n_kv);
@@ -108,7 +111,8 @@ constexpr PrefixPlan prefix_plan(int B, int T, int n_q, int n_kv, int P, int S) 
     const long long items = (long long)n_kv * p.prefix_tiles;
     const long long prefix = (long long)p.prefix_tiles * P, own = (long long)B * S;
     const long long most = (p.shared ? 512 : 256) / items;
-    const long long share = p.shared ? ceil_div(512 * prefix, (prefix + own) * items) : most;
+    const long long even = p.shared ? ceil_div(512 * prefix, (prefix + own) * items) : most;
+    const long long share = even * items < kPrefixLeastPlaces ? ceil_div(kPrefixLeastPlaces, items) : even;
     const long long wanted = share < most ? share : most;
     const int chunk = ceil_div(ceil_div(P, wanted > 1 ? wanted : 1), unit) * unit;
     p.prefix_chunk = chunk < least ? least : chunk;

@@ -42,7 +42,7 @@
 // a graph):
 //   1x5 300+64      9.2 us, one launch: latency (the bytes are 0.3 us)
 //   12x1 1024+512  10.6 us, of it 4 the second launch
-//   64x1 8191+1088  47 us: 166 MB, 4.2 TB/s in the first launch (a copy reaches 4.8)
+//   64x1 8191+1088  48 us: 166 MB, 4.1 TB/s in the first launch (a copy reaches 4.8)
 //   48x4 16000+320  82 us: 51 GFLOP, 760 TFLOP/s in the first launch (a large matrix
 //     product reaches 1214).  A step of a wave is 512 cycles of MFMA, some 500 of the
 //     softmax's VALU and 128 of a CU's LDS: two waves per SIMD overlap them in part.
