@@ -100,7 +100,8 @@ constexpr PrefixPlan prefix_plan(int B, int T, int n_q, int n_kv, int P, int S) 
   PrefixPlan p = {false, false, 0, 128, 0, ceil_div((long long)T * (n_q / n_kv), 32), 128, 0};
   const long long rows = (long long)B * T * (n_q / n_kv);
   const long long own_items = (long long)n_kv * B * p.own_tiles;
-  if ((long long)P + S <= kPrefixJointRows && own_items <= kPrefixJointItems) {
+  // (with no key row at all there are no parts to add up)
+  if (((long long)P + S <= kPrefixJointRows && own_items <= kPrefixJointItems) || (P == 0 && S == 0)) {
     p.joint = true;
     return p;
   }
