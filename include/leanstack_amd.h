@@ -328,7 +328,8 @@ int lsk_lm_head_argmax_noalloc_bf16(const void* w_packed, int layout_id, int V, 
                                     float* logits_opt, int logits_mode, long long* out_idx,
                                     void* hip_stream);
 
-/* Device workspace of lsk_prefix_attention_bf16 (any contents; 0: none). */
+/* Device workspace of lsk_prefix_attention_bf16 (any contents; 0: none, or sizes
+ * that it refuses). */
 size_t lsk_prefix_attention_workspace_bytes(int B, int T, int n_q, int n_kv, int P, int S);
 
 /* Attention of a batch of requests that share a prefix: query token t of request
@@ -363,7 +364,8 @@ int lsk_prefix_attention_bf16(const void* q, long long q_batch_stride, long long
                               const int* lens, float scale, void* out, void* workspace, size_t ws_bytes,
                               void* hip_stream);
 
-/* Device workspace of lsk_lora_add_bf16 for these sizes (any contents; 0: none). */
+/* Device workspace of lsk_lora_add_bf16 for these sizes (any contents; 0: none, or
+ * sizes that it refuses). */
 size_t lsk_lora_workspace_bytes(int M, int N, int K, int rank_tiles, int count, int epilogue);
 
 /* Low-rank adapters of many requests beside a shared projection: for row m with

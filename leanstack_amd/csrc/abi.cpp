@@ -395,7 +395,7 @@ int lsk_rmsnorm_lm_head_argmax_bf16(const void* w_packed, int layout_id, int V, 
 extern "C" {
 
 size_t lsk_prefix_attention_workspace_bytes(int B, int T, int n_q, int n_kv, int P, int S) {
-  if (B < 1 || T < 1 || n_kv < 1 || n_q < n_kv || n_q % n_kv != 0 || P < 0 || S < 0) return 0;
+  if (lsk::check_prefix_sizes(B, T, n_q, n_kv, P, S) != LSK_OK) return 0;
   return (size_t)lsk::prefix_workspace_bytes(lsk::prefix_plan(B, T, n_q, n_kv, P, S), B, T, n_q);
 }
 
@@ -459,7 +459,7 @@ int lsk_prefix_attention_bf16(const void* q, long long q_batch_stride, long long
 extern "C" {
 
 size_t lsk_lora_workspace_bytes(int M, int N, int K, int rank_tiles, int count, int epilogue) {
-  if (M < 1 || N < 1 || K < lsk::kTileK || count < 1 || !lsk::adapter_rank_supported(rank_tiles)) return 0;
+  if (lsk::check_lora_sizes(M, N, K, rank_tiles, count, epilogue) != LSK_OK) return 0;
   return (size_t)lsk::adapter_workspace_bytes(lsk::adapter_plan(M, N, K, rank_tiles, count, epilogue == LSK_EPI_SILU_MUL), rank_tiles);
 }
 

@@ -190,24 +190,33 @@ int check_constrain_args(const void* logits, int logits_mode, int M, int V, long
   return LSK_OK;
 }
 
+int check_prefix_sizes(int B, int T, int n_q, int n_kv, int P, int S) {
+  if (n_kv < 1 || n_q < n_kv || n_q % n_kv != 0)
+    return fail(LSK_ERR_INVALID, "n_q=%d must be a multiple of n_kv=%d", n_q, n_kv);
+  if (B < 1 || T < 1 || P < 0 || S < 0) return fail(LSK_ERR_INVALID, "B=%d, T=%d, P=%d, S=%d rows", B, T, P, S);
+  // Query rows and grids are counted in 32 bits, key rows addressed with 31 (the plan
+  // is made of sizes that keep to both).
+  const long long most = 0xffffffffLL / kPrefixThreads;
+  if ((long long)B * T > most || (long long)B * T * n_q > most)
+    return fail(LSK_ERR_INVALID, "B=%d, T=%d, n_q=%d: too many query rows", B, T, n_q);
+  constexpr int most_rows = ((1 << 30) - 1) / kAttnHeadDim;
+  if (P > most_rows || S > most_rows)
+    return fail(LSK_ERR_INVALID, "%d and %d rows: a head's rows must stay below 2^31 bytes", P, S);
+  const PrefixPlan p = prefix_plan(B, T, n_q, n_kv, P, S);
+  const long long prefix_items = (long long)n_kv * p.prefix_tiles * p.prefix_parts;
+  const long long own_items = (long long)n_kv * B * p.own_tiles;
+  if (own_items > most || prefix_items > most || prefix_items + own_items * (p.joint ? 1 : p.own_parts) > most)
+    return fail(LSK_ERR_INVALID, "B=%d, T=%d, n_q=%d over %d + %d rows: too many items", B, T, n_q, P, S);
+  return LSK_OK;
+}
+
 int check_prefix_args(const void* q, long long q_batch, long long q_head, long long q_token, int B, int T, int n_q,
                       int n_kv, int head_dim, const void* prefix_k, const void* prefix_v, long long prefix_head,
                       int prefix_row, int P, const void* k, const void* v, long long batch, long long head, int row,
                       int S, const int* lens, float scale, const void* out) {
   if (head_dim != kAttnHeadDim)
     return fail(LSK_ERR_INVALID, "head_dim=%d: the attention kernel is built for %d", head_dim, kAttnHeadDim);
-  if (n_kv < 1 || n_q < n_kv || n_q % n_kv != 0)
-    return fail(LSK_ERR_INVALID, "n_q=%d must be a multiple of n_kv=%d", n_q, n_kv);
-  if (B < 1 || T < 1 || P < 0 || S < 0) return fail(LSK_ERR_INVALID, "B=%d, T=%d, P=%d, S=%d rows", B, T, P, S);
-  // Query rows and grids are counted in 32 bits, key rows addressed with 31.
-  const long long most = 0xffffffffLL / kPrefixThreads;
-  if ((long long)B * T > most || (long long)B * T * n_q > most)
-    return fail(LSK_ERR_INVALID, "B=%d, T=%d, n_q=%d: too many query rows", B, T, n_q);
-  const PrefixPlan p = prefix_plan(B, T, n_q, n_kv, P, S);
-  const long long prefix_items = (long long)n_kv * p.prefix_tiles * p.prefix_parts;
-  const long long own_items = (long long)n_kv * B * p.own_tiles;
-  if (own_items > most || prefix_items > most || prefix_items + own_items * (p.joint ? 1 : p.own_parts) > most)
-    return fail(LSK_ERR_INVALID, "B=%d, T=%d, n_q=%d over %d + %d rows: too many items", B, T, n_q, P, S);
+  if (int st = check_prefix_sizes(B, T, n_q, n_kv, P, S)) return st;
   // (a few steps past the last row are addressed, out of range: their offsets must not wrap)
   if (prefix_row < head_dim || row < head_dim || prefix_row % 8 != 0 || row % 8 != 0 ||
       prefix_row > kMaxActivationStride || row > kMaxActivationStride)
@@ -230,9 +239,7 @@ int check_prefix_args(const void* q, long long q_batch, long long q_head, long l
   return LSK_OK;
 }
 
-int check_lora_args(const void* y, int M, int N, int ldy, const void* x, int K, int ldx, const void* a_tiles,
-                    const void* b_tiles, const float* scale, const int* ranks, int count, int rank_tiles,
-                    const int* index, int epilogue, const void* out) {
+int check_lora_sizes(int M, int N, int K, int rank_tiles, int count, int epilogue) {
   if (epilogue != LSK_EPI_NONE && epilogue != LSK_EPI_SILU_MUL)
     return fail(LSK_ERR_INVALID, "epilogue %d: the adapters take none or SiLU*up", epilogue);
   if (int st = check_shape(epilogue == LSK_EPI_SILU_MUL ? LSK_LAYOUT_MFMA16X32_GATEUP : LSK_LAYOUT_MFMA16X32, N, K))
@@ -246,6 +253,13 @@ int check_lora_args(const void* y, int M, int N, int ldy, const void* x, int K, 
   const long long groups = (long long)p.tiles * p.slots;
   if (groups * (p.ranges > p.splits ? p.ranges : p.splits) > 0xffffffffLL / kAdapterThreads)
     return fail(LSK_ERR_INVALID, "M=%d rows are too many", M);  // a grid's threads are counted in 32 bits
+  return LSK_OK;
+}
+
+int check_lora_args(const void* y, int M, int N, int ldy, const void* x, int K, int ldx, const void* a_tiles,
+                    const void* b_tiles, const float* scale, const int* ranks, int count, int rank_tiles,
+                    const int* index, int epilogue, const void* out) {
+  if (int st = check_lora_sizes(M, N, K, rank_tiles, count, epilogue)) return st;
   if (ldx < K || ldx % 8 != 0 || ldx > kMaxActivationStride)
     return fail(LSK_ERR_INVALID, "ldx=%d must be a multiple of 8, K=%d..%d", ldx, K, kMaxActivationStride);
   if (ldy < N || ldy % 8 != 0 || ldy > kMaxActivationStride)

@@ -132,7 +132,9 @@ constexpr unsigned long long prefix_workspace_bytes(const PrefixPlan& p, int B, 
   return (unsigned long long)(p.prefix_parts + p.own_parts) * B * T * n_q * (kAttnHeadDim + 2) * 4ull;
 }
 
-// Argument rules of lsk_prefix_attention_bf16 (all but the workspace's size).
+// The sizes that prefix_plan takes, and argument rules of lsk_prefix_attention_bf16
+// (all but the workspace's size).
+int check_prefix_sizes(int B, int T, int n_q, int n_kv, int P, int S);
 int check_prefix_args(const void* q, long long q_batch, long long q_head, long long q_token, int B, int T, int n_q,
                       int n_kv, int head_dim, const void* prefix_k, const void* prefix_v, long long prefix_head,
                       int prefix_row, int P, const void* k, const void* v, long long batch, long long head, int row,
@@ -152,7 +154,7 @@ constexpr int kConstrainCounterWords = 16;  // a row's counter has 64 bytes to i
 constexpr int constrain_slice(int M, int V) {
   const int least = (V + kConstrainMaxSlice - 1) / kConstrainMaxSlice;
   const int most = V / 2048 < 32 ? V / 2048 + 1 : 32;
-  const int wanted = (1024 + M - 1) / M;
+  const int wanted = M >= 1024 ? 1 : (1024 + M - 1) / M;
   const int some = wanted > most ? most : wanted;
   const int slices = some < least ? least : some;
   const int slice = ((V + slices - 1) / slices + 63) / 64 * 64;
@@ -235,7 +237,9 @@ constexpr unsigned long long adapter_workspace_bytes(const AdapterPlan& p, int r
   return (unsigned long long)p.splits * (unsigned long long)p.tiles * (unsigned long long)(rank_tiles * p.rows) * 64;
 }
 
-// Argument rules of lsk_lora_add_bf16 (all but the workspace's size).
+// The sizes that adapter_plan takes, and argument rules of lsk_lora_add_bf16 (all but the
+// workspace's size).
+int check_lora_sizes(int M, int N, int K, int rank_tiles, int count, int epilogue);
 int check_lora_args(const void* y, int M, int N, int ldy, const void* x, int K, int ldx, const void* a_tiles,
                     const void* b_tiles, const float* scale, const int* ranks, int count, int rank_tiles,
                     const int* index, int epilogue, const void* out);
