@@ -44,7 +44,8 @@ def _pack_b(b: torch.Tensor, gate_up: bool) -> torch.Tensor:
 class AdapterStore:
     """`count` adapters of rank up to `rank` for projections of [n, k] weights,
     all empty (they add nothing) until loaded.  gate_up: the projection is a
-    fused [gate; up] one, whose SiLU(gate) * up is taken after the adapters."""
+    fused [gate; up] one, whose SiLU(gate) * up is taken after the adapters.  A
+    store holds values: of adapters that require gradients, no graph."""
 
     def __init__(self, count: int, n: int, k: int, rank: int, *, gate_up: bool = False,
                  device: torch.device | str = "cuda") -> None:
@@ -65,6 +66,7 @@ class AdapterStore:
     def device(self) -> torch.device:
         return self.a_tiles.device
 
+    @torch.no_grad()
     def load(self, slot: int, a: torch.Tensor, b: torch.Tensor, scale: float = 1.0) -> None:
         """Put A [r, k] and B [n, r] (bfloat16, r up to the store's rank; a
         gate_up B's gate rows first) into a slot, on the current stream."""
@@ -84,6 +86,7 @@ class AdapterStore:
         self.scales[slot:slot + 1].fill_(scale)
         self.ranks[slot:slot + 1].fill_(r)
 
+    @torch.no_grad()
     def load_parts(self, slot: int, parts: list[tuple[torch.Tensor, torch.Tensor]], scale: float = 1.0) -> None:
         """One adapter per part of a fused projection ((A, B) of q, k and v, or
         of gate and up, in the order of the fused rows): their ranks stand
@@ -93,6 +96,7 @@ class AdapterStore:
         a = torch.cat([pa for pa, _ in parts]).to(self.device)
         self.load(slot, a, torch.block_diag(*(pb for _, pb in parts)).to(device=self.device, dtype=a.dtype), scale)
 
+    @torch.no_grad()
     def clear(self, slot: int) -> None:
         """Empty a slot: rows that name it get nothing added."""
         if not 0 <= slot < self.count:
@@ -101,6 +105,7 @@ class AdapterStore:
         self.ranks[slot:slot + 1].fill_(0)
 
     @classmethod
+    @torch.no_grad()
     def of(cls, a: torch.Tensor, b: torch.Tensor, scales: torch.Tensor, *, gate_up: bool = False) -> "AdapterStore":
         """A store of adapters held as A [count, r, k] and B [count, n, r] with scales [count]."""
         if a.dim() != 3 or b.dim() != 3 or a.shape[0] != b.shape[0] or a.shape[1] != b.shape[2] \
