@@ -704,6 +704,11 @@ def _lora_workspace_bytes(m: int, n: int, k: int, rank_tiles: int, count: int, e
     return _lib.load().lsk_lora_workspace_bytes(m, n, k, rank_tiles, count, epilogue)
 
 
+def _check_index(index: torch.Tensor, m: int) -> None:
+    if index.dtype is not torch.int32 or index.numel() != m or not index.is_contiguous():
+        raise ValueError(f"index must be a contiguous int32 tensor of {m} values, got {index.dtype} {tuple(index.shape)}")
+
+
 def lora_add(y: torch.Tensor, x: torch.Tensor, store: AdapterStore, index: torch.Tensor, *,
              epilogue: int = _lib.EPI_NONE, out: torch.Tensor | None = None) -> torch.Tensor:
     """The rows' own low-rank adapters added to what a shared projection gave:
@@ -725,8 +730,7 @@ def lora_add(y: torch.Tensor, x: torch.Tensor, store: AdapterStore, index: torch
     x2, xm, ldx = _rows(x, k, "x")
     if xm != m:
         raise ValueError(f"x has {xm} rows, y has {m}")
-    if index.dtype is not torch.int32 or index.numel() != m or not index.is_contiguous():
-        raise ValueError(f"index must be a contiguous int32 tensor of {m} values, got {index.dtype} {tuple(index.shape)}")
+    _check_index(index, m)
     n_out = n // 2 if silu else n
     if out is not None:
         _check_out(out, m, n_out, torch.bfloat16)
@@ -768,6 +772,11 @@ def lora_linear(x: torch.Tensor, weight: PackedWeight, store: AdapterStore, inde
         raise ValueError("a gate_up weight takes a gate_up store and EPI_SILU_MUL, and no other does")
     if out is not None and (out.data_ptr() % 16 or _overlap(out, x)):
         raise ValueError("out must be 16-byte aligned and not overlap x")
+    # (lora_add's checks, in front of the projection: a refused call has written nothing)
+    if x.shape[-1] == weight.k:
+        _check_index(index, x.numel() // weight.k)
+    if not (store.a_tiles.get_device() == index.get_device() == x.get_device()):
+        _one_device(x, (store.a_tiles, "store"), (index, "index"))
     if epilogue == _lib.EPI_SILU_MUL:
         # the same tiles read as a plain weight give both halves, before SiLU, in packed order
         if residual is not None:
