@@ -504,7 +504,7 @@ def _key_rows(k: torch.Tensor, v: torch.Tensor, what: str) -> tuple[int, ...]:
     d = k.shape[-1]
     strides = k.stride()
     if (k.dtype is torch.bfloat16 is v.dtype and k.shape == v.shape and strides == v.stride() and strides[-1] == 1
-            and strides[-2] >= d and not (strides[0] | strides[1] | strides[-2]) & 7):
+            and d <= strides[-2] <= _lib.MAX_ACTIVATION_STRIDE and not (strides[0] | strides[1] | strides[-2]) & 7):
         return strides  # (the library checks the addresses)
     if k.dtype is not torch.bfloat16 or v.dtype is not torch.bfloat16 or k.shape != v.shape:
         raise ValueError(f"{what} must be bfloat16 tensors of one shape, got {k.dtype} {tuple(k.shape)} / {v.dtype} "
@@ -513,9 +513,10 @@ def _key_rows(k: torch.Tensor, v: torch.Tensor, what: str) -> tuple[int, ...]:
         return (0,) * (k.dim() - 2) + (d,)
     strides = [s if n > 1 else 0 for n, s in zip(k.shape[:-1], k.stride())]
     if strides != [s if n > 1 else 0 for n, s in zip(v.shape[:-1], v.stride())] or k.stride(-1) != 1 or v.stride(-1) != 1 \
-            or any(s % 8 for s in strides) or k.data_ptr() % 16 or v.data_ptr() % 16 or 0 < strides[-1] < d:
-        raise ValueError(f"{what} must have equal strides, multiples of 8, rows of unit stride and 16-byte alignment, got "
-                         f"strides {k.stride()} / {v.stride()}")
+            or any(s % 8 for s in strides) or k.data_ptr() % 16 or v.data_ptr() % 16 or 0 < strides[-1] < d \
+            or strides[-1] > _lib.MAX_ACTIVATION_STRIDE:
+        raise ValueError(f"{what} must have equal strides, multiples of 8 (of rows up to {_lib.MAX_ACTIVATION_STRIDE}), rows "
+                         f"of unit stride and 16-byte alignment, got strides {k.stride()} / {v.stride()}")
     if k.shape[-2] > 1 and strides[-1] == 0:
         raise ValueError(f"{what}: the rows must not repeat (stride 0)")
     strides[-1] = strides[-1] or d
@@ -540,8 +541,9 @@ def shared_prefix_attention(q: torch.Tensor, prefix_k: torch.Tensor, prefix_v: t
     ends).  Query t sees the prefix and the first lens - (T - 1 - t) own rows.  Rows
     behind the written ones are not read; a query that sees no row gives zeros.
     bfloat16, d = 128, q heads in groups of n_q / n_kv.  Caches are read in place at
-    any strides that are multiples of 8; lens is read on the device, so a captured
-    call follows it.  out: a contiguous [B, T, n_q * d] tensor."""
+    any strides that are multiples of 8 (rows up to 2^22 - 8 elements apart, a head's
+    rows below 2^31 bytes); lens is read on the device, so a captured call follows
+    it.  out: a contiguous [B, T, n_q * d] tensor."""
     if q.dim() != 4 or prefix_k.dim() != 3 or k.dim() != 4:
         raise ValueError(f"q, prefix_k / prefix_v and k / v must be [B, n_q, T, d], [n_kv, P, d] and [B, n_kv, S, d], got "
                          f"{tuple(q.shape)}, {tuple(prefix_k.shape)} and {tuple(k.shape)}")
