@@ -530,16 +530,27 @@ __device__ __forceinline__ void own_item(const PrefixArgs& a, int j, int b, int 
   if constexpr (CAUSAL) {
     // Infinite and NaN values of rows that only some query rows see: to those.
     const bool any = __syncthreads_or(special);
-    const int first = max(begin, least);
+    int first = max(begin, least);
+    asm("" : "+v"(first));  // (a vector register: scalar ones are short in the loops before)
     write_item<NW, true, JOINT>(a, st, slots, ms, ls, part, find,
                                 [&](const Query& q, int d, float sum, f32x4_t& o) __attribute__((always_inline)) {
       if (!any) return;
       for (int i = first; i < min(stop, written - (a.T - 1 - q.t)); ++i) {
-        const bf16x4_t v = *reinterpret_cast<const bf16x4_t*>(a.v + base + (size_t)i * a.k_row + d);
+        const unsigned row = (unsigned)i * (unsigned)a.k_row;  // (a head's rows span less than 2^30 values)
+        const bf16x4_t v = *reinterpret_cast<const bf16x4_t*>(a.v + base + (row + (unsigned)d));
+        // 0, or NaN for what is not finite.  A row whose key is not finite scores -inf, and 0
+        // times the value is NaN, too, or makes all of the query's output NaN.
+        float key = 0.f;
+#pragma unroll 1
+        for (int e = 0; e < D; e += 4) {
+          const bf16x4_t k = *reinterpret_cast<const bf16x4_t*>(a.k + base + (row + (unsigned)e));
+#pragma unroll
+          for (int u = 0; u < 4; ++u) key += static_cast<float>(k[u]) * 0.f;
+        }
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const float f = static_cast<float>(v[e]);
-          if (!(fabsf(f) < __builtin_huge_valf())) o[e] += sum != 0.f ? f : f * 0.f;  // (of no weight: NaN)
+          if (!(fabsf(f) < __builtin_huge_valf())) o[e] += sum != 0.f ? f + key : f * 0.f;  // (of no weight: NaN)
         }
       }
     });
