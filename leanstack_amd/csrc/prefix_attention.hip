@@ -185,21 +185,14 @@ __device__ __forceinline__ bf16x8_t k_operand(lds_byte_t* k, const Lane& a, int 
   return *reinterpret_cast<__attribute__((address_space(3))) const bf16x8_t*>(k + (a.k_read ^ (unsigned)(ks << 5)));
 }
 
-// S^T = K Q^T of N steps of key rows.  A product waits twice its time for the one that it
-// adds to: N products by turns, of one step two half sums.
-template <int N>
-__device__ __forceinline__ void step_scores(lds_byte_t* k, const Lane& a, const bf16x8_t (&qf)[8], f32x16_t (&s)[N]) {
-  constexpr int kChains = N > 1 ? N : 2;
-  f32x16_t c[kChains] = {};
+// S^T = K Q^T of a step's key rows.  A product waits twice its time for the one that it
+// adds to: two half sums by turns.
+__device__ __forceinline__ f32x16_t step_scores(lds_byte_t* k, const Lane& a, const bf16x8_t (&qf)[8]) {
+  f32x16_t c[2] = {};
 #pragma unroll
   for (int ks = 0; ks < 8; ++ks)
-#pragma unroll
-    for (int n = 0; n < N; ++n) {
-      const int chain = N > 1 ? n : ks & 1;
-      c[chain] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k_operand(k + n * kHalfSlot, a, ks), qf[ks], c[chain], 0, 0, 0);
-    }
-#pragma unroll
-  for (int n = 0; n < N; ++n) s[n] = N > 1 ? c[n] : c[0] + c[1];
+    c[ks & 1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k_operand(k, a, ks), qf[ks], c[ks & 1], 0, 0, 0);
+  return c[0] + c[1];
 }
 
 // V^T of rows 16 s .. + 15 (in the lanes' order: slot e of half h is row
@@ -212,23 +205,21 @@ __device__ __forceinline__ bf16x8_t v_operand(lds_byte_t* v, const Lane& a, int 
   return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
 }
 
-// The weights P of N steps (bf16, the B operands of two products each), and m, l, O
-// brought to the new maximum.  limit: key rows that the lane's query row sees, in
-// rows of the steps.
-template <int N, bool MASK>
-__device__ __forceinline__ void step_weights(f32x16_t (&s)[N], float c2, int limit, State& st, bf16x8_t (&p)[2 * N]) {
+// The weights P of a step (bf16, the B operands of two products), and m, l, O
+// brought to the new maximum.  limit: key rows of the step that the lane's query row
+// sees.
+template <bool MASK>
+__device__ __forceinline__ void step_weights(f32x16_t s, float c2, int limit, State& st, bf16x8_t (&p)[2]) {
   const int h = (threadIdx.x & 63) >> 5;
-  auto seen = [&](int n, int i) { return 32 * n + 8 * (i / 4) + 4 * h + i % 4 < limit; };
+  auto seen = [&](int i) { return 8 * (i / 4) + 4 * h + i % 4 < limit; };
   if constexpr (MASK) {
 #pragma unroll
-    for (int n = 0; n < N; ++n)
-#pragma unroll
-      for (int i = 0; i < 16; ++i)
-        if (!seen(n, i)) s[n][i] = neg_inf();
+    for (int i = 0; i < 16; ++i)
+      if (!seen(i)) s[i] = neg_inf();
   }
-  float mx = s[0][0];
+  float mx = s[0];
 #pragma unroll
-  for (int i = 1; i < 16 * N; ++i) mx = fmaxf(mx, s[i / 16][i % 16]);
+  for (int i = 1; i < 16; ++i) mx = fmaxf(mx, s[i]);
   mx = other_half_max(mx) * c2;
   if (MASK && limit <= 0) mx = neg_inf();  // (-inf times a scale of zero)
   const bool raise = mx > st.m + kRaise;
@@ -244,24 +235,19 @@ __device__ __forceinline__ void step_weights(f32x16_t (&s)[N], float c2, int lim
   const float m = st.m == neg_inf() ? 0.f : st.m;
   const bf16x2_t ones = {static_cast<__bf16>(1.f), static_cast<__bf16>(1.f)};
 #pragma unroll
-  for (int n = 0; n < N; ++n) {
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[n][i], c2, -m));
-      if (MASK && !seen(n, i)) e = 0.f;
-      p[2 * n + i / 8][i % 8] = static_cast<__bf16>(e);
-    }
-#pragma unroll
-    for (int i = 0; i < 16; i += 2)
-      st.l = __builtin_amdgcn_fdot2_f32_bf16(bf16x2_t{p[2 * n + i / 8][i % 8], p[2 * n + i / 8][i % 8 + 1]}, ones, st.l,
-                                             false);
+  for (int i = 0; i < 16; ++i) {
+    float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], c2, -m));
+    if (MASK && !seen(i)) e = 0.f;
+    p[i / 8][i % 8] = static_cast<__bf16>(e);
   }
+#pragma unroll
+  for (int i = 0; i < 16; i += 2)
+    st.l = __builtin_amdgcn_fdot2_f32_bf16(bf16x2_t{p[i / 8][i % 8], p[i / 8][i % 8 + 1]}, ones, st.l, false);
 }
 
-template <int N>
-__device__ __forceinline__ void step_accumulate(lds_byte_t* v, const Lane& a, const bf16x8_t (&p)[N], State& st) {
+__device__ __forceinline__ void step_accumulate(lds_byte_t* v, const Lane& a, const bf16x8_t (&p)[2], State& st) {
 #pragma unroll
-  for (int s = 0; s < N; ++s)
+  for (int s = 0; s < 2; ++s)
 #pragma unroll
     for (int db = 0; db < 4; ++db)
       st.o[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v_operand(v, a, s, db), p[s], st.o[db], 0, 0, 0);
@@ -323,17 +309,16 @@ __device__ __forceinline__ bool attend_split(const Rows& src, const bf16x8_t (&q
   auto step = [&](auto masked) __attribute__((always_inline)) {
     constexpr bool kMask = decltype(masked)::value;
     wait_half();  // K is here
-    f32x16_t s[1];
-    step_scores<1>(slot, a, qf, s);
+    const f32x16_t s = step_scores(slot, a, qf);
     wait_reads();
     off += (unsigned)(NW * kStep) * (unsigned)(src.stride * 2);
     load_k(buf, a, off, at);
     bf16x8_t p[2];
-    step_weights<1, kMask>(s, c2, min(limit, src.end) - row0, st, p);
+    step_weights<kMask>(s, c2, min(limit, src.end) - row0, st, p);
     wait_half();  // V is here
     if constexpr (kMask && CAUSAL)
       special |= mask_values(slots + wave * kSlot + kHalfSlot, least - row0, src.end - row0);
-    step_accumulate<2>(slot + kHalfSlot, a, p, st);
+    step_accumulate(slot + kHalfSlot, a, p, st);
     wait_reads();
     load_v(buf, a, off, at + kHalfSlot);
     row0 += NW * kStep;
@@ -380,11 +365,10 @@ __device__ __forceinline__ void attend_shared(const Rows& src, const bf16x8_t (&
     // slot the next load takes.
     asm volatile("s_waitcnt vmcnt(8) lgkmcnt(0)\n\ts_barrier" ::: "memory");
     load();
-    f32x16_t s[1];
-    step_scores<1>(ring + from, a, qf, s);
+    const f32x16_t s = step_scores(ring + from, a, qf);
     bf16x8_t p[2];
-    step_weights<1, decltype(masked)::value>(s, c2, src.end - row0, st, p);
-    step_accumulate<2>(ring + from + kHalfSlot, a, p, st);
+    step_weights<decltype(masked)::value>(s, c2, src.end - row0, st, p);
+    step_accumulate(ring + from + kHalfSlot, a, p, st);
     from = (from + kSlot) & (kRing - 1);
     row0 += kStep;
   };
