@@ -389,7 +389,8 @@ size_t lsk_lora_workspace_bytes(int M, int N, int K, int rank_tiles, int count, 
  *              gate rows, n0 = 32j + 8(c/4) + c%4, p = 1 their up rows, N/2
  *              further on.  Rows past N (or N/2) are zero.
  *   scale, ranks   device fp32 / int32 [count]; of A_a's rows and B_a's columns the
- *              first ranks[a] count
+ *              first ranks[a] count: A_a's others may hold anything, B_a's have to
+ *              be finite (they meet zeros)
  *   rank_tiles 1, 2, 3, 4, 6 or 8 (rank 16 to 128)
  *   index      device int32 [M]
  *   out        [M][N] (or [M][N/2]) contiguous, 16-byte aligned; may be y itself
