@@ -14,7 +14,7 @@
 //
 // h is held in fp32 and multiplied as the sum of two bf16 parts, h = hi + lo
 // (lo the rounding error of hi, itself rounded): 2^-17 of h is lost instead of
-// 2^-9, for one more MFMA per tile, which the bytes hide.  z is rounded once.
+// 2^-8, for one more MFMA per tile, which the bytes hide.  z is rounded once.
 // A row's result depends on its own x, y and adapter alone: products of other
 // rows or adapters are dropped by selection, never multiplied by zero.
 //
@@ -25,13 +25,17 @@
 // and the rows of a group: 64 share an adapter's tiles among four times the
 // rows, 16 keep a small batch's groups small.
 //
-// Bound by bytes for many rows or adapters, by the chain x, A, h, B, z for few:
-//   1 row, o (2560 x 4096), rank 8                        5.1 us
-//   16 rows, QKV (6144 x 2560), 24 of rank 16             6.3 us (4.1 MB)
-//   64 rows, down (2560 x 9728), 32 of rank 64           15.5 us (52 MB, most of
-//     them A, which the first launch reads in 10.3)
-//   2000 rows, gate_up (19456 x 2560), 8 of rank 32        44 us (135 MB: the first
-//     launch 7.6, the second 36.3 for 117 MB, 3.2 TB/s; a copy reaches 4.8)
+// Bound by bytes for many rows or adapters, by the chain x, A, h, B, z for few (medians
+// of the launches by themselves):
+//   1 row, o (2560 x 4096), rank 8                     5.2 us
+//   16 rows, QKV (6144 x 2560), 24 of rank 16          6.4 us (4.1 MB)
+//   64 rows, down (2560 x 9728), 32 of rank 64         9.9 + 4.9 us (52 MB, most of them
+//     A: 41 MB fetched by the first launch, each adapter's once)
+//   2000 rows, gate_up (19456 x 2560), 8 of rank 32    7.6 + 35.1 us (135 MB: the second
+//     launch 117 MB, 3.3 TB/s; a copy reaches 4.8)
+// 17 to 128 rows that name few adapters of a store of many leave workgroups idle, and
+// above 128 rows the time grows with the adapters that 64 neighbouring rows name:
+// adapter_plan has the figures.
 
 #include <hip/hip_runtime.h>
 

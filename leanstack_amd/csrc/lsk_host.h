@@ -190,14 +190,25 @@ constexpr bool adapter_rank_supported(int rank_tiles) {
 // tiles, and the second launch takes y once whatever its rows name.  Slots beyond
 // the first few would be workgroups that find nothing to do (2000 rows of gate_up
 // with 4 slots per tile instead of 1: 14.9 instead of 7.6 us for the first launch).
+// Each form is the slower one for the other's rows; all launches of a call, us, in
+// tiles of 16 rows and of 64, where the rows name one adapter of the store and where
+// each row names its own:
+//                                128 rows: one        own      256 rows: one        own
+//   o, 48 adapters of rank 16       9.7, 10.5  11.1, 35.4    15.1, 11.8  12.9, 43.5
+//   o, 48 of rank 128              17.6, 18.3  21.5, 77.9    28.1, 19.8  28.9, 98.5
+//   QKV, 48 of rank 16             14.3, 10.9  10.4, 35.5    22.0, 11.2  12.8, 43.8
+//   gate_up, 8 of rank 32          16.7, 14.1  15.6, 23.7    26.4, 15.4  23.2, 25.4
+// The host knows the store's count and not what the rows name: slots go by the count, so
+// that one adapter out of a store of many has fewer workgroups than out of a store of one
+// (gate_up, rank 16, 128 rows: 23.1 us of 32 adapters, 11.3 of one).
 struct AdapterPlan {
   int rows, tiles, slots, ranges, splits;
 };
 constexpr int adapter_blocks(int N, bool silu) { return silu ? (N + 63) / 64 : (N + 31) / 32; }
 // Column ranges of `tiles` 64-row tiles in the second launch.  A workgroup takes some 4 us
 // until y streams, then about 13 bytes a nanosecond (a CU's share of 3.3 TB/s), a
-// block per wave at a time; a CU runs one, so a few workgroups more than CUs would
-// cost a whole round: gate_up, rank 32, with one round and with two: 512 rows 13.2, 20.5
+// block per wave at a time; a CU runs one (of plain rank 16, whose registers allow two, it is
+// taken to run one as well), so a few workgroups more than CUs would cost a whole round: gate_up, rank 32, with one round and with two: 512 rows 13.2, 20.5
 // us, 1024 rows 18.2, 23.9; o, 2000 rows 9.5, 12.0.
 constexpr int adapter_rows_ranges(int tiles, int N, bool silu) {
   const int blocks = adapter_blocks(N, silu), most = (blocks + 7) / 8;

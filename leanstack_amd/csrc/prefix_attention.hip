@@ -20,14 +20,16 @@
 //     if the 16 key rows of a product are taken in the order that the lanes hold
 //     them in, so P needs no transposition; V^T comes from LDS by
 //     ds_read_b64_tr_b16.
-// P is rounded to bf16, at most 2^-9 of each weight, and l sums the rounded
+// P is rounded to bf16, at most 2^-8 of each weight, and l sums the rounded
 // weights: the result is exactly that of slightly other weights, whose errors
-// average out over the rows (the output's own rounding is as large).
+// average out over the rows (the output's own rounding is as large: 0.0018 to 0.0022
+// from 64 bits in all, relative 2-norm, 0.0017 with weights in fp32, which P V
+// on matrix instructions would take twice the products for).
 //
 // K and V rows go to LDS by DMA, their 16-byte chunks permuted by row so that
-// neither the reads of K (one row per lane) nor of V (four rows per 16 lanes)
-// meet in a bank.  Rows past the last visible one are out of the buffers' range
-// and come as zeros: what lies behind the written rows is never read.
+// neither 16 lanes' reads of K (one row per lane) nor of V (four rows) meet in a
+// bank.  Rows past the last visible one are out of the buffers' range and come as
+// zeros: what lies behind the written rows is never read.
 //
 // Items whose waves share query rows (own rows; a prefix with few query rows) split
 // the key rows, each wave with a slot of its own and no barrier: the next step's K
@@ -38,16 +40,20 @@
 // row's items up; a short context runs in one launch, each request's items
 // reading the prefix and its own rows.
 //
-// What it measured (32 q, 8 kv heads; B requests of T tokens, P + S rows; the kernels in
-// a graph):
-//   1x5 300+64      9.2 us, one launch: latency (the bytes are 0.3 us)
-//   12x1 1024+512  10.6 us, of it 4 the second launch
-//   64x1 8191+1088  48 us: 166 MB, 4.1 TB/s in the first launch (a copy reaches 4.8)
-//   48x4 16000+320  82 us: 51 GFLOP, 760 TFLOP/s in the first launch (a large matrix
-//     product reaches 1214).  A step of a wave is 512 cycles of MFMA, some 500 of the
-//     softmax's VALU and 128 of a CU's LDS: two waves per SIMD overlap them in part.
+// What it measured (32 q, 8 kv heads; B requests of T tokens, P + S rows; medians of
+// the launches by themselves):
+//   1x5 300+64       8.8 us, one launch: latency (the bytes are 0.3 us)
+//   12x1 1024+512    7.0 + 4.0 us
+//   64x1 8191+1088  41.4 + 5.0 us: 166 MB, 4.0 TB/s in the first launch (a copy reaches 4.8)
+//   48x4 16000+320  65.4 + 8.5 us: 51 GFLOP, 777 TFLOP/s in the first launch (a large matrix
+//     product reaches 1214).  A step of a wave is 512 cycles of MFMA; by the counters
+//     products are under way in 42 % of the cycles of a busy CU, vector instructions
+//     (most of them the softmax's) in 52 %, its LDS pipe in 34 % (105 cycles a step, 33
+//     of them bank conflicts): the first two take turns more than they overlap.
 //     Tried and no faster: 8 waves with 256 query rows (74 us for 67), pairs of steps,
 //     half the waves a barrier behind the others (79), 64 query rows per wave (70).
+//   prompts: 1x256 1024+256  21.0 + 7.7 us; 1x512 4096+512  57.2 + 14.6 us, 640 TFLOP/s;
+//     4x256 2048+256  59.5 + 23.2 us
 
 #include <hip/hip_runtime.h>
 
