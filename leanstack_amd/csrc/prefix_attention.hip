@@ -15,7 +15,8 @@
 //     one query row, and the other 16 are in the other half-wave;
 //   the running maximum m and sum l of the softmax, in base 2, in fp32.  m is
 //     raised only where a step exceeds it by 2^8 (weights up to 2^8 are as exact
-//     as weights up to 1, and the sums, rescaled on a raise, stay in range);
+//     as weights up to 1, and the sums, rescaled on a raise, stay in range of
+//     values up to some 2^110);
 //   O^T += V^T P^T on the same MFMA.  The scores' lanes are those of the B operand
 //     if the 16 key rows of a product are taken in the order that the lanes hold
 //     them in, so P needs no transposition; V^T comes from LDS by
@@ -75,6 +76,7 @@ constexpr int kStep = 32;                  // key rows, and query rows of a wave
 constexpr int kHalfSlot = kStep * D * 2;   // bytes of a step's K, or V
 constexpr int kSlot = 2 * kHalfSlot;
 constexpr float kRaise = 8.f;
+constexpr float kFar = 0x1p30f;
 constexpr int kJointWaves = 8;             // of an item of a short context
 constexpr int kWaves = 4;                  // of another item
 static_assert(kPrefixSharedRows == 32 * kWaves, "query rows of an item whose waves have some of their own");
@@ -117,9 +119,10 @@ struct Rows {
 };
 
 // A wave's softmax state for its 32 query rows: lane (h, c) holds row c, of O the
-// dims 32 db + 8 (i / 4) + 4 h + i % 4, of l the share of the lane's scores.
+// dims 32 db + 8 (i / 4) + 4 h + i % 4, of l the share of the lane's scores, and
+// of m the factor c2 that takes its scores to base 2.
 struct State {
-  float m, l;
+  float m, l, c2;
   f32x16_t o[4];
 };
 
@@ -214,6 +217,11 @@ __device__ __forceinline__ bf16x8_t v_operand(lds_byte_t* v, const Lane& a, int 
 // The weights P of a step (bf16, the B operands of two products), and m, l, O
 // brought to the new maximum.  limit: key rows of the step that the lane's query row
 // sees.
+//
+// Exponents are s c2 - m with one rounding, m being the rounded top c2: far from zero
+// (kFar) its rounding error would be more than 2^x holds.  There scores that are not
+// equal are 2^6 and more apart in base 2, so any factor gives the same weights, if m's
+// order stays: the next power of two above c2, whose products are exact.
 template <bool MASK>
 __device__ __forceinline__ void step_weights(f32x16_t s, float c2, int limit, State& st, bf16x8_t (&p)[2]) {
   const int h = (threadIdx.x & 63) >> 5;
@@ -223,13 +231,17 @@ __device__ __forceinline__ void step_weights(f32x16_t s, float c2, int limit, St
     for (int i = 0; i < 16; ++i)
       if (!seen(i)) s[i] = neg_inf();
   }
-  float mx = s[0];
+  float top = s[0];
 #pragma unroll
-  for (int i = 1; i < 16; ++i) mx = fmaxf(mx, s[i]);
-  mx = other_half_max(mx) * c2;
+  for (int i = 1; i < 16; ++i) top = fmaxf(top, s[i]);
+  top = other_half_max(top);
+  float mx = top * st.c2;
   if (MASK && limit <= 0) mx = neg_inf();  // (-inf times a scale of zero)
   const bool raise = mx > st.m + kRaise;
   if (__ballot(raise)) {  // (a query row's maximum goes by its own scores alone)
+    const float above = __builtin_bit_cast(float, (__builtin_bit_cast(unsigned, c2) + 0x007fffffu) & 0x7f800000u);
+    st.c2 = !raise ? st.c2 : fabsf(top * c2) < kFar ? c2 : above;
+    mx = top * st.c2;
     const float f = raise ? __builtin_amdgcn_exp2f(st.m - mx) : 1.f;
     st.m = raise ? mx : st.m;
     st.l *= f;
@@ -242,7 +254,7 @@ __device__ __forceinline__ void step_weights(f32x16_t s, float c2, int limit, St
   const bf16x2_t ones = {static_cast<__bf16>(1.f), static_cast<__bf16>(1.f)};
 #pragma unroll
   for (int i = 0; i < 16; ++i) {
-    float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], c2, -m));
+    float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], st.c2, -m));
     if (MASK && !seen(i)) e = 0.f;
     p[i / 8][i % 8] = static_cast<__bf16>(e);
   }
@@ -474,10 +486,11 @@ __device__ __forceinline__ void load_q(const PrefixArgs& a, const Query& q, bf16
   }
 }
 
-__device__ __forceinline__ State empty_state() {
+__device__ __forceinline__ State empty_state(float c2) {
   State st;
   st.m = neg_inf();
   st.l = 0.f;
+  st.c2 = c2;
 #pragma unroll
   for (int db = 0; db < 4; ++db) st.o[db] = f32x16_t{};
   return st;
@@ -499,8 +512,8 @@ __device__ __forceinline__ void own_item(const PrefixArgs& a, int j, int b, int 
   load_q(a, mine, qf);
   const int written = __builtin_amdgcn_readfirstlane(own_written(a, b));
   if (!JOINT && begin >= written) return;  // (the second launch knows this, too)
-  State st = empty_state();
   const float c2 = fabsf(a.scale) * 1.44269504088896341f;
+  State st = empty_state(c2);
   if (JOINT && a.P > 0) {
     const Rows src = {a.pk + (size_t)j * a.p_h, a.pv + (size_t)j * a.p_h, a.p_row, 0, a.P};
     attend_split<NW, false>(src, qf, c2, a.P, a.P, 0, slots, st);
@@ -563,8 +576,8 @@ __device__ __forceinline__ void prefix_item(const PrefixArgs& a, int j, int r0, 
   const int i = (SHARED ? (threadIdx.x >> 6) * 32 : 0) + (threadIdx.x & 31);
   bf16x8_t qf[8];
   load_q(a, find(min(i, rows - 1 - r0)), qf);
-  State st = empty_state();
   const float c2 = fabsf(a.scale) * 1.44269504088896341f;
+  State st = empty_state(c2);
   const Rows src = {a.pk + (size_t)j * a.p_h, a.pv + (size_t)j * a.p_h, a.p_row, begin, end};
   if constexpr (SHARED)
     attend_shared(src, qf, c2, slots, st);
