@@ -235,7 +235,8 @@ int check_prefix_args(const void* q, long long q_batch, long long q_head, long l
   for (const void* w : wide)
     if (!aligned(w, 16)) return fail(LSK_ERR_INVALID, "q, the keys and values and out must be 16-byte aligned");
   if (!aligned(lens, 4)) return fail(LSK_ERR_INVALID, "lens must be 4-byte aligned");
-  if (!std::isfinite(scale)) return fail(LSK_ERR_INVALID, "scale must be finite");
+  if (!std::isfinite(scale * 1.44269504088896341f))  // (scores are taken to base 2)
+    return fail(LSK_ERR_INVALID, "scale=%g must be finite, also times log2(e)", (double)scale);
   return LSK_OK;
 }
 

@@ -33,6 +33,15 @@ def test_adapter_workspace_of_sizes_it_does_not_serve(m, n, k, rank_tiles, count
     assert _lib.load().lsk_lora_workspace_bytes(m, n, k, rank_tiles, count, epilogue) == 0
 
 
+@pytest.mark.parametrize("scale", [3e38, -3.4e38])
+def test_attention_scales_that_overflow_in_base_2(scale):
+    """scale * log2(e) has to be finite, or equal scores of zero would give NaN."""
+    at = 0x10000  # aligned, never dereferenced
+    status = _lib.load().lsk_prefix_attention_bf16(at, 1024, 128, 1024, 1, 1, 8, 2, 128, at, at, 128 * 64, 128, 64, at, at, 2 * 128 * 8,
+                                                   128 * 8, 128, 8, at, scale, at, None, 0, None)
+    assert status == _lib.ERR_INVALID and "scale" in _lib.last_error()
+
+
 @pytest.mark.skipif(shutil.which("g++") is None, reason="needs g++")
 def test_size_rules_under_asan_and_ubsan(tmp_path):
     exe = tmp_path / "batch_rules_driver"
