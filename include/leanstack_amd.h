@@ -339,7 +339,8 @@ size_t lsk_prefix_attention_workspace_bytes(int B, int T, int n_q, int n_kv, int
  *   out[b][t][h][d] = softmax(scale * q K^T) V,  q head h reading kv head
  * h / (n_q / n_kv); scores, maxima and sums in fp32, the weights of V rounded to bf16 and normalised by
  * the sum of the rounded ones, bf16 output.  A query that sees no row gives
- * zeros; one whose rows all score -inf gives NaN.
+ * zeros; one whose rows all score -inf gives NaN.  Weights reach 2^8 before they are
+ * normalised: finite values of v above some 2^110 may give infinities.
  *   q            device bf16, [d] at q + b * q_batch_stride + h * q_head_stride +
  *                t * q_token_stride (elements; multiples of 8)
  *   prefix_k, prefix_v   device bf16, row i of kv head j at j *
