@@ -446,6 +446,93 @@ int lsk_constrain_logits(const void* logits, int logits_mode, int M, int V, long
                          void* out, long long* tokens, void* workspace, size_t ws_bytes, void* hip_stream);
 
 /* ------------------------------------------------------------------------
+ * A paged key/value cache in 8 bits.
+ *
+ * 16 rows of one kv head are a block of 2048 bytes, row t, dim d at
+ *   keys    (d / 64) * 1024 + ((d / 16) % 4 * 16 + t) * 16 + d % 16
+ *   values  (d / 16 % 2) * 1024 + (t / 4 * 16 + d % 16) * 16 + d / 32 * 4 + t % 4
+ * each an e4m3 number (OCP, 4 exponent and 3 fraction bits, 0x7f and 0xff NaN), with
+ * one exponent byte x per block: a value is its byte's number times 2^(x - 127).  A
+ * page is page_rows / 16 blocks of each kv head, [n_kv][page_rows / 16][2048] bytes; a
+ * request's row r lies in page table[b][r / page_rows].  Entries outside 0..pages - 1
+ * name no page: rows written there are dropped, rows there are seen by no query
+ * and read back as zeros.
+ * ------------------------------------------------------------------------ */
+
+typedef struct lsk_paged_pool {
+  void* k_blocks;        /* [pages][n_kv][page_rows / 16][2048], 16-byte aligned */
+  void* v_blocks;
+  void* k_exponents;     /* [pages][n_kv][page_rows / 16] */
+  void* v_exponents;
+  int pages;
+  int n_kv;
+  int page_rows;         /* 16, 32, .. 1024 (a power of two) */
+  int table_pages;       /* entries of a request's row of the table */
+  const int* table;      /* device int32, request b's at table + b * table_stride */
+  long long table_stride;
+} lsk_paged_pool;
+
+/* New rows into a layer's pages: rows t = 0 .. counts[b] - 1 of request b become its
+ * rows lens[b] - counts[b] + t, rounded to 8 bits; rows in front of row 0 and past the
+ * table are dropped.  A block's exponent is the least e in -100..119 with |x| <= 448 2^e
+ * over its rows' finite values (larger ones become +-448 2^e); where a block already
+ * holds rows in front of the new ones it does not fall, and those rows are rounded again if
+ * it rises.  Every rounding is to the nearest, ties to even; infinities and NaN become
+ * NaN.  Rows behind the last new one keep their bytes.
+ *   k, v       device bf16, row t of request b, kv head j at b * batch + j * head + t *
+ *              token (elements; multiples of 8), 16-byte aligned
+ *   lens       device int32 [B]: a request's rows, the new ones included
+ *   counts     NULL (T), or device int32 [B], taken within 0..T
+ * No two requests may append to the same block.  head_dim is 128.  Takes the place of the
+ * cache append of src/leanstack/runtime/kv_cache.py:222-245. */
+int lsk_paged_append_bf16(const lsk_paged_pool* pool, const void* k, long long k_batch_stride,
+                          long long k_head_stride, long long k_token_stride, const void* v, long long v_batch_stride,
+                          long long v_head_stride, long long v_token_stride, int B, int T, const int* lens,
+                          const int* counts, void* hip_stream);
+
+/* Rows back: k_out / v_out [B][n_kv][rows][128] bf16, contiguous, of rows starts[b] ..
+ * starts[b] + rows - 1 (device int32 [B]; negative ones are taken as 0).  Exact.  Rows from
+ * lens[b] on (lens NULL: none) and rows without a page are zeros. */
+int lsk_paged_read_bf16(const lsk_paged_pool* pool, const int* starts, const int* lens, int B, int rows, void* k_out,
+                        void* v_out, void* hip_stream);
+
+/* Pages copied in every layer: for i < n, page src[i] to page dst[i] (device int32) in each
+ * of `planes` planes (the keys and the values of each layer), storage [planes][pages]
+ * [page_blocks][2048] and exponents [planes][pages][page_blocks], page_blocks the blocks
+ * of all kv heads of a page.  Entries outside 0..pages - 1 copy nothing.  A page that is
+ * a destination must not be named again. */
+int lsk_paged_copy(void* storage, void* exponents, int planes, int pages, int page_blocks, const int* src,
+                   const int* dst, int n, void* hip_stream);
+
+/* Device workspace of lsk_paged_attention_bf16 for requests of up to `capacity` rows (any
+ * contents; 0: none, or sizes that it refuses). */
+size_t lsk_paged_attention_workspace_bytes(int B, int T, int n_q, int n_kv, int capacity);
+
+/* Attention of T query tokens of each of B requests over their pages: query token t <
+ * counts[b] attends the request's first lens[b] - (counts[b] - 1 - t) rows (the new
+ * tokens' rows are the last of lens[b]; appended before),
+ *   out[b][t][h][d] = softmax(scale * q K^T) V,  q head h reading kv head h / (n_q / n_kv);
+ * scores, maxima and sums in fp32, the weights of V rounded to bf16 and normalised by the sum
+ * of the rounded ones, bf16 output.  Query tokens from counts[b] on, and those that see
+ * no row, give zeros; one whose rows all score -inf gives NaN.  Weights reach 2^8 before they are
+ * normalised: finite values above some 2^110 may give infinities.
+ *   q          device bf16, [d] at q + b * q_batch_stride + h * q_head_stride + t *
+ *              q_token_stride (elements; multiples of 8), 16-byte aligned
+ *   lens, counts   as for lsk_paged_append_bf16 (lens past the table's rows: those)
+ *   out        [B][T][n_q * d] contiguous, 16-byte aligned
+ *   workspace  lsk_paged_attention_workspace_bytes(B, T, n_q, n_kv, table_pages *
+ *              page_rows) bytes, 16-byte aligned; calls that share one must be
+ *              stream-ordered.
+ * head_dim must be 128, |scale| at most 2^120.  Rows that no query sees are not read.  Results do not depend on
+ * timing: every sum has a fixed order.  Takes the place of
+ * F.scaled_dot_product_attention over a contiguous bf16 cache
+ * (src/leanstack/runtime/qwen_explicit.py:894-912, :1000-1039). */
+int lsk_paged_attention_bf16(const lsk_paged_pool* pool, const void* q, long long q_batch_stride,
+                             long long q_head_stride, long long q_token_stride, int B, int T, int n_q, int head_dim,
+                             const int* lens, const int* counts, float scale, void* out, void* workspace,
+                             size_t ws_bytes, void* hip_stream);
+
+/* ------------------------------------------------------------------------
  * Stack programs: a whole decode / verify step of projections in ONE launch.
  *
  * A program is a list of projections with the semantics of lsk_linear_bf16

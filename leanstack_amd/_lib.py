@@ -126,6 +126,41 @@ _SIGNATURES: dict[str, tuple[type | None, list]] = {
     ),
 }
 
+class PagedPool(ctypes.Structure):
+    """struct lsk_paged_pool (include/leanstack_amd.h)."""
+
+    _fields_ = [
+        ("k_blocks", _c_void),
+        ("v_blocks", _c_void),
+        ("k_exponents", _c_void),
+        ("v_exponents", _c_void),
+        ("pages", _c_int),
+        ("n_kv", _c_int),
+        ("page_rows", _c_int),
+        ("table_pages", _c_int),
+        ("table", _c_void),
+        ("table_stride", ctypes.c_longlong),
+    ]
+
+
+_SIGNATURES.update({
+    "lsk_paged_append_bf16": (
+        _c_int,
+        [ctypes.POINTER(PagedPool), _c_void, ctypes.c_longlong, ctypes.c_longlong, ctypes.c_longlong, _c_void,
+         ctypes.c_longlong, ctypes.c_longlong, ctypes.c_longlong, _c_int, _c_int, _c_void, _c_void, _c_void],
+    ),
+    "lsk_paged_read_bf16": (
+        _c_int, [ctypes.POINTER(PagedPool), _c_void, _c_void, _c_int, _c_int, _c_void, _c_void, _c_void]),
+    "lsk_paged_copy": (_c_int, [_c_void, _c_void, _c_int, _c_int, _c_int, _c_void, _c_void, _c_int, _c_void]),
+    "lsk_paged_attention_workspace_bytes": (_c_size, [_c_int] * 5),
+    "lsk_paged_attention_bf16": (
+        _c_int,
+        [ctypes.POINTER(PagedPool), _c_void, ctypes.c_longlong, ctypes.c_longlong, ctypes.c_longlong, _c_int, _c_int,
+         _c_int, _c_int, _c_void, _c_void, ctypes.c_float, _c_void, _c_void, _c_size, _c_void],
+    ),
+})
+
+
 class Projection(ctypes.Structure):
     """struct lsk_projection (include/leanstack_amd.h)."""
 

@@ -24,7 +24,7 @@ BUILD_DIR = PACKAGE_DIR / "_build"
 LIBRARY = PACKAGE_DIR / "libleanstack_amd.so"
 
 SOURCES = ("abi.cpp", "host_rules.cpp", "decode.hip", "skinny.hip", "gemm.hip", "stack.hip", "attention.hip", "rows.hip",
-           "prefix_attention.hip",
+           "prefix_attention.hip", "paged_cache.hip", "paged_attention.hip",
            "adapters.hip", "constrain.hip", "noalloc.hip", "probe.hip")
 OFFLOAD_ARCH = "gfx950"
 

@@ -454,6 +454,125 @@ int lsk_prefix_attention_bf16(const void* q, long long q_batch_stride, long long
 
 }  // extern "C"
 
+// ------------------------------------------------------------- paged 8-bit cache
+
+namespace {
+
+lsk::PagedPool paged_pool(const lsk_paged_pool& p) {
+  lsk::PagedPool r;
+  r.k = static_cast<unsigned char*>(p.k_blocks);
+  r.v = static_cast<unsigned char*>(p.v_blocks);
+  r.k_exp = static_cast<unsigned char*>(p.k_exponents);
+  r.v_exp = static_cast<unsigned char*>(p.v_exponents);
+  r.table = p.table;
+  r.table_ld = (size_t)p.table_stride;
+  r.n_kv = p.n_kv;
+  r.pages = p.pages;
+  const int page_blocks = p.page_rows / lsk::kPagedBlockRows;
+  r.page_shift = __builtin_ctz((unsigned)page_blocks);
+  r.blocks = p.table_pages * page_blocks;
+  return r;
+}
+
+}  // namespace
+
+extern "C" {
+
+int lsk_paged_append_bf16(const lsk_paged_pool* pool, const void* k, long long k_batch_stride,
+                          long long k_head_stride, long long k_token_stride, const void* v, long long v_batch_stride,
+                          long long v_head_stride, long long v_token_stride, int B, int T, const int* lens,
+                          const int* counts, void* hip_stream) {
+  lsk::clear_error();
+  if (int st = lsk::check_paged_append(pool, k, k_batch_stride, k_head_stride, k_token_stride, v, v_batch_stride,
+                                       v_head_stride, v_token_stride, B, T, lens, counts))
+    return st;
+  lsk::PagedAppendArgs a;
+  a.pool = paged_pool(*pool);
+  a.k = static_cast<const __bf16*>(k);
+  a.v = static_cast<const __bf16*>(v);
+  a.lens = lens;
+  a.counts = counts;
+  a.k_b = (size_t)k_batch_stride;
+  a.k_h = (size_t)k_head_stride;
+  a.k_t = (size_t)k_token_stride;
+  a.v_b = (size_t)v_batch_stride;
+  a.v_h = (size_t)v_head_stride;
+  a.v_t = (size_t)v_token_stride;
+  a.B = B;
+  a.T = T;
+  a.windows = lsk::paged_windows(T);
+  hipError_t err = lsk::launch_paged_append(a, static_cast<hipStream_t>(hip_stream));
+  return err == hipSuccess ? LSK_OK : hip_fail(err, "paged append kernel launch");
+}
+
+int lsk_paged_read_bf16(const lsk_paged_pool* pool, const int* starts, const int* lens, int B, int rows, void* k_out,
+                        void* v_out, void* hip_stream) {
+  lsk::clear_error();
+  if (int st = lsk::check_paged_read(pool, starts, lens, B, rows, k_out, v_out)) return st;
+  lsk::PagedReadArgs a;
+  a.pool = paged_pool(*pool);
+  a.k = static_cast<__bf16*>(k_out);
+  a.v = static_cast<__bf16*>(v_out);
+  a.starts = starts;
+  a.lens = lens;
+  a.B = B;
+  a.rows = rows;
+  a.windows = lsk::paged_windows(rows);
+  hipError_t err = lsk::launch_paged_read(a, static_cast<hipStream_t>(hip_stream));
+  return err == hipSuccess ? LSK_OK : hip_fail(err, "paged read kernel launch");
+}
+
+int lsk_paged_copy(void* storage, void* exponents, int planes, int pages, int page_blocks, const int* src,
+                   const int* dst, int n, void* hip_stream) {
+  lsk::clear_error();
+  if (int st = lsk::check_paged_copy(storage, exponents, planes, pages, page_blocks, src, dst, n)) return st;
+  lsk::PagedCopyArgs a;
+  a.storage = static_cast<unsigned char*>(storage);
+  a.exponents = static_cast<unsigned char*>(exponents);
+  a.src = src;
+  a.dst = dst;
+  a.n = n;
+  a.planes = planes;
+  a.pages = pages;
+  a.page_blocks = page_blocks;
+  a.parts = 0;
+  hipError_t err = lsk::launch_paged_copy(a, static_cast<hipStream_t>(hip_stream));
+  return err == hipSuccess ? LSK_OK : hip_fail(err, "page copy kernel launch");
+}
+
+size_t lsk_paged_attention_workspace_bytes(int B, int T, int n_q, int n_kv, int capacity) {
+  if (lsk::check_paged_attention_sizes(B, T, n_q, n_kv, capacity) != LSK_OK) return 0;
+  return 0;
+}
+
+int lsk_paged_attention_bf16(const lsk_paged_pool* pool, const void* q, long long q_batch_stride,
+                             long long q_head_stride, long long q_token_stride, int B, int T, int n_q, int head_dim,
+                             const int* lens, const int* counts, float scale, void* out, void* workspace,
+                             size_t ws_bytes, void* hip_stream) {
+  lsk::clear_error();
+  if (int st = lsk::check_paged_attention(pool, q, q_batch_stride, q_head_stride, q_token_stride, B, T, n_q, head_dim,
+                                          lens, counts, scale, out))
+    return st;
+  lsk::PagedAttentionArgs a;
+  a.pool = paged_pool(*pool);
+  a.q = static_cast<const __bf16*>(q);
+  a.lens = lens;
+  a.counts = counts;
+  a.out = static_cast<__bf16*>(out);
+  a.q_b = (size_t)q_batch_stride;
+  a.q_h = (size_t)q_head_stride;
+  a.q_t = (size_t)q_token_stride;
+  a.B = B;
+  a.T = T;
+  a.G = n_q / pool->n_kv;
+  a.n_q = n_q;
+  a.scale = scale;
+  hipError_t err = lsk::launch_paged_attention(a, static_cast<hipStream_t>(hip_stream));
+  return err == hipSuccess ? LSK_OK : hip_fail(err, "paged attention kernel launch");
+}
+
+}  // extern "C"
+
 // ------------------------------------------------------------- low-rank adapters
 
 extern "C" {

@@ -6,6 +6,7 @@
 // src/leanstack/runtime/cutile_logits.py:44-53 rejects bad input before
 // launching.
 
+#include <climits>
 #include <cmath>
 #include <cstdarg>
 #include <cstdio>
@@ -237,6 +238,110 @@ int check_prefix_args(const void* q, long long q_batch, long long q_head, long l
   if (!aligned(lens, 4)) return fail(LSK_ERR_INVALID, "lens must be 4-byte aligned");
   if (!std::isfinite(scale * 1.44269504088896341f))  // (scores are taken to base 2)
     return fail(LSK_ERR_INVALID, "scale=%g must be finite, also times log2(e)", (double)scale);
+  return LSK_OK;
+}
+
+int check_paged_pool(const lsk_paged_pool* p) {
+  if (p == nullptr) return fail(LSK_ERR_INVALID, "null pool");
+  if (p->page_rows < kPagedBlockRows || p->page_rows > kPagedMostPageRows || (p->page_rows & (p->page_rows - 1)) != 0)
+    return fail(LSK_ERR_INVALID, "page_rows=%d must be a power of two, %d..%d", p->page_rows, kPagedBlockRows,
+                kPagedMostPageRows);
+  if (p->pages < 1 || p->n_kv < 1 || p->table_pages < 1)
+    return fail(LSK_ERR_INVALID, "pages=%d, n_kv=%d and table_pages=%d must be positive", p->pages, p->n_kv, p->table_pages);
+  // Blocks are numbered in 31 bits, and so are a request's rows with some to spare.
+  const long long page_blocks = p->page_rows / kPagedBlockRows;
+  if ((long long)p->n_kv * page_blocks > INT_MAX / p->pages)
+    return fail(LSK_ERR_INVALID, "%d pages of %d heads: a layer must hold fewer than 2^31 blocks", p->pages, p->n_kv);
+  if ((long long)p->table_pages * p->page_rows > (1LL << 30))
+    return fail(LSK_ERR_INVALID, "%d pages of %d rows: a request holds at most 2^30", p->table_pages, p->page_rows);
+  if (p->table_stride < p->table_pages)
+    return fail(LSK_ERR_INVALID, "table_stride=%lld must be at least %d", p->table_stride, p->table_pages);
+  const void* wide[] = {p->k_blocks, p->v_blocks};
+  for (const void* w : wide)
+    if (w == nullptr || !aligned(w, 16)) return fail(LSK_ERR_INVALID, "the pool's blocks must be 16-byte aligned");
+  if (p->k_exponents == nullptr || p->v_exponents == nullptr) return fail(LSK_ERR_INVALID, "null exponents");
+  if (p->table == nullptr || !aligned(p->table, 4)) return fail(LSK_ERR_INVALID, "the table must be 4-byte aligned");
+  return LSK_OK;
+}
+
+namespace {
+
+// One wave per unit: a grid's threads are counted in 32 bits.
+int check_units(long long a, long long b, long long c) {
+  constexpr long long most = 0xffffffffLL / 64 - 4;
+  if (a > most || b > most || a * b > most || c > most || a * b * c > most)
+    return fail(LSK_ERR_INVALID, "%lld x %lld x %lld: too many blocks for one call", a, b, c);
+  return LSK_OK;
+}
+
+}  // namespace
+
+int check_paged_append(const lsk_paged_pool* pool, const void* k, long long k_batch, long long k_head, long long k_token,
+                       const void* v, long long v_batch, long long v_head, long long v_token, int B, int T,
+                       const int* lens, const int* counts) {
+  if (int st = check_paged_pool(pool)) return st;
+  if (B < 1 || T < 1) return fail(LSK_ERR_INVALID, "B=%d requests of T=%d rows must be positive", B, T);
+  if (int st = check_units(B, paged_windows(T), 2LL * pool->n_kv)) return st;
+  const long long strides[] = {k_batch, k_head, k_token, v_batch, v_head, v_token};
+  for (long long s : strides)
+    if (s < 0 || s % 8 != 0) return fail(LSK_ERR_INVALID, "strides must be multiples of 8, not negative (%lld)", s);
+  if (k == nullptr || v == nullptr || lens == nullptr) return fail(LSK_ERR_INVALID, "null device pointer");
+  if (!aligned(k, 16) || !aligned(v, 16)) return fail(LSK_ERR_INVALID, "k and v must be 16-byte aligned");
+  if (!aligned(lens, 4) || !aligned(counts, 4)) return fail(LSK_ERR_INVALID, "lens and counts must be 4-byte aligned");
+  return LSK_OK;
+}
+
+int check_paged_read(const lsk_paged_pool* pool, const int* starts, const int* lens, int B, int rows, const void* k,
+                     const void* v) {
+  if (int st = check_paged_pool(pool)) return st;
+  if (B < 1 || rows < 1) return fail(LSK_ERR_INVALID, "B=%d requests of %d rows must be positive", B, rows);
+  if (int st = check_units(B, paged_windows(rows), 2LL * pool->n_kv)) return st;
+  if (starts == nullptr || k == nullptr || v == nullptr) return fail(LSK_ERR_INVALID, "null device pointer");
+  if (!aligned(k, 16) || !aligned(v, 16)) return fail(LSK_ERR_INVALID, "the outputs must be 16-byte aligned");
+  if (!aligned(starts, 4) || !aligned(lens, 4)) return fail(LSK_ERR_INVALID, "starts and lens must be 4-byte aligned");
+  return LSK_OK;
+}
+
+int check_paged_copy(const void* storage, const void* exponents, int planes, int pages, int page_blocks, const int* src,
+                     const int* dst, int n) {
+  if (planes < 1 || pages < 1 || page_blocks < 1 || n < 1)
+    return fail(LSK_ERR_INVALID, "planes=%d, pages=%d, page_blocks=%d and n=%d must be positive", planes, pages,
+                page_blocks, n);
+  if (page_blocks > (1 << 20)) return fail(LSK_ERR_INVALID, "page_blocks=%d must be at most 2^20", page_blocks);
+  // (16 KB to a workgroup of 4 waves)
+  if (int st = check_units(n, planes, 4LL * ((page_blocks + 7) / 8))) return st;
+  if (storage == nullptr || exponents == nullptr || src == nullptr || dst == nullptr)
+    return fail(LSK_ERR_INVALID, "null device pointer");
+  if (!aligned(storage, 16)) return fail(LSK_ERR_INVALID, "storage must be 16-byte aligned");
+  if (!aligned(src, 4) || !aligned(dst, 4)) return fail(LSK_ERR_INVALID, "src and dst must be 4-byte aligned");
+  return LSK_OK;
+}
+
+int check_paged_attention_sizes(int B, int T, int n_q, int n_kv, int capacity) {
+  if (n_kv < 1 || n_q < n_kv || n_q % n_kv != 0)
+    return fail(LSK_ERR_INVALID, "n_q=%d must be a multiple of n_kv=%d", n_q, n_kv);
+  if (B < 1 || T < 1 || capacity < kPagedBlockRows || capacity % kPagedBlockRows != 0 || capacity > (1 << 30))
+    return fail(LSK_ERR_INVALID, "B=%d, T=%d, %d rows", B, T, capacity);
+  const long long most = 0xffffffffLL / 512;
+  if ((long long)B * T > most || (long long)B * T * n_q > most)
+    return fail(LSK_ERR_INVALID, "B=%d, T=%d, n_q=%d: too many query rows", B, T, n_q);
+  return LSK_OK;
+}
+
+int check_paged_attention(const lsk_paged_pool* pool, const void* q, long long q_batch, long long q_head,
+                          long long q_token, int B, int T, int n_q, int head_dim, const int* lens, const int* counts,
+                          float scale, const void* out) {
+  if (head_dim != kAttnHeadDim)
+    return fail(LSK_ERR_INVALID, "head_dim=%d: the attention kernel is built for %d", head_dim, kAttnHeadDim);
+  if (int st = check_paged_pool(pool)) return st;
+  if (int st = check_paged_attention_sizes(B, T, n_q, pool->n_kv, pool->table_pages * pool->page_rows)) return st;
+  const long long strides[] = {q_batch, q_head, q_token};
+  for (long long s : strides)
+    if (s < 0 || s % 8 != 0) return fail(LSK_ERR_INVALID, "strides must be multiples of 8, not negative (%lld)", s);
+  if (q == nullptr || lens == nullptr || out == nullptr) return fail(LSK_ERR_INVALID, "null device pointer");
+  if (!aligned(q, 16) || !aligned(out, 16)) return fail(LSK_ERR_INVALID, "q and out must be 16-byte aligned");
+  if (!aligned(lens, 4) || !aligned(counts, 4)) return fail(LSK_ERR_INVALID, "lens and counts must be 4-byte aligned");
+  if (!(std::fabs(scale) <= 0x1p120f)) return fail(LSK_ERR_INVALID, "scale=%g must be at most 2^120", (double)scale);
   return LSK_OK;
 }
 

@@ -140,6 +140,31 @@ int check_prefix_args(const void* q, long long q_batch, long long q_head, long l
                       int prefix_row, int P, const void* k, const void* v, long long batch, long long head, int row,
                       int S, const int* lens, float scale, const void* out);
 
+// Pages of an 8-bit key/value cache (paged_cache.hip, paged_attention.hip): blocks of
+// kPagedBlockRows rows of one kv head with an exponent, a power of two of blocks to a page.
+constexpr int kPagedBlockRows = 16;
+constexpr int kPagedBlockBytes = kPagedBlockRows * kAttnHeadDim;
+constexpr int kPagedLeastExponent = -100;  // of a block: 2^-100 .. 2^119, so that 448 times it is finite
+constexpr int kPagedMostExponent = 119;
+constexpr int kPagedMostPageRows = 1024;
+
+// Blocks that `rows` rows from any row on can touch.
+constexpr int paged_windows(int rows) { return (int)(((long long)rows + 2 * kPagedBlockRows - 2) / kPagedBlockRows); }
+
+// Argument rules of the lsk_paged entry points (all but workspaces' sizes).
+int check_paged_pool(const lsk_paged_pool* pool);
+int check_paged_append(const lsk_paged_pool* pool, const void* k, long long k_batch, long long k_head, long long k_token,
+                       const void* v, long long v_batch, long long v_head, long long v_token, int B, int T,
+                       const int* lens, const int* counts);
+int check_paged_read(const lsk_paged_pool* pool, const int* starts, const int* lens, int B, int rows, const void* k,
+                     const void* v);
+int check_paged_copy(const void* storage, const void* exponents, int planes, int pages, int page_blocks, const int* src,
+                     const int* dst, int n);
+int check_paged_attention_sizes(int B, int T, int n_q, int n_kv, int capacity);
+int check_paged_attention(const lsk_paged_pool* pool, const void* q, long long q_batch, long long q_head,
+                          long long q_token, int B, int T, int n_q, int head_dim, const int* lens, const int* counts,
+                          float scale, const void* out);
+
 // Constrained logits (constrain.hip): a row's vocabulary is cut into slices, one
 // workgroup each; a slice's counts are one LDS word per entry.
 constexpr int kConstrainMaxHistory = 1 << 20;

@@ -319,6 +319,51 @@ struct AdapterArgs {
 // rows: 16 or 64 per tile.
 hipError_t launch_adapters(const AdapterArgs& a, int rank_tiles, int rows, bool silu, hipStream_t stream);
 
+// A layer of a paged cache as the kernels take it: blocks and exponents of K and V, and
+// the requests' page table (page_shift: log2 of a page's blocks; blocks: those that the
+// table's rows can name).
+struct PagedPool {
+  unsigned char *k, *v, *k_exp, *v_exp;
+  const int* table;
+  size_t table_ld;
+  int n_kv, pages, page_shift, blocks;
+};
+// New rows into their blocks (paged_cache.hip): `windows` blocks from each request's first on.
+struct PagedAppendArgs {
+  PagedPool pool;
+  const __bf16 *k, *v;
+  const int *lens, *counts;
+  size_t k_b, k_h, k_t, v_b, v_h, v_t;
+  int B, T, windows;
+};
+hipError_t launch_paged_append(const PagedAppendArgs& a, hipStream_t stream);
+// Rows of the cache as bf16, [B][n_kv][rows][128].
+struct PagedReadArgs {
+  PagedPool pool;
+  __bf16 *k, *v;
+  const int *starts, *lens;
+  int B, rows, windows;
+};
+hipError_t launch_paged_read(const PagedReadArgs& a, hipStream_t stream);
+// Pages src[i] to dst[i] in every plane (K and V of each layer) of `pages` pages.
+struct PagedCopyArgs {
+  unsigned char *storage, *exponents;
+  const int *src, *dst;
+  int n, planes, pages, page_blocks, parts;
+};
+hipError_t launch_paged_copy(PagedCopyArgs a, hipStream_t stream);
+// Attention of T query tokens of B requests over their pages (paged_attention.hip).
+struct PagedAttentionArgs {
+  PagedPool pool;
+  const __bf16* q;
+  const int *lens, *counts;
+  __bf16* out;
+  size_t q_b, q_h, q_t;
+  int B, T, G, n_q;
+  float scale;
+};
+hipError_t launch_paged_attention(const PagedAttentionArgs& a, hipStream_t stream);
+
 // Number of scoring workgroups (= argmax partials per row) the lm_head
 // kernel uses for V vocab rows (V % 16 == 0): with NB = V / 16 row-blocks,
 // NB if NB <= 512, else (NB - T) / 2 + T with T = 512 + (NB - 512) % 2 (pairs

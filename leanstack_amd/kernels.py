@@ -18,6 +18,7 @@ import torch
 from . import _lib
 from .adapters import AdapterStore
 from .layout import PackedWeight
+from .paged_cache import PagedKVCache
 
 
 # The wrappers run for every projection of every token, so their host time is
@@ -586,6 +587,165 @@ def shared_prefix_attention(q: torch.Tensor, prefix_k: torch.Tensor, prefix_v: t
             strides[1], strides[2], rows, lens_at, float(scale), out.data_ptr(), _ptr(workspace), nbytes,
             torch._C._cuda_getCurrentRawStream(index))
     _lib.check(status, "lsk_prefix_attention_bf16")
+    return out
+
+
+def _pool(cache: PagedKVCache, layer: int, table: torch.Tensor) -> tuple[_lib.PagedPool, int, int]:
+    """(struct, B, device index) of a layer's pages and the batch's page table."""
+    if not isinstance(cache, PagedKVCache):
+        raise ValueError("cache must be a PagedKVCache")
+    if not 0 <= layer < cache.num_layers:
+        raise ValueError(f"layer {layer} of a cache of {cache.num_layers}")
+    if table.dtype is not torch.int32 or table.dim() != 2 or table.shape[1] < 1 or table.stride(1) != 1 and table.shape[1] > 1:
+        raise ValueError(f"table must be int32 [B, pages] with contiguous rows, got {table.dtype} {tuple(table.shape)} of "
+                         f"strides {table.stride()}")
+    b, width = table.shape
+    stride = table.stride(0) if b > 1 else width
+    if stride < width:
+        raise ValueError(f"table must not repeat or interleave its rows (stride {stride} of {width} entries)")
+    index = cache.storage.get_device()
+    if table.get_device() != index:
+        raise ValueError(f"table is on {table.device}, the cache on {cache.storage.device}")
+    keys = cache.storage.data_ptr()
+    exponents = cache.exponents.data_ptr()
+    plane = cache.num_pages * cache.num_key_value_heads * (cache.page_rows // 16)  # blocks of a layer's keys
+    at = 2 * layer * plane
+    return _lib.PagedPool(keys + at * 2048, keys + (at + plane) * 2048, exponents + at, exponents + at + plane,
+                          cache.num_pages, cache.num_key_value_heads, cache.page_rows, width, table.data_ptr(),
+                          stride), b, index
+
+
+def _head_rows(x: torch.Tensor, what: str) -> tuple[torch.Tensor, tuple[int, ...]]:
+    """x [B, heads, T, d] as the paged kernels read it in place, copied if they cannot, and its strides."""
+    strides = x.stride()
+    if strides[3] != 1 or (strides[0] | strides[1] | strides[2]) & 7 or x.data_ptr() % 16:
+        x = x.clone(memory_format=torch.contiguous_format)
+        strides = x.stride()
+    return x, strides
+
+
+def paged_append(cache: PagedKVCache, layer: int, k: torch.Tensor, v: torch.Tensor, table: torch.Tensor,
+                 lens: torch.Tensor, *, counts: torch.Tensor | None = None) -> None:
+    """New key and value rows of a batch into their pages, rounded to 8 bits.
+
+    k / v: [B, n_kv, T, d] bfloat16, d = 128 (views of the QKV projection's rows are read in
+    place); table: int32 [B, pages]; lens: int32 [B], a request's rows with the new ones;
+    counts: int32 [B], how many of the T are real (the first; all without).  Row t goes to
+    the request's row lens - counts + t; rows in front of row 0, past the table or in an entry
+    that names no page are dropped.  The three are read on the device, so a captured call
+    follows them.  No two requests may append to one page (PagedKVCache.reserve sees to it)."""
+    pool, b, index = _pool(cache, layer, table)
+    n_kv = cache.num_key_value_heads
+    if k.dim() != 4 or k.shape != v.shape or k.shape[0] != b or k.shape[1] != n_kv or k.shape[3] != 128 \
+            or k.dtype is not torch.bfloat16 or v.dtype is not torch.bfloat16:
+        raise ValueError(f"k and v must be bfloat16 [{b}, {n_kv}, T, 128], got {k.dtype} {tuple(k.shape)} and {v.dtype} "
+                         f"{tuple(v.shape)}")
+    lens_at = _per_row(lens, b, torch.int32, index, "lens")
+    counts_at = _per_row(counts, b, torch.int32, index, "counts")
+    if not (k.get_device() == v.get_device() == index):
+        _one_device(cache.storage, (k, "k"), (v, "v"))
+    _require_device(cache.storage, "cache")
+    t = k.shape[2]
+    if b * t == 0:
+        return
+    k, ks = _head_rows(k, "k")
+    v, vs = _head_rows(v, "v")
+    with _on_index(index):
+        status = _lib.load().lsk_paged_append_bf16(
+            ctypes.byref(pool), k.data_ptr(), ks[0], ks[1], ks[2], v.data_ptr(), vs[0], vs[1], vs[2], b, t, lens_at,
+            counts_at, torch._C._cuda_getCurrentRawStream(index))
+    _lib.check(status, "lsk_paged_append_bf16")
+
+
+def paged_read(cache: PagedKVCache, layer: int, table: torch.Tensor, starts: torch.Tensor, rows: int, *,
+               lens: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """(k, v) [B, n_kv, rows, 128] bfloat16: what the cache stands for in rows starts[b] ..
+    starts[b] + rows - 1 (int32 [B] on the device).  Rows from lens[b] on and rows without
+    a page are zeros."""
+    pool, b, index = _pool(cache, layer, table)
+    starts_at = _per_row(starts, b, torch.int32, index, "starts")
+    lens_at = _per_row(lens, b, torch.int32, index, "lens")
+    if rows < 0:
+        raise ValueError(f"rows={rows} must not be negative")
+    _require_device(cache.storage, "cache")
+    k = cache.storage.new_empty((b, cache.num_key_value_heads, rows, 128), dtype=torch.bfloat16)
+    v = torch.empty_like(k)
+    if b * rows == 0:
+        return k, v
+    with _on_index(index):
+        status = _lib.load().lsk_paged_read_bf16(ctypes.byref(pool), starts_at, lens_at, b, rows, k.data_ptr(), v.data_ptr(),
+                                                 torch._C._cuda_getCurrentRawStream(index))
+    _lib.check(status, "lsk_paged_read_bf16")
+    return k, v
+
+
+def copy_pages(cache: PagedKVCache, src: torch.Tensor, dst: torch.Tensor) -> None:
+    """Page src[i] to page dst[i] in every layer, keys, values and exponents (int32 [n] on
+    the pool's device).  Entries outside 0..num_pages - 1 copy nothing.  A destination must
+    not be named again, neither as a destination nor as a source."""
+    if not isinstance(cache, PagedKVCache):
+        raise ValueError("cache must be a PagedKVCache")
+    n = src.numel()
+    index = cache.storage.get_device()
+    src_at = _per_row(src, n, torch.int32, index, "src")
+    dst_at = _per_row(dst, n, torch.int32, index, "dst")
+    _require_device(cache.storage, "cache")
+    if n == 0:
+        return
+    with _on_index(index):
+        status = _lib.load().lsk_paged_copy(
+            cache.storage.data_ptr(), cache.exponents.data_ptr(), 2 * cache.num_layers, cache.num_pages,
+            cache.num_key_value_heads * (cache.page_rows // 16), src_at, dst_at, n,
+            torch._C._cuda_getCurrentRawStream(index))
+    _lib.check(status, "lsk_paged_copy")
+
+
+@functools.lru_cache(maxsize=4096)
+def _paged_workspace_bytes(b: int, t: int, n_q: int, n_kv: int, capacity: int) -> int:
+    return _lib.load().lsk_paged_attention_workspace_bytes(b, t, n_q, n_kv, capacity)
+
+
+def paged_attention(q: torch.Tensor, cache: PagedKVCache, layer: int, table: torch.Tensor, lens: torch.Tensor,
+                    scale: float, *, counts: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """softmax(q k^T * scale) v of T query tokens of each of B requests over their pages ->
+    [B, T, n_q * d].
+
+    q: [B, n_q, T, d] bfloat16, d = 128, q heads in groups of n_q / n_kv; table, lens and
+    counts as for paged_append, which the new tokens' rows went through before: query t sees
+    the first lens - (counts - 1 - t) rows.  Query tokens from counts on, and those that see
+    no row, give zeros.  T = 1 is a decode step, a few tokens a verify block, thousands a
+    prompt (in chunks if wanted).  out: a contiguous [B, T, n_q * d] tensor."""
+    pool, b, index = _pool(cache, layer, table)
+    n_kv = cache.num_key_value_heads
+    if q.dim() != 4 or q.dtype is not torch.bfloat16 or q.shape[0] != b or q.shape[3] != 128 or q.shape[1] < 1 \
+            or q.shape[1] % n_kv:
+        raise ValueError(f"q must be bfloat16 [{b}, a multiple of {n_kv}, T, 128], got {q.dtype} {tuple(q.shape)}")
+    n_q, t = q.shape[1], q.shape[2]
+    lens_at = _per_row(lens, b, torch.int32, index, "lens")
+    counts_at = _per_row(counts, b, torch.int32, index, "counts")
+    if q.get_device() != index:
+        _one_device(cache.storage, (q, "q"))
+    if out is not None:
+        _one_device(cache.storage, (out, "out"))
+        if tuple(out.shape) != (b, t, n_q * 128) or out.dtype is not torch.bfloat16 or not out.is_contiguous() \
+                or out.data_ptr() % 16:
+            raise ValueError(f"out must be a contiguous, 16-byte aligned bfloat16 [{b}, {t}, {n_q * 128}] tensor, got "
+                             f"{out.dtype} {tuple(out.shape)}")
+        if q.numel() and _overlap(out, q):
+            raise ValueError("out must not overlap q")
+    _require_device(cache.storage, "cache")
+    if out is None:
+        out = q.new_empty((b, t, n_q * 128))
+    if b * t == 0:
+        return out
+    q, qs = _head_rows(q, "q")
+    nbytes = _paged_workspace_bytes(b, t, n_q, n_kv, table.shape[1] * cache.page_rows)
+    workspace = q.new_empty((nbytes // 2,)) if nbytes else None
+    with _on_index(index):
+        status = _lib.load().lsk_paged_attention_bf16(
+            ctypes.byref(pool), q.data_ptr(), qs[0], qs[1], qs[2], b, t, n_q, 128, lens_at, counts_at, float(scale),
+            out.data_ptr(), _ptr(workspace), nbytes, torch._C._cuda_getCurrentRawStream(index))
+    _lib.check(status, "lsk_paged_attention_bf16")
     return out
 
 
