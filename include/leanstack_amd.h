@@ -445,6 +445,35 @@ int lsk_constrain_logits(const void* logits, int logits_mode, int M, int V, long
                          long long bias_ld, int bias_count, const int* allowed, long long allowed_ld,
                          void* out, long long* tokens, void* workspace, size_t ws_bytes, void* hip_stream);
 
+/* Device workspace of lsk_sample_logits (0: none, or sizes that it refuses). */
+size_t lsk_sample_workspace_bytes(int logits_mode, int M, int V);
+
+/* A token drawn from each row of logits by a given random number.  With weights
+ *   w[v] = 2^-44 * round(2^44 * exp((x[v] - max x) / temperature)),
+ * tokens ordered by larger x, then lower index:
+ *   kept are the first top_k; of those, the ones with w >= min_p; of those, the shortest
+ *   prefix (one token at least) whose sum reaches top_p times their sum;
+ *   tokens[m] = the first token, in the order of indices, at which the running sum of the
+ *   kept weights exceeds uniforms[m] times their sum, logprobs[m] = log(its weight / their sum).
+ * A row that holds a NaN, or nothing but -inf, has no distribution: token -1, logprob NaN.
+ * Values of +inf weigh 1 each, all others then nothing.
+ *   logits        device, fp32 (LSK_LOGITS_FP32) or bf16 (LSK_LOGITS_BF16), row m at
+ *                 logits + m * logits_ld; V at most 2^19
+ *   uniforms      device fp32 [M], in [0, 1) (below and NaN: 0; above: the last kept token)
+ *   temperature   NULL (1), or device fp32 [M]; 0, below and NaN: the largest logit's token
+ *                 (the lowest index of several), logprob 0
+ *   top_k         NULL, or device int32 [M]; below 1: all
+ *   top_p, min_p  NULL, or device fp32 [M]; top_p from 1 on and NaN: all, up to 0: one;
+ *                 min_p up to 0 and NaN: all, above 1: as 1
+ *   tokens        device int64 [M]
+ *   logprobs      device fp32 [M]
+ *   workspace     lsk_sample_workspace_bytes(...) bytes, 16-byte aligned; calls that share
+ *                 one must be stream-ordered.
+ * The reference's head is greedy (src/leanstack/runtime/cutile_logits.py:37-69). */
+int lsk_sample_logits(const void* logits, int logits_mode, int M, int V, long long logits_ld, const float* uniforms,
+                      const float* temperature, const int* top_k, const float* top_p, const float* min_p,
+                      long long* tokens, float* logprobs, void* workspace, size_t ws_bytes, void* hip_stream);
+
 /* ------------------------------------------------------------------------
  * A paged key/value cache in 8 bits.
  *

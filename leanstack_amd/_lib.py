@@ -41,6 +41,8 @@ DECODE_MAX_M = 16
 # Longest token history and bias list of constrain_logits (kConstrainMax... in the library).
 CONSTRAIN_MAX_HISTORY = 1 << 20
 CONSTRAIN_MAX_BIAS = 1023
+# Largest vocabulary of sample_logits (kSampleMaxVocab).
+SAMPLE_MAX_VOCAB = 1 << 19
 # Largest activation row stride in elements (kMaxActivationStride).
 MAX_ACTIVATION_STRIDE = (1 << 22) - 8
 
@@ -144,6 +146,12 @@ class PagedPool(ctypes.Structure):
 
 
 _SIGNATURES.update({
+    "lsk_sample_workspace_bytes": (_c_size, [_c_int] * 3),
+    "lsk_sample_logits": (
+        _c_int,
+        [_c_void, _c_int, _c_int, _c_int, ctypes.c_longlong, _c_void, _c_void, _c_void, _c_void, _c_void, _c_void, _c_void,
+         _c_void, _c_size, _c_void],
+    ),
     "lsk_paged_append_bf16": (
         _c_int,
         [ctypes.POINTER(PagedPool), _c_void, ctypes.c_longlong, ctypes.c_longlong, ctypes.c_longlong, _c_void,

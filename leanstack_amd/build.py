@@ -25,7 +25,7 @@ LIBRARY = PACKAGE_DIR / "libleanstack_amd.so"
 
 SOURCES = ("abi.cpp", "host_rules.cpp", "decode.hip", "skinny.hip", "gemm.hip", "stack.hip", "attention.hip", "rows.hip",
            "prefix_attention.hip", "paged_cache.hip", "paged_attention.hip",
-           "adapters.hip", "constrain.hip", "noalloc.hip", "probe.hip")
+           "adapters.hip", "constrain.hip", "sample.hip", "noalloc.hip", "probe.hip")
 OFFLOAD_ARCH = "gfx950"
 
 # -packed-fp32-ops: keep the compiler from forming packed FP32 VALU ops.

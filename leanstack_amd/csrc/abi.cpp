@@ -454,6 +454,40 @@ int lsk_prefix_attention_bf16(const void* q, long long q_batch_stride, long long
 
 }  // extern "C"
 
+// ------------------------------------------------------------- sampled tokens
+
+extern "C" {
+
+size_t lsk_sample_workspace_bytes(int logits_mode, int M, int V) {
+  if (lsk::check_sample_sizes(logits_mode, M, V) != LSK_OK) return 0;
+  return 0;
+}
+
+int lsk_sample_logits(const void* logits, int logits_mode, int M, int V, long long logits_ld, const float* uniforms,
+                      const float* temperature, const int* top_k, const float* top_p, const float* min_p,
+                      long long* tokens, float* logprobs, void* workspace, size_t ws_bytes, void* hip_stream) {
+  lsk::clear_error();
+  if (int st = lsk::check_sample_args(logits, logits_mode, M, V, logits_ld, uniforms, temperature, top_k, top_p, min_p,
+                                      tokens, logprobs))
+    return st;
+  lsk::SampleArgs a;
+  a.logits = logits;
+  a.uniforms = uniforms;
+  a.temperature = temperature;
+  a.top_k = top_k;
+  a.top_p = top_p;
+  a.min_p = min_p;
+  a.tokens = tokens;
+  a.logprobs = logprobs;
+  a.logits_ld = (size_t)logits_ld;
+  a.M = M;
+  a.V = V;
+  hipError_t err = lsk::launch_sample(a, logits_mode == LSK_LOGITS_BF16, static_cast<hipStream_t>(hip_stream));
+  return err == hipSuccess ? LSK_OK : hip_fail(err, "sampling kernel launch");
+}
+
+}  // extern "C"
+
 // ------------------------------------------------------------- paged 8-bit cache
 
 namespace {

@@ -288,6 +288,18 @@ struct ConstrainArgs {
 };
 hipError_t launch_constrain(const ConstrainArgs& a, bool bf16, hipStream_t stream);
 
+// A token drawn from each of M rows of logits (sample.hip).  Optional pointers are NULL.
+struct SampleArgs {
+  const void* logits;
+  const float *uniforms, *temperature, *top_p, *min_p;
+  const int* top_k;
+  long long* tokens;
+  float* logprobs;
+  size_t logits_ld;
+  int M, V;
+};
+hipError_t launch_sample(const SampleArgs& a, bool bf16, hipStream_t stream);
+
 // Attention of T query tokens of B requests over P shared and up to S own rows
 // (prefix_attention.hip).  Strides in elements; part_ml / part_o: (m, l) and O of
 // every part and query row (rows = B T n_q), m in base 2.

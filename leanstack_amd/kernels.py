@@ -1101,6 +1101,66 @@ def _constrain_workspace_bytes(m: int, v: int) -> int:
     return _lib.load().lsk_constrain_workspace_bytes(m, v)
 
 
+def sample_logits(logits: torch.Tensor, uniforms: torch.Tensor, *, temperature: torch.Tensor | None = None,
+                  top_k: torch.Tensor | None = None, top_p: torch.Tensor | None = None,
+                  min_p: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """A token drawn from each request's row of logits [M, V] (float32 or bfloat16), and the
+    logarithm of its probability among the kept ones: (int64 [M], float32 [M]).
+
+    Of the probabilities at `temperature` (1 without; 0 and below: the largest logit's token)
+    the top_k largest are kept (all without, or below 1; the lower index of equal logits
+    first), of those the ones of at least min_p times the largest, of those the shortest
+    prefix that holds top_p of their sum.  The token is the first, in the order of
+    indices, at which the running sum of the kept ones exceeds uniforms[m] (float32, in
+    [0, 1), from a generator of the caller's) times their sum.  Weights are whole
+    multiples of 2^-44 of the largest, so that the result depends on nothing but the
+    arguments.  A row with a NaN, or of -inf alone, gives token -1 and NaN.
+
+    uniforms, temperature, top_p, min_p: float32 [M], top_k: int32 [M], read on the
+    device, so a captured call follows them.  V at most 2^19."""
+    dtype = logits.dtype
+    if dtype is torch.float32:
+        mode = _lib.LOGITS_FP32
+    elif dtype is torch.bfloat16:
+        mode = _lib.LOGITS_BF16
+    else:
+        raise ValueError(f"logits must be float32 or bfloat16, got {dtype}")
+    if logits.dim() != 2 or not 1 <= logits.shape[1] <= _lib.SAMPLE_MAX_VOCAB:
+        raise ValueError(f"logits must be [M, V] with V up to {_lib.SAMPLE_MAX_VOCAB}, got {tuple(logits.shape)}")
+    m, v = logits.shape
+    index = logits.get_device()
+    if uniforms is None:
+        raise ValueError("uniforms must be given")
+    uniforms_at = _per_row(uniforms, m, torch.float32, index, "uniforms")
+    temperature_at = _per_row(temperature, m, torch.float32, index, "temperature")
+    k_at = _per_row(top_k, m, torch.int32, index, "top_k")
+    p_at = _per_row(top_p, m, torch.float32, index, "top_p")
+    min_p_at = _per_row(min_p, m, torch.float32, index, "min_p")
+    _require_device(logits, "logits")
+    ld, unit = logits.stride()
+    if (v > 1 and unit != 1) or (m > 1 and ld < v):
+        logits, ld = logits.contiguous(), v
+    elif m == 1:
+        ld = v
+    tokens = logits.new_empty((m,), dtype=torch.long)
+    logprobs = logits.new_empty((m,), dtype=torch.float32)
+    if m == 0:
+        return tokens, logprobs
+    nbytes = _sample_workspace_bytes(mode, m, v)
+    workspace = logits.new_empty((nbytes,), dtype=torch.uint8) if nbytes else None
+    with _on_index(index):
+        status = _lib.load().lsk_sample_logits(
+            logits.data_ptr(), mode, m, v, ld, uniforms_at, temperature_at, k_at, p_at, min_p_at, tokens.data_ptr(),
+            logprobs.data_ptr(), _ptr(workspace), nbytes, torch._C._cuda_getCurrentRawStream(index))
+    _lib.check(status, "lsk_sample_logits")
+    return tokens, logprobs
+
+
+@functools.lru_cache(maxsize=1024)
+def _sample_workspace_bytes(mode: int, m: int, v: int) -> int:
+    return _lib.load().lsk_sample_workspace_bytes(mode, m, v)
+
+
 def _ptr(t: torch.Tensor | None) -> int | None:
     return None if t is None else t.data_ptr()
 
