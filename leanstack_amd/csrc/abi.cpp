@@ -576,7 +576,7 @@ int lsk_paged_copy(void* storage, void* exponents, int planes, int pages, int pa
 
 size_t lsk_paged_attention_workspace_bytes(int B, int T, int n_q, int n_kv, int capacity) {
   if (lsk::check_paged_attention_sizes(B, T, n_q, n_kv, capacity) != LSK_OK) return 0;
-  return 0;
+  return (size_t)lsk::paged_workspace_bytes(lsk::paged_plan(B, T, n_q, n_kv, capacity), n_kv);
 }
 
 int lsk_paged_attention_bf16(const lsk_paged_pool* pool, const void* q, long long q_batch_stride,
@@ -587,6 +587,11 @@ int lsk_paged_attention_bf16(const lsk_paged_pool* pool, const void* q, long lon
   if (int st = lsk::check_paged_attention(pool, q, q_batch_stride, q_head_stride, q_token_stride, B, T, n_q, head_dim,
                                           lens, counts, scale, out))
     return st;
+  const lsk::PagedPlan p = lsk::paged_plan(B, T, n_q, pool->n_kv, pool->table_pages * pool->page_rows);
+  const size_t need = (size_t)lsk::paged_workspace_bytes(p, pool->n_kv);
+  if (need > 0 && (workspace == nullptr || ws_bytes < need || !aligned(workspace, 16)))
+    return fail(LSK_ERR_WORKSPACE, "the attention needs a workspace of %zu bytes, 16-byte aligned (got %zu)", need,
+                workspace ? ws_bytes : 0);
   lsk::PagedAttentionArgs a;
   a.pool = paged_pool(*pool);
   a.q = static_cast<const __bf16*>(q);
@@ -601,7 +606,17 @@ int lsk_paged_attention_bf16(const lsk_paged_pool* pool, const void* q, long lon
   a.G = n_q / pool->n_kv;
   a.n_q = n_q;
   a.scale = scale;
-  hipError_t err = lsk::launch_paged_attention(a, static_cast<hipStream_t>(hip_stream));
+  a.tiles = p.tiles;
+  a.items = (int)p.items;
+  a.places = (int)p.places;
+  a.workers = (int)p.workers;
+  a.least_units = p.least_units;
+  a.slot_rows = p.slot_rows;
+  const size_t begins = (size_t)lsk::paged_begins_bytes(p), slots = (size_t)p.slots * pool->n_kv * p.slot_rows;
+  a.begins = static_cast<int*>(workspace);
+  a.part_o = need > 0 ? reinterpret_cast<float*>(static_cast<char*>(workspace) + begins) : nullptr;
+  a.part_ml = need > 0 ? a.part_o + slots * lsk::kAttnHeadDim : nullptr;
+  hipError_t err = lsk::launch_paged_attention(a, p, static_cast<hipStream_t>(hip_stream));
   return err == hipSuccess ? LSK_OK : hip_fail(err, "paged attention kernel launch");
 }
 

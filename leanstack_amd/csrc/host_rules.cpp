@@ -346,9 +346,15 @@ int check_paged_attention_sizes(int B, int T, int n_q, int n_kv, int capacity) {
     return fail(LSK_ERR_INVALID, "n_q=%d must be a multiple of n_kv=%d", n_q, n_kv);
   if (B < 1 || T < 1 || capacity < kPagedBlockRows || capacity % kPagedBlockRows != 0 || capacity > (1 << 30))
     return fail(LSK_ERR_INVALID, "B=%d, T=%d, %d rows", B, T, capacity);
+  // Query rows and grids (of 512 threads a workgroup at most) are counted in 32 bits, units of
+  // all a head's items in 31.
   const long long most = 0xffffffffLL / 512;
   if ((long long)B * T > most || (long long)B * T * n_q > most)
     return fail(LSK_ERR_INVALID, "B=%d, T=%d, n_q=%d: too many query rows", B, T, n_q);
+  const PagedPlan p = paged_plan(B, T, n_q, n_kv, capacity);
+  if (p.items * n_kv * (p.rows / 16) > most || p.workers * n_kv > most ||
+      p.items * ((capacity + p.unit - 1) / p.unit) > INT_MAX)
+    return fail(LSK_ERR_INVALID, "B=%d, T=%d, n_q=%d over %d rows: too many items", B, T, n_q, capacity);
   return LSK_OK;
 }
 

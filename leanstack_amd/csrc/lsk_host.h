@@ -151,6 +151,45 @@ constexpr int kPagedMostPageRows = 1024;
 // Blocks that `rows` rows from any row on can touch.
 constexpr int paged_windows(int rows) { return (int)(((long long)rows + 2 * kPagedBlockRows - 2) / kPagedBlockRows); }
 
+// How an attention call runs.  An item is `rows` query rows (16, 32 or 64, or 128 where
+// waves have rows of their own) of one request and kv head.  one_launch: a workgroup per
+// item.  Else few rows are cut into chunks of at least `least_units` units of key rows, a
+// wave each, `places` per kv head and one more per item at most; of 128 rows `workers`
+// workgroups per kv head share all units.
+constexpr int kPagedFewUnit = 32;
+constexpr int kPagedManyUnit = 64;
+constexpr int kPagedManyRows = 128;
+constexpr int kPagedShortRows = 1024;
+struct PagedPlan {
+  bool one_launch;
+  int rows, slot_rows, unit, least_units, tiles;
+  long long items, places, workers, slots;  // slots: of parts, per kv head
+};
+constexpr PagedPlan paged_plan(int B, int T, int n_q, int n_kv, int capacity) {
+  const long long rows = (long long)T * (n_q / n_kv);
+  PagedPlan p = {false, rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : kPagedManyRows, 0, kPagedFewUnit, 4, 0, 0, 0, 0, 0};
+  const bool many = p.rows == kPagedManyRows;
+  if (many) p.unit = kPagedManyUnit;
+  p.slot_rows = rows < p.rows ? (int)rows : p.rows;
+  p.tiles = (int)((rows + p.rows - 1) / p.rows);
+  p.items = (long long)B * p.tiles;
+  p.one_launch = !many && capacity <= kPagedShortRows;
+  const int all = many ? 512 : 2048;
+  const long long most = p.items * ((capacity + p.unit - 1) / p.unit);
+  p.places = all / n_kv > 1 ? all / n_kv : 1;
+  if (p.places > most) p.places = most;
+  p.workers = many ? p.places : p.places + p.items;
+  p.slots = many ? 2 * p.workers : p.workers;
+  return p;
+}
+// (m, l) and O of every slot, and where the items begin.
+constexpr unsigned long long paged_begins_bytes(const PagedPlan& p) { return ((unsigned long long)p.items * 4 + 4 + 15) / 16 * 16; }
+constexpr unsigned long long paged_workspace_bytes(const PagedPlan& p, int n_kv) {
+  return p.one_launch ? 0
+                      : paged_begins_bytes(p) + (unsigned long long)p.slots * (unsigned long long)n_kv *
+                                                    (unsigned long long)p.slot_rows * (kAttnHeadDim + 2) * 4ull;
+}
+
 // Argument rules of the lsk_paged entry points (all but workspaces' sizes).
 int check_paged_pool(const lsk_paged_pool* pool);
 int check_paged_append(const lsk_paged_pool* pool, const void* k, long long k_batch, long long k_head, long long k_token,

@@ -365,16 +365,20 @@ struct PagedCopyArgs {
 };
 hipError_t launch_paged_copy(PagedCopyArgs a, hipStream_t stream);
 // Attention of T query tokens of B requests over their pages (paged_attention.hip).
+// begins: the first chunk, or unit, of each item (items + 1 words, left by the first
+// launch); part_ml / part_o: (m, l) and O, slots of slot_rows query rows, m in base 2.
 struct PagedAttentionArgs {
   PagedPool pool;
   const __bf16* q;
   const int *lens, *counts;
   __bf16* out;
+  int* begins;
+  float *part_ml, *part_o;
   size_t q_b, q_h, q_t;
-  int B, T, G, n_q;
+  int B, T, G, n_q, tiles, items, places, workers, least_units, slot_rows;
   float scale;
 };
-hipError_t launch_paged_attention(const PagedAttentionArgs& a, hipStream_t stream);
+hipError_t launch_paged_attention(const PagedAttentionArgs& a, const PagedPlan& plan, hipStream_t stream);
 
 // Number of scoring workgroups (= argmax partials per row) the lm_head
 // kernel uses for V vocab rows (V % 16 == 0): with NB = V / 16 row-blocks,

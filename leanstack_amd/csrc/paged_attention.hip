@@ -4,8 +4,21 @@
 //
 //   out = sum_i e^(s_i - m) v_i / sum_i e^(s_i - m),  s = scale q . k,
 // k and v being e4m3 bytes times a power of two per 16 rows and head (paged_cache.hip
-// has the format).  A wave takes two blocks, 32 key rows, a step, for up to 4 x 16 query
-// rows of one kv head:
+// has the format).
+//
+// An item is up to 64 (T n_q / n_kv rows are few) or 128 query rows of one request and kv
+// head, over the rows that its last one sees.  How many those are only the device
+// knows; every wave counts the items' units of key rows (lens is read once more by each).
+// Few query rows: an item is cut into chunks of equal length, as many as let all the
+// chunks run at once, one wave each.  Many: a kv head's items are laid end to end and
+// its workgroups take equal shares of the line (the end of one item, whole items, the start
+// of another), because an item more or less per CU would cost a whole round.  Whole items
+// are written to the output, parts as (m, l, O) in fp32 to the workspace, and a second
+// launch adds an item's parts up in their order.  A context that is short for certain runs
+// in one launch, an item per workgroup.
+//
+// Few query rows (decode, verify).  A wave takes two blocks, 32 key rows, a step, for up to
+// 4 x 16 query rows:
 //   bytes to bf16 with their scale, two values an instruction, exact;
 //   S = K Q^T on v_mfma_f32_16x16x32_bf16: a lane holds 2 x 4 scores of one query row;
 //   the running maximum m and sum l of the softmax in base 2, in fp32, m raised only
@@ -15,10 +28,19 @@
 //     blocks of V lie in memory as the other operand's lanes take them.
 // Nothing goes through LDS but the waves' sums at the end.
 //
-// P is rounded to bf16, at most 2^-9 of each weight, and l sums the rounded weights: the
+// Many query rows (prompts).  Four waves of 32 query rows share the key rows of a step (64)
+// through a ring in LDS, filled by DMA.  K is multiplied as it is, in 8 bits with its
+// scales, on v_mfma_scale_f32_32x32x64_f8f6f4: q, of 8 significant bits, is the sum of two
+// e4m3 numbers of 4, so two products at twice the rate of bf16 give the same scores
+// without converting K (q's parts are exact down to 2^-23 of the row's largest).  V is
+// converted on its way out of LDS for v_mfma_f32_32x32x16_bf16.
+//
+// P is rounded to bf16, at most 2^-8 of each weight, and l sums the rounded weights: the
 // result is exactly that of slightly other weights.
 
 #include <hip/hip_runtime.h>
+
+#include <type_traits>
 
 #include "lsk_internal.h"
 
@@ -26,13 +48,15 @@ namespace lsk {
 namespace {
 
 typedef unsigned u32x4_t __attribute__((ext_vector_type(4)));
+typedef int i32x8_t __attribute__((ext_vector_type(8)));
+typedef float f32x2_t __attribute__((ext_vector_type(2)));
 typedef float f32x4_t __attribute__((ext_vector_type(4)));
+typedef float f32x16_t __attribute__((ext_vector_type(16)));
 typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x4_t __attribute__((ext_vector_type(4)));
 
 constexpr int D = kAttnHeadDim;
-constexpr int kWaves = 4;
-constexpr int kThreads = 64 * kWaves;
+constexpr int kFewWaves = 4, kShortWaves = 8;  // of a workgroup for few query rows
 constexpr float kRaise = 8.f;
 constexpr float kFar = 0x1p30f;
 constexpr float kLowest = -3.402823466e38f;
@@ -42,6 +66,199 @@ __device__ __forceinline__ float neg_inf() { return -__builtin_huge_valf(); }
 __device__ __forceinline__ float power_of_two(int n) {
   return n < -126 ? 0.f : __builtin_bit_cast(float, (unsigned)(n + 127) << 23);
 }
+
+// Four bytes times a power of two.
+__device__ __forceinline__ bf16x4_t four(unsigned w, float scale) {
+  const bf16x2_t a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, scale, false);
+  const bf16x2_t b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, scale, true);
+  return bf16x4_t{a[0], a[1], b[0], b[1]};
+}
+__device__ __forceinline__ bf16x8_t eight(unsigned w0, unsigned w1, float scale0, float scale1) {
+  return __builtin_shufflevector(four(w0, scale0), four(w1, scale1), 0, 1, 2, 3, 4, 5, 6, 7);
+}
+
+// Bytes of a word that are NaN, as 0xff each.
+__device__ __forceinline__ unsigned nan_bytes(unsigned w) {
+  const unsigned t = ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
+  return (t >> 7) * 0xffu;
+}
+// ... as ones (e4m3 0x38).
+__device__ __forceinline__ unsigned nan_ones(unsigned w) { return nan_bytes(w) & 0x38383838u; }
+
+// What a request has, and what its query token t sees (those behind the last real one: as
+// many rows as that).
+struct Request {
+  int len, count, most;
+  __device__ __forceinline__ int visible(int t) const { return min(max(len - max(count - 1 - t, 0), 0), most); }
+};
+__device__ __forceinline__ Request request_of(const PagedAttentionArgs& a, int b) {
+  return {max(a.lens[b], 0), a.counts ? min(max(a.counts[b], 0), a.T) : a.T, 16 * a.pool.blocks};
+}
+
+// Query rows r0 .. + ROWS - 1 of request b: rows that the last one sees.
+template <int ROWS>
+__device__ __forceinline__ int item_rows(const PagedAttentionArgs& a, const Request& q, int tile) {
+  if (a.tiles == 1) return q.count > 0 ? q.visible(a.T - 1) : 0;
+  const int r0 = tile * ROWS;
+  if (q.count <= r0 / a.G) return 0;
+  return q.visible((min(r0 + ROWS, a.T * a.G) - 1) / a.G);
+}
+template <int ROWS>
+__device__ __forceinline__ int item_units(const PagedAttentionArgs& a, int item) {
+  constexpr int kUnit = ROWS == kPagedManyRows ? kPagedManyUnit : kPagedFewUnit;
+  const int b = a.tiles == 1 ? item : item / a.tiles;
+  return max((item_rows<ROWS>(a, request_of(a, b), item - b * a.tiles) + kUnit - 1) / kUnit, 1);
+}
+
+// Inclusive sums over a wave's lanes.
+__device__ __forceinline__ int wave_sums(int v) {
+  const int lane = threadIdx.x & 63;
+#pragma unroll
+  for (int s = 1; s < 64; s <<= 1) {
+    const int o = __shfl_up(v, s);
+    if (lane >= s) v += o;
+  }
+  return v;
+}
+
+// The items in 64 runs, one per lane: each(i) adds up over a lane's.
+template <typename Each>
+__device__ __forceinline__ int lane_items(const PagedAttentionArgs& a, Each each) {
+  const int lane = threadIdx.x & 63, n = (a.items + 63) / 64;
+  const int i0 = min(lane * n, a.items), i1 = min(i0 + n, a.items);
+  int sum = 0;
+  for (int i = i0; i < i1; ++i) sum += each(i);
+  return sum;
+}
+
+// The item at `place` of a line on which each(i) places are item i's, and the place where
+// that one begins; mine, before: the lane's items' places, and those in front of them.
+struct Found {
+  int item, begin;
+};
+template <typename Each>
+__device__ __forceinline__ Found item_at(const PagedAttentionArgs& a, int place, int mine, int before, Each each) {
+  const int lane = threadIdx.x & 63, n = (a.items + 63) / 64;
+  const int i1 = min((lane + 1) * n, a.items);
+  // the last lane whose items do not begin behind it
+  const int from = 63 - __builtin_clzll(__ballot(mine > 0 && before <= place));
+  int i = min(lane * n, a.items), at = before;
+  for (; i < i1 - 1; ++i) {
+    const int here = each(i);
+    if (place < at + here) break;
+    at += here;
+  }
+  return {__builtin_amdgcn_readlane(i, from), __builtin_amdgcn_readlane(at, from)};
+}
+
+// Where the items begin, for the second launch.
+template <typename Each>
+__device__ __forceinline__ void write_begins(const PagedAttentionArgs& a, int before, int total, Each each) {
+  const int lane = threadIdx.x & 63, n = (a.items + 63) / 64;
+  const int i1 = min((lane + 1) * n, a.items);
+  for (int i = min(lane * n, a.items), at = before; i < i1; ++i) {
+    a.begins[i] = at;
+    at += each(i);
+  }
+  if (lane == 0) a.begins[a.items] = total;
+}
+
+// Worker w's chunk: units [first, last) of an item (none: first = last).
+struct Chunk {
+  int item, first, last;
+  bool whole;
+};
+template <int ROWS>
+__device__ __forceinline__ Chunk chunk_of(const PagedAttentionArgs& a, int w, bool write) {
+  auto units_of = [&](int i) { return item_units<ROWS>(a, i); };
+  const int total = __builtin_amdgcn_readlane(wave_sums(lane_items(a, units_of)), 63);
+  const int most = max((total + a.places - 1) / a.places, a.least_units);  // units of a chunk
+  auto chunks_of = [&](int i) { return (item_units<ROWS>(a, i) + most - 1) / most; };
+  const int mine = lane_items(a, chunks_of), up_to = wave_sums(mine);
+  const int chunks = __builtin_amdgcn_readlane(up_to, 63);
+  if (write) write_begins(a, up_to - mine, chunks, chunks_of);
+  if (w >= chunks) return {0, 0, 0, false};
+  const Found f = item_at(a, w, mine, up_to - mine, chunks_of);
+  const int units = item_units<ROWS>(a, f.item), n = (units + most - 1) / most;
+  const int each = (units + n - 1) / n;  // (at most `most`: none of the n is empty)
+  const int first = (w - f.begin) * each;
+  return {f.item, first, min(first + each, units), n == 1};
+}
+
+// Where worker w's share of the line begins.
+__device__ __forceinline__ int share_begin(long long units, int w, int workers) { return (int)(units * w / workers); }
+
+// The item in which worker w's share begins, the units of it in front of the share, and
+// the share's length.
+struct Share {
+  int item, skip, units;
+};
+template <int ROWS>
+__device__ __forceinline__ Share share_of(const PagedAttentionArgs& a, int w, bool write) {
+  auto units_of = [&](int i) { return item_units<ROWS>(a, i); };
+  const int mine = lane_items(a, units_of), up_to = wave_sums(mine);
+  const int total = __builtin_amdgcn_readlane(up_to, 63);
+  if (write) write_begins(a, up_to - mine, total, units_of);
+  const int begin = share_begin(total, w, a.workers);
+  const Found f = item_at(a, begin, mine, up_to - mine, units_of);
+  return {f.item, begin - f.begin, share_begin(total, w + 1, a.workers) - begin};
+}
+
+struct Part {
+  float* o;   // [rows][D]
+  float* ml;  // [rows][2]
+};
+__device__ __forceinline__ Part part_of(const PagedAttentionArgs& a, size_t slot) {
+  return {a.part_o + slot * a.slot_rows * D, a.part_ml + slot * a.slot_rows * 2};
+}
+
+// The weights of V and the running sums.
+//
+// Exponents are s c2 - m with one rounding, m being the rounded top c2: far from zero
+// (kFar) its rounding error would be more than 2^x holds.  There scores that are not
+// equal are 2^6 and more apart in base 2, so any factor gives the same weights, if m's
+// order stays: the next power of two above c2, whose products are exact.
+// m starts at the lowest finite number, so that scores of -inf have no weight; whether any row
+// was seen is known apart.
+struct Sums {
+  float m, l, c2;
+};
+__device__ __forceinline__ Sums no_sums(float c2) { return {kLowest, 0.f, c2}; }
+
+// Raises m to the row's maximum `top` and returns what the sums so far are multiplied by.
+__device__ __forceinline__ float raised(Sums& st, float top, float c2) {
+  const bool raise = top * st.c2 > st.m + kRaise;
+  const float above = __builtin_bit_cast(float, (__builtin_bit_cast(unsigned, c2) + 0x007fffffu) & 0x7f800000u);
+  st.c2 = !raise ? st.c2 : fabsf(top * c2) < kFar ? c2 : above;
+  const float mx = top * st.c2;
+  const float f = raise ? __builtin_amdgcn_exp2f(st.m - mx) : 1.f;
+  st.m = raise ? mx : st.m;
+  st.l *= f;
+  return f;
+}
+
+// What brings scores to base 2, and what is done to q's bits: a negative scale's sign goes
+// into q, and a scale of zero leaves zeros (an unseen row's score of -inf has to
+// meet a factor above zero), infinities and NaN of q aside.
+struct Scale {
+  float c2;
+  unsigned flip;
+  bool zero;
+};
+__device__ __forceinline__ Scale scale_of(float scale) {
+  const bool zero = scale == 0.f;
+  return {zero ? 1.f : fabsf(scale) * 1.44269504088896341f, scale < 0.f ? 0x80008000u : 0u, zero};
+}
+__device__ __forceinline__ unsigned scaled_bits(unsigned w, const Scale& sc) {
+  w ^= sc.flip;
+  if (sc.zero) {
+    const bool low = (w & 0x7f80u) == 0x7f80u, high = (w & 0x7f800000u) == 0x7f800000u;
+    w &= (low ? 0xffffu : 0u) | (high ? 0xffff0000u : 0u);
+  }
+  return w;
+}
+
+// ------------------------------------------------------------------ few query rows
 
 // The four lanes that hold a query row's scores: c, c + 16, c + 32, c + 48.
 __device__ __forceinline__ float rows_max(float v) {
@@ -53,108 +270,58 @@ __device__ __forceinline__ float rows_sum(float v) {
   return v + __shfl_xor(v, 32);
 }
 
-// Eight bytes times a power of two.
-__device__ __forceinline__ bf16x8_t eight(unsigned w0, unsigned w1, float scale0, float scale1) {
-  const bf16x2_t a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w0, scale0, false);
-  const bf16x2_t b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w0, scale0, true);
-  const bf16x2_t c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w1, scale1, false);
-  const bf16x2_t d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w1, scale1, true);
-  return bf16x8_t{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
-}
-
-// Bytes of a word that are NaN, as 0xff each.
-__device__ __forceinline__ unsigned nan_bytes(unsigned w) {
-  const unsigned t = ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
-  return (t >> 7) * 0xffu;
-}
-
-// A wave's softmax state for 16 query rows: lane (c, g) holds row c, of O the dims
-// 16 i + 4 g .. + 3, of l the share of the lane's scores, and of m the factor c2 that
-// takes its scores to base 2.  m = -inf: no row seen.
+// A wave's state for 16 query rows: lane (c, g) holds row c, of O the dims 16 i + 4 g .. + 3,
+// of l the share of the lane's scores.
 struct State {
-  float m, l, c2;
+  Sums sums;
   f32x4_t o[8];
 };
 
-__device__ __forceinline__ State empty_state(float c2) {
-  State st;
-  st.m = neg_inf();
-  st.l = 0.f;
-  st.c2 = c2;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) st.o[i] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-  return st;
-}
-
-// 1 KB of a block, 16 bytes a lane; zeros and no access where there is none.
+// 1 KB of a block, 16 bytes a lane; zeros and no access where there is none.  Past the caches
+// (nt): a block is read once, by the four waves of a workgroup by turns (64 requests over 17..8001 rows:
+// 105 us for 116).
+constexpr int kStream = 2;
 __device__ __forceinline__ u32x4_t load_1k(const unsigned char* blocks, int at, int half) {
   const __amdgpu_buffer_rsrc_t block = __builtin_amdgcn_make_buffer_rsrc(
       const_cast<unsigned char*>(blocks) + (size_t)(at < 0 ? 0 : at) * kPagedBlockBytes, (short)0,
       at < 0 ? 0 : kPagedBlockBytes, 0x00020000);
-  return __builtin_bit_cast(u32x4_t, __builtin_amdgcn_raw_buffer_load_b128(block, (threadIdx.x & 63) * 16, half * 1024, 0));
+  return __builtin_bit_cast(u32x4_t, __builtin_amdgcn_raw_buffer_load_b128(block, (threadIdx.x & 63) * 16, half * 1024, kStream));
 }
 
 // The weights P of a step as the operand of the second product, and m, l, O brought to
-// the new maximum.  s[m][i]: row 16 m + 4 g + i of the step.  seen(m, i): whether the lane's
-// query row sees it (MASK).
-//
-// Exponents are s c2 - m with one rounding, m being the rounded top c2: far from zero
-// (kFar) its rounding error would be more than 2^x holds.  There scores that are not
-// equal are 2^6 and more apart in base 2, so any factor gives the same weights, if m's
-// order stays: the next power of two above c2, whose products are exact.
-template <bool MASK, typename Seen>
-__device__ __forceinline__ bf16x8_t step_weights(f32x4_t (&s)[2], float c2, State& st, Seen seen) {
-  bool any = !MASK;
-  if constexpr (MASK) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const bool ok = seen(i / 4, i % 4);
-      any |= ok;
-      if (!ok) s[i / 4][i % 4] = neg_inf();
-    }
-  }
+// the new maximum.  s[m][i]: row 16 m + 4 g + i of the step, -inf where it is not seen.
+__device__ __forceinline__ bf16x8_t step_weights(const f32x4_t (&s)[2], float c2, State& st) {
   float top = fmaxf(s[0][0], s[0][1]);
 #pragma unroll
   for (int i = 2; i < 8; ++i) top = fmaxf(top, s[i / 4][i % 4]);
-  // (a row that is seen raises m from -inf whatever its score: sums of 0 are then NaN)
-  const float mine = any ? fmaxf(top * st.c2, kLowest) : neg_inf();
-  if (__ballot(mine > st.m + kRaise)) {
-    top = rows_max(top);
-    const bool raise = rows_max(mine) > st.m + kRaise;
-    const float above = __builtin_bit_cast(float, (__builtin_bit_cast(unsigned, c2) + 0x007fffffu) & 0x7f800000u);
-    st.c2 = !raise ? st.c2 : fabsf(top * c2) < kFar ? c2 : above;
-    const float mx = fmaxf(top * st.c2, kLowest);
-    const float f = raise ? __builtin_amdgcn_exp2f(st.m - mx) : 1.f;
-    st.m = raise ? mx : st.m;
-    st.l *= f;
+  if (__ballot(top * st.sums.c2 > st.sums.m + kRaise)) {
+    const float f = raised(st.sums, rows_max(top), c2);
 #pragma unroll
     for (int i = 0; i < 8; ++i)
 #pragma unroll
       for (int e = 0; e < 4; ++e) st.o[i][e] *= f;
   }
-  const float m = st.m == neg_inf() ? 0.f : st.m;
   bf16x8_t p;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i / 4][i % 4], st.c2, -m));
-    if (MASK && !seen(i / 4, i % 4)) e = 0.f;
-    p[i] = static_cast<__bf16>(e);
-  }
+  for (int i = 0; i < 8; ++i)
+    p[i] = static_cast<__bf16>(__builtin_amdgcn_exp2f(__builtin_fmaf(s[i / 4][i % 4], st.sums.c2, -st.sums.m)));
   const bf16x2_t ones = {static_cast<__bf16>(1.f), static_cast<__bf16>(1.f)};
 #pragma unroll
-  for (int i = 0; i < 8; i += 2) st.l = __builtin_amdgcn_fdot2_f32_bf16(bf16x2_t{p[i], p[i + 1]}, ones, st.l, false);
+  for (int i = 0; i < 8; i += 2)
+    st.sums.l = __builtin_amdgcn_fdot2_f32_bf16(bf16x2_t{p[i], p[i + 1]}, ones, st.sums.l, false);
   return p;
 }
 
-// What the wave's lane l knows of block 2 (first + kWaves (l / 2)) + l % 2: its place in the pool
+// What the wave's lane l knows of block 2 (first + NW (l / 2)) + l % 2: its place in the pool
 // (-1: no row of it is read) and its scales.
 struct Blocks {
   int at;
   float ks, vs;
 };
+template <int NW>
 __device__ __forceinline__ Blocks blocks_from(const PagedPool& p, int b, int j, int first, int end) {
   const int lane = threadIdx.x & 63;
-  const int block = 2 * (first + kWaves * (lane >> 1)) + (lane & 1);
+  const int block = 2 * (first + NW * (lane >> 1)) + (lane & 1);
   Blocks r = {-1, 1.f, 1.f};
   if (block < end) {
     const int page = p.table[(size_t)b * p.table_ld + (block >> p.page_shift)];
@@ -167,56 +334,98 @@ __device__ __forceinline__ Blocks blocks_from(const PagedPool& p, int b, int j, 
   return r;
 }
 
-// Grid: kv head (fastest), request, 16 NT query rows.
+// threadIdx.x, anew: what is made of it is not kept in registers from one item to the next.
+__device__ __forceinline__ int own_thread() {
+  int tid = threadIdx.x;
+  asm volatile("" : "+v"(tid));
+  return tid;
+}
+
+// Query rows of more than one tile are kept in LDS (16 registers each).
 template <int NT>
-__global__ __launch_bounds__(kThreads) void paged_attention_kernel(PagedAttentionArgs a) {
-  __shared__ float os[kWaves][16][D + 4];
-  __shared__ float ms[kWaves][16], ls[kWaves][16];
+constexpr bool kQueriesInLds = NT > 1;
+template <int NT>
+struct Queries {
+  u32x4_t q[kQueriesInLds<NT> ? NT : 1][4][64];
+};
+
+// A wave's steps first_step + i NW (up to stop_step), i = 0, 1, .., for query rows 16 NT tile .. of
+// kv head j of request b.  any[n]: whether the lane has met a row that its query row sees.
+template <int NT, int NW>
+__device__ __forceinline__ void few_steps(const PagedAttentionArgs& a, Queries<NT>& lds, int j, int b, int tile, int first_step,
+                                          int stop_step, const Request& rq, State (&st)[NT], bool (&any)[NT]) {
+  constexpr bool kInLds = kQueriesInLds<NT>;
+  constexpr int kAhead = NT > 2 ? 1 : 2;  // steps on their way
   const PagedPool& p = a.pool;
-  const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  int id = blockIdx.x;
-  const int j = id % p.n_kv;
-  id /= p.n_kv;
-  const int b = id % a.B;
-  const int r0 = id / a.B * 16 * NT;
-  const int rows = a.T * a.G;
+  const int lane = own_thread() & 63, c = lane & 15, g = lane >> 4;
+  const int r0 = tile * 16 * NT, rows = a.T * a.G;
+  const int least = rq.count > r0 / a.G ? rq.visible(r0 / a.G) : 0;
+  const int end_block = (item_rows<16 * NT>(a, rq, tile) + 15) / 16, stop = min(stop_step, (end_block + 1) / 2);
+  // 32 steps' blocks in the lanes at a time; the first steps' rows are on their way before anything else.
+  Blocks blocks;
+  int here = 0;
+  struct Held {
+    u32x4_t k[2][2], v[2][2];
+  } held[kAhead];
+  auto load_k = [&](int i, u32x4_t (&kq)[2][2]) __attribute__((always_inline)) {
+#pragma unroll
+    for (int m = 0; m < 2; ++m) {
+      const int at = i < here ? __builtin_amdgcn_readlane(blocks.at, 2 * i + m) : -1;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) kq[m][h] = load_1k(p.k, at, h);
+    }
+  };
+  auto load_v = [&](int i, u32x4_t (&vq)[2][2]) __attribute__((always_inline)) {
+#pragma unroll
+    for (int m = 0; m < 2; ++m) {
+      const int at = i < here ? __builtin_amdgcn_readlane(blocks.at, 2 * i + m) : -1;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) vq[m][h] = load_1k(p.v, at, h);
+    }
+  };
+  auto begin_group = [&](int first) __attribute__((always_inline)) {
+    blocks = blocks_from<NW>(p, b, j, first, end_block);
+    here = min(32, (stop - first + NW - 1) / NW);
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      load_k(i, held[i].k);
+      load_v(i, held[i].v);
+    }
+  };
+  begin_group(first_step);
 
-  const int len = max(a.lens[b], 0);
-  const int count = a.counts ? min(max(a.counts[b], 0), a.T) : a.T;
-  // Rows that query t sees (those behind the last real one: as many as that).
-  auto visible = [&](int t) { return min(max(len - max(count - 1 - t, 0), 0), 16 * p.blocks); };
-  const int t_first = r0 / a.G, t_last = min(r0 + 16 * NT, rows) - 1;
-  const int least = count > t_first ? visible(t_first) : 0;
-  const int most = count > t_first ? visible(t_last / a.G) : 0;
-  const int end_block = (most + 15) / 16, steps = (end_block + 1) / 2;
-
-  bf16x8_t q[NT][4];
+  const Scale sc = scale_of(a.scale);
+  bf16x8_t q[kInLds ? 1 : NT][4];
   int limit[NT];
-  State st[NT];
-  const float c2 = fabsf(a.scale) * 1.44269504088896341f;
-  const unsigned flip = a.scale < 0.f ? 0x80008000u : 0u;
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
+    any[n] = false;
     const int r = min(r0 + 16 * n + c, rows - 1);
     const int t = r / a.G, h = j * a.G + r % a.G;
-    limit[n] = visible(t);
-    st[n] = empty_state(c2);
+    limit[n] = rq.visible(t);
+    st[n].sums = no_sums(sc.c2);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) st[n].o[i] = f32x4_t{0.f, 0.f, 0.f, 0.f};
     const __bf16* from = a.q + (size_t)b * a.q_b + (size_t)h * a.q_h + (size_t)t * a.q_t + 16 * g;
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
       u32x4_t w = *reinterpret_cast<const u32x4_t*>(from + 64 * (k >> 1) + 8 * (k & 1));
 #pragma unroll
-      for (int e = 0; e < 4; ++e) w[e] ^= flip;
-      q[n][k] = __builtin_bit_cast(bf16x8_t, w);
+      for (int e = 0; e < 4; ++e) w[e] = scaled_bits(w[e], sc);
+      if constexpr (kInLds)
+        lds.q[n][k][lane] = w;  // (a wave's own)
+      else
+        q[n][k] = __builtin_bit_cast(bf16x8_t, w);
     }
   }
+  if constexpr (kInLds) wave_lds_order();
 
-  for (int first = wave; first < steps; first += 32 * kWaves) {
-    const Blocks blocks = blocks_from(p, b, j, first, end_block);
-    const int here = min(32, (steps - first + kWaves - 1) / kWaves);
-    for (int i = 0; i < here; ++i) {
-      const int row0 = 32 * (first + kWaves * i);
+  for (int first = first_step; first < stop; first += 32 * NW) {
+    if (first != first_step) begin_group(first);
+    auto step = [&](int i, Held& hold) __attribute__((always_inline)) {
+      u32x4_t (&kq)[2][2] = hold.k;
+      u32x4_t (&vq)[2][2] = hold.v;
+      const int row0 = 32 * (first + NW * i);
       int at[2];
       float ks[2], vs[2];
 #pragma unroll
@@ -225,34 +434,46 @@ __global__ __launch_bounds__(kThreads) void paged_attention_kernel(PagedAttentio
         ks[m] = row_lane(blocks.ks, 2 * i + m);
         vs[m] = row_lane(blocks.vs, 2 * i + m);
       }
-      u32x4_t kq[2][2], vq[2][2];
-#pragma unroll
-      for (int m = 0; m < 2; ++m)
-#pragma unroll
-        for (int h = 0; h < 2; ++h) kq[m][h] = load_1k(p.k, at[m], h);
-#pragma unroll
-      for (int m = 0; m < 2; ++m)
-#pragma unroll
-        for (int h = 0; h < 2; ++h) vq[m][h] = load_1k(p.v, at[m], h);
-
       f32x4_t s[NT][2];
 #pragma unroll
-      for (int m = 0; m < 2; ++m)
+      for (int k = 0; k < 4; ++k) {
+        bf16x8_t key[2];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const bf16x8_t key = eight(kq[m][k >> 1][2 * (k & 1)], kq[m][k >> 1][2 * (k & 1) + 1], ks[m], ks[m]);
+        for (int m = 0; m < 2; ++m) key[m] = eight(kq[m][k >> 1][2 * (k & 1)], kq[m][k >> 1][2 * (k & 1) + 1], ks[m], ks[m]);
 #pragma unroll
-          for (int n = 0; n < NT; ++n)
-            s[n][m] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(key, q[n][k], k ? s[n][m] : f32x4_t{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
+        for (int n = 0; n < NT; ++n) {
+          bf16x8_t query;
+          if constexpr (kInLds)
+            query = __builtin_bit_cast(bf16x8_t, lds.q[n][k][lane]);
+          else
+            query = q[n][k];
+#pragma unroll
+          for (int m = 0; m < 2; ++m)
+            s[n][m] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(key[m], query, k ? s[n][m] : f32x4_t{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
         }
+      }
+      load_k(i + kAhead, kq);  // on its way while this step's weights and second product run
       const bool masked = row0 + 32 > least || at[0] < 0 || at[1] < 0;
-      bf16x8_t w[NT];
-      if (!masked) {
+      auto seen = [&](int n, int i) { return row0 + 16 * (i / 4) + 4 * g + i % 4 < limit[n] && at[i / 4] >= 0; };
+      if (masked) {
 #pragma unroll
-        for (int n = 0; n < NT; ++n) w[n] = step_weights<false>(s[n], c2, st[n], [](int, int) { return true; });
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const bool ok = seen(n, i);
+            any[n] |= ok;
+            s[n][i / 4][i % 4] = ok ? s[n][i / 4][i % 4] : neg_inf();
+          }
       } else {
-        // (a weight of zero does not take a NaN out of a product: those become zero here
-        // and come back for the query rows that see them)
+#pragma unroll
+        for (int n = 0; n < NT; ++n) any[n] = true;
+      }
+      bf16x8_t w[NT];
+#pragma unroll
+      for (int n = 0; n < NT; ++n) w[n] = step_weights(s[n], sc.c2, st[n]);
+      if (masked) {
+        // A weight of zero does not take a NaN out of a product: those become zero here and
+        // come back for the query rows that see them.
         unsigned found = 0;
 #pragma unroll
         for (int m = 0; m < 2; ++m)
@@ -260,28 +481,23 @@ __global__ __launch_bounds__(kThreads) void paged_attention_kernel(PagedAttentio
           for (int h = 0; h < 2; ++h)
 #pragma unroll
             for (int e = 0; e < 4; ++e) found |= nan_bytes(vq[m][h][e]);
-        const bool special = __ballot(found != 0) != 0;
+        if (__ballot(found != 0)) {
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          auto seen = [&](int m, int e) { return row0 + 16 * m + 4 * g + e < limit[n] && at[m] >= 0; };
-          w[n] = step_weights<true>(s[n], c2, st[n], seen);
-          if (special) {
+          for (int n = 0; n < NT; ++n) {
             bf16x8_t sees;
 #pragma unroll
-            for (int e = 0; e < 8; ++e) sees[e] = static_cast<__bf16>(seen(e / 4, e % 4) ? 1.f : 0.f);
+            for (int e = 0; e < 8; ++e) sees[e] = static_cast<__bf16>(seen(n, e) ? 1.f : 0.f);
 #pragma unroll
             for (int d = 0; d < 8; ++d) {
-              const bf16x8_t nans = eight(nan_bytes(vq[0][d & 1][d >> 1]) & 0x38383838u,
-                                          nan_bytes(vq[1][d & 1][d >> 1]) & 0x38383838u, 1.f, 1.f);
+              const bf16x8_t nans = eight(nan_ones(vq[0][d & 1][d >> 1]), nan_ones(vq[1][d & 1][d >> 1]), 1.f, 1.f);
               const f32x4_t met =
                   __builtin_amdgcn_mfma_f32_16x16x32_bf16(nans, sees, f32x4_t{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
 #pragma unroll
               for (int e = 0; e < 4; ++e)
                 if (met[e] > 0.f) st[n].o[d][e] = __builtin_nanf("");
+              __builtin_amdgcn_sched_barrier(0);  // (one at a time: registers)
             }
           }
-        }
-        if (special) {
 #pragma unroll
           for (int m = 0; m < 2; ++m)
 #pragma unroll
@@ -297,57 +513,530 @@ __global__ __launch_bounds__(kThreads) void paged_attention_kernel(PagedAttentio
         for (int n = 0; n < NT; ++n)
           st[n].o[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(value, w[n], st[n].o[d], 0, 0, 0);
       }
+      load_v(i + kAhead, vq);
+    };
+    for (int i = 0; i < here; i += kAhead) {
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u)
+        if (u == 0 || i + u < here) step(i + u, held[u]);
     }
   }
 
+}
+
+// Whether one of the row's four lanes has met a row; all lanes of the wave ask.
+__device__ __forceinline__ bool met_any(bool any, int c) { return (__ballot(any) >> c & 0x0001000100010001ull) != 0; }
+
+// Grid: kv head (fastest), four of its workers: a wave each.
+template <int NT>
+__global__ __launch_bounds__(64 * kFewWaves, 2) void few_attention_kernel(PagedAttentionArgs a) {
+  __shared__ Queries<NT> queries[kFewWaves];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int j = blockIdx.x % a.pool.n_kv, w = (blockIdx.x / a.pool.n_kv) * kFewWaves + wave;
+  if (w >= a.workers) return;
+  const Chunk ch = chunk_of<16 * NT>(a, w, j == 0 && w == 0);
+  if (ch.first == ch.last) return;
+  const int b = a.tiles == 1 ? ch.item : ch.item / a.tiles, tile = ch.item - b * a.tiles;
+  State st[NT];
+  bool any[NT];
+  const Request rq = request_of(a, b);
+  few_steps<NT, 1>(a, queries[wave], j, b, tile, ch.first, ch.last, rq, st, any);
+  const int lane = own_thread() & 63, c = lane & 15, g = lane >> 4;
+  const Part part = part_of(a, (size_t)j * a.workers + w);
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
-    if (n) __syncthreads();
-    const float l = rows_sum(st[n].l);
+    const int r = 16 * n + c, row = tile * 16 * NT + r;
+    const float l = rows_sum(st[n].sums.l);
+    const bool met = met_any(any[n], c);
+    if (row >= a.T * a.G) continue;
+    if (ch.whole) {
+      const int t = row / a.G, h = j * a.G + row % a.G;
+      const bool none = t >= rq.count || !met;
+      const float share = none ? 0.f : 1.f / l;  // (of a sum of 0: infinite, and 0 times that NaN)
+      __bf16* out = a.out + (((size_t)b * a.T + t) * a.n_q + h) * D + 4 * g;
 #pragma unroll
-    for (int d = 0; d < 8; ++d) *reinterpret_cast<f32x4_t*>(&os[wave][c][16 * d + 4 * g]) = st[n].o[d];
-    if (g == 0) {
-      ms[wave][c] = st[n].m;
-      ls[wave][c] = l;
+      for (int d = 0; d < 8; ++d) {
+        bf16x4_t o;
+#pragma unroll
+        for (int u = 0; u < 4; ++u) o[u] = static_cast<__bf16>(none ? 0.f : st[n].o[d][u] * share);
+        *reinterpret_cast<bf16x4_t*>(out + 16 * d) = o;
+      }
+    } else {
+      float* out = part.o + (size_t)r * D + 4 * g;
+#pragma unroll
+      for (int d = 0; d < 8; ++d) *reinterpret_cast<f32x4_t*>(out + 16 * d) = st[n].o[d];
+      if (g == 0) *reinterpret_cast<f32x2_t*>(part.ml + r * 2) = f32x2_t{met ? st[n].sums.m : neg_inf(), l};
+    }
+  }
+}
+
+// One launch, an item per workgroup whose waves take its steps by turns.  Grid: kv head (fastest), item.
+template <int NT>
+__global__ __launch_bounds__(64 * kShortWaves, 2) void short_attention_kernel(PagedAttentionArgs a) {
+  constexpr int NW = kShortWaves;
+  __shared__ union {
+    Queries<NT> queries[NW];
+    float os[NW][16][D + 4];
+  } sh;
+  __shared__ float ms[NW][16], ls[NW][16];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int j = blockIdx.x % a.pool.n_kv, item = blockIdx.x / a.pool.n_kv;
+  const int b = a.tiles == 1 ? item : item / a.tiles, tile = item - b * a.tiles;
+  State st[NT];
+  bool any[NT];
+  const Request rq = request_of(a, b);
+  few_steps<NT, NW>(a, sh.queries[wave], j, b, tile, wave, 1 << 26, rq, st, any);
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    __syncthreads();  // the queries, or the last tile's sums, have been read
+    const int tid = own_thread();
+    const float l = rows_sum(st[n].sums.l);
+    {
+      const int c = tid & 15, g = tid >> 4 & 3;
+#pragma unroll
+      for (int d = 0; d < 8; ++d) *reinterpret_cast<f32x4_t*>(&sh.os[wave][c][16 * d + 4 * g]) = st[n].o[d];
+      const bool met = met_any(any[n], c);
+      if (g == 0) {
+        ms[wave][c] = met ? st[n].sums.m : neg_inf();
+        ls[wave][c] = l;
+      }
     }
     __syncthreads();
-    // 16 lanes to a query row, 8 dims each
-    const int r = threadIdx.x >> 4;
-    const int row = r0 + 16 * n + r;
-    if (row < rows) {
+    // 32 lanes to a query row, 4 dims each
+    static_assert(NW * 64 == 16 * 32, "lanes to a query row");
+    const int r = tid >> 5, d0 = (tid & 31) * 4;
+    const int row = (tile * NT + n) * 16 + r;
+    if (row < a.T * a.G) {
       const int t = row / a.G, h = j * a.G + row % a.G;
-      float m = neg_inf(), sum = 0.f, w[kWaves];
+      float m = neg_inf(), sum = 0.f, w[NW];
 #pragma unroll
-      for (int i = 0; i < kWaves; ++i) m = fmaxf(m, ms[i][r]);
+      for (int i = 0; i < NW; ++i) m = fmaxf(m, ms[i][r]);
 #pragma unroll
-      for (int i = 0; i < kWaves; ++i) {
+      for (int i = 0; i < NW; ++i) {
         w[i] = ms[i][r] == m ? 1.f : __builtin_amdgcn_exp2f(ms[i][r] - m);
         sum += w[i] * ls[i][r];
       }
-      const bool none = t >= count || m == neg_inf();
-      bf16x8_t o;
+      const bool none = t >= rq.count || m == neg_inf();
+      const float share = none ? 0.f : 1.f / sum;
+      f32x4_t x = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int e = 0; e < 8; e += 4) {
-        f32x4_t x = {0.f, 0.f, 0.f, 0.f};
+      for (int i = 0; i < NW; ++i) x += w[i] * *reinterpret_cast<const f32x4_t*>(&sh.os[i][r][d0]);
+      bf16x4_t o;
 #pragma unroll
-        for (int i = 0; i < kWaves; ++i) x += w[i] * *reinterpret_cast<const f32x4_t*>(&os[i][r][8 * (threadIdx.x & 15) + e]);
-#pragma unroll
-        for (int u = 0; u < 4; ++u) o[e + u] = static_cast<__bf16>(none ? 0.f : x[u] / sum);
-      }
-      *reinterpret_cast<bf16x8_t*>(a.out + (((size_t)b * a.T + t) * a.n_q + h) * D + 8 * (threadIdx.x & 15)) = o;
+      for (int u = 0; u < 4; ++u) o[u] = static_cast<__bf16>(none ? 0.f : x[u] * share);
+      *reinterpret_cast<bf16x4_t*>(a.out + (((size_t)b * a.T + t) * a.n_q + h) * D + d0) = o;
     }
+  }
+}
+
+// Adds up the parts of items that were cut.  Grid: kv head (fastest), item, 16 rows of it.
+constexpr int kJoinThreads = 256;
+template <bool MANY>
+__global__ __launch_bounds__(kJoinThreads) void join_kernel(PagedAttentionArgs a, int rows) {
+  int id = blockIdx.x;
+  const int j = id % a.pool.n_kv;
+  id /= a.pool.n_kv;
+  const int groups = rows / 16;
+  const int item = id / groups, group = id % groups;
+  const int begin = a.begins[item], end = a.begins[item + 1];
+  // parts `from` .. `last`: a slot per chunk, or the second slot of the worker that has the first unit
+  // and the first slots of those up to the last unit's
+  int from = begin, last = end - 1;
+  const int units = MANY ? a.begins[a.items] : 0;
+  if constexpr (MANY) {
+    auto worker_of = [&](int unit) {
+      int w = (int)((long long)unit * a.workers / units);
+      while (share_begin(units, w + 1, a.workers) <= unit) ++w;
+      while (share_begin(units, w, a.workers) > unit) --w;
+      return w;
+    };
+    from = worker_of(begin), last = worker_of(end - 1);
+  }
+  if (from == last) return;
+  const int b = a.tiles == 1 ? item : item / a.tiles, tile = item - b * a.tiles;
+  const int r = group * 16 + (threadIdx.x >> 4), row = tile * rows + r, d0 = (threadIdx.x & 15) * 8;
+  if (row >= a.T * a.G) return;
+  const int t = row / a.G, h = j * a.G + row % a.G;
+  float m = neg_inf(), l = 0.f;
+  f32x4_t o[2] = {};
+  // kJoinAhead parts on their way at a time (past the last the last again, unused)
+  constexpr int kJoinAhead = 4;
+  for (int w0 = from; w0 <= last; w0 += kJoinAhead) {
+    f32x2_t ml[kJoinAhead];
+    f32x4_t x[kJoinAhead][2];
+#pragma unroll
+    for (int i = 0; i < kJoinAhead; ++i) {
+      const int w = min(w0 + i, last);
+      const size_t slot = (size_t)j * a.workers + w;
+      const Part part = part_of(a, MANY ? slot * 2 + (w == from ? 1 : 0) : slot);
+      ml[i] = *reinterpret_cast<const f32x2_t*>(part.ml + r * 2);
+#pragma unroll
+      for (int e = 0; e < 2; ++e) x[i][e] = *reinterpret_cast<const f32x4_t*>(part.o + (size_t)r * D + d0 + 4 * e);
+    }
+#pragma unroll
+    for (int i = 0; i < kJoinAhead; ++i) {
+      if (w0 + i > last) break;
+      if (MANY && share_begin(units, w0 + i, a.workers) == share_begin(units, w0 + i + 1, a.workers))
+        continue;  // (fewer units than workers: one without a share)
+      const float top = fmaxf(m, ml[i][0]);
+      const float was = m == top ? 1.f : __builtin_amdgcn_exp2f(m - top);
+      const float now = ml[i][0] == top ? 1.f : __builtin_amdgcn_exp2f(ml[i][0] - top);
+      l = l * was + ml[i][1] * now;
+#pragma unroll
+      for (int e = 0; e < 2; ++e) o[e] = o[e] * was + x[i][e] * now;
+      m = top;
+    }
+  }
+  const bool none = t >= request_of(a, b).count || m == neg_inf();
+  const float share = none ? 0.f : 1.f / l;
+  bf16x8_t x;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) x[e] = static_cast<__bf16>(none ? 0.f : o[e / 4][e % 4] * share);
+  *reinterpret_cast<bf16x8_t*>(a.out + (((size_t)b * a.T + t) * a.n_q + h) * D + d0) = x;
+}
+
+// ------------------------------------------------------------------ many query rows
+
+constexpr int kManyWaves = 4;
+constexpr int kManyRows = 32 * kManyWaves;
+constexpr int kStep = 64;                           // key rows, one block per wave
+constexpr int kRing = 3;
+constexpr int kSlot = 2 * 4 * kPagedBlockBytes;     // K, then V, of a step
+static_assert(kManyRows == kPagedManyRows && kStep == kPagedManyUnit, "as the host counts them");
+
+// Both halves' values of a lane pair 32 apart, in both lanes.  (The compiler takes
+// a swap of a value with itself for two equal results: it is given a copy that it
+// does not know to be one.)
+__device__ __forceinline__ f32x2_t both_halves(float v) {
+  const unsigned a = __builtin_bit_cast(unsigned, v);
+  unsigned b = a;
+  asm("" : "+v"(b));
+  const auto r = __builtin_amdgcn_permlane32_swap(a, b, false, false);
+  return f32x2_t{__builtin_bit_cast(float, (unsigned)r[0]), __builtin_bit_cast(float, (unsigned)r[1])};
+}
+
+struct ManyShared {
+  unsigned char ring[kRing * kSlot];
+};
+
+typedef __attribute__((address_space(3))) const unsigned char lds_byte_t;
+__device__ __forceinline__ u32x4_t lds_16(lds_byte_t* at) {
+  return *reinterpret_cast<__attribute__((address_space(3))) const u32x4_t*>(at);
+}
+
+// q as two e4m3 numbers per value: 32 values in units of 2^e, and what they leave in units of 2^(e - 4).
+struct QueryParts {
+  i32x8_t high[2], low[2];  // dims 64 k + 32 h .. + 31
+  int high_scale, low_scale;
+};
+
+__device__ __forceinline__ QueryParts query_parts(const __bf16* from, const Scale& sc) {
+  const int h = (threadIdx.x & 63) >> 5;
+  u32x4_t w[2][4];
+  unsigned top = 0;
+  bool fine = true;
+#pragma unroll
+  for (int k = 0; k < 2; ++k)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      w[k][i] = *reinterpret_cast<const u32x4_t*>(from + 64 * k + 32 * h + 8 * i);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const unsigned lo = w[k][i][e] & 0x7fffu, hi = (w[k][i][e] >> 16) & 0x7fffu;
+        top = max(top, max(lo, hi));
+        w[k][i][e] = scaled_bits(w[k][i][e], sc);
+      }
+    }
+  top = max(top, (unsigned)__shfl_xor((int)top, 32));
+  fine = top < 0x7f80u;
+  // the least e with |q| <= 256 2^e, so that no high part rounds past 448
+  const int e = min(max((int)(top >> 7) - 127 - 7, -120), 119);
+  const float factor = power_of_two(-e);
+  QueryParts q;
+  q.high_scale = e + 127;
+  q.low_scale = e - 4 + 127;
+#pragma unroll
+  for (int k = 0; k < 2; ++k)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const unsigned w0 = w[k][i >> 1][2 * (i & 1)], w1 = w[k][i >> 1][2 * (i & 1) + 1];
+      float x[4] = {__builtin_bit_cast(float, w0 << 16), __builtin_bit_cast(float, w0 & 0xffff0000u),
+                    __builtin_bit_cast(float, w1 << 16), __builtin_bit_cast(float, w1 & 0xffff0000u)};
+#pragma unroll
+      for (int u = 0; u < 4; ++u) x[u] *= factor;
+      int high = __builtin_amdgcn_cvt_pk_fp8_f32(x[0], x[1], 0, false);
+      high = __builtin_amdgcn_cvt_pk_fp8_f32(x[2], x[3], high, true);
+      const f32x2_t a = __builtin_amdgcn_cvt_pk_f32_fp8(high, false), b = __builtin_amdgcn_cvt_pk_f32_fp8(high, true);
+      int low = __builtin_amdgcn_cvt_pk_fp8_f32((x[0] - a[0]) * 16.f, (x[1] - a[1]) * 16.f, 0, false);
+      low = __builtin_amdgcn_cvt_pk_fp8_f32((x[2] - b[0]) * 16.f, (x[3] - b[1]) * 16.f, low, true);
+      // (a query with an infinity or a NaN has no finite score: NaN)
+      q.high[k][i] = fine ? high : 0x7f7f7f7f;
+      q.low[k][i] = fine ? low : 0;
+    }
+  return q;
+}
+
+// S^T of 32 key rows, blocks 2 m and 2 m + 1 of a slot: lane (h, c) holds query row c, key rows
+// 8 (i / 4) + 4 h + i % 4.  scale: exponent byte of the block that the lane's key row c is in.
+__device__ __forceinline__ f32x16_t many_scores(lds_byte_t* slot, int m, const QueryParts& q, int scale) {
+  const int lane = threadIdx.x & 63, c = lane & 31, h = lane >> 5;
+  lds_byte_t* at = slot + (2 * m + (c >> 4)) * kPagedBlockBytes + (32 * h + (c & 15)) * 16;
+  f32x16_t s = {};
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    const u32x4_t lo = lds_16(at + k * 1024), hi = lds_16(at + k * 1024 + 256);
+    const i32x8_t key = {(int)lo[0], (int)lo[1], (int)lo[2], (int)lo[3], (int)hi[0], (int)hi[1], (int)hi[2], (int)hi[3]};
+    s = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(key, q.low[k], s, 0, 0, 0, scale, 0, q.low_scale);
+    s = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(key, q.high[k], s, 0, 0, 0, scale, 0, q.high_scale);
+  }
+  return s;
+}
+
+struct ManyState {
+  Sums sums;
+  f32x16_t o[4];  // dims 32 d + 8 (i / 4) + 4 h + i % 4 of query row c
+};
+
+// As step_weights, for 32 key rows; p[u]: those of the u-th block.
+__device__ __forceinline__ void many_weights(const f32x16_t& s, float c2, ManyState& st, bf16x8_t (&p)[2]) {
+  float top = s[0];
+#pragma unroll
+  for (int i = 1; i < 16; ++i) top = fmaxf(top, s[i]);
+  if (__ballot(top * st.sums.c2 > st.sums.m + kRaise)) {
+    const f32x2_t tops = both_halves(top);
+    const float f = raised(st.sums, fmaxf(tops[0], tops[1]), c2);
+#pragma unroll
+    for (int d = 0; d < 4; ++d)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) st.o[d][i] *= f;
+  }
+#pragma unroll
+  for (int i = 0; i < 16; ++i)
+    p[i / 8][i % 8] = static_cast<__bf16>(__builtin_amdgcn_exp2f(__builtin_fmaf(s[i], st.sums.c2, -st.sums.m)));
+  const bf16x2_t ones = {static_cast<__bf16>(1.f), static_cast<__bf16>(1.f)};
+#pragma unroll
+  for (int i = 0; i < 16; i += 2)
+    st.sums.l = __builtin_amdgcn_fdot2_f32_bf16(bf16x2_t{p[i / 8][i % 8], p[i / 8][i % 8 + 1]}, ones, st.sums.l, false);
+}
+
+// O^T += V^T P^T over block `block` of a slot.  masked: some query row does not see some of
+// its rows; sees(e): whether the lane's sees the e-th of its eight.
+template <typename Sees>
+__device__ __forceinline__ void many_values(lds_byte_t* slot, int block, float scale, const bf16x8_t& p, bool masked, Sees sees,
+                                            ManyState& st) {
+  const int lane = threadIdx.x & 63, c = lane & 31, h = lane >> 5;
+  lds_byte_t* at = slot + (4 + block) * kPagedBlockBytes + (c >> 4) * 1024 + (16 * h + (c & 15)) * 16;
+  u32x4_t lo = lds_16(at), hi = lds_16(at + 512);
+  if (masked) {  // (as for few query rows)
+    unsigned found = 0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) found |= nan_bytes(lo[e]) | nan_bytes(hi[e]);
+    if (__ballot(found != 0)) {
+      bf16x8_t one;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) one[e] = static_cast<__bf16>(sees(e) ? 1.f : 0.f);
+#pragma unroll
+      for (int d = 0; d < 4; ++d) {
+        const f32x16_t met =
+            __builtin_amdgcn_mfma_f32_32x32x16_bf16(eight(nan_ones(lo[d]), nan_ones(hi[d]), 1.f, 1.f), one, f32x16_t{}, 0, 0, 0);
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          if (met[i] > 0.f) st.o[d][i] = __builtin_nanf("");
+        lo[d] &= ~nan_bytes(lo[d]);
+        hi[d] &= ~nan_bytes(hi[d]);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+  }
+#pragma unroll
+  for (int d = 0; d < 4; ++d)
+    st.o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(eight(lo[d], hi[d], scale, scale), p, st.o[d], 0, 0, 0);
+}
+
+// Lane l: block `first` + l of the item (-1: none of its rows is read) and its exponent bytes.
+struct ManyBlocks {
+  int at, ke, ve;
+};
+__device__ __forceinline__ ManyBlocks many_blocks(const PagedPool& p, int b, int j, int first, int end) {
+  const int block = first + (threadIdx.x & 63);
+  ManyBlocks r = {-1, 127, 127};
+  if (block < end) {
+    const int page = p.table[(size_t)b * p.table_ld + (block >> p.page_shift)];
+    if ((unsigned)page < (unsigned)p.pages) {
+      r.at = ((page * p.n_kv + j) << p.page_shift) | (block & ((1 << p.page_shift) - 1));
+      r.ke = p.k_exp[r.at];
+      r.ve = p.v_exp[r.at];
+    }
+  }
+  return r;
+}
+
+// Query rows of a tile over steps [first_step, stop_step) of 64 key rows.
+__device__ __forceinline__ void many_rows(const PagedAttentionArgs& a, ManyShared& sh, int j, int b, int tile, int first_step,
+                                          int stop_step, bool whole, size_t slot_index) {
+  const PagedPool& p = a.pool;
+  const int lane = threadIdx.x & 63, c = lane & 31, h = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int rows = a.T * a.G, row = tile * kManyRows + 32 * wave + c;
+  const Request rq = request_of(a, b);
+  const int most = item_rows<kManyRows>(a, rq, tile);
+  const int end_block = (most + 15) / 16;
+  const int stop = min(stop_step, (end_block + 3) / 4);
+  const int t = min(row, rows - 1) / a.G, head = j * a.G + min(row, rows - 1) % a.G;
+  const int limit = rq.visible(t);
+  // (the wave's first row sees the fewest)
+  const int least = rq.visible(min(tile * kManyRows + 32 * wave, rows - 1) / a.G);
+  const Scale sc = scale_of(a.scale);
+  const QueryParts q = query_parts(a.q + (size_t)b * a.q_b + (size_t)head * a.q_h + (size_t)t * a.q_t, sc);
+  bool any = false;
+  ManyState st;
+  st.sums = no_sums(sc.c2);
+#pragma unroll
+  for (int d = 0; d < 4; ++d) st.o[d] = f32x16_t{};
+
+  auto* ring = (lds_byte_t*)sh.ring;
+  const unsigned ring_at = (unsigned)(size_t)ring;
+  // 16 steps' blocks in the lanes, this group's and the next one's
+  ManyBlocks now = many_blocks(p, b, j, 4 * first_step, end_block), next = now;
+  int group = first_step;  // the step of lane 0
+  auto load = [&](int step, unsigned slot) __attribute__((always_inline)) {
+    const int i = 4 * (step - group) + wave;  // (0..127)
+    const int at = step < stop ? __builtin_amdgcn_readlane(i < 64 ? now.at : next.at, i & 63) : -1;
+    const size_t from = (size_t)(at < 0 ? 0 : at) * kPagedBlockBytes;
+    lds_load_words_t k = buffer_words(p.k + from, at < 0 ? 0 : kPagedBlockBytes);
+    lds_load_words_t v = buffer_words(p.v + from, at < 0 ? 0 : kPagedBlockBytes);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) k[e] = __builtin_amdgcn_readfirstlane(k[e]), v[e] = __builtin_amdgcn_readfirstlane(v[e]);
+    const unsigned to = ring_at + slot * kSlot + wave * kPagedBlockBytes;
+    dma_1k<false>(k, lane * 16, 0, to);
+    dma_1k<false>(k, lane * 16 + 1024, 0, to + 1024);
+    dma_1k<false>(v, lane * 16, 0, to + 4 * kPagedBlockBytes);
+    dma_1k<false>(v, lane * 16 + 1024, 0, to + 4 * kPagedBlockBytes + 1024);
+  };
+  __syncthreads();  // (the ring of the item before has been read)
+  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");  // (loads counted by the compiler are not among those counted here)
+  load(first_step, 0);
+  load(first_step + 1, 1);
+  unsigned slot = 0;
+  for (int step = first_step; step < stop; ++step) {
+    if (step - group == 12) next = many_blocks(p, b, j, 4 * (group + 16), end_block);
+    if (step - group == 16) {
+      now = next;
+      group = step;
+    }
+    // The step's loads have landed (the next one's 4 are behind them), and with the barrier
+    // every wave's; every wave is done with the step before it, whose slot the next takes.
+    asm volatile("s_waitcnt vmcnt(4) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    load(step + 2, slot >= 1 ? slot - 1 : kRing - 1);
+    lds_byte_t* here = ring + slot * kSlot;
+    const int i = 4 * (step - group);
+    int at[4], ke[4], ve[4];
+#pragma unroll
+    for (int m = 0; m < 4; ++m) {
+      at[m] = __builtin_amdgcn_readlane(now.at, i + m);
+      ke[m] = __builtin_amdgcn_readlane(now.ke, i + m);
+      ve[m] = __builtin_amdgcn_readlane(now.ve, i + m);
+    }
+    const int row0 = kStep * step;
+    const bool masked = row0 + kStep > least || (at[0] | at[1] | at[2] | at[3]) < 0;
+    f32x16_t s[2];
+#pragma unroll
+    for (int m = 0; m < 2; ++m) s[m] = many_scores(here, m, q, c < 16 ? ke[2 * m] : ke[2 * m + 1]);
+    auto seen = [&](int m, int e) { return row0 + 32 * m + 8 * (e / 4) + 4 * h + e % 4 < limit && at[2 * m + e / 8] >= 0; };
+    if (masked) {
+#pragma unroll
+      for (int m = 0; m < 2; ++m)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const bool ok = seen(m, e);
+          any |= ok;
+          s[m][e] = ok ? s[m][e] : neg_inf();
+        }
+    } else {
+      any = true;
+    }
+#pragma unroll
+    for (int m = 0; m < 2; ++m) {
+      bf16x8_t w[2];
+      many_weights(s[m], sc.c2, st, w);
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+        many_values(here, 2 * m + u, power_of_two(ve[2 * m + u] - 127), w[u], masked, [&](int e) { return seen(m, 8 * u + e); }, st);
+    }
+    slot = slot + 1 == kRing ? 0 : slot + 1;
+  }
+  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+
+  const f32x2_t ls = both_halves(st.sums.l);
+  const float l = ls[0] + ls[1];
+  const bool met = (__ballot(any) >> c & 0x0000000100000001ull) != 0;  // one of the row's two lanes has
+  const float m = met ? st.sums.m : neg_inf();
+  if (row >= rows) return;
+  const bool none = t >= rq.count || m == neg_inf();
+  const float share = none ? 0.f : 1.f / l;
+  const Part part = part_of(a, slot_index);
+  const int r = 32 * wave + c;
+#pragma unroll
+  for (int d = 0; d < 4; ++d)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int dim = 32 * d + 8 * i + 4 * h;
+      if (whole) {
+        bf16x4_t o;
+#pragma unroll
+        for (int u = 0; u < 4; ++u) o[u] = static_cast<__bf16>(none ? 0.f : st.o[d][4 * i + u] * share);
+        *reinterpret_cast<bf16x4_t*>(a.out + (((size_t)b * a.T + t) * a.n_q + head) * D + dim) = o;
+      } else {
+        *reinterpret_cast<f32x4_t*>(part.o + (size_t)r * D + dim) =
+            f32x4_t{st.o[d][4 * i], st.o[d][4 * i + 1], st.o[d][4 * i + 2], st.o[d][4 * i + 3]};
+      }
+    }
+  if (!whole && h == 0) *reinterpret_cast<f32x2_t*>(part.ml + r * 2) = f32x2_t{m, l};
+}
+
+// Grid: kv head (fastest: with 8 of them each XCD's L2 holds one head's rows), worker.
+// A share that does not reach an item's start leaves its part in the worker's slot 0, one
+// that starts the item and does not end it in slot 1.
+__global__ __launch_bounds__(64 * kManyWaves, 2) void many_attention_kernel(PagedAttentionArgs a) {
+  __shared__ __align__(1024) ManyShared sh;
+  const int j = blockIdx.x % a.pool.n_kv, w = blockIdx.x / a.pool.n_kv;
+  const Share s = share_of<kManyRows>(a, w, blockIdx.x == 0 && threadIdx.x < 64);
+  int item = s.item, skip = s.skip, left = s.units;
+  while (left > 0) {
+    const int b = a.tiles == 1 ? item : item / a.tiles;
+    const int units = item_units<kManyRows>(a, item);
+    const int last = min(skip + left, units);
+    many_rows(a, sh, j, b, item - b * a.tiles, skip, last, skip == 0 && last == units,
+              ((size_t)j * a.workers + w) * 2 + (skip == 0 ? 1 : 0));
+    left -= last - skip;
+    skip = 0;
+    ++item;
   }
 }
 
 }  // namespace
 
-hipError_t launch_paged_attention(const PagedAttentionArgs& a, hipStream_t stream) {
-  const int rows = a.T * a.G;
-  const int nt = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
-  const dim3 grid((unsigned)a.pool.n_kv * a.B * ceil_div(rows, 16 * nt));
-  if (nt == 1) launch_kernel(paged_attention_kernel<1>, grid, dim3(kThreads), 0, stream, a);
-  if (nt == 2) launch_kernel(paged_attention_kernel<2>, grid, dim3(kThreads), 0, stream, a);
-  if (nt == 4) launch_kernel(paged_attention_kernel<4>, grid, dim3(kThreads), 0, stream, a);
+hipError_t launch_paged_attention(const PagedAttentionArgs& a, const PagedPlan& plan, hipStream_t stream) {
+  const unsigned n_kv = (unsigned)a.pool.n_kv;
+  if (plan.one_launch) {
+    const dim3 grid(n_kv * a.items);
+    if (plan.rows == 16) launch_kernel(short_attention_kernel<1>, grid, dim3(64 * kShortWaves), 0, stream, a);
+    if (plan.rows == 32) launch_kernel(short_attention_kernel<2>, grid, dim3(64 * kShortWaves), 0, stream, a);
+    if (plan.rows == 64) launch_kernel(short_attention_kernel<4>, grid, dim3(64 * kShortWaves), 0, stream, a);
+    return hipGetLastError();
+  }
+  const dim3 grid(n_kv * (plan.rows == kManyRows ? a.workers : ceil_div(a.workers, kFewWaves)));
+  if (plan.rows == 16) launch_kernel(few_attention_kernel<1>, grid, dim3(64 * kFewWaves), 0, stream, a);
+  if (plan.rows == 32) launch_kernel(few_attention_kernel<2>, grid, dim3(64 * kFewWaves), 0, stream, a);
+  if (plan.rows == 64) launch_kernel(few_attention_kernel<4>, grid, dim3(64 * kFewWaves), 0, stream, a);
+  if (plan.rows == kManyRows) launch_kernel(many_attention_kernel, grid, dim3(64 * kManyWaves), 0, stream, a);
+  hipError_t err = hipGetLastError();
+  if (err != hipSuccess) return err;
+  const dim3 joins((unsigned)a.items * n_kv * (plan.rows / 16));
+  if (plan.rows == kManyRows)
+    launch_kernel(join_kernel<true>, joins, dim3(kJoinThreads), 0, stream, a, plan.rows);
+  else
+    launch_kernel(join_kernel<false>, joins, dim3(kJoinThreads), 0, stream, a, plan.rows);
   return hipGetLastError();
 }
 
