@@ -177,6 +177,8 @@ constexpr PagedPlan paged_plan(int B, int T, int n_q, int n_kv, int capacity) {
   const int all = many ? 512 : 2048;
   const long long most = p.items * ((capacity + p.unit - 1) / p.unit);
   p.places = all / n_kv > 1 ? all / n_kv : 1;
+  // (an item more or less than a chunk adds one: all chunks are to run at once)
+  if (!many && p.places > 1) p.places = p.items < p.places / 2 ? p.places - p.items : p.places / 2;
   if (p.places > most) p.places = most;
   p.workers = many ? p.places : p.places + p.items;
   p.slots = many ? 2 * p.workers : p.workers;

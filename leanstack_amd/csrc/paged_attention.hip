@@ -57,7 +57,7 @@ typedef __bf16 bf16x4_t __attribute__((ext_vector_type(4)));
 
 constexpr int D = kAttnHeadDim;
 constexpr int kFewWaves = 4, kShortWaves = 8;  // of a workgroup for few query rows
-constexpr float kRaise = 8.f;
+constexpr float kRaise = 8.f, kMostWeight = 256.f;  // in base 2
 constexpr float kFar = 0x1p30f;
 constexpr float kLowest = -3.402823466e38f;
 
@@ -700,7 +700,7 @@ __global__ __launch_bounds__(kJoinThreads) void join_kernel(PagedAttentionArgs a
 constexpr int kManyWaves = 4;
 constexpr int kManyRows = 32 * kManyWaves;
 constexpr int kStep = 64;                           // key rows, one block per wave
-constexpr int kRing = 3;
+constexpr int kRing = 4;
 constexpr int kSlot = 2 * 4 * kPagedBlockBytes;     // K, then V, of a step
 static_assert(kManyRows == kPagedManyRows && kStep == kPagedManyUnit, "as the host counts them");
 
@@ -776,18 +776,30 @@ __device__ __forceinline__ QueryParts query_parts(const __bf16* from, const Scal
   return q;
 }
 
-// S^T of 32 key rows, blocks 2 m and 2 m + 1 of a slot: lane (h, c) holds query row c, key rows
-// 8 (i / 4) + 4 h + i % 4.  scale: exponent byte of the block that the lane's key row c is in.
-__device__ __forceinline__ f32x16_t many_scores(lds_byte_t* slot, int m, const QueryParts& q, int scale) {
+// 32 key rows of K, blocks 2 m and 2 m + 1 of a slot, as the lanes multiply them.
+struct Keys {
+  i32x8_t k[2];
+};
+__device__ __forceinline__ Keys many_keys(lds_byte_t* slot, int m) {
   const int lane = threadIdx.x & 63, c = lane & 31, h = lane >> 5;
   lds_byte_t* at = slot + (2 * m + (c >> 4)) * kPagedBlockBytes + (32 * h + (c & 15)) * 16;
-  f32x16_t s = {};
+  Keys keys;
 #pragma unroll
   for (int k = 0; k < 2; ++k) {
     const u32x4_t lo = lds_16(at + k * 1024), hi = lds_16(at + k * 1024 + 256);
-    const i32x8_t key = {(int)lo[0], (int)lo[1], (int)lo[2], (int)lo[3], (int)hi[0], (int)hi[1], (int)hi[2], (int)hi[3]};
-    s = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(key, q.low[k], s, 0, 0, 0, scale, 0, q.low_scale);
-    s = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(key, q.high[k], s, 0, 0, 0, scale, 0, q.high_scale);
+    keys.k[k] = i32x8_t{(int)lo[0], (int)lo[1], (int)lo[2], (int)lo[3], (int)hi[0], (int)hi[1], (int)hi[2], (int)hi[3]};
+  }
+  return keys;
+}
+
+// S^T of 32 key rows: lane (h, c) holds query row c, key rows 8 (i / 4) + 4 h + i % 4.  scale:
+// exponent byte of the block that key row c is in.
+__device__ __forceinline__ f32x16_t many_scores(const Keys& keys, const QueryParts& q, int scale) {
+  f32x16_t s = {};
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    s = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(keys.k[k], q.low[k], s, 0, 0, 0, scale, 0, q.low_scale);
+    s = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(keys.k[k], q.high[k], s, 0, 0, 0, scale, 0, q.high_scale);
   }
   return s;
 }
@@ -797,60 +809,51 @@ struct ManyState {
   f32x16_t o[4];  // dims 32 d + 8 (i / 4) + 4 h + i % 4 of query row c
 };
 
-// As step_weights, for 32 key rows; p[u]: those of the u-th block.
-__device__ __forceinline__ void many_weights(const f32x16_t& s, float c2, ManyState& st, bf16x8_t (&p)[2]) {
-  float top = s[0];
-#pragma unroll
-  for (int i = 1; i < 16; ++i) top = fmaxf(top, s[i]);
-  if (__ballot(top * st.sums.c2 > st.sums.m + kRaise)) {
-    const f32x2_t tops = both_halves(top);
-    const float f = raised(st.sums, fmaxf(tops[0], tops[1]), c2);
-#pragma unroll
-    for (int d = 0; d < 4; ++d)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) st.o[d][i] *= f;
-  }
+// The weights of 32 key rows, p[u] those of the u-th block, and their sum.
+__device__ __forceinline__ float many_weights(const f32x16_t& s, const Sums& sums, bf16x8_t (&p)[2]) {
 #pragma unroll
   for (int i = 0; i < 16; ++i)
-    p[i / 8][i % 8] = static_cast<__bf16>(__builtin_amdgcn_exp2f(__builtin_fmaf(s[i], st.sums.c2, -st.sums.m)));
+    p[i / 8][i % 8] = static_cast<__bf16>(__builtin_amdgcn_exp2f(__builtin_fmaf(s[i], sums.c2, -sums.m)));
   const bf16x2_t ones = {static_cast<__bf16>(1.f), static_cast<__bf16>(1.f)};
+  float sum = 0.f;
 #pragma unroll
   for (int i = 0; i < 16; i += 2)
-    st.sums.l = __builtin_amdgcn_fdot2_f32_bf16(bf16x2_t{p[i / 8][i % 8], p[i / 8][i % 8 + 1]}, ones, st.sums.l, false);
+    sum = __builtin_amdgcn_fdot2_f32_bf16(bf16x2_t{p[i / 8][i % 8], p[i / 8][i % 8 + 1]}, ones, sum, false);
+  return sum;
 }
 
-// O^T += V^T P^T over block `block` of a slot.  masked: some query row does not see some of
-// its rows; sees(e): whether the lane's sees the e-th of its eight.
-template <typename Sees>
-__device__ __forceinline__ void many_values(lds_byte_t* slot, int block, float scale, const bf16x8_t& p, bool masked, Sees sees,
-                                            ManyState& st) {
+// V of block `block` of a slot: dims 32 d .. of lane c, rows 4 h .. + 3 and 8 + 4 h .. + 3.
+struct Values {
+  u32x4_t lo, hi;
+};
+__device__ __forceinline__ Values many_values(lds_byte_t* slot, int block) {
   const int lane = threadIdx.x & 63, c = lane & 31, h = lane >> 5;
   lds_byte_t* at = slot + (4 + block) * kPagedBlockBytes + (c >> 4) * 1024 + (16 * h + (c & 15)) * 16;
-  u32x4_t lo = lds_16(at), hi = lds_16(at + 512);
-  if (masked) {  // (as for few query rows)
-    unsigned found = 0;
+  return {lds_16(at), lds_16(at + 512)};
+}
+
+// NaN of rows that some query row does not see: to those that do (as for few query rows).
+// sees(e): whether the lane's query row sees the e-th of its eight.
+template <typename Sees>
+__device__ __forceinline__ void many_nans(Values& v, Sees sees, ManyState& st) {
+  unsigned found = 0;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) found |= nan_bytes(lo[e]) | nan_bytes(hi[e]);
-    if (__ballot(found != 0)) {
-      bf16x8_t one;
+  for (int e = 0; e < 4; ++e) found |= nan_bytes(v.lo[e]) | nan_bytes(v.hi[e]);
+  if (__ballot(found != 0) == 0) return;
+  bf16x8_t one;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) one[e] = static_cast<__bf16>(sees(e) ? 1.f : 0.f);
+  for (int e = 0; e < 8; ++e) one[e] = static_cast<__bf16>(sees(e) ? 1.f : 0.f);
 #pragma unroll
-      for (int d = 0; d < 4; ++d) {
-        const f32x16_t met =
-            __builtin_amdgcn_mfma_f32_32x32x16_bf16(eight(nan_ones(lo[d]), nan_ones(hi[d]), 1.f, 1.f), one, f32x16_t{}, 0, 0, 0);
+  for (int d = 0; d < 4; ++d) {
+    const f32x16_t met =
+        __builtin_amdgcn_mfma_f32_32x32x16_bf16(eight(nan_ones(v.lo[d]), nan_ones(v.hi[d]), 1.f, 1.f), one, f32x16_t{}, 0, 0, 0);
 #pragma unroll
-        for (int i = 0; i < 16; ++i)
-          if (met[i] > 0.f) st.o[d][i] = __builtin_nanf("");
-        lo[d] &= ~nan_bytes(lo[d]);
-        hi[d] &= ~nan_bytes(hi[d]);
-        __builtin_amdgcn_sched_barrier(0);
-      }
-    }
+    for (int i = 0; i < 16; ++i)
+      if (met[i] > 0.f) st.o[d][i] = __builtin_nanf("");
+    v.lo[d] &= ~nan_bytes(v.lo[d]);
+    v.hi[d] &= ~nan_bytes(v.hi[d]);
+    __builtin_amdgcn_sched_barrier(0);
   }
-#pragma unroll
-  for (int d = 0; d < 4; ++d)
-    st.o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(eight(lo[d], hi[d], scale, scale), p, st.o[d], 0, 0, 0);
 }
 
 // Lane l: block `first` + l of the item (-1: none of its rows is read) and its exponent bytes.
@@ -915,55 +918,98 @@ __device__ __forceinline__ void many_rows(const PagedAttentionArgs& a, ManyShare
   };
   __syncthreads();  // (the ring of the item before has been read)
   asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");  // (loads counted by the compiler are not among those counted here)
-  load(first_step, 0);
-  load(first_step + 1, 1);
-  unsigned slot = 0;
-  for (int step = first_step; step < stop; ++step) {
+  // Half steps of 32 key rows.  A wave issues in order, so the products of the next half's
+  // scores stand between the exponentials of this one's weights.
+  auto key_scale = [&](int step, int m) __attribute__((always_inline)) {
+    const int i = 4 * (step - group) + 2 * m;
+    const int lo = __builtin_amdgcn_readlane(now.ke, i), hi = __builtin_amdgcn_readlane(now.ke, i + 1);
+    return c < 16 ? lo : hi;
+  };
+  // The step's loads have landed (the next ones' are behind them), and with the barrier
+  // every wave's; every wave is done with the step two before it, whose slot the load takes.
+  auto begin_step = [&](int step) __attribute__((always_inline)) {
     if (step - group == 12) next = many_blocks(p, b, j, 4 * (group + 16), end_block);
-    if (step - group == 16) {
-      now = next;
-      group = step;
-    }
-    // The step's loads have landed (the next one's 4 are behind them), and with the barrier
-    // every wave's; every wave is done with the step before it, whose slot the next takes.
     asm volatile("s_waitcnt vmcnt(4) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-    load(step + 2, slot >= 1 ? slot - 1 : kRing - 1);
-    lds_byte_t* here = ring + slot * kSlot;
-    const int i = 4 * (step - group);
-    int at[4], ke[4], ve[4];
+    load(step + 2, (step - first_step + 2) & (kRing - 1));
+  };
+  if (first_step < stop) {
+    load(first_step, 0);
+    load(first_step + 1, 1);
+    begin_step(first_step);
+    Keys keys = many_keys(ring, 0);
+    f32x16_t s = many_scores(keys, q, key_scale(first_step, 0));
+    keys = many_keys(ring, 1);
+    for (int step = first_step; step < stop; ++step) {
+      lds_byte_t* slot = ring + ((step - first_step) & (kRing - 1)) * kSlot;
+      lds_byte_t* after = ring + ((step + 1 - first_step) & (kRing - 1)) * kSlot;
 #pragma unroll
-    for (int m = 0; m < 4; ++m) {
-      at[m] = __builtin_amdgcn_readlane(now.at, i + m);
-      ke[m] = __builtin_amdgcn_readlane(now.ke, i + m);
-      ve[m] = __builtin_amdgcn_readlane(now.ve, i + m);
-    }
-    const int row0 = kStep * step;
-    const bool masked = row0 + kStep > least || (at[0] | at[1] | at[2] | at[3]) < 0;
-    f32x16_t s[2];
+      for (int m = 0; m < 2; ++m) {
+        const int i = 4 * (step - group) + 2 * m, row0 = kStep * step + 32 * m;
+        int at[2], ve[2];
 #pragma unroll
-    for (int m = 0; m < 2; ++m) s[m] = many_scores(here, m, q, c < 16 ? ke[2 * m] : ke[2 * m + 1]);
-    auto seen = [&](int m, int e) { return row0 + 32 * m + 8 * (e / 4) + 4 * h + e % 4 < limit && at[2 * m + e / 8] >= 0; };
-    if (masked) {
-#pragma unroll
-      for (int m = 0; m < 2; ++m)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const bool ok = seen(m, e);
-          any |= ok;
-          s[m][e] = ok ? s[m][e] : neg_inf();
+        for (int u = 0; u < 2; ++u) {
+          at[u] = __builtin_amdgcn_readlane(now.at, i + u);
+          ve[u] = __builtin_amdgcn_readlane(now.ve, i + u);
         }
-    } else {
-      any = true;
-    }
+        Values v[2] = {many_values(slot, 2 * m), many_values(slot, 2 * m + 1)};
+        if (m == 1 && step + 1 - group == 16) {  // (this step's have been taken out)
+          now = next;
+          group = step + 1;
+        }
+        const int scale = key_scale(m == 0 ? step : step + 1, 1 - m);
+        const bool masked = row0 + 32 > least || (at[0] | at[1]) < 0;
+        auto seen = [&](int e) { return row0 + 8 * (e / 4) + 4 * h + e % 4 < limit && at[e / 8] >= 0; };
+        if (masked) {
 #pragma unroll
-    for (int m = 0; m < 2; ++m) {
-      bf16x8_t w[2];
-      many_weights(s[m], sc.c2, st, w);
+          for (int e = 0; e < 16; ++e) {
+            const bool ok = seen(e);
+            any |= ok;
+            s[e] = ok ? s[e] : neg_inf();
+          }
+        } else {
+          any = true;
+        }
+        bf16x8_t w[2];
+        const f32x16_t then = many_scores(keys, q, scale);
+        float sum = many_weights(s, st.sums, w);
+        asm volatile("" : "+v"(sum) : "v"(then[0]));  // (the products stay in front of the branch)
+        // A weight above 2^8 shows in their sum: then m is raised, and they are computed again.
+        if (__ballot(sum > 16.f * kMostWeight)) {
+          float top = s[0];
 #pragma unroll
-      for (int u = 0; u < 2; ++u)
-        many_values(here, 2 * m + u, power_of_two(ve[2 * m + u] - 127), w[u], masked, [&](int e) { return seen(m, 8 * u + e); }, st);
+          for (int e = 1; e < 16; ++e) top = fmaxf(top, s[e]);
+          const f32x2_t tops = both_halves(top);
+          const float f = raised(st.sums, fmaxf(tops[0], tops[1]), sc.c2);
+#pragma unroll
+          for (int d = 0; d < 4; ++d)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) st.o[d][e] *= f;
+          sum = many_weights(s, st.sums, w);
+        }
+        st.sums.l += sum;
+        // The half after the next: of this step, or of the one that begins here.
+        if (m == 0) {
+          begin_step(step + 1);
+          keys = many_keys(after, 0);
+        } else {
+          keys = many_keys(after, 1);
+        }
+        if (masked) {
+#pragma unroll
+          for (int u = 0; u < 2; ++u) many_nans(v[u], [&](int e) { return seen(8 * u + e); }, st);
+        }
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const float vs = power_of_two(ve[u] - 127);
+          if (u == 0) __builtin_amdgcn_s_setprio(1);  // products before the other wave's exponentials
+#pragma unroll
+          for (int d = 0; d < 4; ++d)
+            st.o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(eight(v[u].lo[d], v[u].hi[d], vs, vs), w[u], st.o[d], 0, 0, 0);
+        }
+        __builtin_amdgcn_s_setprio(0);
+        s = then;
+      }
     }
-    slot = slot + 1 == kRing ? 0 : slot + 1;
   }
   asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
 
