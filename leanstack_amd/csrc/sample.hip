@@ -14,6 +14,12 @@
 // by 2048 bins, even in x, down from the maximum to where weights vanish; then the
 // places of the one bin in which the cut lies, ranked against each other, or, where
 // they are many (ties, narrow logits), binned again by their bits first.
+//
+// One workgroup per row.  With top-k or min-p few tokens can be kept, and two sweeps over the
+// row do: the first takes the maximum of each of 4096 groups of values, of which the k-th
+// largest is a bound below which none of the first k lies; the second lists what is above
+// it.  All else works on the list, in LDS.  Without either (top-p or the temperature alone)
+// every weight counts, and each step is a sweep.
 
 #include <hip/hip_runtime.h>
 
@@ -26,9 +32,13 @@ typedef unsigned long long u64;
 
 constexpr int kThreads = 1024;
 constexpr int kWaves = kThreads / 64;
-constexpr int kBins = 2048;
-constexpr int kList = 1024;
-constexpr int kParts = 16;      // of a wave's share of the row, for the draw
+constexpr int kBins = 2 * kThreads;
+constexpr int kRanked = 1024;               // places ranked against each other
+constexpr int kListed = 4096;               // tokens that may be kept
+constexpr int kGroups = 4;                  // of values per thread, whose maxima bound the k-th
+constexpr int kMostK = kGroups * kThreads / 2;
+constexpr int kAhead = 4;                   // 16-byte loads of a thread in flight
+constexpr int kParts = kSampleMaxVocab / 256 + 2;
 constexpr double kUnit = 17592186044416.0;  // 2^44
 constexpr float kOctaves = 46.f;            // below the maximum: weights round to zero
 
@@ -37,8 +47,26 @@ __device__ __forceinline__ unsigned value_order(float v) {
   const unsigned b = __builtin_bit_cast(unsigned, v + 0.f);
   return b ^ ((unsigned)((int)b >> 31) | 0x80000000u);
 }
+__device__ __forceinline__ float ordered_value(unsigned o) {
+  return __builtin_bit_cast(float, o ^ ((unsigned)((int)~o >> 31) | 0x80000000u));
+}
 
 __device__ __forceinline__ u64 place_of(float x, int v) { return (u64)value_order(x) << 32 | (0xffffffffu - (unsigned)v); }
+__device__ __forceinline__ int index_of(u64 place) { return (int)(0xffffffffu - (unsigned)place); }
+__device__ __forceinline__ float value_of(u64 place) { return ordered_value((unsigned)(place >> 32)); }
+
+// 2^t for t in -47..0, to 2^-50 of it: 2^n times the series of e^(f ln 2), |f| <= 1/2.
+__device__ __forceinline__ double power_of_2(double t) {
+  const double n = __builtin_rint(t), f = t - n;
+  // ln(2)^i / i!
+  constexpr double c[] = {1.0, 0.69314718055994531, 0.24022650695910071, 0.055504108664821580, 0.0096181291076284772,
+                          0.0013333558146428443, 0.00015403530393381610, 1.5252733804059840e-05, 1.3215486790144309e-06,
+                          1.0178086009239699e-07, 7.0549116208011233e-09, 4.4455382718708115e-10, 2.5678435993488206e-11};
+  double p = c[12];
+#pragma unroll
+  for (int i = 11; i >= 0; --i) p = __builtin_fma(p, f, c[i]);
+  return p * __builtin_bit_cast(double, (u64)(1023 + (int)n) << 52);
+}
 
 template <typename V>
 __device__ __forceinline__ V wave_inclusive(V v) {
@@ -50,23 +78,98 @@ __device__ __forceinline__ V wave_inclusive(V v) {
   }
   return v;
 }
+template <typename V>
+__device__ __forceinline__ V wave_total(V v) {
+#pragma unroll
+  for (int s = 1; s < 64; s <<= 1) v += __shfl_xor(v, s);
+  return v;
+}
 
 struct Shared {
-  u64 weight[kBins], before[kBins];      // of the bins; and of those in front
+  u64 weight[kBins], before[kBins];  // of the bins; and of those in front
   unsigned count[kBins], counted[kBins];
-  u64 sub_weight[kBins];
-  unsigned sub_count[kBins];
-  u64 list[kList], list_weight[kList];
+  union {
+    struct {
+      u64 weight[kBins];
+      unsigned count[kBins];
+    } sub;
+    u64 parts[kParts];
+  };
+  u64 ranked[kRanked], ranked_weight[kRanked];
+  u64 listed[kListed];
   u64 wave_weight[kWaves];
   unsigned wave_count[kWaves];
-  u64 parts[kWaves * kParts];
+  float wave_max[kWaves];
   u64 lo, hi, kept;
-  unsigned n;
-  int found, nan;
+  unsigned n, listed_n;
+  int found;
+};
+
+// A row in accesses of 16 bytes from its first aligned value on: access q holds the kVec
+// values from head + q kVec on; those around them are taken one by one.
+template <typename T>
+struct Row {
+  static constexpr int kVec = 16 / sizeof(T);
+  typedef T vec_t __attribute__((ext_vector_type(kVec)));
+  const T* at;
+  int V, head, vecs;
+  __device__ __forceinline__ Row(const T* p, int n) : at(p), V(n) {
+    head = min((int)((16 - (reinterpret_cast<uintptr_t>(p) & 15)) & 15) / (int)sizeof(T), n);
+    vecs = (n - head) / kVec;
+  }
+  __device__ __forceinline__ float value(int v) const { return static_cast<float>(at[v]); }
+  // access(v0, x): kVec values from index v0 on; one(v, x): a value apart.  All threads.
+  template <typename Access, typename One>
+  __device__ __forceinline__ void sweep(Access access, One one) const {
+    const int tid = threadIdx.x;
+    if (tid < head) one(tid, value(tid));
+    const vec_t* body = reinterpret_cast<const vec_t*>(at + head);
+    for (int q0 = tid; q0 < vecs; q0 += kAhead * kThreads) {
+      vec_t x[kAhead];
+#pragma unroll
+      for (int k = 0; k < kAhead; ++k) x[k] = body[min(q0 + k * kThreads, vecs - 1)];
+#pragma unroll
+      for (int k = 0; k < kAhead; ++k) {
+        if (q0 + k * kThreads >= vecs) break;
+        float f[kVec];
+#pragma unroll
+        for (int e = 0; e < kVec; ++e) f[e] = static_cast<float>(x[k][e]);
+        access(head + (q0 + k * kThreads) * kVec, f);
+      }
+    }
+    const int tail = head + vecs * kVec + tid;
+    if (tail < V) one(tail, value(tail));
+  }
+  template <typename Each>
+  __device__ __forceinline__ void each(Each f) const {
+    sweep([&](int v0, const float (&x)[kVec]) {
+#pragma unroll
+      for (int e = 0; e < kVec; ++e) f(v0 + e, x[e]);
+    }, f);
+  }
+};
+
+// How a row's values weigh, and the bins that they fall into.
+struct Rule {
+  float top, per_bin;
+  double to_base2, least;
+  // Weight in units; 0 also for what min_p drops (a token without weight counts for nothing).
+  __device__ __forceinline__ u64 weight(float x) const {
+    if (x == top) return 1ull << 44;
+    const double t = ((double)x - (double)top) * to_base2;
+    if (!(t > -kOctaves)) return 0;
+    const double w = __builtin_rint(power_of_2(t) * kUnit);
+    return w >= least ? (u64)w : 0;
+  }
+  // Bins down from the maximum, monotone in x.
+  __device__ __forceinline__ int bin(float x) const {
+    const float f = (top - x) * per_bin;
+    return x == top ? 0 : f < (float)(kBins - 1) ? (int)f : kBins - 1;
+  }
 };
 
 // Exclusive sums of count and weight over the bins; found: the first bin at which `reached`
-// (count and weight up to and with it), kBins if there is none.  Returns whether there is.
+// (count and weight up to and with it), kBins if there is none.
 template <typename Reached>
 __device__ void scan_bins(Shared& s, const unsigned* count, const u64* weight, unsigned* counted, u64* before,
                           Reached reached) {
@@ -76,7 +179,6 @@ __device__ void scan_bins(Shared& s, const unsigned* count, const u64* weight, u
   const unsigned c = wave_inclusive(c0 + c1);
   const u64 w = wave_inclusive(w0 + w1);
   if (tid == 0) s.found = kBins;
-  __syncthreads();
   if (lane == 63) s.wave_count[wave] = c, s.wave_weight[wave] = w;
   __syncthreads();
   unsigned cb = c - c0 - c1;
@@ -86,9 +188,170 @@ __device__ void scan_bins(Shared& s, const unsigned* count, const u64* weight, u
     counted[2 * tid] = cb, counted[2 * tid + 1] = cb + c0;
     before[2 * tid] = wb, before[2 * tid + 1] = wb + w0;
   }
-  if (c0 && reached(cb + c0, wb + w0)) atomicMin(&s.found, 2 * tid);
-  if (c1 && reached(cb + c0 + c1, wb + w0 + w1)) atomicMin(&s.found, 2 * tid + 1);
+  if (c0 && reached(cb + c0, wb + w0))
+    atomicMin(&s.found, 2 * tid);
+  else if (c1 && reached(cb + c0 + c1, wb + w0 + w1))
+    atomicMin(&s.found, 2 * tid + 1);
   __syncthreads();
+}
+
+// The lowest kept place of the bin in which a cut lies: the first `want` by count, or those with
+// less than `target` in front of them.  base_c, base_w: what lies in front of the bin.
+// each(f): f(v, x) for all tokens.  Returns the place; s.kept: the weight up to it.
+template <typename Each>
+__device__ u64 cut_in_bin(Shared& s, const Rule& rule, Each each, int bin, unsigned base_c, u64 base_w, bool by_count,
+                          unsigned want, double target) {
+  const int tid = threadIdx.x;
+  __syncthreads();
+  if (tid == 0) s.lo = ~0ull, s.hi = 0, s.n = 0;
+  __syncthreads();
+  {
+    u64 lo = ~0ull, hi = 0;
+    unsigned n = 0;
+    each([&](int v, float x) {
+      if (rule.bin(x) == bin && rule.weight(x)) {
+        const u64 p = place_of(x, v);
+        lo = p < lo ? p : lo, hi = p > hi ? p : hi, ++n;
+      }
+    });
+    if (n) atomicMin(&s.lo, lo), atomicMax(&s.hi, hi), atomicAdd(&s.n, n);
+  }
+  __syncthreads();
+  u64 lo = s.lo, hi = s.hi;
+  unsigned n = s.n;
+  __syncthreads();
+  while (n > kRanked) {
+    const int bits = 64 - __clzll((long long)(hi - lo));
+    const int shift = bits > 11 ? bits - 11 : 0;
+    for (int i = tid; i < kBins; i += kThreads) s.sub.count[i] = 0, s.sub.weight[i] = 0;
+    __syncthreads();
+    each([&](int v, float x) {
+      if (rule.bin(x) != bin) return;
+      const u64 p = place_of(x, v);
+      if (p < lo || p > hi) return;
+      const u64 w = rule.weight(x);
+      if (!w) return;
+      const int at = (int)((hi - p) >> shift);
+      atomicAdd(&s.sub.count[at], 1u);
+      atomicAdd(&s.sub.weight[at], w);
+    });
+    __syncthreads();
+    scan_bins(s, s.sub.count, s.sub.weight, nullptr, nullptr, [&](unsigned c, u64 w) {
+      return by_count ? base_c + c >= want : (double)(base_w + w) >= target;
+    });
+    // (rounding can leave the target out of reach: then the last)
+    int at = s.found;
+    if (at == kBins) at = (int)((hi - lo) >> shift);
+    if (tid == 0) s.lo = 0, s.hi = 0;
+    __syncthreads();
+    u64 c = 0, w = 0;
+    for (int i = tid; i < at; i += kThreads) c += s.sub.count[i], w += s.sub.weight[i];
+    if (c) atomicAdd(&s.lo, c), atomicAdd(&s.hi, w);
+    __syncthreads();
+    base_c += (unsigned)s.lo, base_w += s.hi;
+    n = s.sub.count[at];
+    const u64 width = (1ull << shift) - 1;
+    hi -= (u64)at << shift;
+    lo = hi >= width && hi - width > lo ? hi - width : lo;
+    __syncthreads();
+  }
+  if (tid == 0) s.n = 0, s.lo = ~0ull, s.kept = base_w;
+  __syncthreads();
+  each([&](int v, float x) {
+    if (rule.bin(x) != bin) return;
+    const u64 p = place_of(x, v);
+    if (p < lo || p > hi) return;
+    const u64 w = rule.weight(x);
+    if (!w) return;
+    const unsigned at = atomicAdd(&s.n, 1u);
+    if (at < kRanked) s.ranked[at] = p, s.ranked_weight[at] = w;
+  });
+  __syncthreads();
+  n = min(s.n, (unsigned)kRanked);
+  if (tid < (int)n) {
+    const u64 mine = s.ranked[tid];
+    unsigned c = base_c;
+    u64 w = base_w;
+    for (unsigned i = 0; i < n; ++i)
+      if (s.ranked[i] > mine) ++c, w += s.ranked_weight[i];
+    if (by_count ? c < want : c == 0 || (double)w < target) {
+      atomicMin(&s.lo, mine);
+      atomicAdd(&s.kept, s.ranked_weight[tid]);
+    }
+  }
+  __syncthreads();
+  return s.lo;
+}
+
+// The lowest kept place under top-k (k below the number of tokens) and top-p (below 1).
+template <typename Each>
+__device__ u64 lowest_kept(Shared& s, const Rule& rule, Each each, bool by_k, unsigned k, bool by_p, float top_p) {
+  const int tid = threadIdx.x;
+  __syncthreads();
+  for (int i = tid; i < kBins; i += kThreads) s.count[i] = 0, s.weight[i] = 0;
+  __syncthreads();
+  each([&](int, float x) {
+    const u64 w = rule.weight(x);
+    if (!w) return;
+    const int at = rule.bin(x);
+    atomicAdd(&s.count[at], 1u);
+    atomicAdd(&s.weight[at], w);
+  });
+  __syncthreads();
+  scan_bins(s, s.count, s.weight, s.counted, s.before, [&](unsigned c, u64) { return by_k && c >= k; });
+  u64 sum = s.before[kBins - 1] + s.weight[kBins - 1], lowest = 0;
+  const int bin = s.found;
+  if (by_k && bin < kBins) {  // (fewer than k have weight: no cut)
+    lowest = cut_in_bin(s, rule, each, bin, s.counted[bin], s.before[bin], true, k, 0.0);
+    sum = s.kept;
+  }
+  if (by_p) {
+    const double target = top_p > 0.f ? (double)top_p * (double)sum : 0.0;
+    __syncthreads();
+    scan_bins(s, s.count, s.weight, s.counted, s.before, [&](unsigned, u64 w) { return (double)w >= target; });
+    const int at = s.found;
+    if (at < kBins) {
+      const u64 p = cut_in_bin(s, rule, each, at, s.counted[at], s.before[at], false, 0, target);
+      lowest = p > lowest ? p : lowest;
+    }
+  }
+  __syncthreads();
+  return lowest;
+}
+
+// Which of `count` (up to kParts) sums in s.parts the drawn token lies in, what is in front
+// of it and all of them: the first at which the running sum exceeds u times the total.
+struct Drawn {
+  int part;
+  u64 before, total, target;
+};
+__device__ Drawn draw_part(Shared& s, int count, float u) {
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int each = (count + kThreads - 1) / kThreads;
+  const int i0 = min(tid * each, count), i1 = min(i0 + each, count);
+  u64 mine = 0;
+  for (int i = i0; i < i1; ++i) mine += s.parts[i];
+  const u64 up_to = wave_inclusive(mine);
+  if (lane == 63) s.wave_weight[wave] = up_to;
+  __syncthreads();
+  u64 before = up_to - mine, total = 0;
+  for (int i = 0; i < kWaves; ++i) {
+    if (i < wave) before += s.wave_weight[i];
+    total += s.wave_weight[i];
+  }
+  u64 target = u > 0.f ? (u64)((double)fminf(u, 1.f) * (double)total) : 0;
+  if (target >= total) target = total - 1;
+  if (before <= target && target < before + mine) {
+    int i = i0;
+    for (; i < i1 - 1; ++i) {
+      if (target < before + s.parts[i]) break;
+      before += s.parts[i];
+    }
+    s.found = i;
+    s.lo = before;
+  }
+  __syncthreads();
+  return {s.found, s.lo, total, target};
 }
 
 template <typename T>
@@ -96,228 +359,154 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleArgs a) {
   extern __shared__ __align__(16) unsigned char shared_bytes[];
   Shared& s = *reinterpret_cast<Shared*>(shared_bytes);
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int row = blockIdx.x;
-  const T* logits = static_cast<const T*>(a.logits) + (size_t)row * a.logits_ld;
-  const int V = a.V;
+  const int m = blockIdx.x, V = a.V;
+  const Row<T> row(static_cast<const T*>(a.logits) + (size_t)m * a.logits_ld, V);
+  constexpr int kVec = Row<T>::kVec;
 
-  // The largest place.
-  if (tid == 0) s.nan = 0, s.hi = 0;
+  // The maxima of the thread's groups of values (NaN if one is), and of all.
+  float maxima[kGroups];
+#pragma unroll
+  for (int g = 0; g < kGroups; ++g) maxima[g] = -__builtin_huge_valf();
+  row.sweep([&](int, const float (&x)[kVec]) {
+#pragma unroll
+    for (int e = 0; e < kVec; ++e) maxima[e % kGroups] = __builtin_elementwise_maximum(maxima[e % kGroups], x[e]);
+  }, [&](int, float x) { maxima[0] = __builtin_elementwise_maximum(maxima[0], x); });
+  float top = maxima[0];
+#pragma unroll
+  for (int g = 1; g < kGroups; ++g) top = __builtin_elementwise_maximum(top, maxima[g]);
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) top = __builtin_elementwise_maximum(top, __shfl_xor(top, d));
+  if (lane == 0) s.wave_max[wave] = top;
+  if (tid == 0) s.found = V, s.listed_n = 0;
   __syncthreads();
-  u64 best = 0;
-  bool nan = false;
-  for (int v = tid; v < V; v += kThreads) {
-    const float x = static_cast<float>(logits[v]);
-    nan |= x != x;
-    const u64 p = place_of(x, v);
-    best = p > best ? p : best;
-  }
-  atomicMax(&s.hi, best);
-  if (nan) s.nan = 1;
-  __syncthreads();
-  best = s.hi;
-  const int best_at = (int)(0xffffffffu - (unsigned)best);
-  const float top = static_cast<float>(logits[best_at]);
-  if (s.nan || top == -__builtin_huge_valf()) {  // no distribution
-    if (tid == 0) a.tokens[row] = -1, a.logprobs[row] = __builtin_nanf("");
+#pragma unroll
+  for (int i = 0; i < kWaves; ++i) top = __builtin_elementwise_maximum(top, s.wave_max[i]);
+  if (!(top > -__builtin_huge_valf())) {  // NaN, or -inf alone: no distribution
+    if (tid == 0) a.tokens[m] = -1, a.logprobs[m] = __builtin_nanf("");
     return;
   }
-  const float temperature = a.temperature ? a.temperature[row] : 1.f;
+  const float temperature = a.temperature ? a.temperature[m] : 1.f;
   if (!(temperature > 0.f)) {  // greedy
-    if (tid == 0) a.tokens[row] = best_at, a.logprobs[row] = 0.f;
+    int first = V;
+    row.each([&](int v, float x) { first = x == top ? min(first, v) : first; });
+    if (first < V) atomicMin(&s.found, first);
+    __syncthreads();
+    if (tid == 0) a.tokens[m] = s.found, a.logprobs[m] = 0.f;
     return;
   }
-  const int k = a.top_k && a.top_k[row] > 0 ? a.top_k[row] : V;
-  const float min_p = a.min_p ? a.min_p[row] : 0.f;
-  const float top_p = a.top_p ? a.top_p[row] : 1.f;
-  const double least = min_p > 0.f ? (double)fminf(min_p, 1.f) * kUnit : 0.0;  // (NaN: off)
-  const bool by_k = k < V, by_p = top_p < 1.f;                                // (NaN: off)
+  const int k = a.top_k && a.top_k[m] > 0 ? a.top_k[m] : V;
+  const float min_p = a.min_p ? a.min_p[m] : 0.f;
+  const float top_p = a.top_p ? a.top_p[m] : 1.f;
+  const bool by_k = k < V, by_p = top_p < 1.f;  // (NaN: off)
+  const Rule rule = {top, (float)kBins * 1.44269504f / (kOctaves * temperature), 1.4426950408889634 / (double)temperature,
+                     min_p > 0.f ? (double)fminf(min_p, 1.f) * kUnit : 0.0};
+  const float u = a.uniforms[m];
 
-  const double to_base2 = 1.4426950408889634 / (double)temperature;
-  // Weight in units; 0 also for what min_p drops (a token without weight counts for nothing).
-  auto weight_of = [&](float x) -> u64 {
-    if (x == top) return 1ull << 44;
-    const double t = ((double)x - (double)top) * to_base2;
-    if (!(t > -kOctaves)) return 0;
-    const double w = __builtin_rint(exp2(t) * kUnit);
-    return w >= least ? (u64)w : 0;
-  };
-  // Bins down from the maximum, monotone in x.
-  const float per_bin = (float)kBins * 1.44269504f / (kOctaves * temperature);
-  auto bin_of = [&](float x) {
-    const float f = (top - x) * per_bin;
-    return x == top ? 0 : f < (float)(kBins - 1) ? (int)f : kBins - 1;
-  };
-  auto each = [&](auto f) {
-    for (int v = tid; v < V; v += kThreads) f(v, static_cast<float>(logits[v]));
-  };
-
-  // The lowest kept place of the bin in which a cut lies: the first k by count, or those with
-  // less than `target` in front of them.  base_c, base_w: what lies in front of the bin.
-  // Returns the place; s.kept: the weight up to it.
-  auto cut_in_bin = [&](int bin, unsigned base_c, u64 base_w, bool count, unsigned want, double target) -> u64 {
-    if (tid == 0) s.lo = ~0ull, s.hi = 0, s.n = 0;
-    __syncthreads();
-    {
-      u64 lo = ~0ull, hi = 0;
-      unsigned n = 0;
-      each([&](int v, float x) {
-        if (bin_of(x) == bin && weight_of(x)) {
-          const u64 p = place_of(x, v);
-          lo = p < lo ? p : lo, hi = p > hi ? p : hi, ++n;
-        }
-      });
-      if (n) atomicMin(&s.lo, lo), atomicMax(&s.hi, hi), atomicAdd(&s.n, n);
-    }
-    __syncthreads();
-    u64 lo = s.lo, hi = s.hi;
-    unsigned n = s.n;
-    while (n > kList) {
-      const int bits = 64 - __clzll((long long)(hi - lo));
-      const int shift = bits > 11 ? bits - 11 : 0;
-      for (int i = tid; i < kBins; i += kThreads) s.sub_count[i] = 0, s.sub_weight[i] = 0;
+  bool listed = (by_k && k <= kMostK) || min_p > 0.f || V <= kListed;
+  if (listed) {
+    // The bin of the k-th largest maximum: at least k values are in it or above.
+    int last = kBins - 1;
+    if (by_k && k <= kMostK) {
+      for (int i = tid; i < kBins; i += kThreads) s.count[i] = 0, s.weight[i] = 0;
       __syncthreads();
-      each([&](int v, float x) {
-        if (bin_of(x) != bin) return;
-        const u64 p = place_of(x, v);
-        if (p < lo || p > hi) return;
-        const u64 w = weight_of(x);
-        if (!w) return;
-        const int at = (int)((hi - p) >> shift);
-        atomicAdd(&s.sub_count[at], 1u);
-        atomicAdd(&s.sub_weight[at], w);
-      });
-      __syncthreads();
-      scan_bins(s, s.sub_count, s.sub_weight, nullptr, nullptr, [&](unsigned c, u64 w) {
-        return count ? base_c + c >= want : (double)(base_w + w) >= target;
-      });
-      // (rounding can leave the target out of reach: then the last)
-      int at = s.found;
-      if (at == kBins) at = (int)((hi - lo) >> shift);
-      __syncthreads();
-      if (tid == 0) s.lo = 0, s.hi = 0;
-      __syncthreads();
-      u64 c = 0, w = 0;
-      for (int i = tid; i < at; i += kThreads) c += s.sub_count[i], w += s.sub_weight[i];
-      if (c) atomicAdd(&s.lo, c), atomicAdd(&s.hi, w);
-      __syncthreads();
-      base_c += (unsigned)s.lo, base_w += s.hi;
-      n = s.sub_count[at];
-      hi -= (u64)at << shift;
-      const u64 low = hi - ((1ull << shift) - 1);
-      lo = hi >= ((1ull << shift) - 1) && low > lo ? low : lo;
-      __syncthreads();
-    }
-    if (tid == 0) s.n = 0, s.lo = ~0ull, s.kept = base_w;
-    __syncthreads();
-    each([&](int v, float x) {
-      if (bin_of(x) != bin) return;
-      const u64 p = place_of(x, v);
-      if (p < lo || p > hi) return;
-      const u64 w = weight_of(x);
-      if (!w) return;
-      const unsigned at = atomicAdd(&s.n, 1u);
-      if (at < kList) s.list[at] = p, s.list_weight[at] = w;
-    });
-    __syncthreads();
-    n = min(s.n, (unsigned)kList);
-    if (tid < (int)n) {
-      const u64 mine = s.list[tid];
-      unsigned c = base_c;
-      u64 w = base_w;
-      for (unsigned i = 0; i < n; ++i)
-        if (s.list[i] > mine) ++c, w += s.list_weight[i];
-      if (count ? c < want : c == 0 || (double)w < target) {
-        atomicMin(&s.lo, mine);
-        atomicAdd(&s.kept, s.list_weight[tid]);
-      }
-    }
-    __syncthreads();
-    return s.lo;
-  };
-
-  u64 lowest = 0;  // kept place
-  if (by_k || by_p) {
-    for (int i = tid; i < kBins; i += kThreads) s.count[i] = 0, s.weight[i] = 0;
-    __syncthreads();
-    each([&](int, float x) {
-      const u64 w = weight_of(x);
-      if (!w) return;
-      const int at = bin_of(x);
-      atomicAdd(&s.count[at], 1u);
-      atomicAdd(&s.weight[at], w);
-    });
-    __syncthreads();
-    scan_bins(s, s.count, s.weight, s.counted, s.before,
-              [&](unsigned c, u64) { return c > (unsigned)k; });  // more than k: a cut
-    u64 sum = s.before[kBins - 1] + s.weight[kBins - 1];
-    // The bin of the k-th: the first at which the count reaches k.
-    if (by_k && s.found < kBins) {
-      __syncthreads();
-      scan_bins(s, s.count, s.weight, s.counted, s.before, [&](unsigned c, u64) { return c >= (unsigned)k; });
-      const int bin = s.found;
-      __syncthreads();
-      lowest = cut_in_bin(bin, s.counted[bin], s.before[bin], true, (unsigned)k, 0.0);
-      sum = s.kept;
-    }
-    if (by_p) {
-      const double target = top_p > 0.f ? (double)top_p * (double)sum : 0.0;
-      __syncthreads();
-      scan_bins(s, s.count, s.weight, s.counted, s.before, [&](unsigned, u64 w) { return (double)w >= target; });
-      const int bin = s.found;
-      __syncthreads();
-      if (bin < kBins) {
-        const u64 p = cut_in_bin(bin, s.counted[bin], s.before[bin], false, 0, target);
-        lowest = p > lowest ? p : lowest;
-      }
-    }
-    __syncthreads();
-  }
-
-  // The draw: sums of kParts parts of each wave's share of the row, in index order.
-  const int share = (V + kWaves * kParts - 1) / (kWaves * kParts);
-  auto kept = [&](int v) -> u64 {
-    const float x = static_cast<float>(logits[v]);
-    return place_of(x, v) >= lowest ? weight_of(x) : 0;
-  };
-  for (int i = 0; i < kParts; ++i) {
-    const int begin = min((wave * kParts + i) * share, V), end = min(begin + share, V);
-    u64 w = 0;
-    for (int v = begin + lane; v < end; v += 64) w += kept(v);
 #pragma unroll
-    for (int d = 1; d < 64; d <<= 1) w += __shfl_xor(w, d);
-    if (lane == 0) s.parts[wave * kParts + i] = w;
+      for (int g = 0; g < kGroups; ++g)
+        if (maxima[g] > -__builtin_huge_valf()) atomicAdd(&s.count[rule.bin(maxima[g])], 1u);
+      __syncthreads();
+      scan_bins(s, s.count, s.weight, nullptr, nullptr, [&](unsigned c, u64) { return c >= (unsigned)k; });
+      last = min(s.found, kBins - 1);
+    }
+    auto list = [&](int v, float x) {
+      if (rule.bin(x) <= last && rule.weight(x)) {
+        const unsigned at = atomicAdd(&s.listed_n, 1u);
+        if (at < kListed) s.listed[at] = place_of(x, v);
+      }
+    };
+    row.sweep([&](int v0, const float (&x)[kVec]) {
+      float most = x[0];
+#pragma unroll
+      for (int e = 1; e < kVec; ++e) most = fmaxf(most, x[e]);
+      if (rule.bin(most) > last) return;
+#pragma unroll
+      for (int e = 0; e < kVec; ++e) list(v0 + e, x[e]);
+    }, list);
+    __syncthreads();
+    listed = s.listed_n <= kListed;  // (else ties, or logits too flat)
+  }
+  const int n = (int)s.listed_n;
+  auto each_listed = [&](auto f) {
+    for (int i = tid; i < n; i += kThreads) f(index_of(s.listed[i]), value_of(s.listed[i]));
+  };
+  auto each_of_row = [&](auto f) { row.each(f); };
+  u64 lowest = 0;
+  if (by_k || by_p)
+    lowest = listed ? lowest_kept(s, rule, each_listed, by_k, (unsigned)k, by_p, top_p)
+                    : lowest_kept(s, rule, each_of_row, by_k, (unsigned)k, by_p, top_p);
+
+  __syncthreads();
+  auto write = [&](int v, u64 w, u64 total) {
+    a.tokens[m] = v;
+    a.logprobs[m] = (float)log((double)w / (double)total);
+  };
+  if (listed) {
+    // Kept weights by ranges of the vocabulary, then token by token in the drawn range.
+    const int width = (V + kRanked - 1) / kRanked;  // (at most 512)
+    for (int i = tid; i < kRanked; i += kThreads) s.parts[i] = 0;
+    if (tid == 0) s.n = 0;
+    __syncthreads();
+    for (int i = tid; i < n; i += kThreads)
+      if (s.listed[i] >= lowest) atomicAdd(&s.parts[index_of(s.listed[i]) / width], rule.weight(value_of(s.listed[i])));
+    __syncthreads();
+    const Drawn d = draw_part(s, kRanked, u);
+    for (int i = tid; i < n; i += kThreads)
+      if (s.listed[i] >= lowest && index_of(s.listed[i]) / width == d.part) {
+        const unsigned at = atomicAdd(&s.n, 1u);
+        s.ranked[at] = s.listed[i];
+        s.ranked_weight[at] = rule.weight(value_of(s.listed[i]));
+      }
+    __syncthreads();
+    if (tid < (int)s.n) {
+      const int mine = index_of(s.ranked[tid]);
+      u64 before = d.before;
+      for (unsigned i = 0; i < s.n; ++i)
+        if (index_of(s.ranked[i]) < mine) before += s.ranked_weight[i];
+      const u64 w = s.ranked_weight[tid];
+      if (before <= d.target && d.target < before + w) write(mine, w, d.total);
+    }
+    return;
+  }
+  // Kept weights by 64 accesses of the row (a wave's), in index order: the values in front
+  // of the first access, the accesses, the values behind the last.
+  auto kept = [&](int v, float x) -> u64 { return place_of(x, v) >= lowest ? rule.weight(x) : 0; };
+  const int parts = (row.vecs + 63) / 64 + 2, tail = row.head + row.vecs * kVec;
+  if (tid == 0) s.parts[0] = 0, s.parts[parts - 1] = 0;
+  __syncthreads();
+  if (tid < row.head) atomicAdd(&s.parts[0], kept(tid, row.value(tid)));
+  if (tail + tid < V) atomicAdd(&s.parts[parts - 1], kept(tail + tid, row.value(tail + tid)));
+  for (int p = wave; p < parts - 2; p += kWaves) {
+    const int q = p * 64 + lane;
+    u64 w = 0;
+    if (q < row.vecs) {
+      const auto x = reinterpret_cast<const typename Row<T>::vec_t*>(row.at + row.head)[q];
+#pragma unroll
+      for (int e = 0; e < kVec; ++e) w += kept(row.head + q * kVec + e, static_cast<float>(x[e]));
+    }
+    w = wave_total(w);
+    if (lane == 0) s.parts[p + 1] = w;
   }
   __syncthreads();
+  const Drawn d = draw_part(s, parts, u);
   if (wave != 0) return;
-  constexpr int kMine = kWaves * kParts / 64;
-  u64 mine = 0;
-#pragma unroll
-  for (int i = 0; i < kMine; ++i) mine += s.parts[lane * kMine + i];
-  const u64 up_to = wave_inclusive(mine);
-  const u64 total = __shfl(up_to, 63);
-  const float u = a.uniforms[row];
-  u64 target = u > 0.f ? (u64)((double)fminf(u, 1.f) * (double)total) : 0;
-  if (target >= total) target = total - 1;
-  const u64 here = __ballot(up_to > target);
-  const int from = __builtin_ctzll(here);
-  u64 sum = __shfl(up_to - mine, from);
-  int part = from * kMine;
-  for (int i = 0; i < kMine - 1; ++i) {
-    const u64 w = s.parts[part];
-    if (sum + w > target) break;
-    sum += w, ++part;
-  }
-  const int begin = part * share, end = min(begin + share, V);
+  const int begin = d.part == 0 ? 0 : d.part == parts - 1 ? tail : row.head + (d.part - 1) * 64 * kVec;
+  const int end = d.part == 0 ? row.head : d.part == parts - 1 ? V : min(begin + 64 * kVec, tail);
+  u64 sum = d.before;
   for (int v0 = begin; v0 < end; v0 += 64) {
     const int v = v0 + lane;
-    const u64 w = v < end ? kept(v) : 0;
+    const u64 w = v < end ? kept(v, row.value(v)) : 0;
     const u64 c = sum + wave_inclusive(w);
-    const u64 there = __ballot(c > target);
+    const u64 there = __ballot(c > d.target);
     if (there) {
-      if (lane == __builtin_ctzll(there)) {
-        a.tokens[row] = v;
-        a.logprobs[row] = (float)log((double)w / (double)total);
-      }
+      if (lane == __builtin_ctzll(there)) write(v, w, d.total);
       return;
     }
     sum = __shfl(c, 63);
@@ -333,6 +522,7 @@ hipError_t launch(const SampleArgs& a, hipStream_t stream) {
 }  // namespace
 
 hipError_t launch_sample(const SampleArgs& a, bool bf16, hipStream_t stream) {
+  static_assert(sizeof(Shared) <= 160 * 1024, "LDS of a CU");
   return bf16 ? launch<__bf16>(a, stream) : launch<float>(a, stream);
 }
 
