@@ -35,12 +35,16 @@ constexpr int kWaves = kThreads / 64;
 constexpr int kBins = 2 * kThreads;
 constexpr int kRanked = 1024;               // places ranked against each other
 constexpr int kListed = 4096;               // tokens that may be kept
+constexpr int kFew = 256;                   // of them, compared each with each
 constexpr int kGroups = 4;                  // of values per thread, whose maxima bound the k-th
 constexpr int kMostK = kGroups * kThreads / 2;
-constexpr int kAhead = 4;                   // 16-byte loads of a thread in flight
+constexpr int kAhead = 8;                   // 16-byte loads of a thread in flight
+constexpr int kAheadDense = 2;              // ... where much is done with each value
 constexpr int kParts = kSampleMaxVocab / 256 + 2;
 constexpr double kUnit = 17592186044416.0;  // 2^44
-constexpr float kOctaves = 46.f;            // below the maximum: weights round to zero
+constexpr float kOctaves = 46.f;            // below the maximum, in the bins
+constexpr int kLastBin = kBins * 45 / 46 + 1;  // from 45 on weights round to zero
+static_assert(kLastBin < kBins - 1, "what lies below all bins is in the last");
 
 // Larger order: larger value; -0 equals +0.  (NaN is seen to apart.)
 __device__ __forceinline__ unsigned value_order(float v) {
@@ -68,20 +72,24 @@ __device__ __forceinline__ double power_of_2(double t) {
   return p * __builtin_bit_cast(double, (u64)(1023 + (int)n) << 52);
 }
 
-template <typename V>
-__device__ __forceinline__ V wave_inclusive(V v) {
-  const int lane = threadIdx.x & 63;
-#pragma unroll
-  for (int s = 1; s < 64; s <<= 1) {
-    const V o = __shfl_up(v, s);
-    if (lane >= s) v += o;
-  }
-  return v;
+// Inclusive sums over a wave's lanes: within rows of 16 (row_shr 1, 2, 4, 8), then rows 1 and 3
+// the row in front of them (row_bcast 15), then the upper half the lower (row_bcast 31).
+template <int kCtrl, int kRows>
+__device__ __forceinline__ unsigned moved(unsigned v) {
+  return (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, kCtrl, kRows, 0xf, false);
+}
+template <int kCtrl, int kRows>
+__device__ __forceinline__ u64 moved(u64 v) {
+  return (u64)moved<kCtrl, kRows>((unsigned)(v >> 32)) << 32 | moved<kCtrl, kRows>((unsigned)v);
 }
 template <typename V>
-__device__ __forceinline__ V wave_total(V v) {
-#pragma unroll
-  for (int s = 1; s < 64; s <<= 1) v += __shfl_xor(v, s);
+__device__ __forceinline__ V wave_inclusive(V v) {
+  v += moved<0x111, 0xf>(v);
+  v += moved<0x112, 0xf>(v);
+  v += moved<0x114, 0xf>(v);
+  v += moved<0x118, 0xf>(v);
+  v += moved<0x142, 0xa>(v);
+  v += moved<0x143, 0xc>(v);
   return v;
 }
 
@@ -119,7 +127,7 @@ struct Row {
   }
   __device__ __forceinline__ float value(int v) const { return static_cast<float>(at[v]); }
   // access(v0, x): kVec values from index v0 on; one(v, x): a value apart.  All threads.
-  template <typename Access, typename One>
+  template <int kAhead, typename Access, typename One>
   __device__ __forceinline__ void sweep(Access access, One one) const {
     const int tid = threadIdx.x;
     if (tid < head) one(tid, value(tid));
@@ -142,7 +150,7 @@ struct Row {
   }
   template <typename Each>
   __device__ __forceinline__ void each(Each f) const {
-    sweep([&](int v0, const float (&x)[kVec]) {
+    sweep<kAheadDense>([&](int v0, const float (&x)[kVec]) {
 #pragma unroll
       for (int e = 0; e < kVec; ++e) f(v0 + e, x[e]);
     }, f);
@@ -183,7 +191,11 @@ __device__ void scan_bins(Shared& s, const unsigned* count, const u64* weight, u
   __syncthreads();
   unsigned cb = c - c0 - c1;
   u64 wb = w - w0 - w1;
-  for (int i = 0; i < wave; ++i) cb += s.wave_count[i], wb += s.wave_weight[i];
+#pragma unroll
+  for (int i = 0; i < kWaves; ++i) {
+    cb += i < wave ? s.wave_count[i] : 0;
+    wb += i < wave ? s.wave_weight[i] : 0;
+  }
   if (counted) {
     counted[2 * tid] = cb, counted[2 * tid + 1] = cb + c0;
     before[2 * tid] = wb, before[2 * tid + 1] = wb + w0;
@@ -195,30 +207,47 @@ __device__ void scan_bins(Shared& s, const unsigned* count, const u64* weight, u
   __syncthreads();
 }
 
+// The first bin at which the count reaches k (kBins: none).
+__device__ __forceinline__ int bin_of_kth(Shared& s, unsigned k) {
+  const int tid = threadIdx.x, wave = tid >> 6;
+  const unsigned c0 = s.count[2 * tid], c1 = s.count[2 * tid + 1];
+  const unsigned up_to = wave_inclusive(c0 + c1);
+  if ((tid & 63) == 63) s.wave_count[wave] = up_to;
+  if (tid == 0) s.found = kBins;
+  __syncthreads();
+  unsigned c = up_to - c0 - c1;
+#pragma unroll
+  for (int i = 0; i < kWaves; ++i) c += i < wave ? s.wave_count[i] : 0;
+  if (c < k && c + c0 >= k)
+    s.found = 2 * tid;
+  else if (c + c0 < k && c + c0 + c1 >= k)
+    s.found = 2 * tid + 1;
+  __syncthreads();
+  return s.found;
+}
+
 // The lowest kept place of the bin in which a cut lies: the first `want` by count, or those with
-// less than `target` in front of them.  base_c, base_w: what lies in front of the bin.
-// each(f): f(v, x) for all tokens.  Returns the place; s.kept: the weight up to it.
+// less than `target` in front of them.  each(f): f(v, x) for all tokens, the bins filled and
+// scanned.  Returns the place; s.kept: the weight up to it.
 template <typename Each>
-__device__ u64 cut_in_bin(Shared& s, const Rule& rule, Each each, int bin, unsigned base_c, u64 base_w, bool by_count,
-                          unsigned want, double target) {
+__device__ u64 cut_in_bin(Shared& s, const Rule& rule, Each each, int bin, bool by_count, unsigned want, double target) {
   const int tid = threadIdx.x;
-  __syncthreads();
-  if (tid == 0) s.lo = ~0ull, s.hi = 0, s.n = 0;
-  __syncthreads();
-  {
-    u64 lo = ~0ull, hi = 0;
-    unsigned n = 0;
+  unsigned n = s.count[bin], base_c = s.counted[bin];
+  u64 lo = 0, hi = ~0ull, base_w = s.before[bin];
+  if (n > kRanked) {
+    if (tid == 0) s.lo = ~0ull, s.hi = 0;
+    __syncthreads();
+    u64 least = ~0ull, most = 0;
     each([&](int v, float x) {
       if (rule.bin(x) == bin && rule.weight(x)) {
         const u64 p = place_of(x, v);
-        lo = p < lo ? p : lo, hi = p > hi ? p : hi, ++n;
+        least = p < least ? p : least, most = p > most ? p : most;
       }
     });
-    if (n) atomicMin(&s.lo, lo), atomicMax(&s.hi, hi), atomicAdd(&s.n, n);
+    if (most) atomicMin(&s.lo, least), atomicMax(&s.hi, most);
+    __syncthreads();
+    lo = s.lo, hi = s.hi;
   }
-  __syncthreads();
-  u64 lo = s.lo, hi = s.hi;
-  unsigned n = s.n;
   __syncthreads();
   while (n > kRanked) {
     const int bits = 64 - __clzll((long long)(hi - lo));
@@ -302,7 +331,7 @@ __device__ u64 lowest_kept(Shared& s, const Rule& rule, Each each, bool by_k, un
   u64 sum = s.before[kBins - 1] + s.weight[kBins - 1], lowest = 0;
   const int bin = s.found;
   if (by_k && bin < kBins) {  // (fewer than k have weight: no cut)
-    lowest = cut_in_bin(s, rule, each, bin, s.counted[bin], s.before[bin], true, k, 0.0);
+    lowest = cut_in_bin(s, rule, each, bin, true, k, 0.0);
     sum = s.kept;
   }
   if (by_p) {
@@ -311,12 +340,18 @@ __device__ u64 lowest_kept(Shared& s, const Rule& rule, Each each, bool by_k, un
     scan_bins(s, s.count, s.weight, s.counted, s.before, [&](unsigned, u64 w) { return (double)w >= target; });
     const int at = s.found;
     if (at < kBins) {
-      const u64 p = cut_in_bin(s, rule, each, at, s.counted[at], s.before[at], false, 0, target);
+      const u64 p = cut_in_bin(s, rule, each, at, false, 0, target);
       lowest = p > lowest ? p : lowest;
     }
   }
   __syncthreads();
   return lowest;
+}
+
+// Where in a sum of kept weights the random number falls.
+__device__ __forceinline__ u64 drawn(float u, u64 total) {
+  const u64 at = u > 0.f ? (u64)((double)fminf(u, 1.f) * (double)total) : 0;
+  return at < total ? at : total - 1;
 }
 
 // Which of `count` (up to kParts) sums in s.parts the drawn token lies in, what is in front
@@ -335,12 +370,12 @@ __device__ Drawn draw_part(Shared& s, int count, float u) {
   if (lane == 63) s.wave_weight[wave] = up_to;
   __syncthreads();
   u64 before = up_to - mine, total = 0;
+#pragma unroll
   for (int i = 0; i < kWaves; ++i) {
-    if (i < wave) before += s.wave_weight[i];
+    before += i < wave ? s.wave_weight[i] : 0;
     total += s.wave_weight[i];
   }
-  u64 target = u > 0.f ? (u64)((double)fminf(u, 1.f) * (double)total) : 0;
-  if (target >= total) target = total - 1;
+  const u64 target = drawn(u, total);
   if (before <= target && target < before + mine) {
     int i = i0;
     for (; i < i1 - 1; ++i) {
@@ -352,6 +387,69 @@ __device__ Drawn draw_part(Shared& s, int count, float u) {
   }
   __syncthreads();
   return {s.found, s.lo, total, target};
+}
+
+// Sums over four neighbouring lanes (quad_perm).
+template <typename V>
+__device__ __forceinline__ V quad_sum(V v) {
+  v += moved<0xb1, 0xf>(v);
+  v += moved<0x4e, 0xf>(v);
+  return v;
+}
+
+// Up to kFew listed tokens, each compared with each by four lanes: its rank and what is in
+// front of it, then what is kept in front of its index.
+template <typename Write>
+__device__ __forceinline__ void few_tokens(Shared& s, const Rule& rule, int n, unsigned k, bool by_p, float top_p, float u,
+                                           Write write) {
+  static_assert(4 * kFew == kThreads, "four lanes to a token");
+  constexpr int kStep = 8;  // tokens of a lane at a time
+  const int tid = threadIdx.x, me = tid >> 2, q = tid & 3;
+  const bool here = me < n;
+  const u64 mine = here ? s.listed[me] : 0, w = here ? rule.weight(value_of(mine)) : 0;
+  const int rounded = (n + 4 * kStep - 1) / (4 * kStep) * (4 * kStep);
+  __syncthreads();
+  if (me < rounded && q == 0) {  // (places of zero are behind all others)
+    s.listed[me] = mine;
+    s.ranked_weight[me] = w;
+  }
+  __syncthreads();
+  unsigned rank = 0;
+  u64 before = 0;
+  if (here) {
+    for (int i0 = q; i0 < n; i0 += 4 * kStep) {
+#pragma unroll
+      for (int i = 0; i < kStep; ++i) {
+        const bool larger = s.listed[i0 + 4 * i] > mine;
+        rank += larger ? 1u : 0u;
+        before += larger ? s.ranked_weight[i0 + 4 * i] : 0;
+      }
+    }
+  }
+  rank = quad_sum(rank);
+  before = quad_sum(before);
+  if (here && rank == min(k, (unsigned)n) - 1) s.kept = before + w;  // the sum of the first k
+  __syncthreads();
+  const double target = top_p > 0.f ? (double)top_p * (double)s.kept : 0.0;
+  const bool kept = here && rank < k && (!by_p || rank == 0 || (double)before < target);
+  if (me < rounded && q == 0) s.ranked[me] = kept ? w : 0;
+  __syncthreads();
+  u64 in_front = 0, total = 0;
+  if (here) {
+    for (int i0 = q; i0 < n; i0 += 4 * kStep) {
+#pragma unroll
+      for (int i = 0; i < kStep; ++i) {
+        const u64 other = s.ranked[i0 + 4 * i];
+        total += other;
+        in_front += (unsigned)s.listed[i0 + 4 * i] > (unsigned)mine ? other : 0;  // (a lower index)
+      }
+    }
+  }
+  total = quad_sum(total);
+  in_front = quad_sum(in_front);
+  if (!kept || q != 0) return;
+  const u64 at = drawn(u, total);
+  if (in_front <= at && at < in_front + w) write(index_of(mine), w, total);
 }
 
 template <typename T>
@@ -367,7 +465,7 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleArgs a) {
   float maxima[kGroups];
 #pragma unroll
   for (int g = 0; g < kGroups; ++g) maxima[g] = -__builtin_huge_valf();
-  row.sweep([&](int, const float (&x)[kVec]) {
+  row.template sweep<kAhead>([&](int, const float (&x)[kVec]) {
 #pragma unroll
     for (int e = 0; e < kVec; ++e) maxima[e % kGroups] = __builtin_elementwise_maximum(maxima[e % kGroups], x[e]);
   }, [&](int, float x) { maxima[0] = __builtin_elementwise_maximum(maxima[0], x); });
@@ -405,28 +503,34 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleArgs a) {
   bool listed = (by_k && k <= kMostK) || min_p > 0.f || V <= kListed;
   if (listed) {
     // The bin of the k-th largest maximum: at least k values are in it or above.
-    int last = kBins - 1;
+    // And none that min-p keeps is far below it (two bins for what the logarithm is off).
+    int last = kLastBin;
+    if (min_p > 0.f) last = (int)fminf((float)last, 2.f - __log2f(fminf(min_p, 1.f)) * ((float)kBins / kOctaves));
     if (by_k && k <= kMostK) {
-      for (int i = tid; i < kBins; i += kThreads) s.count[i] = 0, s.weight[i] = 0;
+      for (int i = tid; i < kBins; i += kThreads) s.count[i] = 0;
       __syncthreads();
 #pragma unroll
-      for (int g = 0; g < kGroups; ++g)
-        if (maxima[g] > -__builtin_huge_valf()) atomicAdd(&s.count[rule.bin(maxima[g])], 1u);
+      for (int g = 0; g < kGroups; ++g) {
+        const int at = rule.bin(maxima[g]);
+        if (at <= kLastBin) atomicAdd(&s.count[at], 1u);
+      }
       __syncthreads();
-      scan_bins(s, s.count, s.weight, nullptr, nullptr, [&](unsigned c, u64) { return c >= (unsigned)k; });
-      last = min(s.found, kBins - 1);
+      last = min(bin_of_kth(s, (unsigned)k), last);
     }
+    // (some may weigh nothing: they change nothing)
+    const float end = (float)(last + 1);
+    auto in_reach = [&](float x) { return (top - x) * rule.per_bin < end || x == top; };
     auto list = [&](int v, float x) {
-      if (rule.bin(x) <= last && rule.weight(x)) {
+      if (in_reach(x)) {
         const unsigned at = atomicAdd(&s.listed_n, 1u);
         if (at < kListed) s.listed[at] = place_of(x, v);
       }
     };
-    row.sweep([&](int v0, const float (&x)[kVec]) {
+    row.template sweep<kAhead>([&](int v0, const float (&x)[kVec]) {
       float most = x[0];
 #pragma unroll
       for (int e = 1; e < kVec; ++e) most = fmaxf(most, x[e]);
-      if (rule.bin(most) > last) return;
+      if (!in_reach(most)) return;
 #pragma unroll
       for (int e = 0; e < kVec; ++e) list(v0 + e, x[e]);
     }, list);
@@ -434,6 +538,14 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleArgs a) {
     listed = s.listed_n <= kListed;  // (else ties, or logits too flat)
   }
   const int n = (int)s.listed_n;
+  auto write = [&](int v, u64 w, u64 total) {
+    a.tokens[m] = v;
+    a.logprobs[m] = (float)log((double)w / (double)total);
+  };
+  if (listed && n <= kFew) {
+    few_tokens(s, rule, n, (unsigned)k, by_p, top_p, u, write);
+    return;
+  }
   auto each_listed = [&](auto f) {
     for (int i = tid; i < n; i += kThreads) f(index_of(s.listed[i]), value_of(s.listed[i]));
   };
@@ -444,10 +556,6 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleArgs a) {
                     : lowest_kept(s, rule, each_of_row, by_k, (unsigned)k, by_p, top_p);
 
   __syncthreads();
-  auto write = [&](int v, u64 w, u64 total) {
-    a.tokens[m] = v;
-    a.logprobs[m] = (float)log((double)w / (double)total);
-  };
   if (listed) {
     // Kept weights by ranges of the vocabulary, then token by token in the drawn range.
     const int width = (V + kRanked - 1) / kRanked;  // (at most 512)
@@ -491,8 +599,8 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleArgs a) {
 #pragma unroll
       for (int e = 0; e < kVec; ++e) w += kept(row.head + q * kVec + e, static_cast<float>(x[e]));
     }
-    w = wave_total(w);
-    if (lane == 0) s.parts[p + 1] = w;
+    w = wave_inclusive(w);
+    if (lane == 63) s.parts[p + 1] = w;
   }
   __syncthreads();
   const Drawn d = draw_part(s, parts, u);
