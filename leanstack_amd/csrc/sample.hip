@@ -59,17 +59,32 @@ __device__ __forceinline__ u64 place_of(float x, int v) { return (u64)value_orde
 __device__ __forceinline__ int index_of(u64 place) { return (int)(0xffffffffu - (unsigned)place); }
 __device__ __forceinline__ float value_of(u64 place) { return ordered_value((unsigned)(place >> 32)); }
 
-// 2^t for t in -47..0, to 2^-50 of it: 2^n times the series of e^(f ln 2), |f| <= 1/2.
-__device__ __forceinline__ double power_of_2(double t) {
-  const double n = __builtin_rint(t), f = t - n;
-  // ln(2)^i / i!
-  constexpr double c[] = {1.0, 0.69314718055994531, 0.24022650695910071, 0.055504108664821580, 0.0096181291076284772,
+// 2^(j / 64), j = 0..63, and then 2^t by the nearest of them below it, 2^n, and the series of
+// e^(f ln(2) / 64), |f| <= 1/2: to 2^-50 of it.
+constexpr int kPowers = 64;
+__device__ __forceinline__ double root_power(int j) {
+  // ln(2)^i / i!, for 2^(j / 64 - 1 / 2)
+  constexpr double c[] = {1.0, 0.69314718055994531, 0.24022650695910072, 0.055504108664821580, 0.0096181291076284772,
                           0.0013333558146428443, 0.00015403530393381610, 1.5252733804059840e-05, 1.3215486790144309e-06,
                           1.0178086009239699e-07, 7.0549116208011233e-09, 4.4455382718708115e-10, 2.5678435993488206e-11};
+  const double f = (double)j / kPowers - 0.5;
   double p = c[12];
 #pragma unroll
   for (int i = 11; i >= 0; --i) p = __builtin_fma(p, f, c[i]);
-  return p * __builtin_bit_cast(double, (u64)(1023 + (int)n) << 52);
+  return p * 1.4142135623730951;
+}
+// Units of 2^(t64 / 64), t64 in -46 * 64..0, as a whole number: the sum with 2^52 rounds it.
+__device__ __forceinline__ u64 units_of(double t64, const double* powers) {
+  const double n = __builtin_rint(t64), f = t64 - n;
+  const int i = (int)n;
+  // (ln(2) / 64)^i / i!
+  constexpr double l = 0.69314718055994531 / kPowers;
+  constexpr double c[] = {1.0, l, l * l / 2, l * l * l / 6, l * l * l * l / 24, l * l * l * l * l / 120};
+  double p = c[5];
+#pragma unroll
+  for (int e = 4; e >= 0; --e) p = __builtin_fma(p, f, c[e]);
+  const double w = __builtin_ldexp(p * powers[i & (kPowers - 1)], 44 + (i >> 6));
+  return __builtin_bit_cast(u64, w + 0x1p52) & ((1ull << 52) - 1);
 }
 
 // Inclusive sums over a wave's lanes: within rows of 16 (row_shr 1, 2, 4, 8), then rows 1 and 3
@@ -94,6 +109,7 @@ __device__ __forceinline__ V wave_inclusive(V v) {
 }
 
 struct Shared {
+  double powers[kPowers];
   u64 weight[kBins], before[kBins];  // of the bins; and of those in front
   unsigned count[kBins], counted[kBins];
   union {
@@ -108,7 +124,7 @@ struct Shared {
   u64 wave_weight[kWaves];
   unsigned wave_count[kWaves];
   float wave_max[kWaves];
-  u64 lo, hi, kept;
+  u64 lo, hi, kept, total, total_listed;
   unsigned n, listed_n;
   int found;
 };
@@ -160,14 +176,16 @@ struct Row {
 // How a row's values weigh, and the bins that they fall into.
 struct Rule {
   float top, per_bin;
-  double to_base2, least;
+  double to_base2;  // and to 64ths
+  double least;
+  const double* powers;
   // Weight in units; 0 also for what min_p drops (a token without weight counts for nothing).
   __device__ __forceinline__ u64 weight(float x) const {
     if (x == top) return 1ull << 44;
     const double t = ((double)x - (double)top) * to_base2;
-    if (!(t > -kOctaves)) return 0;
-    const double w = __builtin_rint(power_of_2(t) * kUnit);
-    return w >= least ? (u64)w : 0;
+    if (!(t > -(double)kOctaves * kPowers)) return 0;
+    const u64 w = units_of(t, powers);
+    return (double)w >= least ? w : 0;
   }
   // Bins down from the maximum, monotone in x.
   __device__ __forceinline__ int bin(float x) const {
@@ -313,8 +331,9 @@ __device__ u64 cut_in_bin(Shared& s, const Rule& rule, Each each, int bin, bool 
 }
 
 // The lowest kept place under top-k (k below the number of tokens) and top-p (below 1).
+// total: of all tokens' weights, where each() leaves some out (else 0).
 template <typename Each>
-__device__ u64 lowest_kept(Shared& s, const Rule& rule, Each each, bool by_k, unsigned k, bool by_p, float top_p) {
+__device__ u64 lowest_kept(Shared& s, const Rule& rule, Each each, bool by_k, unsigned k, bool by_p, float top_p, u64 total) {
   const int tid = threadIdx.x;
   __syncthreads();
   for (int i = tid; i < kBins; i += kThreads) s.count[i] = 0, s.weight[i] = 0;
@@ -328,7 +347,7 @@ __device__ u64 lowest_kept(Shared& s, const Rule& rule, Each each, bool by_k, un
   });
   __syncthreads();
   scan_bins(s, s.count, s.weight, s.counted, s.before, [&](unsigned c, u64) { return by_k && c >= k; });
-  u64 sum = s.before[kBins - 1] + s.weight[kBins - 1], lowest = 0;
+  u64 sum = total ? total : s.before[kBins - 1] + s.weight[kBins - 1], lowest = 0;
   const int bin = s.found;
   if (by_k && bin < kBins) {  // (fewer than k have weight: no cut)
     lowest = cut_in_bin(s, rule, each, bin, true, k, 0.0);
@@ -400,8 +419,8 @@ __device__ __forceinline__ V quad_sum(V v) {
 // Up to kFew listed tokens, each compared with each by four lanes: its rank and what is in
 // front of it, then what is kept in front of its index.
 template <typename Write>
-__device__ __forceinline__ void few_tokens(Shared& s, const Rule& rule, int n, unsigned k, bool by_p, float top_p, float u,
-                                           Write write) {
+__device__ __forceinline__ void few_tokens(Shared& s, const Rule& rule, int n, unsigned k, bool by_p, float top_p, u64 all,
+                                           float u, Write write) {
   static_assert(4 * kFew == kThreads, "four lanes to a token");
   constexpr int kStep = 8;  // tokens of a lane at a time
   const int tid = threadIdx.x, me = tid >> 2, q = tid & 3;
@@ -430,7 +449,7 @@ __device__ __forceinline__ void few_tokens(Shared& s, const Rule& rule, int n, u
   before = quad_sum(before);
   if (here && rank == min(k, (unsigned)n) - 1) s.kept = before + w;  // the sum of the first k
   __syncthreads();
-  const double target = top_p > 0.f ? (double)top_p * (double)s.kept : 0.0;
+  const double target = top_p > 0.f ? (double)top_p * (double)(all ? all : s.kept) : 0.0;
   const bool kept = here && rank < k && (!by_p || rank == 0 || (double)before < target);
   if (me < rounded && q == 0) s.ranked[me] = kept ? w : 0;
   __syncthreads();
@@ -475,7 +494,8 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleArgs a) {
 #pragma unroll
   for (int d = 1; d < 64; d <<= 1) top = __builtin_elementwise_maximum(top, __shfl_xor(top, d));
   if (lane == 0) s.wave_max[wave] = top;
-  if (tid == 0) s.found = V, s.listed_n = 0;
+  if (tid == 0) s.found = V, s.listed_n = 0, s.total = s.total_listed = 0;
+  if (tid < kPowers) s.powers[tid] = root_power(tid);
   __syncthreads();
 #pragma unroll
   for (int i = 0; i < kWaves; ++i) top = __builtin_elementwise_maximum(top, s.wave_max[i]);
@@ -496,17 +516,21 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleArgs a) {
   const float min_p = a.min_p ? a.min_p[m] : 0.f;
   const float top_p = a.top_p ? a.top_p[m] : 1.f;
   const bool by_k = k < V, by_p = top_p < 1.f;  // (NaN: off)
-  const Rule rule = {top, (float)kBins * 1.44269504f / (kOctaves * temperature), 1.4426950408889634 / (double)temperature,
-                     min_p > 0.f ? (double)fminf(min_p, 1.f) * kUnit : 0.0};
+  const Rule rule = {top, (float)kBins * 1.44269504f / (kOctaves * temperature),
+                     kPowers * 1.4426950408889634 / (double)temperature, min_p > 0.f ? (double)fminf(min_p, 1.f) * kUnit : 0.0,
+                     s.powers};
   const float u = a.uniforms[m];
 
-  bool listed = (by_k && k <= kMostK) || min_p > 0.f || V <= kListed;
+  // Top-p alone: the sum is one of all weights, and the cut mostly among the first few thousand.
+  const bool sums = by_p && !by_k && !(min_p > 0.f);
+  u64 all = 0;
+  bool listed = (by_k && k <= kMostK) || min_p > 0.f || V <= kListed || sums;
   if (listed) {
     // The bin of the k-th largest maximum: at least k values are in it or above.
     // And none that min-p keeps is far below it (two bins for what the logarithm is off).
     int last = kLastBin;
     if (min_p > 0.f) last = (int)fminf((float)last, 2.f - __log2f(fminf(min_p, 1.f)) * ((float)kBins / kOctaves));
-    if (by_k && k <= kMostK) {
+    if ((by_k && k <= kMostK) || sums) {
       for (int i = tid; i < kBins; i += kThreads) s.count[i] = 0;
       __syncthreads();
 #pragma unroll
@@ -515,7 +539,7 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleArgs a) {
         if (at <= kLastBin) atomicAdd(&s.count[at], 1u);
       }
       __syncthreads();
-      last = min(bin_of_kth(s, (unsigned)k), last);
+      last = min(bin_of_kth(s, (unsigned)(sums ? kMostK : k)), last);
     }
     // (some may weigh nothing: they change nothing)
     const float end = (float)(last + 1);
@@ -526,7 +550,17 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleArgs a) {
         if (at < kListed) s.listed[at] = place_of(x, v);
       }
     };
-    row.template sweep<kAhead>([&](int v0, const float (&x)[kVec]) {
+    if (sums) {
+      u64 total = 0, reached = 0;
+      row.each([&](int v, float x) {
+        const u64 w = rule.weight(x);
+        total += w;
+        if (in_reach(x)) reached += w;
+        list(v, x);
+      });
+      total = wave_inclusive(total), reached = wave_inclusive(reached);
+      if (lane == 63) atomicAdd(&s.total, total), atomicAdd(&s.total_listed, reached);
+    } else row.template sweep<kAhead>([&](int v0, const float (&x)[kVec]) {
       float most = x[0];
 #pragma unroll
       for (int e = 1; e < kVec; ++e) most = fmaxf(most, x[e]);
@@ -535,7 +569,9 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleArgs a) {
       for (int e = 0; e < kVec; ++e) list(v0 + e, x[e]);
     }, list);
     __syncthreads();
-    listed = s.listed_n <= kListed;  // (else ties, or logits too flat)
+    all = s.total;
+    listed = s.listed_n <= kListed &&  // (else ties, or logits too flat)
+             (!sums || s.total_listed == all || (double)s.total_listed >= (double)top_p * (double)all);
   }
   const int n = (int)s.listed_n;
   auto write = [&](int v, u64 w, u64 total) {
@@ -543,7 +579,7 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleArgs a) {
     a.logprobs[m] = (float)log((double)w / (double)total);
   };
   if (listed && n <= kFew) {
-    few_tokens(s, rule, n, (unsigned)k, by_p, top_p, u, write);
+    few_tokens(s, rule, n, (unsigned)k, by_p, top_p, all, u, write);
     return;
   }
   auto each_listed = [&](auto f) {
@@ -552,8 +588,8 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleArgs a) {
   auto each_of_row = [&](auto f) { row.each(f); };
   u64 lowest = 0;
   if (by_k || by_p)
-    lowest = listed ? lowest_kept(s, rule, each_listed, by_k, (unsigned)k, by_p, top_p)
-                    : lowest_kept(s, rule, each_of_row, by_k, (unsigned)k, by_p, top_p);
+    lowest = listed ? lowest_kept(s, rule, each_listed, by_k, (unsigned)k, by_p, top_p, all)
+                    : lowest_kept(s, rule, each_of_row, by_k, (unsigned)k, by_p, top_p, 0);
 
   __syncthreads();
   if (listed) {
