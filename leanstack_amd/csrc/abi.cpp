@@ -458,14 +458,9 @@ int lsk_prefix_attention_bf16(const void* q, long long q_batch_stride, long long
 
 extern "C" {
 
-size_t lsk_sample_workspace_bytes(int logits_mode, int M, int V) {
-  if (lsk::check_sample_sizes(logits_mode, M, V) != LSK_OK) return 0;
-  return 0;
-}
-
 int lsk_sample_logits(const void* logits, int logits_mode, int M, int V, long long logits_ld, const float* uniforms,
                       const float* temperature, const int* top_k, const float* top_p, const float* min_p,
-                      long long* tokens, float* logprobs, void* workspace, size_t ws_bytes, void* hip_stream) {
+                      long long* tokens, float* logprobs, void* hip_stream) {
   lsk::clear_error();
   if (int st = lsk::check_sample_args(logits, logits_mode, M, V, logits_ld, uniforms, temperature, top_k, top_p, min_p,
                                       tokens, logprobs))

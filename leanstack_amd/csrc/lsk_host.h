@@ -233,7 +233,6 @@ constexpr int constrain_slices(int M, int V) {
 
 // Sampled tokens (sample.hip): a row's weights, whole numbers up to 2^44, add up in 63 bits.
 constexpr int kSampleMaxVocab = 1 << 19;
-int check_sample_sizes(int logits_mode, int M, int V);
 int check_sample_args(const void* logits, int logits_mode, int M, int V, long long logits_ld, const float* uniforms,
                       const float* temperature, const int* top_k, const float* top_p, const float* min_p,
                       const long long* tokens, const float* logprobs);

@@ -1146,19 +1146,12 @@ def sample_logits(logits: torch.Tensor, uniforms: torch.Tensor, *, temperature: 
     logprobs = logits.new_empty((m,), dtype=torch.float32)
     if m == 0:
         return tokens, logprobs
-    nbytes = _sample_workspace_bytes(mode, m, v)
-    workspace = logits.new_empty((nbytes,), dtype=torch.uint8) if nbytes else None
     with _on_index(index):
         status = _lib.load().lsk_sample_logits(
             logits.data_ptr(), mode, m, v, ld, uniforms_at, temperature_at, k_at, p_at, min_p_at, tokens.data_ptr(),
-            logprobs.data_ptr(), _ptr(workspace), nbytes, torch._C._cuda_getCurrentRawStream(index))
+            logprobs.data_ptr(), torch._C._cuda_getCurrentRawStream(index))
     _lib.check(status, "lsk_sample_logits")
     return tokens, logprobs
-
-
-@functools.lru_cache(maxsize=1024)
-def _sample_workspace_bytes(mode: int, m: int, v: int) -> int:
-    return _lib.load().lsk_sample_workspace_bytes(mode, m, v)
 
 
 def _ptr(t: torch.Tensor | None) -> int | None:

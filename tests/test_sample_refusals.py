@@ -8,7 +8,7 @@ import torch
 from leanstack_amd import _lib, kernels
 
 FAKE = 0x10000  # aligned, never dereferenced
-INVALID, WORKSPACE = -1, -4
+INVALID = -1
 
 
 @pytest.mark.parametrize("bad,code", [
@@ -20,10 +20,9 @@ INVALID, WORKSPACE = -1, -4
 ])
 def test_entry_point_rejects_before_launch(bad, code):
     lib = _lib.load()
-    a = dict(x=FAKE, mode=0, m=3, v=1000, ld=1000, u=FAKE, t=None, k=None, p=None, mp=None, tokens=FAKE, logs=FAKE, ws=FAKE,
-             ws_bytes=1 << 30) | bad
+    a = dict(x=FAKE, mode=0, m=3, v=1000, ld=1000, u=FAKE, t=None, k=None, p=None, mp=None, tokens=FAKE, logs=FAKE) | bad
     status = lib.lsk_sample_logits(a["x"], a["mode"], a["m"], a["v"], a["ld"], a["u"], a["t"], a["k"], a["p"], a["mp"],
-                                   a["tokens"], a["logs"], a["ws"], a["ws_bytes"], None)
+                                   a["tokens"], a["logs"], None)
     assert status == code
     assert lib.lsk_last_error()
 
