@@ -538,8 +538,8 @@ size_t lsk_paged_attention_workspace_bytes(int B, int T, int n_q, int n_kv, int 
  *   out[b][t][h][d] = softmax(scale * q K^T) V,  q head h reading kv head h / (n_q / n_kv);
  * scores, maxima and sums in fp32, the weights of V rounded to bf16 and normalised by the sum
  * of the rounded ones, bf16 output.  Query tokens from counts[b] on, and those that see
- * no row, give zeros; one whose rows all score -inf gives NaN.  Weights reach 2^8 before they are
- * normalised: finite values above some 2^110 may give infinities.
+ * no row, give zeros; one whose rows all score -inf gives NaN.  Weights reach 2^12 before they
+ * are normalised: over n rows, finite values above 2^115 / n may give infinities.
  *   q          device bf16, [d] at q + b * q_batch_stride + h * q_head_stride + t *
  *              q_token_stride (elements; multiples of 8), 16-byte aligned
  *   lens, counts   as for lsk_paged_append_bf16 (lens past the table's rows: those)

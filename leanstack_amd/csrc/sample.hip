@@ -176,6 +176,7 @@ struct Row {
 // How a row's values weigh, and the bins that they fall into.
 struct Rule {
   float top, per_bin;
+  float part, part_top;  // distances from the maximum are taken of half the values where they could overflow
   double to_base2;  // and to 64ths
   double least;
   const double* powers;
@@ -188,8 +189,9 @@ struct Rule {
     return (double)w >= least ? w : 0;
   }
   // Bins down from the maximum, monotone in x.
+  __device__ __forceinline__ float in_bins(float x) const { return __builtin_fmaf(x, -part, part_top) * per_bin; }
   __device__ __forceinline__ int bin(float x) const {
-    const float f = (top - x) * per_bin;
+    const float f = in_bins(x);
     return x == top ? 0 : f < (float)(kBins - 1) ? (int)f : kBins - 1;
   }
 };
@@ -516,7 +518,8 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleArgs a) {
   const float min_p = a.min_p ? a.min_p[m] : 0.f;
   const float top_p = a.top_p ? a.top_p[m] : 1.f;
   const bool by_k = k < V, by_p = top_p < 1.f;  // (NaN: off)
-  const Rule rule = {top, (float)kBins * 1.44269504f / (kOctaves * temperature),
+  const float part = top > 0x1p100f ? 0.5f : 1.f;
+  const Rule rule = {top, (float)kBins * 1.44269504f / (kOctaves * part) / temperature, part, top * part,
                      kPowers * 1.4426950408889634 / (double)temperature, min_p > 0.f ? (double)fminf(min_p, 1.f) * kUnit : 0.0,
                      s.powers};
   const float u = a.uniforms[m];
@@ -543,7 +546,7 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleArgs a) {
     }
     // (some may weigh nothing: they change nothing)
     const float end = (float)(last + 1);
-    auto in_reach = [&](float x) { return (top - x) * rule.per_bin < end || x == top; };
+    auto in_reach = [&](float x) { return rule.in_bins(x) < end || x == top; };
     auto list = [&](int v, float x) {
       if (in_reach(x)) {
         const unsigned at = atomicAdd(&s.listed_n, 1u);

@@ -190,6 +190,11 @@ class PagedKVCache:
             raise ValueError(f"one number of new rows (>= 0) per request is needed, got {counts}")
         return counts
 
+    def _reserved(self, requests: list[Request], counts: list[int]) -> None:
+        for r, n in zip(requests, counts):
+            if r.rows + n > len(r.pages) * self.page_rows:
+                raise ValueError(f"{r.rows} + {n} rows do not fit the request's {len(r.pages)} pages: reserve them first")
+
     def _copy(self, src: list[int], dst: list[int]) -> None:
         if not src:
             return
@@ -204,9 +209,7 @@ class PagedKVCache:
     def advance(self, requests: list[Request], new: int | list[int]) -> None:
         """Count rows that were appended (in every layer)."""
         counts = self._counts(requests, new)
-        for r, n in zip(requests, counts):
-            if r.rows + n > len(r.pages) * self.page_rows:
-                raise ValueError(f"{r.rows} + {n} rows do not fit the request's {len(r.pages)} pages: reserve them first")
+        self._reserved(requests, counts)
         for r, n in zip(requests, counts):
             r.rows += n
 
@@ -233,9 +236,10 @@ class PagedKVCache:
         their pages, -1 behind the last, and their rows with `new` ones that a step appends.
         table / lens: existing tensors to fill (a captured step's), wide enough."""
         counts = self._counts(requests, new)
-        for r, n in zip(requests, counts):
-            if r.rows + n > len(r.pages) * self.page_rows:
-                raise ValueError(f"{r.rows} + {n} rows do not fit the request's {len(r.pages)} pages: reserve them first")
+        self._reserved(requests, counts)
+        for r, n in zip(requests, counts):  # (a fork since reserve(); only the begun page can be another's too)
+            if n > 0 and r.rows % self.page_rows and self._holders[r.pages[r.rows // self.page_rows]] > 1:
+                raise ValueError(f"row {r.rows} would go to a page that another request holds: reserve it first")
         width = max([1] + [len(r.pages) for r in requests])
         if table is not None:
             if table.dim() != 2 or table.shape[0] != len(requests) or table.shape[1] < width or table.dtype is not torch.int32:

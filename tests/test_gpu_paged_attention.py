@@ -123,6 +123,27 @@ def test_many_requests(gpu):
     check(gpu, cache, queries(130, 8, 2, seed=35), table, lens, D ** -0.5, [i % 3 for i in range(130)])
 
 
+@pytest.mark.parametrize("t,n_q", [(1, 4), (5, 4), (90, 2)])
+def test_a_million_rows(gpu, t, n_q):
+    """A context of 2^20 rows, of 16 pages named again and again: the result is that of rows which
+    all weigh as often as they are named (the last, begun round aside, whose rows are left out).
+    Sums of 2^20 weights in fp32, in chunks: 2^-24 for each of a chunk's, at most 2^14 in a row."""
+    n_kv, page_rows, pages = 1, 64, 16
+    cache, table = setup(gpu, n_kv, page_rows, [pages * page_rows], seed=31)
+    named = table[0][:pages]
+    rounds = 1024
+    q = queries(1, n_q, t, seed=32)
+    # the same rows for every query token: the last rounds have no page
+    wide = named * rounds + [-1] * (t // page_rows + 1)
+    got = kernels.paged_attention(q.to(gpu), cache, 0, ints(gpu, [wide]), ints(gpu, [pages * page_rows * rounds + t - 1]), 0.1)
+    pool = Pool(cache.storage[0], cache.exponents[0])
+    for i in range(t):
+        want, bound = attention(pool, q[:, :, i:i + 1], [named], [pages * page_rows], 0.1)
+        most = pool.dense(named, pages * page_rows)[1].abs().max()
+        off = (got[:, i].cpu().double().view(1, 1, n_q, D) - want).abs()
+        assert bool((off <= bound + 2 * 2.0 ** -10 * most).all())
+
+
 @pytest.mark.parametrize("t", [1, 6, 70])
 @pytest.mark.parametrize("scale", [-0.1, 0.0, 1.0, 1e-30, 40.0])
 def test_scales(gpu, t, scale):

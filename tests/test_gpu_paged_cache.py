@@ -205,6 +205,28 @@ def test_copy_whole_pages_of_any_size(gpu, n_kv, page_rows):
     assert torch.equal(cache.storage, storage) and torch.equal(cache.exponents, exponents)
 
 
+def test_pages_past_four_gib(gpu):
+    """Rows, copies and attention in pages whose bytes lie past 2^32 of a layer's keys, as in a small pool."""
+    n_kv, page_rows, far, middle = 8, 1024, 4299, 2100
+    large, small = PagedKVCache(1, n_kv, far + 1, page_rows=page_rows, device=gpu), PagedKVCache(1, n_kv, 4, page_rows=page_rows, device=gpu)
+    where, lens = {0: far, 1: middle, 2: far - 1, 3: 7}, [1000, 1500]
+    k, v = (x.to(gpu) for x in new_rows(2, n_kv, 700, seed=40))
+    q = new_rows(2, 4 * n_kv, 40, seed=41)[0].to(gpu)
+    results = []
+    for cache, name in ((small, lambda p: p), (large, lambda p: where[p])):
+        table = tables(gpu, [[name(0), name(1)], [name(2), name(3)]])
+        kernels.paged_append(cache, 0, k, v, table, ints(gpu, lens))
+        kernels.copy_pages(cache, ints(gpu, [name(0)]), ints(gpu, [name(1)]))
+        results.append([*kernels.paged_read(cache, 0, table, ints(gpu, [300, 800]), 1200), *(
+            kernels.paged_attention(q[:, :, :t].contiguous(), cache, 0, table, ints(gpu, lens), 0.1) for t in (1, 7, 40))])
+    assert all(torch.equal(x, y) for x, y in zip(*results))
+    for p, at in where.items():
+        assert torch.equal(small.storage[:, :, p], large.storage[:, :, at])
+        assert torch.equal(small.exponents[:, :, p], large.exponents[:, :, at])
+    others = [p for p in (0, 1, 2, 3, 4, 5, 6, 8, middle - 1, middle + 1, far - 2)]
+    assert not bool(large.storage[:, :, others].any())
+
+
 def test_captured_append_follows_lens_counts_and_table(gpu):
     cache = random_pool(gpu, 1, 2, 6, 16, seed=16)
     pool = Pool(cache.storage[0], cache.exponents[0])

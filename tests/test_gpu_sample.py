@@ -97,6 +97,18 @@ def test_rows_of_their_own(gpu, m):
         top_p=rng.choice([0.0, -1.0, 0.1, 0.9, 1.0, 2.0], m).tolist(), min_p=rng.choice([0.0, -0.5, 1e-4, 0.1, 1.0, 3.0], m).tolist())
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("v", [500, 9001])
+@pytest.mark.parametrize("temperature", [1e37, 1e38, 3e38, math.inf])
+def test_values_further_apart_than_the_largest_number(gpu, temperature, v, dtype):
+    """Differences that overflow in 32 bits, at temperatures that make them small."""
+    logits = logits_of(3, v, seed=21, std=1.0, dtype=dtype).clamp(-3.3, 3.3) * 1e38
+    if math.isfinite(temperature):
+        logits[2, ::7] = -math.inf
+    for i, options in enumerate(({}, dict(top_k=40), dict(top_k=400, top_p=0.7), dict(top_p=0.6), dict(min_p=0.01), dict(min_p=0.9))):
+        run(gpu, logits, uniforms_of(3, seed=22 + i), temperature=[temperature] * 3, **{k: [x] * 3 for k, x in options.items()})
+
+
 @pytest.mark.parametrize("std", [0.0, 1e-6, 0.01, 30.0, 1e4, 1e30])
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_flat_and_steep(gpu, std, dtype):

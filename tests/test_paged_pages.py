@@ -106,6 +106,25 @@ def test_fork_of_reserved_pages():
     assert b.pages[1] not in a.pages
 
 
+def test_rows_for_a_shared_page_are_refused():
+    """A fork between reserve() and batch(): the new row would be written into both."""
+    cache = cache_of()
+    a, full = cache.open(), cache.open()
+    grow(cache, [a, full], [5, 16])
+    cache.reserve([a], 3)
+    b = cache.fork(a)
+    cache.fork(full)
+    for call in (lambda: cache.batch([a], 1), lambda: cache.batch([full, b], [0, 1])):
+        with pytest.raises(ValueError, match="another request holds"):
+            call()
+    cache.batch([a, b, full])
+    cache.reserve([b], 3)
+    for r in (a, b):
+        assert cache.batch([r], 3)[1].tolist() == [8]
+    cache.reserve([full], 1)
+    cache.batch([full], 1)
+
+
 def test_truncate():
     cache = cache_of()
     a = cache.open()
