@@ -606,6 +606,7 @@ int lsk_paged_attention_bf16(const lsk_paged_pool* pool, const void* q, long lon
   a.places = (int)p.places;
   a.workers = (int)p.workers;
   a.least_units = p.least_units;
+  a.join_shift = p.join_shift;
   a.slot_rows = p.slot_rows;
   const size_t begins = (size_t)lsk::paged_begins_bytes(p), slots = (size_t)p.slots * pool->n_kv * p.slot_rows;
   a.begins = static_cast<int*>(workspace);

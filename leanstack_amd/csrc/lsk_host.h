@@ -151,30 +151,50 @@ constexpr int kPagedMostPageRows = 1024;
 // Blocks that `rows` rows from any row on can touch.
 constexpr int paged_windows(int rows) { return (int)(((long long)rows + 2 * kPagedBlockRows - 2) / kPagedBlockRows); }
 
-// How an attention call runs.  An item is `rows` query rows (16, 32 or 64, or 128 where
-// waves have rows of their own) of one request and kv head.  one_launch: a workgroup per
-// item.  Else few rows are cut into chunks of at least `least_units` units of key rows, a
-// wave each, `places` per kv head and one more per item at most; of 128 rows `workers`
-// workgroups per kv head share all units.
+// How an attention call runs.  An item is `rows` query rows of one request and kv head.
+// - Up to 64 rows over a context that is short for certain run in one launch, a workgroup per
+//   item, while the chip holds all the workgroups: 24 requests over 2048 rows 21 us, 26 in two
+//   launches; 1 request 14 us for 13, so few workgroups have the lower limit.  From
+//   kPagedShortGroups workgroups on (64 requests of 8 kv heads) two launches take as long (20 us
+//   over 512 rows), with 128 requests 29 us for 39.
+// - Else up to 32 rows are cut into chunks of at least `least_units` units of key rows, a wave
+//   each, at most `places` per kv head and one more per item.  2048 waves in all for up to 16
+//   rows (64 requests over 4096 rows: 95 us, with 1024 waves 115), 1024 for 32, whose waves do
+//   more with a row (24 x 5 tokens over 2000 rows: 24 us, with 2048 waves 26, with 512 37).
+//   Chunks of 4 units: 1 request over 8192 rows 13.5 us, of 2 15.3, of 8 15.6.
+// - More are taken 128 at a time by workgroups of which `workers` per kv head share all units,
+//   512 in all (256 were 342 us for 276 in prompts of 1500 tokens).  Also 33..64 rows: 8 x 16
+//   tokens over 8192 rows 55 us, 71 by waves of 64 rows.
+// The second launch adds up parts, 2^join_shift query rows to a workgroup; with more parts than
+// its threads can take at once it has fewer rows (1 request over 32768 rows, 256 parts: 6.4 us, 39
+// with 16 rows); with many query rows more of them, `join_passes` times, so that fewer
+// workgroups wait for their first loads (4 x 2000 tokens: 16 us, 32 with one pass).
 constexpr int kPagedFewUnit = 32;
 constexpr int kPagedManyUnit = 64;
 constexpr int kPagedManyRows = 128;
-constexpr int kPagedShortRows = 1024;
+constexpr int kPagedShortRows = 2048, kPagedShortFewRows = 1536, kPagedShortFewGroups = 128, kPagedShortGroups = 512;
+constexpr int kPagedJoinGroups = 2048, kPagedJoinPasses = 4;
 struct PagedPlan {
   bool one_launch;
   int rows, slot_rows, unit, least_units, tiles;
+  int join_shift;   // a workgroup of the second launch adds up the parts of 2^join_shift query rows
+  int join_passes;  // .. times this many, one behind the other
+  bool join_wide;   // .. with 1024 threads, not 256
   long long items, places, workers, slots;  // slots: of parts, per kv head
 };
 constexpr PagedPlan paged_plan(int B, int T, int n_q, int n_kv, int capacity) {
   const long long rows = (long long)T * (n_q / n_kv);
-  PagedPlan p = {false, rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : kPagedManyRows, 0, kPagedFewUnit, 4, 0, 0, 0, 0, 0};
+  PagedPlan p = {false, rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : kPagedManyRows, 0, kPagedFewUnit, 4, 0, 0, 1, false, 0, 0, 0, 0};
+  const long long groups = (long long)B * n_kv;
+  p.one_launch = rows <= 64 && groups < kPagedShortGroups &&
+                 capacity <= (groups < kPagedShortFewGroups ? kPagedShortFewRows : kPagedShortRows);
+  if (rows > 32 && !p.one_launch) p.rows = kPagedManyRows;
   const bool many = p.rows == kPagedManyRows;
   if (many) p.unit = kPagedManyUnit;
   p.slot_rows = rows < p.rows ? (int)rows : p.rows;
   p.tiles = (int)((rows + p.rows - 1) / p.rows);
   p.items = (long long)B * p.tiles;
-  p.one_launch = !many && capacity <= kPagedShortRows;
-  const int all = many ? 512 : 2048;
+  const int all = many ? 512 : p.rows == 32 ? 1024 : 2048;
   const long long most = p.items * ((capacity + p.unit - 1) / p.unit);
   p.places = all / n_kv > 1 ? all / n_kv : 1;
   // (an item more or less than a chunk adds one: all chunks are to run at once)
@@ -182,6 +202,12 @@ constexpr PagedPlan paged_plan(int B, int T, int n_q, int n_kv, int capacity) {
   if (p.places > most) p.places = most;
   p.workers = many ? p.places : p.places + p.items;
   p.slots = many ? 2 * p.workers : p.workers;
+  const long long shortest = many ? p.unit : p.unit * p.least_units, longest = (capacity + shortest - 1) / shortest;
+  const long long parts = p.workers / p.items < longest ? p.workers / p.items : longest;
+  p.join_shift = 4;
+  while (p.join_shift > 0 && (p.slot_rows <= 1 << (p.join_shift - 1) || (64 >> p.join_shift) < parts)) --p.join_shift;
+  p.join_wide = parts >= 128;
+  p.join_passes = many && p.join_shift == 4 && p.items * n_kv * ((p.slot_rows + 15) / 16) > kPagedJoinGroups ? kPagedJoinPasses : 1;
   return p;
 }
 // (m, l) and O of every slot, and where the items begin.

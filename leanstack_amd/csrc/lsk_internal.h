@@ -375,7 +375,7 @@ struct PagedAttentionArgs {
   int* begins;
   float *part_ml, *part_o;
   size_t q_b, q_h, q_t;
-  int B, T, G, n_q, tiles, items, places, workers, least_units, slot_rows;
+  int B, T, G, n_q, tiles, items, places, workers, least_units, slot_rows, join_shift;
   float scale;
 };
 hipError_t launch_paged_attention(const PagedAttentionArgs& a, const PagedPlan& plan, hipStream_t stream);

@@ -59,6 +59,7 @@ constexpr int D = kAttnHeadDim;
 constexpr int kFewWaves = 4, kShortWaves = 8;  // of a workgroup for few query rows
 constexpr float kRaise = 8.f, kMostWeight = 256.f;  // in base 2
 constexpr float kFar = 0x1p30f;
+constexpr int kJoinThreads = 256, kJoinWide = 1024;
 constexpr float kLowest = -3.402823466e38f;
 
 __device__ __forceinline__ float neg_inf() { return -__builtin_huge_valf(); }
@@ -629,15 +630,20 @@ __global__ __launch_bounds__(64 * kShortWaves, 2) void short_attention_kernel(Pa
   }
 }
 
-// Adds up the parts of items that were cut.  Grid: kv head (fastest), item, 16 rows of it.
-constexpr int kJoinThreads = 256;
-template <bool MANY>
-__global__ __launch_bounds__(kJoinThreads) void join_kernel(PagedAttentionArgs a, int rows) {
+// Adds up the parts of items that were cut.  Grid: kv head (fastest), item, `1 << a.join_shift` query
+// rows of it; 16 threads take 8 dims each of a part's row, and the rest of the workgroup other rows
+// or, with few rows, further parts: stream s the parts s, s + streams, ..
+template <bool MANY, int THREADS, int PASSES>
+__global__ __launch_bounds__(THREADS) void join_kernel(PagedAttentionArgs a, int rows) {
+  constexpr int kSlots = THREADS / 16;
+  __shared__ __align__(16) float os[kSlots][D];
+  __shared__ float ms[kSlots], ls[kSlots];
   int id = blockIdx.x;
   const int j = id % a.pool.n_kv;
   id /= a.pool.n_kv;
-  const int groups = rows / 16;
-  const int item = id / groups, group = id % groups;
+  const int own = 1 << a.join_shift, streams = kSlots >> a.join_shift;  // rows at a time; and of each
+  const int groups = (min(rows, a.T * a.G) + own * PASSES - 1) / (own * PASSES);
+  const int item = id / groups, group = id - item * groups;
   const int begin = a.begins[item], end = a.begins[item + 1];
   // parts `from` .. `last`: a slot per chunk, or the second slot of the worker that has the first unit
   // and the first slots of those up to the last unit's
@@ -654,45 +660,88 @@ __global__ __launch_bounds__(kJoinThreads) void join_kernel(PagedAttentionArgs a
   }
   if (from == last) return;
   const int b = a.tiles == 1 ? item : item / a.tiles, tile = item - b * a.tiles;
-  const int r = group * 16 + (threadIdx.x >> 4), row = tile * rows + r, d0 = (threadIdx.x & 15) * 8;
-  if (row >= a.T * a.G) return;
-  const int t = row / a.G, h = j * a.G + row % a.G;
-  float m = neg_inf(), l = 0.f;
-  f32x4_t o[2] = {};
-  // kJoinAhead parts on their way at a time (past the last the last again, unused)
-  constexpr int kJoinAhead = 4;
-  for (int w0 = from; w0 <= last; w0 += kJoinAhead) {
-    f32x2_t ml[kJoinAhead];
-    f32x4_t x[kJoinAhead][2];
+  const int slot = threadIdx.x >> 4, d0 = (threadIdx.x & 15) * 8;
+  const int stream = slot >> a.join_shift;
+  const int r0 = group * own * PASSES + (slot & (own - 1)), end_row = min(rows, a.T * a.G - tile * rows);
+  float m[PASSES], l[PASSES];
+  f32x4_t o[PASSES][2];
+#pragma unroll
+  for (int p = 0; p < PASSES; ++p) m[p] = neg_inf(), l[p] = 0.f, o[p][0] = o[p][1] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  // kJoinAhead parts of each row on their way at a time (past the last the last again, unused)
+  constexpr int kJoinAhead = PASSES > 1 ? 2 : 4;
+  for (int w0 = from + stream; w0 <= last; w0 += kJoinAhead * streams) {
+    f32x2_t ml[kJoinAhead][PASSES];
+    f32x4_t x[kJoinAhead][PASSES][2];
 #pragma unroll
     for (int i = 0; i < kJoinAhead; ++i) {
-      const int w = min(w0 + i, last);
-      const size_t slot = (size_t)j * a.workers + w;
-      const Part part = part_of(a, MANY ? slot * 2 + (w == from ? 1 : 0) : slot);
-      ml[i] = *reinterpret_cast<const f32x2_t*>(part.ml + r * 2);
+      const int w = min(w0 + i * streams, last);
+      const size_t at = (size_t)j * a.workers + w;
+      const Part part = part_of(a, MANY ? at * 2 + (w == from ? 1 : 0) : at);
 #pragma unroll
-      for (int e = 0; e < 2; ++e) x[i][e] = *reinterpret_cast<const f32x4_t*>(part.o + (size_t)r * D + d0 + 4 * e);
+      for (int p = 0; p < PASSES; ++p) {
+        const int r = min(r0 + p * own, end_row - 1);
+        ml[i][p] = *reinterpret_cast<const f32x2_t*>(part.ml + r * 2);
+#pragma unroll
+        for (int e = 0; e < 2; ++e) x[i][p][e] = *reinterpret_cast<const f32x4_t*>(part.o + (size_t)r * D + d0 + 4 * e);
+      }
     }
 #pragma unroll
     for (int i = 0; i < kJoinAhead; ++i) {
-      if (w0 + i > last) break;
-      if (MANY && share_begin(units, w0 + i, a.workers) == share_begin(units, w0 + i + 1, a.workers))
+      const int w = w0 + i * streams;
+      if (w > last) break;
+      if (MANY && share_begin(units, w, a.workers) == share_begin(units, w + 1, a.workers))
         continue;  // (fewer units than workers: one without a share)
-      const float top = fmaxf(m, ml[i][0]);
-      const float was = m == top ? 1.f : __builtin_amdgcn_exp2f(m - top);
-      const float now = ml[i][0] == top ? 1.f : __builtin_amdgcn_exp2f(ml[i][0] - top);
-      l = l * was + ml[i][1] * now;
 #pragma unroll
-      for (int e = 0; e < 2; ++e) o[e] = o[e] * was + x[i][e] * now;
-      m = top;
+      for (int p = 0; p < PASSES; ++p) {
+        const float top = fmaxf(m[p], ml[i][p][0]);
+        const float was = m[p] == top ? 1.f : __builtin_amdgcn_exp2f(m[p] - top);
+        const float now = ml[i][p][0] == top ? 1.f : __builtin_amdgcn_exp2f(ml[i][p][0] - top);
+        l[p] = l[p] * was + ml[i][p][1] * now;
+#pragma unroll
+        for (int e = 0; e < 2; ++e) o[p][e] = o[p][e] * was + x[i][p][e] * now;
+        m[p] = top;
+      }
     }
   }
-  const bool none = t >= request_of(a, b).count || m == neg_inf();
-  const float share = none ? 0.f : 1.f / l;
-  bf16x8_t x;
+  auto place = [&](int of) {
+    const int t = of / a.G, h = j * a.G + of % a.G;
+    return a.out + (((size_t)b * a.T + t) * a.n_q + h) * D;
+  };
+  const int count = request_of(a, b).count;
+  if (PASSES > 1 || streams == 1) {
 #pragma unroll
-  for (int e = 0; e < 8; ++e) x[e] = static_cast<__bf16>(none ? 0.f : o[e / 4][e % 4] * share);
-  *reinterpret_cast<bf16x8_t*>(a.out + (((size_t)b * a.T + t) * a.n_q + h) * D + d0) = x;
+    for (int p = 0; p < PASSES; ++p) {
+      const int r = r0 + p * own, row = tile * rows + r;
+      if (r >= end_row) break;
+      const bool none = row / a.G >= count || m[p] == neg_inf();
+      const float share = none ? 0.f : 1.f / l[p];
+      bf16x8_t x;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[e] = static_cast<__bf16>(none ? 0.f : o[p][e / 4][e % 4] * share);
+      *reinterpret_cast<bf16x8_t*>(place(row) + d0) = x;
+    }
+    return;
+  }
+  // The streams' sums in their order: a thread per row and dim.
+#pragma unroll
+  for (int e = 0; e < 2; ++e) *reinterpret_cast<f32x4_t*>(&os[slot][d0 + 4 * e]) = o[0][e];
+  if (d0 == 0) ms[slot] = m[0], ls[slot] = l[0];
+  __syncthreads();
+  for (int i = threadIdx.x; i < own * D; i += THREADS) {
+    const int mine = i / D, d = i % D, to = tile * rows + group * own + mine;
+    if (group * own + mine >= end_row) continue;
+    float most = ms[mine];
+    for (int s = 1; s < streams; ++s) most = fmaxf(most, ms[s * own + mine]);
+    float sum = 0.f, x = 0.f;
+    for (int s = 0; s < streams; ++s) {
+      const float part = ms[s * own + mine];
+      const float weight = part == most ? 1.f : __builtin_amdgcn_exp2f(part - most);
+      sum += ls[s * own + mine] * weight;
+      x += os[s * own + mine][d] * weight;
+    }
+    const bool none = to / a.G >= count || most == neg_inf();
+    place(to)[d] = static_cast<__bf16>(none ? 0.f : x * (1.f / sum));
+  }
 }
 
 // ------------------------------------------------------------------ many query rows
@@ -1074,15 +1123,17 @@ hipError_t launch_paged_attention(const PagedAttentionArgs& a, const PagedPlan& 
   const dim3 grid(n_kv * (plan.rows == kManyRows ? a.workers : ceil_div(a.workers, kFewWaves)));
   if (plan.rows == 16) launch_kernel(few_attention_kernel<1>, grid, dim3(64 * kFewWaves), 0, stream, a);
   if (plan.rows == 32) launch_kernel(few_attention_kernel<2>, grid, dim3(64 * kFewWaves), 0, stream, a);
-  if (plan.rows == 64) launch_kernel(few_attention_kernel<4>, grid, dim3(64 * kFewWaves), 0, stream, a);
   if (plan.rows == kManyRows) launch_kernel(many_attention_kernel, grid, dim3(64 * kManyWaves), 0, stream, a);
   hipError_t err = hipGetLastError();
   if (err != hipSuccess) return err;
-  const dim3 joins((unsigned)a.items * n_kv * (plan.rows / 16));
-  if (plan.rows == kManyRows)
-    launch_kernel(join_kernel<true>, joins, dim3(kJoinThreads), 0, stream, a, plan.rows);
+  const dim3 joins((unsigned)a.items * n_kv * (unsigned)ceil_div(plan.slot_rows, plan.join_passes << plan.join_shift));
+  auto join = [&](auto kernel, int threads) { launch_kernel(kernel, joins, dim3(threads), 0, stream, a, plan.rows); };
+  if (plan.rows != kManyRows)
+    plan.join_wide ? join(join_kernel<false, kJoinWide, 1>, kJoinWide) : join(join_kernel<false, kJoinThreads, 1>, kJoinThreads);
+  else if (plan.join_passes > 1)
+    join(join_kernel<true, kJoinThreads, kPagedJoinPasses>, kJoinThreads);
   else
-    launch_kernel(join_kernel<false>, joins, dim3(kJoinThreads), 0, stream, a, plan.rows);
+    plan.join_wide ? join(join_kernel<true, kJoinWide, 1>, kJoinWide) : join(join_kernel<true, kJoinThreads, 1>, kJoinThreads);
   return hipGetLastError();
 }
 

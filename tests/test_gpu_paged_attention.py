@@ -144,6 +144,21 @@ def test_a_million_rows(gpu, t, n_q):
         assert bool((off <= bound + 2 * 2.0 ** -10 * most).all())
 
 
+@pytest.mark.parametrize("n_q,n_kv,t,lens,counts", [
+    (4, 1, 1, [16500], None), (32, 8, 1, [9000, 33, 0, 2500], None), (3, 1, 1, [20000, 7], None),   # many parts of few rows
+    (4, 1, 5, [17000], None), (8, 2, 5, [5000, 3, 2100, 5], [5, 3, 4, 0]), (2, 2, 32, [2100, 40], None),
+    (4, 1, 10, [3000], None), (8, 2, 16, [2300, 16, 9], [16, 16, 3]),   # 33..64 rows in two launches
+    (4, 1, 20, [9000], None), (2, 1, 33, [8500, 12], [33, 1]),          # .. many parts of them
+    (32, 8, 128, [128, 300, 129, 5, 192, 200, 128, 130, 131], [128, 128, 128, 5, 128, 100, 1, 128, 0]),
+    (4, 4, 1, [33 + 8 * i for i in range(140)], None), (8, 8, 3, [33 + 8 * i for i in range(70)], None),  # whole and cut ones
+])
+def test_parts(gpu, n_q, n_kv, t, lens, counts):
+    """Contexts cut into any number of parts, joined by workgroups of each kind."""
+    cache, table = setup(gpu, n_kv, 64, lens, seed=41)
+    wide = [row + [-1] * 33 for row in table]   # (a table of more than 2048 rows: no call in one launch)
+    check(gpu, cache, queries(len(lens), n_q, t, seed=42), wide, lens, 0.1, counts)
+
+
 @pytest.mark.parametrize("t", [1, 6, 70])
 @pytest.mark.parametrize("scale", [-0.1, 0.0, 1.0, 1e-30, 40.0])
 def test_scales(gpu, t, scale):

@@ -22,14 +22,14 @@ FAKE = 0x10000  # aligned, never dereferenced
     (MOST, MOST, MOST, MOST, MOST), (1 << 20, 1 << 20, 32, 8, 4096), (MOST, 1, 1, 1, 4096), (1, MOST, 8, 8, 4096),
     (0, 1, 8, 8, 4096), (1, 0, 8, 8, 4096), (1, 1, 8, 0, 4096), (1, 1, 7, 8, 4096), (1, 1, 12, 8, 4096), (1, 1, 8, 8, 0),
     (1, 1, 8, 8, -16), (1, 1, 8, 8, 4095), (1, 1, 8, 8, MOST), (1, 1, 8, 8, (1 << 30) + 16), (1 << 16, 64, 8, 8, 1 << 30),
-    (4, 1, 32, 8, 1024),   # (served by one launch without a workspace)
+    (4, 1, 32, 8, 1536), (16, 5, 32, 8, 2048), (63, 16, 32, 8, 2048),   # (served by one launch without a workspace)
 ])
 def test_no_workspace(b, t, n_q, n_kv, capacity):
     assert _lib.load().lsk_paged_attention_workspace_bytes(b, t, n_q, n_kv, capacity) == 0
 
 
 @pytest.mark.parametrize("b,t,n_q,n_kv,capacity", [
-    (1, 1, 32, 8, 1040), (64, 1, 32, 8, 1 << 16), (24, 5, 32, 8, 4096), (2, 1500, 32, 8, 2048), (1, 1, 8, 8, 1 << 30),
+    (1, 1, 32, 8, 1552), (16, 5, 32, 8, 2064), (64, 1, 32, 8, 64), (64, 1, 32, 8, 1 << 16), (24, 5, 32, 8, 4096), (2, 1500, 32, 8, 2048), (1, 1, 8, 8, 1 << 30),
     (1, 17, 32, 8, 64), (4096, 1, 32, 8, 8192), (1, 1, 4096, 4096, 2048),
 ])
 @pytest.mark.parametrize("bad", ["none", "small", "misaligned"])
