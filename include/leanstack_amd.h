@@ -445,6 +445,11 @@ int lsk_constrain_logits(const void* logits, int logits_mode, int M, int V, long
                          long long bias_ld, int bias_count, const int* allowed, long long allowed_ld,
                          void* out, long long* tokens, void* workspace, size_t ws_bytes, void* hip_stream);
 
+/* Device workspace of lsk_sample_logits (any contents; 0: none, or sizes that it refuses): few rows
+ * without top_k and min_p are worked on by several workgroups each.  by_*: whether the
+ * argument is given. */
+size_t lsk_sample_workspace_bytes(int logits_mode, int M, int V, int by_top_k, int by_top_p, int by_min_p);
+
 /* A token drawn from each row of logits by a given random number.  With weights
  *   w[v] = 2^-44 * round(2^44 * exp((x[v] - max x) / temperature)),
  * tokens ordered by larger x, then lower index:
@@ -464,10 +469,12 @@ int lsk_constrain_logits(const void* logits, int logits_mode, int M, int V, long
  *                 min_p up to 0 and NaN: all, above 1: as 1
  *   tokens        device int64 [M]
  *   logprobs      device fp32 [M]
+ *   workspace     lsk_sample_workspace_bytes(...) bytes, 16-byte aligned; calls that share
+ *                 one must be stream-ordered
  * The reference's head is greedy (src/leanstack/runtime/cutile_logits.py:37-69). */
 int lsk_sample_logits(const void* logits, int logits_mode, int M, int V, long long logits_ld, const float* uniforms,
                       const float* temperature, const int* top_k, const float* top_p, const float* min_p,
-                      long long* tokens, float* logprobs, void* hip_stream);
+                      long long* tokens, float* logprobs, void* workspace, size_t ws_bytes, void* hip_stream);
 
 /* ------------------------------------------------------------------------
  * A paged key/value cache in 8 bits.

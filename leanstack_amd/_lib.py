@@ -146,10 +146,11 @@ class PagedPool(ctypes.Structure):
 
 
 _SIGNATURES.update({
+    "lsk_sample_workspace_bytes": (_c_size, [_c_int] * 6),
     "lsk_sample_logits": (
         _c_int,
         [_c_void, _c_int, _c_int, _c_int, ctypes.c_longlong, _c_void, _c_void, _c_void, _c_void, _c_void, _c_void, _c_void,
-         _c_void],
+         _c_void, _c_size, _c_void],
     ),
     "lsk_paged_append_bf16": (
         _c_int,

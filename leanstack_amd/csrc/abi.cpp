@@ -458,9 +458,14 @@ int lsk_prefix_attention_bf16(const void* q, long long q_batch_stride, long long
 
 extern "C" {
 
+size_t lsk_sample_workspace_bytes(int logits_mode, int M, int V, int by_top_k, int by_top_p, int by_min_p) {
+  if (lsk::check_sample_sizes(logits_mode, M, V) != LSK_OK) return 0;
+  return (size_t)M * lsk::sample_row_bytes(lsk::sample_slices(M, V, by_top_k || by_min_p), V, by_top_p);
+}
+
 int lsk_sample_logits(const void* logits, int logits_mode, int M, int V, long long logits_ld, const float* uniforms,
                       const float* temperature, const int* top_k, const float* top_p, const float* min_p,
-                      long long* tokens, float* logprobs, void* hip_stream) {
+                      long long* tokens, float* logprobs, void* workspace, size_t ws_bytes, void* hip_stream) {
   lsk::clear_error();
   if (int st = lsk::check_sample_args(logits, logits_mode, M, V, logits_ld, uniforms, temperature, top_k, top_p, min_p,
                                       tokens, logprobs))
@@ -477,6 +482,14 @@ int lsk_sample_logits(const void* logits, int logits_mode, int M, int V, long lo
   a.logits_ld = (size_t)logits_ld;
   a.M = M;
   a.V = V;
+  a.slices = lsk::sample_slices(M, V, top_k != nullptr || min_p != nullptr);
+  a.max_parts = lsk::sample_max_parts(V);
+  a.workspace = static_cast<unsigned char*>(workspace);
+  a.row_bytes = (size_t)lsk::sample_row_bytes(a.slices, V, top_p != nullptr);
+  const size_t need = (size_t)M * a.row_bytes;
+  if (need > 0 && (workspace == nullptr || ws_bytes < need || !aligned(workspace, 16)))
+    return fail(LSK_ERR_WORKSPACE, "these logits need a workspace of %zu bytes, 16-byte aligned (got %zu)", need,
+                workspace ? ws_bytes : 0);
   hipError_t err = lsk::launch_sample(a, logits_mode == LSK_LOGITS_BF16, static_cast<hipStream_t>(hip_stream));
   return err == hipSuccess ? LSK_OK : hip_fail(err, "sampling kernel launch");
 }

@@ -191,14 +191,19 @@ int check_constrain_args(const void* logits, int logits_mode, int M, int V, long
   return LSK_OK;
 }
 
-int check_sample_args(const void* logits, int logits_mode, int M, int V, long long logits_ld, const float* uniforms,
-                      const float* temperature, const int* top_k, const float* top_p, const float* min_p,
-                      const long long* tokens, const float* logprobs) {
+int check_sample_sizes(int logits_mode, int M, int V) {
   if (logits_mode != LSK_LOGITS_FP32 && logits_mode != LSK_LOGITS_BF16)
     return fail(LSK_ERR_INVALID, "unknown logits mode %d", logits_mode);
   if (M < 1 || V < 1 || V > kSampleMaxVocab)
     return fail(LSK_ERR_INVALID, "M=%d rows of V=%d values (at most %d)", M, V, kSampleMaxVocab);
   if (M > (int)(0xffffffffLL / 1024)) return fail(LSK_ERR_INVALID, "M=%d rows are too many", M);
+  return LSK_OK;
+}
+
+int check_sample_args(const void* logits, int logits_mode, int M, int V, long long logits_ld, const float* uniforms,
+                      const float* temperature, const int* top_k, const float* top_p, const float* min_p,
+                      const long long* tokens, const float* logprobs) {
+  if (int st = check_sample_sizes(logits_mode, M, V)) return st;
   if (logits_ld < V) return fail(LSK_ERR_INVALID, "logits_ld=%lld must be at least V=%d", logits_ld, V);
   if (logits == nullptr || uniforms == nullptr || tokens == nullptr || logprobs == nullptr)
     return fail(LSK_ERR_INVALID, "null device pointer");

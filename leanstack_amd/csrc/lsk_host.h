@@ -259,6 +259,23 @@ constexpr int constrain_slices(int M, int V) {
 
 // Sampled tokens (sample.hip): a row's weights, whole numbers up to 2^44, add up in 63 bits.
 constexpr int kSampleMaxVocab = 1 << 19;
+
+// Rows without top-k and min-p are cut into slices while the chip has room for all, of at least
+// kSampleLeastSlice values.
+constexpr int kSampleMaxSlices = 16, kSampleLeastSlice = 8192, kSamplePlaces = 512;
+constexpr int kSampleBins = 2048, kSampleSliceListed = 512, kSampleRowBytes = 256;
+constexpr int sample_slices(int M, int V, bool ranked) {
+  const int room = kSamplePlaces / M, most = V / kSampleLeastSlice;
+  const int slices = room < most ? room : most;
+  return ranked || slices < 2 ? 1 : slices < kSampleMaxSlices ? slices : kSampleMaxSlices;
+}
+// (parts of 64 accesses of 16 bytes)
+constexpr int sample_max_parts(int V) { return V / 256 + 3; }
+constexpr unsigned long long sample_row_bytes(int slices, int V, bool by_p) {
+  const unsigned long long words = sample_max_parts(V) + (by_p ? slices * (unsigned long long)(kSampleSliceListed + kSampleBins) : 0);
+  return slices < 2 ? 0 : (kSampleRowBytes + words * 8 + 255) / 256 * 256;
+}
+int check_sample_sizes(int logits_mode, int M, int V);
 int check_sample_args(const void* logits, int logits_mode, int M, int V, long long logits_ld, const float* uniforms,
                       const float* temperature, const int* top_k, const float* top_p, const float* min_p,
                       const long long* tokens, const float* logprobs);

@@ -297,6 +297,10 @@ struct SampleArgs {
   float* logprobs;
   size_t logits_ld;
   int M, V;
+  // Rows cut into slices (1: not), and what they leave, row_bytes for each row.
+  int slices, max_parts;
+  unsigned char* workspace;
+  size_t row_bytes;
 };
 hipError_t launch_sample(const SampleArgs& a, bool bf16, hipStream_t stream);
 

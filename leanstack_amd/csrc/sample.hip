@@ -19,7 +19,8 @@
 // row do: the first takes the maximum of each of 4096 groups of values, of which the k-th
 // largest is a bound below which none of the first k lies; the second lists what is above
 // it.  All else works on the list, in LDS.  Without either (top-p or the temperature alone)
-// every weight counts, and each step is a sweep.
+// every weight counts, and a workgroup is bound by the arithmetic of the weights: few rows
+// are cut into slices, a workgroup each, which leave sums for the row's own.
 
 #include <hip/hip_runtime.h>
 
@@ -32,7 +33,8 @@ typedef unsigned long long u64;
 
 constexpr int kThreads = 1024;
 constexpr int kWaves = kThreads / 64;
-constexpr int kBins = 2 * kThreads;
+constexpr int kBins = kSampleBins;
+static_assert(kBins == 2 * kThreads, "two to a thread");
 constexpr int kRanked = 1024;               // places ranked against each other
 constexpr int kListed = 4096;               // tokens that may be kept
 constexpr int kFew = 256;                   // of them, compared each with each
@@ -129,6 +131,12 @@ struct Shared {
   int found;
 };
 
+// Accesses [first, end) of a row, and the values in front of the first and behind the last.
+struct Range {
+  int first, end;
+  bool head, tail;
+};
+
 // A row in accesses of 16 bytes from its first aligned value on: access q holds the kVec
 // values from head + q kVec on; those around them are taken one by one.
 template <typename T>
@@ -145,16 +153,20 @@ struct Row {
   // access(v0, x): kVec values from index v0 on; one(v, x): a value apart.  All threads.
   template <int kAhead, typename Access, typename One>
   __device__ __forceinline__ void sweep(Access access, One one) const {
-    const int tid = threadIdx.x;
-    if (tid < head) one(tid, value(tid));
+    sweep<kAhead>(Range{0, vecs, true, true}, access, one);
+  }
+  template <int kAhead, typename Access, typename One>
+  __device__ __forceinline__ void sweep(const Range& r, Access access, One one) const {
+    const int tid = threadIdx.x, first = r.first, end = r.end;
+    if (r.head && tid < head) one(tid, value(tid));
     const vec_t* body = reinterpret_cast<const vec_t*>(at + head);
-    for (int q0 = tid; q0 < vecs; q0 += kAhead * kThreads) {
+    for (int q0 = first + tid; q0 < end; q0 += kAhead * kThreads) {
       vec_t x[kAhead];
 #pragma unroll
-      for (int k = 0; k < kAhead; ++k) x[k] = body[min(q0 + k * kThreads, vecs - 1)];
+      for (int k = 0; k < kAhead; ++k) x[k] = body[min(q0 + k * kThreads, end - 1)];
 #pragma unroll
       for (int k = 0; k < kAhead; ++k) {
-        if (q0 + k * kThreads >= vecs) break;
+        if (q0 + k * kThreads >= end) break;
         float f[kVec];
 #pragma unroll
         for (int e = 0; e < kVec; ++e) f[e] = static_cast<float>(x[k][e]);
@@ -162,14 +174,22 @@ struct Row {
       }
     }
     const int tail = head + vecs * kVec + tid;
-    if (tail < V) one(tail, value(tail));
+    if (r.tail && tail < V) one(tail, value(tail));
   }
   template <typename Each>
-  __device__ __forceinline__ void each(Each f) const {
-    sweep<kAheadDense>([&](int v0, const float (&x)[kVec]) {
+  __device__ __forceinline__ void each(const Range& r, Each f) const {
+    sweep<kAheadDense>(r, [&](int v0, const float (&x)[kVec]) {
 #pragma unroll
       for (int e = 0; e < kVec; ++e) f(v0 + e, x[e]);
     }, f);
+  }
+  template <typename Each>
+  __device__ __forceinline__ void each(Each f) const { each(Range{0, vecs, true, true}, f); }
+  // Parts of the row in index order: the values in front of the first access, the accesses by
+  // 64 (a wave's), the values behind the last.
+  __device__ __forceinline__ int parts() const { return (vecs + 63) / 64 + 2; }
+  __device__ __forceinline__ int part_of(int v) const {
+    return v < head ? 0 : v >= head + vecs * kVec ? parts() - 1 : (v - head) / (64 * kVec) + 1;
   }
 };
 
@@ -195,6 +215,12 @@ struct Rule {
     return x == top ? 0 : f < (float)(kBins - 1) ? (int)f : kBins - 1;
   }
 };
+
+__device__ __forceinline__ Rule rule_of(float top, float temperature, float min_p, const double* powers) {
+  const float part = top > 0x1p100f ? 0.5f : 1.f;
+  return {top, (float)kBins * 1.44269504f / (kOctaves * part) / temperature, part, top * part,
+          kPowers * 1.4426950408889634 / (double)temperature, min_p > 0.f ? (double)fminf(min_p, 1.f) * kUnit : 0.0, powers};
+}
 
 // Exclusive sums of count and weight over the bins; found: the first bin at which `reached`
 // (count and weight up to and with it), kBins if there is none.
@@ -473,7 +499,242 @@ __device__ __forceinline__ void few_tokens(Shared& s, const Rule& rule, int n, u
   if (in_front <= at && at < in_front + w) write(index_of(mine), w, total);
 }
 
+// ------------------------------------------------------------------ few rows, all weights
+
+// What a row's slices leave for each other: their maxima; the bin in which top-p cuts (kBins: no
+// cut) and the weight in front of it; and of each slice the first index of the maximum (for
+// rows without a temperature) and how many tokens of that bin it has (more than
+// kSampleSliceListed: too many).
+struct RowSums {
+  u64 before, total;
+  int bin;
+  float max[kSampleMaxSlices];
+  int first[kSampleMaxSlices];
+  unsigned n[kSampleMaxSlices];
+};
+static_assert(sizeof(RowSums) <= kSampleRowBytes, "as the host counts it");
+struct Space {
+  RowSums* row;
+  u64* parts;   // [parts] weights in front of the cut, by the row's parts
+  u64* listed;  // [slices][kSampleSliceListed] places of the bin of the cut
+  u64* bins;    // [slices][kBins] weights
+};
+__device__ __forceinline__ Space space_of(const SampleArgs& a, int m) {
+  unsigned char* at = a.workspace + (size_t)m * a.row_bytes;
+  Space s;
+  s.row = reinterpret_cast<RowSums*>(at);
+  s.parts = reinterpret_cast<u64*>(at + kSampleRowBytes);
+  s.listed = s.parts + a.max_parts;
+  s.bins = s.listed + (size_t)a.slices * kSampleSliceListed;
+  return s;
+}
+// Slice i of a row: whole parts.
 template <typename T>
+__device__ __forceinline__ Range slice_of(const SampleArgs& a, const Row<T>& row, int i) {
+  const int each = ((row.vecs + 63) / 64 + a.slices - 1) / a.slices * 64;
+  const int first = min(i * each, row.vecs);
+  return {first, min(first + each, row.vecs), i == 0, i == a.slices - 1};
+}
+// The row's maximum (NaN if there is one), by all threads.
+__device__ __forceinline__ float row_top(const SampleArgs& a, const RowSums& r) {
+  float top = r.max[0];
+  for (int i = 1; i < a.slices; ++i) top = __builtin_elementwise_maximum(top, r.max[i]);
+  return top;
+}
+
+// Grid of these three: slice (fastest), row.
+template <typename T>
+__global__ __launch_bounds__(kThreads) void slice_top_kernel(SampleArgs a) {
+  __shared__ float wave_max[kWaves];
+  const int m = blockIdx.x / a.slices, i = blockIdx.x % a.slices;
+  const Row<T> row(static_cast<const T*>(a.logits) + (size_t)m * a.logits_ld, a.V);
+  const Range sl = slice_of(a, row, i);
+  float top = -__builtin_huge_valf();
+  row.template sweep<kAheadDense>(sl, [&](int, const float (&x)[Row<T>::kVec]) {
+#pragma unroll
+    for (int e = 0; e < Row<T>::kVec; ++e) top = __builtin_elementwise_maximum(top, x[e]);
+  }, [&](int, float x) { top = __builtin_elementwise_maximum(top, x); });
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) top = __builtin_elementwise_maximum(top, __shfl_xor(top, d));
+  if ((threadIdx.x & 63) == 0) wave_max[threadIdx.x >> 6] = top;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int w = 1; w < kWaves; ++w) top = __builtin_elementwise_maximum(top, wave_max[w]);
+    space_of(a, m).row->max[i] = top;
+  }
+}
+
+// Weights by bins, of rows that top-p cuts.
+template <typename T>
+__global__ __launch_bounds__(kThreads) void slice_bins_kernel(SampleArgs a) {
+  __shared__ u64 weight[kBins];
+  __shared__ double powers[kPowers];
+  const int m = blockIdx.x / a.slices, i = blockIdx.x % a.slices, tid = threadIdx.x;
+  const Space at = space_of(a, m);
+  const float temperature = a.temperature ? a.temperature[m] : 1.f, top = row_top(a, *at.row);
+  if (!(top > -__builtin_huge_valf()) || !(temperature > 0.f) || !(a.top_p[m] < 1.f)) return;
+  if (tid < kPowers) powers[tid] = root_power(tid);
+  weight[2 * tid] = weight[2 * tid + 1] = 0;
+  __syncthreads();
+  const Rule rule = rule_of(top, temperature, 0.f, powers);
+  const Row<T> row(static_cast<const T*>(a.logits) + (size_t)m * a.logits_ld, a.V);
+  const Range sl = slice_of(a, row, i);
+  row.each(sl, [&](int, float x) {
+    const u64 w = rule.weight(x);
+    if (w) atomicAdd(&weight[rule.bin(x)], w);
+  });
+  __syncthreads();
+  u64* out = at.bins + (size_t)i * kBins;
+  out[2 * tid] = weight[2 * tid], out[2 * tid + 1] = weight[2 * tid + 1];
+}
+
+// Weights by parts: all, or those in front of the bin in which top-p cuts, whose tokens are listed.
+template <typename T>
+__global__ __launch_bounds__(kThreads) void slice_parts_kernel(SampleArgs a) {
+  constexpr int kVec = Row<T>::kVec;
+  __shared__ double powers[kPowers];
+  __shared__ u64 wave_weight[kWaves], before_bin;
+  __shared__ int found;
+  __shared__ unsigned listed;
+  const int m = blockIdx.x / a.slices, i = blockIdx.x % a.slices, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const Space at = space_of(a, m);
+  const float temperature = a.temperature ? a.temperature[m] : 1.f, top = row_top(a, *at.row);
+  if (!(top > -__builtin_huge_valf())) return;
+  const Row<T> row(static_cast<const T*>(a.logits) + (size_t)m * a.logits_ld, a.V);
+  const Range sl = slice_of(a, row, i);
+  if (tid < kPowers) powers[tid] = root_power(tid);
+  if (tid == 0) found = a.V > kBins ? a.V : kBins, listed = 0;
+  __syncthreads();
+  if (!(temperature > 0.f)) {
+    int first = a.V;
+    row.each(sl, [&](int v, float x) { first = x == top ? min(first, v) : first; });
+    if (first < a.V) atomicMin(&found, first);
+    __syncthreads();
+    if (tid == 0) at.row->first[i] = found;
+    return;
+  }
+  const Rule rule = rule_of(top, temperature, 0.f, powers);
+  const float top_p = a.top_p ? a.top_p[m] : 1.f;
+  int bin = kBins;
+  if (top_p < 1.f) {
+    u64 w0 = 0, w1 = 0;
+    for (int s = 0; s < a.slices; ++s) {
+      const u64* bins = at.bins + (size_t)s * kBins + 2 * tid;
+      w0 += bins[0], w1 += bins[1];
+    }
+    const u64 up_to = wave_inclusive(w0 + w1);
+    if (lane == 63) wave_weight[wave] = up_to;
+    __syncthreads();
+    u64 before = up_to - w0 - w1, total = 0;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+      before += w < wave ? wave_weight[w] : 0;
+      total += wave_weight[w];
+    }
+    const double target = top_p > 0.f ? (double)top_p * (double)total : 0.0;
+    const bool first = w0 && (double)(before + w0) >= target, second = w1 && (double)(before + w0 + w1) >= target;
+    if (first || second) atomicMin(&found, first ? 2 * tid : 2 * tid + 1);
+    __syncthreads();
+    bin = found;  // (the sum of all is no less than the target)
+    if (bin >> 1 == tid) before_bin = before + (bin & 1 ? w0 : 0);
+    __syncthreads();
+    if (i == 0 && tid == 0) at.row->before = before_bin, at.row->total = total;
+  }
+  if (i == 0 && tid == 0) at.row->bin = bin;
+  auto kept = [&](int v, float x) -> u64 {
+    const u64 w = rule.weight(x);
+    if (bin == kBins || !w) return w;
+    const int here = rule.bin(x);
+    if (here == bin) {
+      const unsigned to = atomicAdd(&listed, 1u);
+      if (to < kSampleSliceListed) at.listed[(size_t)i * kSampleSliceListed + to] = place_of(x, v);
+    }
+    return here < bin ? w : 0;
+  };
+  const auto* body = reinterpret_cast<const typename Row<T>::vec_t*>(row.at + row.head);
+  const int tail = row.head + row.vecs * kVec;
+  if (i == 0 && wave == 0) {
+    const u64 w = wave_inclusive(lane < row.head ? kept(lane, row.value(lane)) : 0);
+    if (lane == 63) at.parts[0] = w;
+  }
+  if (i == a.slices - 1 && wave == 0) {
+    const u64 w = wave_inclusive(tail + lane < a.V ? kept(tail + lane, row.value(tail + lane)) : 0);
+    if (lane == 63) at.parts[row.parts() - 1] = w;
+  }
+  for (int q0 = sl.first + 64 * wave; q0 < sl.end; q0 += kThreads) {
+    u64 w = 0;
+    if (q0 + lane < sl.end) {
+      const auto x = body[q0 + lane];
+#pragma unroll
+      for (int e = 0; e < kVec; ++e) w += kept(row.head + (q0 + lane) * kVec + e, static_cast<float>(x[e]));
+    }
+    w = wave_inclusive(w);
+    if (lane == 63) at.parts[q0 / 64 + 1] = w;
+  }
+  __syncthreads();
+  if (tid == 0) at.row->n[i] = listed;
+}
+
+// The drawn token of a row whose kept weights are in s.parts.
+template <typename T, typename Write>
+__device__ __forceinline__ void draw_of_parts(Shared& s, const Rule& rule, const Row<T>& row, u64 lowest, float u, Write write) {
+  constexpr int kVec = Row<T>::kVec;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int parts = row.parts(), tail = row.head + row.vecs * kVec;
+  const Drawn d = draw_part(s, parts, u);
+  if (wave != 0) return;
+  const int begin = d.part == 0 ? 0 : d.part == parts - 1 ? tail : row.head + (d.part - 1) * 64 * kVec;
+  const int end = d.part == 0 ? row.head : d.part == parts - 1 ? row.V : min(begin + 64 * kVec, tail);
+  u64 sum = d.before;
+  for (int v0 = begin; v0 < end; v0 += 64) {
+    const int v = v0 + lane;
+    const float x = row.value(min(v, end - 1));
+    const u64 w = v < end && place_of(x, v) >= lowest ? rule.weight(x) : 0;
+    const u64 c = sum + wave_inclusive(w);
+    const u64 there = __ballot(c > d.target);
+    if (there) {
+      if (lane == __builtin_ctzll(there)) write(v, w, d.total);
+      return;
+    }
+    sum = __shfl(c, 63);
+  }
+}
+
+// The end of a row whose slices have been summed; false: too many tokens in the bin of the cut.
+template <typename T, typename Write>
+__device__ bool draw_of_slices(Shared& s, const SampleArgs& a, const Rule& rule, const Row<T>& row, const Space& at, float top_p,
+                               float u, Write write) {
+  const int tid = threadIdx.x, bin = at.row->bin;
+  u64 lowest = 0;
+  unsigned n = 0;
+  if (bin < kBins) {
+    bool fits = true;
+    for (int i = 0; i < a.slices; ++i) {
+      const unsigned here = at.row->n[i];
+      fits = fits && here <= kSampleSliceListed;
+      n += here;
+      if (tid < (int)here && fits && n <= kListed) s.listed[n - here + tid] = at.listed[(size_t)i * kSampleSliceListed + tid];
+    }
+    if (!fits || n > kListed) return false;
+    if (tid == 0) s.count[bin] = n, s.counted[bin] = 0, s.before[bin] = at.row->before;
+    __syncthreads();
+    const double target = top_p > 0.f ? (double)top_p * (double)at.row->total : 0.0;
+    lowest = cut_in_bin(s, rule, [&](auto f) {
+      for (int i = tid; i < (int)n; i += kThreads) f(index_of(s.listed[i]), value_of(s.listed[i]));
+    }, bin, false, 0, target);
+    __syncthreads();
+  }
+  for (int i = tid; i < row.parts(); i += kThreads) s.parts[i] = at.parts[i];
+  __syncthreads();
+  for (int i = tid; i < (int)n; i += kThreads)
+    if (s.listed[i] >= lowest) atomicAdd(&s.parts[row.part_of(index_of(s.listed[i]))], rule.weight(value_of(s.listed[i])));
+  __syncthreads();
+  draw_of_parts(s, rule, row, lowest, u, write);
+  return true;
+}
+
+// SLICED: the slices' kernels have run.
+template <typename T, bool SLICED>
 __global__ __launch_bounds__(kThreads) void sample_kernel(SampleArgs a) {
   extern __shared__ __align__(16) unsigned char shared_bytes[];
   Shared& s = *reinterpret_cast<Shared*>(shared_bytes);
@@ -481,6 +742,29 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleArgs a) {
   const int m = blockIdx.x, V = a.V;
   const Row<T> row(static_cast<const T*>(a.logits) + (size_t)m * a.logits_ld, V);
   constexpr int kVec = Row<T>::kVec;
+  auto write = [&](int v, u64 w, u64 total) {
+    a.tokens[m] = v;
+    a.logprobs[m] = (float)log((double)w / (double)total);
+  };
+  if constexpr (SLICED) {
+    const Space at = space_of(a, m);
+    const float top = row_top(a, *at.row), temperature = a.temperature ? a.temperature[m] : 1.f;
+    if (!(top > -__builtin_huge_valf())) {
+      if (tid == 0) a.tokens[m] = -1, a.logprobs[m] = __builtin_nanf("");
+      return;
+    }
+    if (!(temperature > 0.f)) {
+      int first = V;
+      for (int i = 0; i < a.slices; ++i) first = min(first, at.row->first[i]);
+      if (tid == 0) a.tokens[m] = first, a.logprobs[m] = 0.f;
+      return;
+    }
+    if (tid < kPowers) s.powers[tid] = root_power(tid);
+    __syncthreads();
+    const Rule rule = rule_of(top, temperature, 0.f, s.powers);
+    if (draw_of_slices(s, a, rule, row, at, a.top_p ? a.top_p[m] : 1.f, a.uniforms[m], write)) return;
+    __syncthreads();
+  }
 
   // The maxima of the thread's groups of values (NaN if one is), and of all.
   float maxima[kGroups];
@@ -518,10 +802,7 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleArgs a) {
   const float min_p = a.min_p ? a.min_p[m] : 0.f;
   const float top_p = a.top_p ? a.top_p[m] : 1.f;
   const bool by_k = k < V, by_p = top_p < 1.f;  // (NaN: off)
-  const float part = top > 0x1p100f ? 0.5f : 1.f;
-  const Rule rule = {top, (float)kBins * 1.44269504f / (kOctaves * part) / temperature, part, top * part,
-                     kPowers * 1.4426950408889634 / (double)temperature, min_p > 0.f ? (double)fminf(min_p, 1.f) * kUnit : 0.0,
-                     s.powers};
+  const Rule rule = rule_of(top, temperature, min_p, s.powers);
   const float u = a.uniforms[m];
 
   // Top-p alone: the sum is one of all weights, and the cut mostly among the first few thousand.
@@ -577,10 +858,6 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleArgs a) {
              (!sums || s.total_listed == all || (double)s.total_listed >= (double)top_p * (double)all);
   }
   const int n = (int)s.listed_n;
-  auto write = [&](int v, u64 w, u64 total) {
-    a.tokens[m] = v;
-    a.logprobs[m] = (float)log((double)w / (double)total);
-  };
   if (listed && n <= kFew) {
     few_tokens(s, rule, n, (unsigned)k, by_p, top_p, all, u, write);
     return;
@@ -622,10 +899,9 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleArgs a) {
     }
     return;
   }
-  // Kept weights by 64 accesses of the row (a wave's), in index order: the values in front
-  // of the first access, the accesses, the values behind the last.
+  // Kept weights by the row's parts.
   auto kept = [&](int v, float x) -> u64 { return place_of(x, v) >= lowest ? rule.weight(x) : 0; };
-  const int parts = (row.vecs + 63) / 64 + 2, tail = row.head + row.vecs * kVec;
+  const int parts = row.parts(), tail = row.head + row.vecs * kVec;
   if (tid == 0) s.parts[0] = 0, s.parts[parts - 1] = 0;
   __syncthreads();
   if (tid < row.head) atomicAdd(&s.parts[0], kept(tid, row.value(tid)));
@@ -642,27 +918,20 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleArgs a) {
     if (lane == 63) s.parts[p + 1] = w;
   }
   __syncthreads();
-  const Drawn d = draw_part(s, parts, u);
-  if (wave != 0) return;
-  const int begin = d.part == 0 ? 0 : d.part == parts - 1 ? tail : row.head + (d.part - 1) * 64 * kVec;
-  const int end = d.part == 0 ? row.head : d.part == parts - 1 ? V : min(begin + 64 * kVec, tail);
-  u64 sum = d.before;
-  for (int v0 = begin; v0 < end; v0 += 64) {
-    const int v = v0 + lane;
-    const u64 w = v < end ? kept(v, row.value(v)) : 0;
-    const u64 c = sum + wave_inclusive(w);
-    const u64 there = __ballot(c > d.target);
-    if (there) {
-      if (lane == __builtin_ctzll(there)) write(v, w, d.total);
-      return;
-    }
-    sum = __shfl(c, 63);
-  }
+  draw_of_parts(s, rule, row, lowest, u, write);
 }
 
 template <typename T>
 hipError_t launch(const SampleArgs& a, hipStream_t stream) {
-  launch_kernel(sample_kernel<T>, dim3((unsigned)a.M), dim3(kThreads), sizeof(Shared), stream, a);
+  if (a.slices > 1) {
+    const dim3 grid((unsigned)a.M * (unsigned)a.slices), threads(kThreads);
+    launch_kernel(slice_top_kernel<T>, grid, threads, 0, stream, a);
+    if (a.top_p) launch_kernel(slice_bins_kernel<T>, grid, threads, 0, stream, a);
+    launch_kernel(slice_parts_kernel<T>, grid, threads, 0, stream, a);
+    launch_kernel(sample_kernel<T, true>, dim3((unsigned)a.M), threads, sizeof(Shared), stream, a);
+  } else {
+    launch_kernel(sample_kernel<T, false>, dim3((unsigned)a.M), dim3(kThreads), sizeof(Shared), stream, a);
+  }
   return hipGetLastError();
 }
 

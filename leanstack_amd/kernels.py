@@ -1117,7 +1117,8 @@ def sample_logits(logits: torch.Tensor, uniforms: torch.Tensor, *, temperature: 
     arguments.  A row with a NaN, or of -inf alone, gives token -1 and NaN.
 
     uniforms, temperature, top_p, min_p: float32 [M], top_k: int32 [M], read on the
-    device, so a captured call follows them.  V at most 2^19."""
+    device, so a captured call follows them.  A filter that no row uses is better left out:
+    what is given decides how the rows are worked on.  V at most 2^19."""
     dtype = logits.dtype
     if dtype is torch.float32:
         mode = _lib.LOGITS_FP32
@@ -1146,12 +1147,19 @@ def sample_logits(logits: torch.Tensor, uniforms: torch.Tensor, *, temperature: 
     logprobs = logits.new_empty((m,), dtype=torch.float32)
     if m == 0:
         return tokens, logprobs
+    nbytes = _sample_workspace_bytes(mode, m, v, k_at is not None, p_at is not None, min_p_at is not None)
+    workspace = logits.new_empty((nbytes,), dtype=torch.uint8) if nbytes else None
     with _on_index(index):
         status = _lib.load().lsk_sample_logits(
             logits.data_ptr(), mode, m, v, ld, uniforms_at, temperature_at, k_at, p_at, min_p_at, tokens.data_ptr(),
-            logprobs.data_ptr(), torch._C._cuda_getCurrentRawStream(index))
+            logprobs.data_ptr(), _ptr(workspace), nbytes, torch._C._cuda_getCurrentRawStream(index))
     _lib.check(status, "lsk_sample_logits")
     return tokens, logprobs
+
+
+@functools.lru_cache(maxsize=1024)
+def _sample_workspace_bytes(mode: int, m: int, v: int, by_k: bool, by_p: bool, by_min_p: bool) -> int:
+    return _lib.load().lsk_sample_workspace_bytes(mode, m, v, by_k, by_p, by_min_p)
 
 
 def _ptr(t: torch.Tensor | None) -> int | None:

@@ -248,3 +248,82 @@ def test_streams(gpu):
     torch.cuda.synchronize()
     for i in range(4):
         assert all(torch.equal(a, want[i][0]) and torch.equal(b, want[i][1]) for a, b in got[i])
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("m,v", [(1, 16384), (1, 16390), (2, 24577), (7, 151936), (1, 1 << 19), (1, (1 << 19) - 3), (128, 40003), (256, 16387),
+                                 (257, 16387)])
+def test_few_rows_without_ranks(gpu, m, v, dtype):
+    """Temperature and top-p alone, rows that several workgroups share: every row with its own options, greedy
+    ones and ones that top-p leaves alone among them."""
+    rng = np.random.default_rng(v)
+    logits = logits_of(m, v, seed=v, dtype=dtype)
+    temperature = rng.choice([0.0, 0.4, 1.0, 1.7], m).tolist()
+    run(gpu, logits, uniforms_of(m, seed=1), temperature=temperature)
+    run(gpu, logits, uniforms_of(m, seed=2))
+    run(gpu, logits, uniforms_of(m, seed=3), temperature=temperature, top_p=rng.choice([0.0, 0.3, 0.9, 0.999, 1.0, math.nan], m).tolist())
+    run(gpu, logits, [0.0, 1.0][: min(m, 2)] + uniforms_of(m, seed=4)[2:], top_p=[0.95] * m)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_where_the_cut_falls_in_sliced_rows(gpu, dtype):
+    """Cuts among equal values all over the row (more than are listed, and fewer), in the first and in the last
+    slice, rows of one value and rows at odd addresses."""
+    v = 65536 + 24
+    base = torch.full((6, v + 5), -20.0)
+    base[0] = 1.0                              # all equal: no list holds them
+    base[1, ::40] = 2.0                        # 1600 equal ones
+    base[2, ::9] = 2.0                         # 7000
+    base[3, :300] = torch.arange(300) / 100    # in the first slice
+    base[4, -300:] = torch.arange(300) / 100   # in the last one
+    base[5, ::3] = torch.randn((len(base[5, ::3]),), generator=torch.Generator().manual_seed(5)) * 0.02
+    wide = base.to(dtype).to(gpu)
+    for at in (0, 1, 3, 5):
+        logits = wide[:, at:at + v]
+        for i, top_p in enumerate((0.01, 0.5, 0.97, 0.99999)):
+            u = uniforms_of(6, seed=50 + i)
+            tokens, logs = kernels.sample_logits(logits, torch.tensor(u, device=gpu), top_p=torch.full((6,), top_p, device=gpu))
+            rows = logits.double().cpu().numpy()
+            for r in range(6):
+                token, log = reference(rows[r], float(torch.tensor(u)[r]), top_p=float(torch.tensor(top_p)))
+                assert int(tokens[r]) == token, f"row {r} at {at}, top_p {top_p}"
+                assert abs(float(logs[r]) - log) <= 2.0 ** -23 * abs(log) + 2.0 ** -40 * math.exp(-log)
+
+
+@pytest.mark.parametrize("at", [0, 9000, 20000, 32767])
+def test_nan_and_infinities_in_sliced_rows(gpu, at):
+    """A NaN in any slice, a row of -inf, one value that is not, values of +inf in several slices."""
+    v = 32768
+    logits = logits_of(5, v, seed=60)
+    logits[0, at] = math.nan
+    logits[1] = -math.inf
+    logits[2] = -math.inf
+    logits[2, at] = -3e38
+    logits[3, at] = logits[3, 77] = logits[3, 30000] = math.inf
+    for options in ({}, dict(top_p=[0.7] * 5), dict(top_p=[0.2] * 5, temperature=[0.0, 0.0, 1.0, 1.0, 0.0])):
+        run(gpu, logits, uniforms_of(5, seed=61), **options)
+
+
+def test_captured_sliced_rows_follow_their_arguments(gpu):
+    """Replays with other logits and options, eager calls in between."""
+    m, v = 4, 50000
+    logits, u = torch.zeros((m, v), device=gpu), torch.zeros(m, device=gpu)
+    temperature, top_p = torch.ones(m, device=gpu), torch.ones(m, device=gpu)
+    stream = torch.cuda.Stream()
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=stream):
+        tokens, logs = kernels.sample_logits(logits, u, temperature=temperature, top_p=top_p)
+        alone, alone_logs = kernels.sample_logits(logits, u, temperature=temperature)
+    rng = np.random.default_rng(70)
+    for i in range(5):
+        fresh = logits_of(m, v, seed=70 + i)
+        options = dict(temperature=rng.choice([0.0, 0.6, 1.2], m).tolist(), top_p=rng.choice([0.2, 0.9, 1.0], m).tolist())
+        given = uniforms_of(m, seed=80 + i)
+        logits.copy_(fresh), u.copy_(torch.tensor(given))
+        temperature.copy_(torch.tensor(options["temperature"])), top_p.copy_(torch.tensor(options["top_p"]))
+        graph.replay()
+        want = run(gpu, fresh, given, **options)
+        assert torch.equal(tokens.cpu(), want[0]) and torch.equal(logs.cpu(), want[1])
+        want = run(gpu, fresh, given, temperature=options["temperature"])
+        assert torch.equal(alone.cpu(), want[0]) and torch.equal(alone_logs.cpu(), want[1])

@@ -8,7 +8,7 @@ import torch
 from leanstack_amd import _lib, kernels
 
 FAKE = 0x10000  # aligned, never dereferenced
-INVALID = -1
+INVALID, WORKSPACE = -1, -4
 
 
 @pytest.mark.parametrize("bad,code", [
@@ -17,12 +17,16 @@ INVALID = -1
     (dict(x=FAKE + 1, mode=1), INVALID), (dict(u=None), INVALID), (dict(u=FAKE + 2), INVALID), (dict(t=FAKE + 2), INVALID),
     (dict(k=FAKE + 1), INVALID), (dict(p=FAKE + 2), INVALID), (dict(mp=FAKE + 2), INVALID), (dict(tokens=None), INVALID),
     (dict(tokens=FAKE + 4), INVALID), (dict(logs=None), INVALID), (dict(logs=FAKE + 2), INVALID),
+    (dict(v=50000, ld=50000, ws=None), WORKSPACE), (dict(v=50000, ld=50000, ws=FAKE + 8), WORKSPACE),
+    (dict(v=50000, ld=50000, ws_bytes=100), WORKSPACE), (dict(v=50000, ld=50000, p=FAKE, ws_bytes=60000), WORKSPACE),
+    (dict(v=1 << 19, ld=1 << 19, m=256, p=FAKE, ws_bytes=0), WORKSPACE),
 ])
 def test_entry_point_rejects_before_launch(bad, code):
     lib = _lib.load()
-    a = dict(x=FAKE, mode=0, m=3, v=1000, ld=1000, u=FAKE, t=None, k=None, p=None, mp=None, tokens=FAKE, logs=FAKE) | bad
+    a = dict(x=FAKE, mode=0, m=3, v=1000, ld=1000, u=FAKE, t=None, k=None, p=None, mp=None, tokens=FAKE, logs=FAKE, ws=FAKE,
+             ws_bytes=1 << 30) | bad
     status = lib.lsk_sample_logits(a["x"], a["mode"], a["m"], a["v"], a["ld"], a["u"], a["t"], a["k"], a["p"], a["mp"],
-                                   a["tokens"], a["logs"], None)
+                                   a["tokens"], a["logs"], a["ws"], a["ws_bytes"], None)
     assert status == code
     assert lib.lsk_last_error()
 
@@ -37,3 +41,16 @@ def test_wrapper_refuses():
                  lambda: kernels.sample_logits(x, u, min_p=u[:, None]), lambda: kernels.sample_logits(x, u)):
         with pytest.raises(ValueError):
             call()
+
+
+@pytest.mark.parametrize("m,v,filters,some", [
+    (1, 151936, (0, 0, 0), True), (1, 151936, (0, 1, 0), True), (256, 16384, (0, 1, 0), True), (1, 1 << 19, (0, 1, 0), True),
+    (1, 151936, (1, 1, 0), False), (1, 151936, (0, 1, 1), False), (257, 151936, (0, 1, 0), False), (1, 16383, (0, 1, 0), False),
+    (0, 151936, (0, 1, 0), False), (1, (1 << 19) + 1, (0, 0, 0), False),
+])
+def test_workspace_bytes(m, v, filters, some):
+    """Only rows that are cut need one: 16 bytes of sums for 512 values, and with top-p 20 KB a slice."""
+    need = [_lib.load().lsk_sample_workspace_bytes(mode, m, v, *filters) for mode in (0, 1)]
+    assert need[0] == need[1] and (need[0] > 0) == some
+    assert need[0] <= m * (512 + v // 256 * 8 + (16 * 20480 if filters[1] else 0))
+    assert _lib.load().lsk_sample_workspace_bytes(2, m, v, *filters) == 0
