@@ -30,12 +30,14 @@ namespace lsk {
 namespace {
 
 typedef unsigned long long u64;
+typedef u64 u64x2_t __attribute__((ext_vector_type(2)));
 
 constexpr int kThreads = 1024;
 constexpr int kWaves = kThreads / 64;
 constexpr int kBins = kSampleBins;
 static_assert(kBins == 2 * kThreads, "two to a thread");
 constexpr int kRanked = 1024;               // places ranked against each other
+constexpr int kRankedListed = 64;           // .. of a list, which is quickly binned again
 constexpr int kListed = 4096;               // tokens that may be kept
 constexpr int kFew = 256;                   // of them, compared each with each
 constexpr int kGroups = 4;                  // of values per thread, whose maxima bound the k-th
@@ -274,28 +276,33 @@ __device__ __forceinline__ int bin_of_kth(Shared& s, unsigned k) {
 
 // The lowest kept place of the bin in which a cut lies: the first `want` by count, or those with
 // less than `target` in front of them.  each(f): f(v, x) for all tokens, the bins filled and
-// scanned.  Returns the place; s.kept: the weight up to it.
+// scanned.  More than `most` places are binned again.  Returns the place; s.kept: the weight up to it.
 template <typename Each>
-__device__ u64 cut_in_bin(Shared& s, const Rule& rule, Each each, int bin, bool by_count, unsigned want, double target) {
+__device__ u64 cut_in_bin(Shared& s, const Rule& rule, Each each, int bin, bool by_count, unsigned want, double target, unsigned most) {
   const int tid = threadIdx.x;
   unsigned n = s.count[bin], base_c = s.counted[bin];
   u64 lo = 0, hi = ~0ull, base_w = s.before[bin];
-  if (n > kRanked) {
+  if (n > most) {
     if (tid == 0) s.lo = ~0ull, s.hi = 0;
     __syncthreads();
-    u64 least = ~0ull, most = 0;
+    u64 least = ~0ull, top = 0;
     each([&](int v, float x) {
       if (rule.bin(x) == bin && rule.weight(x)) {
         const u64 p = place_of(x, v);
-        least = p < least ? p : least, most = p > most ? p : most;
+        least = p < least ? p : least, top = p > top ? p : top;
       }
     });
-    if (most) atomicMin(&s.lo, least), atomicMax(&s.hi, most);
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const u64 l = __shfl_xor(least, d), h = __shfl_xor(top, d);
+      least = l < least ? l : least, top = h > top ? h : top;
+    }
+    if ((tid & 63) == 0 && top) atomicMin(&s.lo, least), atomicMax(&s.hi, top);
     __syncthreads();
     lo = s.lo, hi = s.hi;
   }
   __syncthreads();
-  while (n > kRanked) {
+  while (n > most) {
     const int bits = 64 - __clzll((long long)(hi - lo));
     const int shift = bits > 11 ? bits - 11 : 0;
     for (int i = tid; i < kBins; i += kThreads) s.sub.count[i] = 0, s.sub.weight[i] = 0;
@@ -321,7 +328,8 @@ __device__ u64 cut_in_bin(Shared& s, const Rule& rule, Each each, int bin, bool 
     __syncthreads();
     u64 c = 0, w = 0;
     for (int i = tid; i < at; i += kThreads) c += s.sub.count[i], w += s.sub.weight[i];
-    if (c) atomicAdd(&s.lo, c), atomicAdd(&s.hi, w);
+    c = wave_inclusive(c), w = wave_inclusive(w);
+    if ((tid & 63) == 63 && c) atomicAdd(&s.lo, c), atomicAdd(&s.hi, w);
     __syncthreads();
     base_c += (unsigned)s.lo, base_w += s.hi;
     n = s.sub.count[at];
@@ -361,7 +369,8 @@ __device__ u64 cut_in_bin(Shared& s, const Rule& rule, Each each, int bin, bool 
 // The lowest kept place under top-k (k below the number of tokens) and top-p (below 1).
 // total: of all tokens' weights, where each() leaves some out (else 0).
 template <typename Each>
-__device__ u64 lowest_kept(Shared& s, const Rule& rule, Each each, bool by_k, unsigned k, bool by_p, float top_p, u64 total) {
+__device__ u64 lowest_kept(Shared& s, const Rule& rule, Each each, bool by_k, unsigned k, bool by_p, float top_p, u64 total,
+                           unsigned most) {
   const int tid = threadIdx.x;
   __syncthreads();
   for (int i = tid; i < kBins; i += kThreads) s.count[i] = 0, s.weight[i] = 0;
@@ -378,7 +387,7 @@ __device__ u64 lowest_kept(Shared& s, const Rule& rule, Each each, bool by_k, un
   u64 sum = total ? total : s.before[kBins - 1] + s.weight[kBins - 1], lowest = 0;
   const int bin = s.found;
   if (by_k && bin < kBins) {  // (fewer than k have weight: no cut)
-    lowest = cut_in_bin(s, rule, each, bin, true, k, 0.0);
+    lowest = cut_in_bin(s, rule, each, bin, true, k, 0.0, most);
     sum = s.kept;
   }
   if (by_p) {
@@ -387,7 +396,7 @@ __device__ u64 lowest_kept(Shared& s, const Rule& rule, Each each, bool by_k, un
     scan_bins(s, s.count, s.weight, s.counted, s.before, [&](unsigned, u64 w) { return (double)w >= target; });
     const int at = s.found;
     if (at < kBins) {
-      const u64 p = cut_in_bin(s, rule, each, at, false, 0, target);
+      const u64 p = cut_in_bin(s, rule, each, at, false, 0, target, most);
       lowest = p > lowest ? p : lowest;
     }
   }
@@ -535,10 +544,11 @@ __device__ __forceinline__ Range slice_of(const SampleArgs& a, const Row<T>& row
   const int first = min(i * each, row.vecs);
   return {first, min(first + each, row.vecs), i == 0, i == a.slices - 1};
 }
-// The row's maximum (NaN if there is one), by all threads.
+// The row's maximum (NaN if there is one), in all threads.
 __device__ __forceinline__ float row_top(const SampleArgs& a, const RowSums& r) {
-  float top = r.max[0];
-  for (int i = 1; i < a.slices; ++i) top = __builtin_elementwise_maximum(top, r.max[i]);
+  float top = r.max[min((int)(threadIdx.x & (kSampleMaxSlices - 1)), a.slices - 1)];
+#pragma unroll
+  for (int d = 1; d < kSampleMaxSlices; d <<= 1) top = __builtin_elementwise_maximum(top, __shfl_xor(top, d));
   return top;
 }
 
@@ -618,9 +628,15 @@ __global__ __launch_bounds__(kThreads) void slice_parts_kernel(SampleArgs a) {
   int bin = kBins;
   if (top_p < 1.f) {
     u64 w0 = 0, w1 = 0;
-    for (int s = 0; s < a.slices; ++s) {
-      const u64* bins = at.bins + (size_t)s * kBins + 2 * tid;
-      w0 += bins[0], w1 += bins[1];
+    const auto* bins = reinterpret_cast<const u64x2_t*>(at.bins) + tid;
+    constexpr int kHeld = 8;  // (16 of them cost the second workgroup of a CU)
+    for (int s0 = 0; s0 < a.slices; s0 += kHeld) {
+      u64x2_t held[kHeld];
+#pragma unroll
+      for (int s = 0; s < kHeld; ++s) held[s] = bins[min(s0 + s, a.slices - 1) * (kBins / 2)];
+#pragma unroll
+      for (int s = 0; s < kHeld; ++s)
+        if (s0 + s < a.slices) w0 += held[s][0], w1 += held[s][1];
     }
     const u64 up_to = wave_inclusive(w0 + w1);
     if (lane == 63) wave_weight[wave] = up_to;
@@ -708,20 +724,21 @@ __device__ bool draw_of_slices(Shared& s, const SampleArgs& a, const Rule& rule,
   u64 lowest = 0;
   unsigned n = 0;
   if (bin < kBins) {
-    bool fits = true;
-    for (int i = 0; i < a.slices; ++i) {
-      const unsigned here = at.row->n[i];
-      fits = fits && here <= kSampleSliceListed;
-      n += here;
-      if (tid < (int)here && fits && n <= kListed) s.listed[n - here + tid] = at.listed[(size_t)i * kSampleSliceListed + tid];
-    }
-    if (!fits || n > kListed) return false;
+    // A wave per slice: the lists one behind the other.
+    static_assert(kWaves == kSampleMaxSlices, "a wave per slice");
+    const int lane = tid & 63, slice = tid >> 6;
+    const unsigned here = lane < a.slices ? at.row->n[lane] : 0, up_to = wave_inclusive(here);
+    n = (unsigned)__builtin_amdgcn_readlane((int)up_to, 63);
+    if (__ballot(here > kSampleSliceListed) || n > kListed) return false;
+    const unsigned mine = (unsigned)__builtin_amdgcn_readlane((int)here, slice);
+    const unsigned from = (unsigned)__builtin_amdgcn_readlane((int)up_to, slice) - mine;
+    for (unsigned i = lane; i < mine; i += 64) s.listed[from + i] = at.listed[(size_t)slice * kSampleSliceListed + i];
     if (tid == 0) s.count[bin] = n, s.counted[bin] = 0, s.before[bin] = at.row->before;
     __syncthreads();
     const double target = top_p > 0.f ? (double)top_p * (double)at.row->total : 0.0;
     lowest = cut_in_bin(s, rule, [&](auto f) {
       for (int i = tid; i < (int)n; i += kThreads) f(index_of(s.listed[i]), value_of(s.listed[i]));
-    }, bin, false, 0, target);
+    }, bin, false, 0, target, kRankedListed);
     __syncthreads();
   }
   for (int i = tid; i < row.parts(); i += kThreads) s.parts[i] = at.parts[i];
@@ -754,8 +771,9 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleArgs a) {
       return;
     }
     if (!(temperature > 0.f)) {
-      int first = V;
-      for (int i = 0; i < a.slices; ++i) first = min(first, at.row->first[i]);
+      int first = at.row->first[min(lane & (kSampleMaxSlices - 1), a.slices - 1)];
+#pragma unroll
+      for (int d = 1; d < kSampleMaxSlices; d <<= 1) first = min(first, __shfl_xor(first, d));
       if (tid == 0) a.tokens[m] = first, a.logprobs[m] = 0.f;
       return;
     }
@@ -785,12 +803,12 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleArgs a) {
   __syncthreads();
 #pragma unroll
   for (int i = 0; i < kWaves; ++i) top = __builtin_elementwise_maximum(top, s.wave_max[i]);
-  if (!(top > -__builtin_huge_valf())) {  // NaN, or -inf alone: no distribution
+  if (__builtin_expect(!(top > -__builtin_huge_valf()), 0)) {  // NaN, or -inf alone: no distribution
     if (tid == 0) a.tokens[m] = -1, a.logprobs[m] = __builtin_nanf("");
     return;
   }
   const float temperature = a.temperature ? a.temperature[m] : 1.f;
-  if (!(temperature > 0.f)) {  // greedy
+  if (__builtin_expect(!(temperature > 0.f), 0)) {  // greedy
     int first = V;
     row.each([&](int v, float x) { first = x == top ? min(first, v) : first; });
     if (first < V) atomicMin(&s.found, first);
@@ -858,7 +876,7 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleArgs a) {
              (!sums || s.total_listed == all || (double)s.total_listed >= (double)top_p * (double)all);
   }
   const int n = (int)s.listed_n;
-  if (listed && n <= kFew) {
+  if (__builtin_expect(listed && n <= kFew, 1)) {
     few_tokens(s, rule, n, (unsigned)k, by_p, top_p, all, u, write);
     return;
   }
@@ -868,8 +886,8 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleArgs a) {
   auto each_of_row = [&](auto f) { row.each(f); };
   u64 lowest = 0;
   if (by_k || by_p)
-    lowest = listed ? lowest_kept(s, rule, each_listed, by_k, (unsigned)k, by_p, top_p, all)
-                    : lowest_kept(s, rule, each_of_row, by_k, (unsigned)k, by_p, top_p, 0);
+    lowest = listed ? lowest_kept(s, rule, each_listed, by_k, (unsigned)k, by_p, top_p, all, kRankedListed)
+                    : lowest_kept(s, rule, each_of_row, by_k, (unsigned)k, by_p, top_p, 0, kRanked);
 
   __syncthreads();
   if (listed) {
