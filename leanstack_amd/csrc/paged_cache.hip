@@ -125,10 +125,10 @@ __global__ __launch_bounds__(kThreads) void append_kernel(PagedAppendArgs a) {
 #pragma unroll
       for (int i = 0; i < 2; ++i) x[h][i] = *reinterpret_cast<const u32x4_t*>(src + 64 * h + 16 * g + 8 * i);
   }
-  // What the block holds: rows in front of the new ones, and for V, whose words hold
-  // four rows, what stands behind them.
+  // What the block holds, of V, whose words hold four rows, next to the new ones.
+  const int new_of_four = min(end, row0 + 4 * g + 4) - max(first, row0 + 4 * g);
   u32x4_t old[2] = {};
-  if (begun > 0 || (kv && end < row0 + 16)) {
+  if (kv && new_of_four > 0 && new_of_four < 4) {
 #pragma unroll
     for (int h = 0; h < 2; ++h) old[h] = *reinterpret_cast<const u32x4_t*>(out + h * 1024 + lane * 16);
   }
@@ -148,6 +148,10 @@ __global__ __launch_bounds__(kThreads) void append_kernel(PagedAppendArgs a) {
   const float factor = power_of_two(-e);
   const bool move = begun > 0 && e != was;
   const float less = power_of_two(was - e);
+  if (move) {  // (seldom: then all in front of the new rows is rounded again)
+#pragma unroll
+    for (int h = 0; h < 2; ++h) old[h] = *reinterpret_cast<const u32x4_t*>(out + h * 1024 + lane * 16);
+  }
 
   u32x4_t q[2];
 #pragma unroll
@@ -192,7 +196,7 @@ __global__ __launch_bounds__(kThreads) void append_kernel(PagedAppendArgs a) {
         if (move) before = (again(before, less) & is_old) | (before & ~is_old);
         o[i] = (t & is_new) | (before & ~is_new);
       }
-      *reinterpret_cast<u32x4_t*>(out + h * 1024 + lane * 16) = o;
+      if (new_of_four > 0 || move) *reinterpret_cast<u32x4_t*>(out + h * 1024 + lane * 16) = o;
     }
   }
   if (lane == 0) *exponent = (unsigned char)(e + 127);
@@ -219,8 +223,12 @@ __global__ __launch_bounds__(kThreads) void read_kernel(PagedReadArgs a) {
   if (row0 < len && row0 / 16 < p.blocks) at = block_in_pool(p, b, j, (int)(row0 / 16));
   if (at >= 0) {
     const unsigned char* from = (kv ? p.v : p.k) + at * kPagedBlockBytes;
+    // the lane's row of K, four rows of V: if one is wanted
+    const long long low = row0 + (kv ? 4 * g : c), high = low + (kv ? 4 : 1);
+    if (high > start && low < (long long)start + a.rows && low < len) {
 #pragma unroll
-    for (int h = 0; h < 2; ++h) q[h] = *reinterpret_cast<const u32x4_t*>(from + h * 1024 + lane * 16);
+      for (int h = 0; h < 2; ++h) q[h] = *reinterpret_cast<const u32x4_t*>(from + h * 1024 + lane * 16);
+    }
     scale = power_of_two((int)(kv ? p.v_exp : p.k_exp)[at] - 127);
     if (kv) {
       auto* bytes = reinterpret_cast<unsigned char*>(&rows[wave][0][0]);
