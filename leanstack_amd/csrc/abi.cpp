@@ -460,7 +460,8 @@ extern "C" {
 
 size_t lsk_sample_workspace_bytes(int logits_mode, int M, int V, int by_top_k, int by_top_p, int by_min_p) {
   if (lsk::check_sample_sizes(logits_mode, M, V) != LSK_OK) return 0;
-  return (size_t)M * lsk::sample_row_bytes(lsk::sample_slices(M, V, by_top_k || by_min_p), V, by_top_p);
+  const bool ranked = by_top_k || by_min_p;
+  return (size_t)M * lsk::sample_row_bytes(lsk::sample_slices(M, V, logits_mode == LSK_LOGITS_BF16 ? 2 : 4, ranked), V, by_top_p, ranked);
 }
 
 int lsk_sample_logits(const void* logits, int logits_mode, int M, int V, long long logits_ld, const float* uniforms,
@@ -482,10 +483,11 @@ int lsk_sample_logits(const void* logits, int logits_mode, int M, int V, long lo
   a.logits_ld = (size_t)logits_ld;
   a.M = M;
   a.V = V;
-  a.slices = lsk::sample_slices(M, V, top_k != nullptr || min_p != nullptr);
+  const bool ranked = top_k != nullptr || min_p != nullptr;
+  a.slices = lsk::sample_slices(M, V, logits_mode == LSK_LOGITS_BF16 ? 2 : 4, ranked);
   a.max_parts = lsk::sample_max_parts(V);
   a.workspace = static_cast<unsigned char*>(workspace);
-  a.row_bytes = (size_t)lsk::sample_row_bytes(a.slices, V, top_p != nullptr);
+  a.row_bytes = (size_t)lsk::sample_row_bytes(a.slices, V, top_p != nullptr, ranked);
   const size_t need = (size_t)M * a.row_bytes;
   if (need > 0 && (workspace == nullptr || ws_bytes < need || !aligned(workspace, 16)))
     return fail(LSK_ERR_WORKSPACE, "these logits need a workspace of %zu bytes, 16-byte aligned (got %zu)", need,

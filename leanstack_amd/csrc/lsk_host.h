@@ -260,19 +260,25 @@ constexpr int constrain_slices(int M, int V) {
 // Sampled tokens (sample.hip): a row's weights, whole numbers up to 2^44, add up in 63 bits.
 constexpr int kSampleMaxVocab = 1 << 19;
 
-// Rows without top-k and min-p are cut into slices while the chip has room for all, of at least
-// kSampleLeastSlice values.
-constexpr int kSampleMaxSlices = 16, kSampleLeastSlice = 8192, kSamplePlaces = 512;
-constexpr int kSampleBins = 2048, kSampleSliceListed = 512, kSampleRowBytes = 256;
-constexpr int sample_slices(int M, int V, bool ranked) {
+// Rows are cut into slices while the chip has room for all, of at least kSampleLeastSlice values.
+// Without top-k and min-p that is always faster (16384 values and 256 rows among them).  With one
+// of them (`ranked`) a second launch costs more than the sweeps of a row that is not
+// kSampleRankedBytes long, or that only two workgroups would share: 16 rows of 151936 fp32 values
+// 17 us for 28, of bf16 16 for 22; of 50257 fp32 values 16 either way, of 32000 15 for 13; 256
+// rows of 151936 64..89 for 68..85.
+constexpr int kSampleMaxSlices = 16, kSampleLeastSlice = 8192, kSamplePlaces = 512, kSampleRankedBytes = 1 << 18;
+constexpr int kSampleBins = 2048, kSampleSliceListed = 512, kSampleRankListed = 2048, kSampleRowBytes = 256;
+constexpr int sample_slices(int M, int V, int value_bytes, bool ranked) {
   const int room = kSamplePlaces / M, most = V / kSampleLeastSlice;
   const int slices = room < most ? room : most;
-  return ranked || slices < 2 ? 1 : slices < kSampleMaxSlices ? slices : kSampleMaxSlices;
+  if (ranked && (V < kSampleRankedBytes / value_bytes || slices < 3)) return 1;
+  return slices < 2 ? 1 : slices < kSampleMaxSlices ? slices : kSampleMaxSlices;
 }
 // (parts of 64 accesses of 16 bytes)
 constexpr int sample_max_parts(int V) { return V / 256 + 3; }
-constexpr unsigned long long sample_row_bytes(int slices, int V, bool by_p) {
-  const unsigned long long words = sample_max_parts(V) + (by_p ? slices * (unsigned long long)(kSampleSliceListed + kSampleBins) : 0);
+constexpr unsigned long long sample_row_bytes(int slices, int V, bool by_p, bool ranked) {
+  const unsigned long long each = ranked ? kSampleRankListed : by_p ? kSampleSliceListed + kSampleBins : 0;
+  const unsigned long long words = slices * each + (ranked ? 0 : sample_max_parts(V));
   return slices < 2 ? 0 : (kSampleRowBytes + words * 8 + 255) / 256 * 256;
 }
 int check_sample_sizes(int logits_mode, int M, int V);

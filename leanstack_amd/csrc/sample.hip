@@ -19,8 +19,8 @@
 // row do: the first takes the maximum of each of 4096 groups of values, of which the k-th
 // largest is a bound below which none of the first k lies; the second lists what is above
 // it.  All else works on the list, in LDS.  Without either (top-p or the temperature alone)
-// every weight counts, and a workgroup is bound by the arithmetic of the weights: few rows
-// are cut into slices, a workgroup each, which leave sums for the row's own.
+// every weight counts, and a workgroup is bound by the arithmetic of the weights.  Few rows
+// are cut into slices, a workgroup each, which leave lists or sums for the row's own.
 
 #include <hip/hip_runtime.h>
 
@@ -112,10 +112,14 @@ __device__ __forceinline__ V wave_inclusive(V v) {
   return v;
 }
 
-struct Shared {
+struct Counts {
+  unsigned count[kBins], wave_count[kWaves];
+  int found;
+};
+struct Shared : Counts {
   double powers[kPowers];
   u64 weight[kBins], before[kBins];  // of the bins; and of those in front
-  unsigned count[kBins], counted[kBins];
+  unsigned counted[kBins];
   union {
     struct {
       u64 weight[kBins];
@@ -126,11 +130,9 @@ struct Shared {
   u64 ranked[kRanked], ranked_weight[kRanked];
   u64 listed[kListed];
   u64 wave_weight[kWaves];
-  unsigned wave_count[kWaves];
   float wave_max[kWaves];
   u64 lo, hi, kept, total, total_listed;
   unsigned n, listed_n;
-  int found;
 };
 
 // Accesses [first, end) of a row, and the values in front of the first and behind the last.
@@ -195,6 +197,24 @@ struct Row {
   }
 };
 
+// The maxima of the thread's groups of values (NaN if one is), and the wave's.
+template <typename T>
+__device__ __forceinline__ float group_maxima(const Row<T>& row, const Range& r, float (&maxima)[kGroups]) {
+  constexpr int kVec = Row<T>::kVec;
+#pragma unroll
+  for (int g = 0; g < kGroups; ++g) maxima[g] = -__builtin_huge_valf();
+  row.template sweep<kAhead>(r, [&](int, const float (&x)[kVec]) {
+#pragma unroll
+    for (int e = 0; e < kVec; ++e) maxima[e % kGroups] = __builtin_elementwise_maximum(maxima[e % kGroups], x[e]);
+  }, [&](int, float x) { maxima[0] = __builtin_elementwise_maximum(maxima[0], x); });
+  float top = maxima[0];
+#pragma unroll
+  for (int g = 1; g < kGroups; ++g) top = __builtin_elementwise_maximum(top, maxima[g]);
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) top = __builtin_elementwise_maximum(top, __shfl_xor(top, d));
+  return top;
+}
+
 // How a row's values weigh, and the bins that they fall into.
 struct Rule {
   float top, per_bin;
@@ -256,7 +276,7 @@ __device__ void scan_bins(Shared& s, const unsigned* count, const u64* weight, u
 }
 
 // The first bin at which the count reaches k (kBins: none).
-__device__ __forceinline__ int bin_of_kth(Shared& s, unsigned k) {
+__device__ __forceinline__ int bin_of_kth(Counts& s, unsigned k) {
   const int tid = threadIdx.x, wave = tid >> 6;
   const unsigned c0 = s.count[2 * tid], c1 = s.count[2 * tid + 1];
   const unsigned up_to = wave_inclusive(c0 + c1);
@@ -508,12 +528,32 @@ __device__ __forceinline__ void few_tokens(Shared& s, const Rule& rule, int n, u
   if (in_front <= at && at < in_front + w) write(index_of(mine), w, total);
 }
 
-// ------------------------------------------------------------------ few rows, all weights
+// Tokens that top-k and min-p may keep are in the first `last` bins or none: where min-p's lowest
+// is (two bins for what the logarithm is off), and where weights vanish.
+__device__ __forceinline__ int last_bin(float min_p) {
+  if (!(min_p > 0.f)) return kLastBin;
+  return (int)fminf((float)kLastBin, 2.f - __log2f(fminf(min_p, 1.f)) * ((float)kBins / kOctaves));
+}
 
-// What a row's slices leave for each other: their maxima; the bin in which top-p cuts (kBins: no
-// cut) and the weight in front of it; and of each slice the first index of the maximum (for
-// rows without a temperature) and how many tokens of that bin it has (more than
-// kSampleSliceListed: too many).
+// The bin of the k-th largest of the threads' maxima: at least k values are in it or above.
+__device__ __forceinline__ int bin_of_maxima(Counts& s, const Rule& rule, const float (&maxima)[kGroups], unsigned k) {
+  for (int i = threadIdx.x; i < kBins; i += kThreads) s.count[i] = 0;
+  __syncthreads();
+#pragma unroll
+  for (int g = 0; g < kGroups; ++g) {
+    const int at = rule.bin(maxima[g]);
+    if (at <= kLastBin) atomicAdd(&s.count[at], 1u);
+  }
+  __syncthreads();
+  return bin_of_kth(s, k);
+}
+
+// ------------------------------------------------------------------ few rows, in slices
+
+// What a row's slices leave for each other and for the row's own workgroup: their maxima; the bin
+// in which top-p cuts (kBins: no cut) and the weight in front of it; and of each slice the first index of
+// the maximum (for rows without a temperature) and how many tokens it has listed (more than
+// the list holds: too many).
 struct RowSums {
   u64 before, total;
   int bin;
@@ -524,17 +564,18 @@ struct RowSums {
 static_assert(sizeof(RowSums) <= kSampleRowBytes, "as the host counts it");
 struct Space {
   RowSums* row;
-  u64* parts;   // [parts] weights in front of the cut, by the row's parts
-  u64* listed;  // [slices][kSampleSliceListed] places of the bin of the cut
+  u64* listed;  // [slices][kSampleRankListed] places that top-k or min-p may keep; or
+  u64* parts;   // [parts] weights in front of top-p's cut, by the row's parts,
+  u64* cut;     // [slices][kSampleSliceListed] places of the bin of the cut
   u64* bins;    // [slices][kBins] weights
 };
 __device__ __forceinline__ Space space_of(const SampleArgs& a, int m) {
   unsigned char* at = a.workspace + (size_t)m * a.row_bytes;
   Space s;
   s.row = reinterpret_cast<RowSums*>(at);
-  s.parts = reinterpret_cast<u64*>(at + kSampleRowBytes);
-  s.listed = s.parts + a.max_parts;
-  s.bins = s.listed + (size_t)a.slices * kSampleSliceListed;
+  s.listed = s.parts = reinterpret_cast<u64*>(at + kSampleRowBytes);
+  s.cut = s.parts + a.max_parts;
+  s.bins = s.cut + (size_t)a.slices * kSampleSliceListed;
   return s;
 }
 // Slice i of a row: whole parts.
@@ -552,7 +593,59 @@ __device__ __forceinline__ float row_top(const SampleArgs& a, const RowSums& r) 
   return top;
 }
 
-// Grid of these three: slice (fastest), row.
+// Grid of these: slice (fastest), row.
+
+// Of rows with top-k or min-p: a slice's tokens that they may keep, by the slice's own maxima.
+template <typename T>
+__global__ __launch_bounds__(kThreads) void slice_list_kernel(SampleArgs a) {
+  constexpr int kVec = Row<T>::kVec;
+  __shared__ Counts s;
+  __shared__ float wave_max[kWaves];
+  __shared__ unsigned listed;
+  __shared__ int found;
+  const int m = blockIdx.x / a.slices, i = blockIdx.x % a.slices, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const Space at = space_of(a, m);
+  const Row<T> row(static_cast<const T*>(a.logits) + (size_t)m * a.logits_ld, a.V);
+  const Range sl = slice_of(a, row, i);
+  float maxima[kGroups];
+  float top = group_maxima(row, sl, maxima);
+  if (lane == 0) wave_max[wave] = top;
+  if (tid == 0) listed = 0, found = a.V;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) top = __builtin_elementwise_maximum(top, wave_max[w]);
+  if (tid == 0) at.row->max[i] = top;
+  const float temperature = a.temperature ? a.temperature[m] : 1.f;
+  if (!(temperature > 0.f)) {
+    int first = a.V;
+    row.each(sl, [&](int v, float x) { first = x == top ? min(first, v) : first; });
+    if (first < a.V) atomicMin(&found, first);
+    __syncthreads();
+    if (tid == 0) at.row->first[i] = found;
+    return;
+  }
+  const int k = a.top_k && a.top_k[m] > 0 ? a.top_k[m] : a.V;
+  const float min_p = a.min_p ? a.min_p[m] : 0.f;
+  const bool by_k = k < a.V && k <= kMostK;
+  if ((by_k || min_p > 0.f) && top > -__builtin_huge_valf()) {
+    const Rule rule = rule_of(top, temperature, min_p, nullptr);
+    int last = last_bin(min_p);
+    if (by_k) last = min(bin_of_maxima(s, rule, maxima, (unsigned)k), last);
+    const float end = (float)(last + 1);
+    auto list = [&](int v, float x) {
+      if (!(rule.in_bins(x) < end || x == top)) return;
+      const unsigned to = atomicAdd(&listed, 1u);
+      if (to < kSampleRankListed) at.listed[(size_t)i * kSampleRankListed + to] = place_of(x, v);
+    };
+    row.template sweep<kAheadDense>(sl, [&](int v0, const float (&x)[kVec]) {
+#pragma unroll
+      for (int e = 0; e < kVec; ++e) list(v0 + e, x[e]);
+    }, list);
+  }
+  __syncthreads();
+  if (tid == 0) at.row->n[i] = listed;
+}
+
 template <typename T>
 __global__ __launch_bounds__(kThreads) void slice_top_kernel(SampleArgs a) {
   __shared__ float wave_max[kWaves];
@@ -663,7 +756,7 @@ __global__ __launch_bounds__(kThreads) void slice_parts_kernel(SampleArgs a) {
     const int here = rule.bin(x);
     if (here == bin) {
       const unsigned to = atomicAdd(&listed, 1u);
-      if (to < kSampleSliceListed) at.listed[(size_t)i * kSampleSliceListed + to] = place_of(x, v);
+      if (to < kSampleSliceListed) at.cut[(size_t)i * kSampleSliceListed + to] = place_of(x, v);
     }
     return here < bin ? w : 0;
   };
@@ -732,7 +825,7 @@ __device__ bool draw_of_slices(Shared& s, const SampleArgs& a, const Rule& rule,
     if (__ballot(here > kSampleSliceListed) || n > kListed) return false;
     const unsigned mine = (unsigned)__builtin_amdgcn_readlane((int)here, slice);
     const unsigned from = (unsigned)__builtin_amdgcn_readlane((int)up_to, slice) - mine;
-    for (unsigned i = lane; i < mine; i += 64) s.listed[from + i] = at.listed[(size_t)slice * kSampleSliceListed + i];
+    for (unsigned i = lane; i < mine; i += 64) s.listed[from + i] = at.cut[(size_t)slice * kSampleSliceListed + i];
     if (tid == 0) s.count[bin] = n, s.counted[bin] = 0, s.before[bin] = at.row->before;
     __syncthreads();
     const double target = top_p > 0.f ? (double)top_p * (double)at.row->total : 0.0;
@@ -750,8 +843,50 @@ __device__ bool draw_of_slices(Shared& s, const SampleArgs& a, const Rule& rule,
   return true;
 }
 
-// SLICED: the slices' kernels have run.
-template <typename T, bool SLICED>
+// The first index of the row's maximum, from its slices'.
+__device__ __forceinline__ int first_of_slices(const SampleArgs& a, const RowSums& r, float top) {
+  const int i = min((int)(threadIdx.x & (kSampleMaxSlices - 1)), a.slices - 1);
+  int first = r.max[i] == top ? r.first[i] : a.V;
+#pragma unroll
+  for (int d = 1; d < kSampleMaxSlices; d <<= 1) first = min(first, __shfl_xor(first, d));
+  return first;
+}
+
+// The slices' lists brought together in s.listed, without what cannot be kept by the whole row's
+// counts; false: too many tokens.
+__device__ __forceinline__ bool gather_lists(Shared& s, const SampleArgs& a, const Rule& rule, const Space& at, bool by_k,
+                                             unsigned k, float min_p) {
+  const int tid = threadIdx.x, lane = tid & 63, slice = tid >> 6;
+  const unsigned here = lane < a.slices ? at.row->n[lane] : 0;
+  if (__ballot(here > kSampleRankListed)) return false;
+  const unsigned n = slice < a.slices ? (unsigned)__shfl((int)here, slice) : 0;
+  const u64* from = at.listed + (size_t)slice * kSampleRankListed;
+  int last = last_bin(min_p);
+  if (by_k) {
+    for (int i = tid; i < kBins; i += kThreads) s.count[i] = 0;
+    __syncthreads();
+    for (unsigned i = lane; i < n; i += 64) {
+      const int bin = rule.bin(value_of(from[i]));
+      if (bin <= kLastBin) atomicAdd(&s.count[bin], 1u);
+    }
+    __syncthreads();
+    last = min(bin_of_kth(s, k), last);
+  }
+  const float end = (float)(last + 1);
+  for (unsigned i = lane; i < n; i += 64) {
+    const u64 place = from[i];
+    const float x = value_of(place);
+    if (!(rule.in_bins(x) < end || x == rule.top)) continue;
+    const unsigned to = atomicAdd(&s.listed_n, 1u);
+    if (to < kListed) s.listed[to] = place;
+  }
+  __syncthreads();
+  return s.listed_n <= kListed;
+}
+
+// Whole rows by themselves, or with what their slices' kernels have left.
+enum Sliced { kWhole, kSummed, kRankedLists };
+template <typename T, Sliced SLICED>
 __global__ __launch_bounds__(kThreads) void sample_kernel(SampleArgs a) {
   extern __shared__ __align__(16) unsigned char shared_bytes[];
   Shared& s = *reinterpret_cast<Shared*>(shared_bytes);
@@ -763,7 +898,7 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleArgs a) {
     a.tokens[m] = v;
     a.logprobs[m] = (float)log((double)w / (double)total);
   };
-  if constexpr (SLICED) {
+  if constexpr (SLICED == kSummed) {
     const Space at = space_of(a, m);
     const float top = row_top(a, *at.row), temperature = a.temperature ? a.temperature[m] : 1.f;
     if (!(top > -__builtin_huge_valf())) {
@@ -771,9 +906,7 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleArgs a) {
       return;
     }
     if (!(temperature > 0.f)) {
-      int first = at.row->first[min(lane & (kSampleMaxSlices - 1), a.slices - 1)];
-#pragma unroll
-      for (int d = 1; d < kSampleMaxSlices; d <<= 1) first = min(first, __shfl_xor(first, d));
+      const int first = first_of_slices(a, *at.row, top);
       if (tid == 0) a.tokens[m] = first, a.logprobs[m] = 0.f;
       return;
     }
@@ -784,19 +917,11 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleArgs a) {
     __syncthreads();
   }
 
-  // The maxima of the thread's groups of values (NaN if one is), and of all.
-  float maxima[kGroups];
-#pragma unroll
-  for (int g = 0; g < kGroups; ++g) maxima[g] = -__builtin_huge_valf();
-  row.template sweep<kAhead>([&](int, const float (&x)[kVec]) {
-#pragma unroll
-    for (int e = 0; e < kVec; ++e) maxima[e % kGroups] = __builtin_elementwise_maximum(maxima[e % kGroups], x[e]);
-  }, [&](int, float x) { maxima[0] = __builtin_elementwise_maximum(maxima[0], x); });
-  float top = maxima[0];
-#pragma unroll
-  for (int g = 1; g < kGroups; ++g) top = __builtin_elementwise_maximum(top, maxima[g]);
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) top = __builtin_elementwise_maximum(top, __shfl_xor(top, d));
+  float maxima[kGroups], top;
+  if constexpr (SLICED == kRankedLists)
+    top = row_top(a, *space_of(a, m).row);
+  else
+    top = group_maxima(row, Range{0, row.vecs, true, true}, maxima);
   if (lane == 0) s.wave_max[wave] = top;
   if (tid == 0) s.found = V, s.listed_n = 0, s.total = s.total_listed = 0;
   if (tid < kPowers) s.powers[tid] = root_power(tid);
@@ -810,7 +935,10 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleArgs a) {
   const float temperature = a.temperature ? a.temperature[m] : 1.f;
   if (__builtin_expect(!(temperature > 0.f), 0)) {  // greedy
     int first = V;
-    row.each([&](int v, float x) { first = x == top ? min(first, v) : first; });
+    if constexpr (SLICED == kRankedLists)
+      first = first_of_slices(a, *space_of(a, m).row, top);
+    else
+      row.each([&](int v, float x) { first = x == top ? min(first, v) : first; });
     if (first < V) atomicMin(&s.found, first);
     __syncthreads();
     if (tid == 0) a.tokens[m] = s.found, a.logprobs[m] = 0.f;
@@ -826,23 +954,14 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleArgs a) {
   // Top-p alone: the sum is one of all weights, and the cut mostly among the first few thousand.
   const bool sums = by_p && !by_k && !(min_p > 0.f);
   u64 all = 0;
-  bool listed = (by_k && k <= kMostK) || min_p > 0.f || V <= kListed || sums;
-  if (listed) {
-    // The bin of the k-th largest maximum: at least k values are in it or above.
-    // And none that min-p keeps is far below it (two bins for what the logarithm is off).
-    int last = kLastBin;
-    if (min_p > 0.f) last = (int)fminf((float)last, 2.f - __log2f(fminf(min_p, 1.f)) * ((float)kBins / kOctaves));
-    if ((by_k && k <= kMostK) || sums) {
-      for (int i = tid; i < kBins; i += kThreads) s.count[i] = 0;
-      __syncthreads();
-#pragma unroll
-      for (int g = 0; g < kGroups; ++g) {
-        const int at = rule.bin(maxima[g]);
-        if (at <= kLastBin) atomicAdd(&s.count[at], 1u);
-      }
-      __syncthreads();
-      last = min(bin_of_kth(s, (unsigned)(sums ? kMostK : k)), last);
-    }
+  const bool few_k = by_k && k <= kMostK;
+  bool listed = few_k || min_p > 0.f || V <= kListed || sums;
+  if (SLICED == kRankedLists && (few_k || min_p > 0.f)) {
+    listed = gather_lists(s, a, rule, space_of(a, m), few_k, (unsigned)k, min_p);
+  } else if (listed) {
+    int last = last_bin(min_p);
+    if constexpr (SLICED == kRankedLists) group_maxima(row, Range{0, row.vecs, true, true}, maxima);
+    if (few_k || sums) last = min(bin_of_maxima(s, rule, maxima, (unsigned)(sums ? kMostK : k)), last);
     // (some may weigh nothing: they change nothing)
     const float end = (float)(last + 1);
     auto in_reach = [&](float x) { return rule.in_bins(x) < end || x == top; };
@@ -941,14 +1060,17 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleArgs a) {
 
 template <typename T>
 hipError_t launch(const SampleArgs& a, hipStream_t stream) {
-  if (a.slices > 1) {
-    const dim3 grid((unsigned)a.M * (unsigned)a.slices), threads(kThreads);
+  const dim3 grid((unsigned)a.M * (unsigned)a.slices), threads(kThreads);
+  if (a.slices > 1 && (a.top_k || a.min_p)) {
+    launch_kernel(slice_list_kernel<T>, grid, threads, 0, stream, a);
+    launch_kernel(sample_kernel<T, kRankedLists>, dim3((unsigned)a.M), threads, sizeof(Shared), stream, a);
+  } else if (a.slices > 1) {
     launch_kernel(slice_top_kernel<T>, grid, threads, 0, stream, a);
     if (a.top_p) launch_kernel(slice_bins_kernel<T>, grid, threads, 0, stream, a);
     launch_kernel(slice_parts_kernel<T>, grid, threads, 0, stream, a);
-    launch_kernel(sample_kernel<T, true>, dim3((unsigned)a.M), threads, sizeof(Shared), stream, a);
+    launch_kernel(sample_kernel<T, kSummed>, dim3((unsigned)a.M), threads, sizeof(Shared), stream, a);
   } else {
-    launch_kernel(sample_kernel<T, false>, dim3((unsigned)a.M), dim3(kThreads), sizeof(Shared), stream, a);
+    launch_kernel(sample_kernel<T, kWhole>, dim3((unsigned)a.M), threads, sizeof(Shared), stream, a);
   }
   return hipGetLastError();
 }

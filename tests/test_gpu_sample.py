@@ -327,3 +327,73 @@ def test_captured_sliced_rows_follow_their_arguments(gpu):
         assert torch.equal(tokens.cpu(), want[0]) and torch.equal(logs.cpu(), want[1])
         want = run(gpu, fresh, given, temperature=options["temperature"])
         assert torch.equal(alone.cpu(), want[0]) and torch.equal(alone_logs.cpu(), want[1])
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("m,v", [(1, 65536), (1, 131072), (2, 131071), (7, 151936), (1, 1 << 19), (1, (1 << 19) - 3), (170, 65541), (171, 65541)])
+def test_few_rows_with_ranks(gpu, m, v, dtype):
+    """top-k and min-p on rows that several workgroups share: every row with its own options, some off, some greedy."""
+    rng = np.random.default_rng(v + 1)
+    logits = logits_of(m, v, seed=v + 1, dtype=dtype)
+    temperature = rng.choice([0.0, 0.4, 1.0, 1.7], m).tolist()
+    top_k = rng.choice([0, 1, 7, 50, 1000, 2048, 2049, 9000], m).tolist()
+    min_p = rng.choice([0.0, 1e-6, 0.03, 0.9, 1.0, math.nan], m).tolist()
+    top_p = rng.choice([0.0, 0.3, 0.95, 1.0], m).tolist()
+    run(gpu, logits, uniforms_of(m, seed=1), temperature=temperature, top_k=top_k)
+    run(gpu, logits, uniforms_of(m, seed=2), temperature=temperature, min_p=min_p)
+    run(gpu, logits, uniforms_of(m, seed=3), temperature=temperature, top_k=top_k, min_p=min_p, top_p=top_p)
+    run(gpu, logits, uniforms_of(m, seed=4), top_k=[50] * m, top_p=[0.9] * m)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_where_the_ranks_fall_in_sliced_rows(gpu, dtype):
+    """The first k among equal values all over the row (more than the lists hold, and fewer), all in one slice, in rows
+    at odd addresses; rows of -inf, NaN and +inf."""
+    v = 131072 + 24
+    base = torch.full((8, v + 5), -20.0)
+    base[0] = 1.0
+    base[1, ::80] = 2.0
+    base[2, ::9] = 2.0
+    base[3, :300] = torch.arange(300) / 100
+    base[4, -300:] = torch.arange(300) / 100
+    base[5] = -math.inf
+    base[5, 40000] = -5.0
+    base[6, 50000] = math.nan
+    base[7, 20000:60000:13000] = math.inf
+    wide = base.to(dtype).to(gpu)
+    for at in (0, 1, 3, 5):
+        logits = wide[:, at:at + v]
+        rows = logits.double().cpu().numpy()
+        for i, (k, min_p, top_p) in enumerate(((1, 0.0, 1.0), (40, 0.0, 0.9), (1700, 0.0, 0.5), (100, 0.02, 1.0), (0, 0.3, 1.0), (2000, 1e-12, 0.99))):
+            u = uniforms_of(8, seed=90 + i)
+            full = [torch.full((8,), x, device=gpu) for x in (k, min_p, top_p)]
+            tokens, logs = kernels.sample_logits(logits, torch.tensor(u, device=gpu), top_k=full[0].int(), min_p=full[1], top_p=full[2])
+            for r in range(8):
+                token, log = reference(rows[r], float(torch.tensor(u)[r]), top_k=k, min_p=float(full[1][r]), top_p=float(full[2][r]))
+                assert int(tokens[r]) == token, f"row {r} at {at}, top_k {k}, min_p {min_p}, top_p {top_p}"
+                assert math.isnan(log) and math.isnan(float(logs[r])) \
+                    or abs(float(logs[r]) - log) <= 2.0 ** -23 * abs(log) + 2.0 ** -40 * math.exp(-log)
+
+
+def test_captured_ranked_rows_follow_their_arguments(gpu):
+    m, v = 5, 66000
+    logits, u = torch.zeros((m, v), device=gpu), torch.zeros(m, device=gpu)
+    given = dict(temperature=torch.ones(m, device=gpu), top_k=torch.ones(m, dtype=torch.int32, device=gpu), top_p=torch.ones(m, device=gpu),
+                 min_p=torch.zeros(m, device=gpu))
+    stream = torch.cuda.Stream()
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=stream):
+        tokens, logs = kernels.sample_logits(logits, u, **given)
+    rng = np.random.default_rng(71)
+    for i in range(5):
+        fresh = logits_of(m, v, seed=170 + i)
+        options = dict(temperature=rng.choice([0.0, 0.6, 1.2], m).tolist(), top_k=rng.choice([0, 3, 60, 900], m).tolist(),
+                       top_p=rng.choice([0.2, 0.9, 1.0], m).tolist(), min_p=rng.choice([0.0, 0.05], m).tolist())
+        draw = uniforms_of(m, seed=180 + i)
+        logits.copy_(fresh), u.copy_(torch.tensor(draw))
+        for name, value in options.items():
+            given[name].copy_(torch.tensor(value))
+        graph.replay()
+        want = run(gpu, fresh, draw, **options)
+        assert torch.equal(tokens.cpu(), want[0]) and torch.equal(logs.cpu(), want[1])

@@ -45,12 +45,15 @@ def test_wrapper_refuses():
 
 @pytest.mark.parametrize("m,v,filters,some", [
     (1, 151936, (0, 0, 0), True), (1, 151936, (0, 1, 0), True), (256, 16384, (0, 1, 0), True), (1, 1 << 19, (0, 1, 0), True),
-    (1, 151936, (1, 1, 0), False), (1, 151936, (0, 1, 1), False), (257, 151936, (0, 1, 0), False), (1, 16383, (0, 1, 0), False),
+    (1, 151936, (1, 1, 0), True), (1, 151936, (0, 1, 1), True), (257, 151936, (0, 1, 0), False), (1, 16383, (0, 1, 0), False),
+    (171, 151936, (1, 0, 0), False), (1, 65535, (1, 0, 1), False),
     (0, 151936, (0, 1, 0), False), (1, (1 << 19) + 1, (0, 0, 0), False),
 ])
 def test_workspace_bytes(m, v, filters, some):
-    """Only rows that are cut need one: 16 bytes of sums for 512 values, and with top-p 20 KB a slice."""
+    """Only rows that are cut need one: with top-k or min-p 16 KB a slice, else 8 bytes of sums for 256 values, and with
+    top-p 20 KB a slice."""
     need = [_lib.load().lsk_sample_workspace_bytes(mode, m, v, *filters) for mode in (0, 1)]
-    assert need[0] == need[1] and (need[0] > 0) == some
-    assert need[0] <= m * (512 + v // 256 * 8 + (16 * 20480 if filters[1] else 0))
+    assert (need[0] > 0) == some and need[1] in (need[0], 0)   # (bf16 rows are half as long)
+    most = 16 * 16384 if filters[0] or filters[2] else v // 256 * 8 + (16 * 20480 if filters[1] else 0)
+    assert need[0] <= m * (512 + most)
     assert _lib.load().lsk_sample_workspace_bytes(2, m, v, *filters) == 0
