@@ -260,19 +260,19 @@ constexpr int constrain_slices(int M, int V) {
 // Sampled tokens (sample.hip): a row's weights, whole numbers up to 2^44, add up in 63 bits.
 constexpr int kSampleMaxVocab = 1 << 19;
 
-// Rows are cut into slices while the chip has room for all, of at least kSampleLeastSlice values.
-// Without top-k and min-p that is always faster (16384 values and 256 rows among them).  With one
-// of them (`ranked`) a second launch costs more than the sweeps of a row that is not
-// kSampleRankedBytes long, or that only two workgroups would share: 16 rows of 151936 fp32 values
-// 17 us for 28, of bf16 16 for 22; of 50257 fp32 values 16 either way, of 32000 15 for 13; 256
-// rows of 151936 64..89 for 68..85.
+// Rows are cut into three slices or more while the chip has room for all, of at least
+// kSampleLeastSlice values.  16 rows of 151936 fp32 values without top-k and min-p 18 us for 75 (top-p 0.9 over flat
+// ones 44 for 283, over peaked ones 36 for 97), of 32000 16 for 22; with two slices some are slower
+// (256 rows 89 for 107, peaked with top-p 146 for 123).  With top-k or min-p (`ranked`) a second
+// launch costs more than the sweeps of a row that is not kSampleRankedBytes long: 16 rows of 151936
+// fp32 values 17 us for 28, of bf16 16 for 22; of 50257 fp32 values 16 either way, of 32000 15 for 13.
 constexpr int kSampleMaxSlices = 16, kSampleLeastSlice = 8192, kSamplePlaces = 512, kSampleRankedBytes = 1 << 18;
 constexpr int kSampleBins = 2048, kSampleSliceListed = 512, kSampleRankListed = 2048, kSampleRowBytes = 256;
 constexpr int sample_slices(int M, int V, int value_bytes, bool ranked) {
   const int room = kSamplePlaces / M, most = V / kSampleLeastSlice;
   const int slices = room < most ? room : most;
-  if (ranked && (V < kSampleRankedBytes / value_bytes || slices < 3)) return 1;
-  return slices < 2 ? 1 : slices < kSampleMaxSlices ? slices : kSampleMaxSlices;
+  if (slices < 3 || (ranked && V < kSampleRankedBytes / value_bytes)) return 1;
+  return slices < kSampleMaxSlices ? slices : kSampleMaxSlices;
 }
 // (parts of 64 accesses of 16 bytes)
 constexpr int sample_max_parts(int V) { return V / 256 + 3; }

@@ -251,8 +251,8 @@ def test_streams(gpu):
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
-@pytest.mark.parametrize("m,v", [(1, 16384), (1, 16390), (2, 24577), (7, 151936), (1, 1 << 19), (1, (1 << 19) - 3), (128, 40003), (256, 16387),
-                                 (257, 16387)])
+@pytest.mark.parametrize("m,v", [(1, 24576), (1, 24583), (2, 32771), (7, 151936), (1, 1 << 19), (1, (1 << 19) - 3), (128, 40003), (170, 24587),
+                                 (171, 24587)])
 def test_few_rows_without_ranks(gpu, m, v, dtype):
     """Temperature and top-p alone, rows that several workgroups share: every row with its own options, greedy
     ones and ones that top-p leaves alone among them."""

@@ -19,7 +19,7 @@ INVALID, WORKSPACE = -1, -4
     (dict(tokens=FAKE + 4), INVALID), (dict(logs=None), INVALID), (dict(logs=FAKE + 2), INVALID),
     (dict(v=50000, ld=50000, ws=None), WORKSPACE), (dict(v=50000, ld=50000, ws=FAKE + 8), WORKSPACE),
     (dict(v=50000, ld=50000, ws_bytes=100), WORKSPACE), (dict(v=50000, ld=50000, p=FAKE, ws_bytes=60000), WORKSPACE),
-    (dict(v=1 << 19, ld=1 << 19, m=256, p=FAKE, ws_bytes=0), WORKSPACE),
+    (dict(v=1 << 19, ld=1 << 19, m=128, p=FAKE, ws_bytes=0), WORKSPACE),
 ])
 def test_entry_point_rejects_before_launch(bad, code):
     lib = _lib.load()
@@ -44,8 +44,8 @@ def test_wrapper_refuses():
 
 
 @pytest.mark.parametrize("m,v,filters,some", [
-    (1, 151936, (0, 0, 0), True), (1, 151936, (0, 1, 0), True), (256, 16384, (0, 1, 0), True), (1, 1 << 19, (0, 1, 0), True),
-    (1, 151936, (1, 1, 0), True), (1, 151936, (0, 1, 1), True), (257, 151936, (0, 1, 0), False), (1, 16383, (0, 1, 0), False),
+    (1, 151936, (0, 0, 0), True), (1, 151936, (0, 1, 0), True), (170, 24576, (0, 1, 0), True), (1, 1 << 19, (0, 1, 0), True),
+    (1, 151936, (1, 1, 0), True), (1, 151936, (0, 1, 1), True), (171, 151936, (0, 1, 0), False), (1, 24575, (0, 1, 0), False),
     (171, 151936, (1, 0, 0), False), (1, 65535, (1, 0, 1), False),
     (0, 151936, (0, 1, 0), False), (1, (1 << 19) + 1, (0, 0, 0), False),
 ])
