@@ -6,8 +6,8 @@
 // k and v being e4m3 bytes times a power of two per 16 rows and head (paged_cache.hip
 // has the format).
 //
-// An item is up to 64 (T n_q / n_kv rows are few) or 128 query rows of one request and kv
-// head, over the rows that its last one sees.  How many those are only the device
+// An item is 16 or 32 query rows (T n_q / n_kv are few; up to 64 in one launch) or 128 of one
+// request and kv head, over the rows that its last one sees.  How many those are only the device
 // knows; every wave counts the items' units of key rows (lens is read once more by each).
 // Few query rows: an item is cut into chunks of equal length, as many as let all the
 // chunks run at once, one wave each.  Many: a kv head's items are laid end to end and
@@ -15,7 +15,13 @@
 // of another), because an item more or less per CU would cost a whole round.  Whole items
 // are written to the output, parts as (m, l, O) in fp32 to the workspace, and a second
 // launch adds an item's parts up in their order.  A context that is short for certain runs
-// in one launch, an item per workgroup.
+// in one launch, an item per workgroup.  (paged_plan in lsk_host.h has the rules.)
+//
+// Bound by: single tokens and a few, the cache's bytes (64 requests over 17..8001 rows, 527 MB: 88 us,
+// 6.0 TB/s, and 4 for the second launch), where there is little to read the chain of lens,
+// table, rows, sums and the second launch (1 request over 32768 rows 17 + 6 us); prompts, the
+// chain of products, exponentials and conversions of two waves that share a SIMD (2 x 1500
+// tokens behind up to 7001 rows: 238 us, 980 TFLOP/s, and 15 for the parts' 130 MB).
 //
 // Few query rows (decode, verify).  A wave takes two blocks, 32 key rows, a step, for up to
 // 4 x 16 query rows:

@@ -21,6 +21,13 @@
 // it.  All else works on the list, in LDS.  Without either (top-p or the temperature alone)
 // every weight counts, and a workgroup is bound by the arithmetic of the weights.  Few rows
 // are cut into slices, a workgroup each, which leave lists or sums for the row's own.
+//
+// 128 rows of 151936 fp32 values with all filters: 24 + 9 us, 6.4 TB/s in the first launch, which
+// reads them twice (kept in registers between the sweeps, 40 of them, they are read once by one
+// workgroup to a CU instead of two: 20 us here and 23 for 21 with 37 rows); 1 row 6 + 8 us, the chain
+// of sweep, groups, list, gathering, ranks and draw.  Without top-k and min-p 64 rows 32 us, with
+// top-p 60..70: the arithmetic of two or three passes of weights (some 30 instructions for a
+// value, half of them in 64 bits).
 
 #include <hip/hip_runtime.h>
 

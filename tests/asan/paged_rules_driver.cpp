@@ -84,6 +84,20 @@ int main() {
     for (int m : kEnds)
       for (int v : kEnds)
         samples += lsk::check_sample_args(p, mode, m, v, v, f32, f32, i32, f32, f32, tokens, f32) == LSK_OK;
+  for (int m : kEnds)
+    for (int v : kEnds) {
+      if (lsk::check_sample_sizes(0, m, v) != LSK_OK) continue;
+      for (int bytes : {2, 4})
+        for (bool ranked : {false, true})
+          for (bool by_p : {false, true}) {
+            const int slices = lsk::sample_slices(m, v, bytes, ranked);
+            const unsigned long long row = lsk::sample_row_bytes(slices, v, by_p, ranked);
+            expect(slices >= 1 && slices <= lsk::kSampleMaxSlices && (long long)m * slices <= (m > 512 ? m : 512) &&
+                       (slices == 1 || v / slices >= lsk::kSampleLeastSlice),
+                   "slices fit the chip and hold values");
+            expect((row == 0) == (slices == 1) && row % 256 == 0 && row < (1u << 20), "a row's sums are less than 1 MB");
+          }
+    }
   expect(pools > 0 && appends > 0 && reads > 0 && copies > 0 && plans > 0 && calls > 0 && samples > 0,
          "some sizes of every kind are served");
 
