@@ -274,8 +274,8 @@ constexpr int sample_slices(int M, int V, int value_bytes, bool ranked) {
   if (slices < 3 || (ranked && V < kSampleRankedBytes / value_bytes)) return 1;
   return slices < kSampleMaxSlices ? slices : kSampleMaxSlices;
 }
-// (parts of 64 accesses of 16 bytes)
-constexpr int sample_max_parts(int V) { return V / 256 + 3; }
+// (parts of 64 accesses of 16 bytes; an even number keeps what follows them at 16 bytes)
+constexpr int sample_max_parts(int V) { return (V / 256 + 4) / 2 * 2; }
 constexpr unsigned long long sample_row_bytes(int slices, int V, bool by_p, bool ranked) {
   const unsigned long long each = ranked ? kSampleRankListed : by_p ? kSampleSliceListed + kSampleBins : 0;
   const unsigned long long words = slices * each + (ranked ? 0 : sample_max_parts(V));

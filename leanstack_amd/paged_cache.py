@@ -19,7 +19,8 @@ kept here, on the host:
 
 Pages have a count of the requests that hold them.  A page that several hold is
 copied before one of them writes into it (``reserve``).  ``truncate`` drops rows of
-rejected drafts, ``compact`` moves the pages in use to the pool's front.
+rejected drafts, ``compact`` moves the pages in use to the pool's front.  One thread at
+a time keeps a cache's accounts; page tables and lengths that were made are tensors of their own.
 """
 
 from __future__ import annotations
