@@ -353,7 +353,7 @@ int check_paged_attention_sizes(int B, int T, int n_q, int n_kv, int capacity) {
     return fail(LSK_ERR_INVALID, "B=%d, T=%d, n_q=%d: too many query rows", B, T, n_q);
   const PagedPlan p = paged_plan(B, T, n_q, n_kv, capacity);
   if (p.items * n_kv * (p.rows / 16) > most || p.workers * n_kv > most ||
-      p.items * ((capacity + p.unit - 1) / p.unit) > INT_MAX)
+      p.items * ((capacity + p.unit - 1) / p.unit + kPagedManyStart) > INT_MAX)
     return fail(LSK_ERR_INVALID, "B=%d, T=%d, n_q=%d over %d rows: too many items", B, T, n_q, capacity);
   return LSK_OK;
 }

@@ -195,19 +195,19 @@ __device__ __forceinline__ Chunk chunk_of(const PagedAttentionArgs& a, int w, bo
 // Where worker w's share of the line begins.
 __device__ __forceinline__ int share_begin(long long units, int w, int workers) { return (int)(units * w / workers); }
 
-// The item in which worker w's share begins, the units of it in front of the share, and
-// the share's length.
+// The item in which worker w's share begins, the places of it in front of the share, and the
+// share's length.  An item's places: kPagedManyStart for its beginning and its end, then its units.
 struct Share {
-  int item, skip, units;
+  int item, skip, places;
 };
 template <int ROWS>
 __device__ __forceinline__ Share share_of(const PagedAttentionArgs& a, int w, bool write) {
-  auto units_of = [&](int i) { return item_units<ROWS>(a, i); };
-  const int mine = lane_items(a, units_of), up_to = wave_sums(mine);
+  auto places_of = [&](int i) { return item_units<ROWS>(a, i) + kPagedManyStart; };
+  const int mine = lane_items(a, places_of), up_to = wave_sums(mine);
   const int total = __builtin_amdgcn_readlane(up_to, 63);
-  if (write) write_begins(a, up_to - mine, total, units_of);
+  if (write) write_begins(a, up_to - mine, total, places_of);
   const int begin = share_begin(total, w, a.workers);
-  const Found f = item_at(a, begin, mine, up_to - mine, units_of);
+  const Found f = item_at(a, begin, mine, up_to - mine, places_of);
   return {f.item, begin - f.begin, share_begin(total, w + 1, a.workers) - begin};
 }
 
@@ -654,15 +654,15 @@ __global__ __launch_bounds__(THREADS) void join_kernel(PagedAttentionArgs a, int
   // parts `from` .. `last`: a slot per chunk, or the second slot of the worker that has the first unit
   // and the first slots of those up to the last unit's
   int from = begin, last = end - 1;
-  const int units = MANY ? a.begins[a.items] : 0;
+  const int places = MANY ? a.begins[a.items] : 0;
   if constexpr (MANY) {
-    auto worker_of = [&](int unit) {
-      int w = (int)((long long)unit * a.workers / units);
-      while (share_begin(units, w + 1, a.workers) <= unit) ++w;
-      while (share_begin(units, w, a.workers) > unit) --w;
+    auto worker_of = [&](int place) {
+      int w = (int)((long long)place * a.workers / places);
+      while (share_begin(places, w + 1, a.workers) <= place) ++w;
+      while (share_begin(places, w, a.workers) > place) --w;
       return w;
     };
-    from = worker_of(begin), last = worker_of(end - 1);
+    from = worker_of(begin + kPagedManyStart), last = worker_of(end - 1);
   }
   if (from == last) return;
   const int b = a.tiles == 1 ? item : item / a.tiles, tile = item - b * a.tiles;
@@ -695,8 +695,8 @@ __global__ __launch_bounds__(THREADS) void join_kernel(PagedAttentionArgs a, int
     for (int i = 0; i < kJoinAhead; ++i) {
       const int w = w0 + i * streams;
       if (w > last) break;
-      if (MANY && share_begin(units, w, a.workers) == share_begin(units, w + 1, a.workers))
-        continue;  // (fewer units than workers: one without a share)
+      if (MANY && share_begin(places, w, a.workers) == share_begin(places, w + 1, a.workers))
+        continue;  // (fewer places than workers: one without a share)
 #pragma unroll
       for (int p = 0; p < PASSES; ++p) {
         const float top = fmaxf(m[p], ml[i][p][0]);
@@ -1102,14 +1102,16 @@ __global__ __launch_bounds__(64 * kManyWaves, 2) void many_attention_kernel(Page
   __shared__ __align__(1024) ManyShared sh;
   const int j = blockIdx.x % a.pool.n_kv, w = blockIdx.x / a.pool.n_kv;
   const Share s = share_of<kManyRows>(a, w, blockIdx.x == 0 && threadIdx.x < 64);
-  int item = s.item, skip = s.skip, left = s.units;
+  int item = s.item, skip = s.skip, left = s.places;
   while (left > 0) {
     const int b = a.tiles == 1 ? item : item / a.tiles;
     const int units = item_units<kManyRows>(a, item);
-    const int last = min(skip + left, units);
-    many_rows(a, sh, j, b, item - b * a.tiles, skip, last, skip == 0 && last == units,
-              ((size_t)j * a.workers + w) * 2 + (skip == 0 ? 1 : 0));
-    left -= last - skip;
+    const int stop = min(skip + left, units + kPagedManyStart);
+    const int first = max(skip - kPagedManyStart, 0), last = stop - kPagedManyStart;
+    if (first < last)
+      many_rows(a, sh, j, b, item - b * a.tiles, first, last, first == 0 && last == units,
+                ((size_t)j * a.workers + w) * 2 + (first == 0 ? 1 : 0));
+    left -= stop - skip;
     skip = 0;
     ++item;
   }
