@@ -625,6 +625,7 @@ int lsk_paged_attention_bf16(const lsk_paged_pool* pool, const void* q, long lon
   a.slot_rows = p.slot_rows;
   const size_t begins = (size_t)lsk::paged_begins_bytes(p), slots = (size_t)p.slots * pool->n_kv * p.slot_rows;
   a.begins = static_cast<int*>(workspace);
+  a.cuts = need > 0 ? a.begins + p.items + 1 : nullptr;
   a.part_o = need > 0 ? reinterpret_cast<float*>(static_cast<char*>(workspace) + begins) : nullptr;
   a.part_ml = need > 0 ? a.part_o + slots * lsk::kAttnHeadDim : nullptr;
   hipError_t err = lsk::launch_paged_attention(a, p, static_cast<hipStream_t>(hip_stream));

@@ -168,7 +168,9 @@ constexpr int paged_windows(int rows) { return (int)(((long long)rows + 2 * kPag
 // The second launch adds up parts, 2^join_shift query rows to a workgroup; with more parts than
 // its threads can take at once it has fewer rows (1 request over 32768 rows, 256 parts: 6.4 us, 39
 // with 16 rows); with many query rows more of them, `join_passes` times, so that fewer
-// workgroups wait for their first loads (4 x 2000 tokens: 16 us, 32 with one pass).
+// workgroups wait for their first loads (2 x 1500 tokens behind 4000 and 7001 rows: 13 us, 14 with
+// one pass or four), and of more items than workers those that a share's beginning cuts (64 prompts
+// of 200 tokens, few of them cut: 4 us, 15 by items).
 constexpr int kPagedFewUnit = 32;
 constexpr int kPagedManyUnit = 64;
 constexpr int kPagedManyRows = 128;
@@ -176,18 +178,18 @@ constexpr int kPagedManyRows = 128;
 // take as long as: 4 prompts of 2000 tokens, whose first items are short, 176 us, 268 counting none.
 constexpr int kPagedManyStart = 6;
 constexpr int kPagedShortRows = 2048, kPagedShortFewRows = 1536, kPagedShortFewGroups = 128, kPagedShortGroups = 512;
-constexpr int kPagedJoinGroups = 2048, kPagedJoinPasses = 4;
+constexpr int kPagedJoinGroups = 2048, kPagedJoinPasses = 2;
 struct PagedPlan {
   bool one_launch;
   int rows, slot_rows, unit, least_units, tiles;
   int join_shift;   // a workgroup of the second launch adds up the parts of 2^join_shift query rows
   int join_passes;  // .. times this many, one behind the other
   bool join_wide;   // .. with 1024 threads, not 256
-  long long items, places, workers, slots;  // slots: of parts, per kv head
+  long long items, places, workers, slots, joins;  // slots: of parts, per kv head; joins: items that may have been cut
 };
 constexpr PagedPlan paged_plan(int B, int T, int n_q, int n_kv, int capacity) {
   const long long rows = (long long)T * (n_q / n_kv);
-  PagedPlan p = {false, rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : kPagedManyRows, 0, kPagedFewUnit, 4, 0, 0, 1, false, 0, 0, 0, 0};
+  PagedPlan p = {false, rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : kPagedManyRows, 0, kPagedFewUnit, 4, 0, 0, 1, false, 0, 0, 0, 0, 0};
   const long long groups = (long long)B * n_kv;
   p.one_launch = rows <= 64 && groups < kPagedShortGroups &&
                  capacity <= (groups < kPagedShortFewGroups ? kPagedShortFewRows : kPagedShortRows);
@@ -210,11 +212,15 @@ constexpr PagedPlan paged_plan(int B, int T, int n_q, int n_kv, int capacity) {
   p.join_shift = 4;
   while (p.join_shift > 0 && (p.slot_rows <= 1 << (p.join_shift - 1) || (64 >> p.join_shift) < parts)) --p.join_shift;
   p.join_wide = parts >= 128;
-  p.join_passes = many && p.join_shift == 4 && p.items * n_kv * ((p.slot_rows + 15) / 16) > kPagedJoinGroups ? kPagedJoinPasses : 1;
+  p.joins = many && p.items > p.workers ? p.workers : p.items;
+  p.join_passes = many && p.join_shift == 4 && p.joins * n_kv * ((p.slot_rows + 15) / 16) > kPagedJoinGroups ? kPagedJoinPasses : 1;
   return p;
 }
-// (m, l) and O of every slot, and where the items begin.
-constexpr unsigned long long paged_begins_bytes(const PagedPlan& p) { return ((unsigned long long)p.items * 4 + 4 + 15) / 16 * 16; }
+// (m, l) and O of every slot, and where the items begin and which of 128 rows are cut.
+constexpr unsigned long long paged_begins_bytes(const PagedPlan& p) {
+  const unsigned long long words = (unsigned long long)p.items + 1 + (p.rows == kPagedManyRows ? (unsigned long long)p.workers : 0);
+  return (words * 4 + 15) / 16 * 16;
+}
 constexpr unsigned long long paged_workspace_bytes(const PagedPlan& p, int n_kv) {
   return p.one_launch ? 0
                       : paged_begins_bytes(p) + (unsigned long long)p.slots * (unsigned long long)n_kv *

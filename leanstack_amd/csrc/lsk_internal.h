@@ -369,14 +369,14 @@ struct PagedCopyArgs {
 };
 hipError_t launch_paged_copy(PagedCopyArgs a, hipStream_t stream);
 // Attention of T query tokens of B requests over their pages (paged_attention.hip).
-// begins: the first chunk, or unit, of each item (items + 1 words, left by the first
-// launch); part_ml / part_o: (m, l) and O, slots of slot_rows query rows, m in base 2.
+// begins: the first chunk, or place on the line, of each item (items + 1 words, left by the
+// first launch); cuts: of 128 query rows, the item that a worker's share is the first to cut, or -1; part_ml / part_o: (m, l) and O, slots of slot_rows query rows, m in base 2.
 struct PagedAttentionArgs {
   PagedPool pool;
   const __bf16* q;
   const int *lens, *counts;
   __bf16* out;
-  int* begins;
+  int *begins, *cuts;
   float *part_ml, *part_o;
   size_t q_b, q_h, q_t;
   int B, T, G, n_q, tiles, items, places, workers, least_units, slot_rows, join_shift;

@@ -197,8 +197,10 @@ __device__ __forceinline__ int share_begin(long long units, int w, int workers) 
 
 // The item in which worker w's share begins, the places of it in front of the share, and the
 // share's length.  An item's places: kPagedManyStart for its beginning and its end, then its units.
+// cuts: whether it is the first share to begin behind the item's first unit.
 struct Share {
   int item, skip, places;
+  bool cuts;
 };
 template <int ROWS>
 __device__ __forceinline__ Share share_of(const PagedAttentionArgs& a, int w, bool write) {
@@ -208,7 +210,9 @@ __device__ __forceinline__ Share share_of(const PagedAttentionArgs& a, int w, bo
   if (write) write_begins(a, up_to - mine, total, places_of);
   const int begin = share_begin(total, w, a.workers);
   const Found f = item_at(a, begin, mine, up_to - mine, places_of);
-  return {f.item, begin - f.begin, share_begin(total, w + 1, a.workers) - begin};
+  const int unit0 = f.begin + kPagedManyStart;
+  return {f.item, begin - f.begin, share_begin(total, w + 1, a.workers) - begin,
+          begin > unit0 && share_begin(total, w - 1, a.workers) <= unit0};
 }
 
 struct Part {
@@ -636,8 +640,8 @@ __global__ __launch_bounds__(64 * kShortWaves, 2) void short_attention_kernel(Pa
   }
 }
 
-// Adds up the parts of items that were cut.  Grid: kv head (fastest), item, `1 << a.join_shift` query
-// rows of it; 16 threads take 8 dims each of a part's row, and the rest of the workgroup other rows
+// Adds up the parts of items that were cut.  Grid: kv head (fastest), item (MANY and more items than
+// workers: worker, whose share may be the first to begin inside one), `1 << a.join_shift` query rows of it; 16 threads take 8 dims each of a part's row, and the rest of the workgroup other rows
 // or, with few rows, further parts: stream s the parts s, s + streams, ..
 template <bool MANY, int THREADS, int PASSES>
 __global__ __launch_bounds__(THREADS) void join_kernel(PagedAttentionArgs a, int rows) {
@@ -649,7 +653,8 @@ __global__ __launch_bounds__(THREADS) void join_kernel(PagedAttentionArgs a, int
   id /= a.pool.n_kv;
   const int own = 1 << a.join_shift, streams = kSlots >> a.join_shift;  // rows at a time; and of each
   const int groups = (min(rows, a.T * a.G) + own * PASSES - 1) / (own * PASSES);
-  const int item = id / groups, group = id - item * groups;
+  const int nth = id / groups, group = id - nth * groups, item = MANY && a.items > a.workers ? a.cuts[nth] : nth;
+  if (item < 0) return;
   const int begin = a.begins[item], end = a.begins[item + 1];
   // parts `from` .. `last`: a slot per chunk, or the second slot of the worker that has the first unit
   // and the first slots of those up to the last unit's
@@ -1102,6 +1107,7 @@ __global__ __launch_bounds__(64 * kManyWaves, 2) void many_attention_kernel(Page
   __shared__ __align__(1024) ManyShared sh;
   const int j = blockIdx.x % a.pool.n_kv, w = blockIdx.x / a.pool.n_kv;
   const Share s = share_of<kManyRows>(a, w, blockIdx.x == 0 && threadIdx.x < 64);
+  if (j == 0 && threadIdx.x == 0) a.cuts[w] = s.cuts ? s.item : -1;
   int item = s.item, skip = s.skip, left = s.places;
   while (left > 0) {
     const int b = a.tiles == 1 ? item : item / a.tiles;
@@ -1134,7 +1140,7 @@ hipError_t launch_paged_attention(const PagedAttentionArgs& a, const PagedPlan& 
   if (plan.rows == kManyRows) launch_kernel(many_attention_kernel, grid, dim3(64 * kManyWaves), 0, stream, a);
   hipError_t err = hipGetLastError();
   if (err != hipSuccess) return err;
-  const dim3 joins((unsigned)a.items * n_kv * (unsigned)ceil_div(plan.slot_rows, plan.join_passes << plan.join_shift));
+  const dim3 joins((unsigned)plan.joins * n_kv * (unsigned)ceil_div(plan.slot_rows, plan.join_passes << plan.join_shift));
   auto join = [&](auto kernel, int threads) { launch_kernel(kernel, joins, dim3(threads), 0, stream, a, plan.rows); };
   if (plan.rows != kManyRows)
     plan.join_wide ? join(join_kernel<false, kJoinWide, 1>, kJoinWide) : join(join_kernel<false, kJoinThreads, 1>, kJoinThreads);

@@ -150,6 +150,8 @@ def test_a_million_rows(gpu, t, n_q):
     (4, 1, 10, [3000], None), (8, 2, 16, [2300, 16, 9], [16, 16, 3]),   # 33..64 rows in two launches
     (4, 1, 20, [9000], None), (2, 1, 33, [8500, 12], [33, 1]),          # .. many parts of them
     (32, 8, 128, [128, 300, 129, 5, 192, 200, 128, 130, 131], [128, 128, 128, 5, 128, 100, 1, 128, 0]),
+    (64, 8, 17, [17 + 11 * i % 150 for i in range(70)], None),          # more items than workers, short and cut ones
+    (32, 8, 150, [150, 700, 151, 0, 160, 170, 155, 900, 150, 180, 200, 151], [150, 150, 9, 0, 150, 1, 150, 150, 40, 150, 150, 150]),
     (4, 4, 1, [33 + 8 * i for i in range(140)], None), (8, 8, 3, [33 + 8 * i for i in range(70)], None),  # whole and cut ones
 ])
 def test_parts(gpu, n_q, n_kv, t, lens, counts):
