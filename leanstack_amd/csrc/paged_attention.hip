@@ -21,7 +21,7 @@
 // 6.0 TB/s, and 4 for the second launch), where there is little to read the chain of lens,
 // table, rows, sums and the second launch (1 request over 32768 rows 17 + 6 us); prompts, the
 // chain of products, exponentials and conversions of two waves that share a SIMD (2 x 1500
-// tokens, the last of 4000 and 7001 rows: 238 us, 980 TFLOP/s, and 15 for the parts' 130 MB).
+// tokens, the last of 4000 and 7001 rows: 238 us, 980 TFLOP/s, and 13 for the parts' 110 MB).
 //
 // Few query rows (decode, verify).  A wave takes two blocks, 32 key rows, a step, for up to
 // 4 x 16 query rows:
