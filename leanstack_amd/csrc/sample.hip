@@ -535,11 +535,13 @@ __device__ __forceinline__ void few_tokens(Shared& s, const Rule& rule, int n, u
   if (in_front <= at && at < in_front + w) write(index_of(mine), w, total);
 }
 
-// Tokens that top-k and min-p may keep are in the first `last` bins or none: where min-p's lowest
-// is (two bins for what the logarithm is off), and where weights vanish.
+// Tokens that top-k and min-p may keep are in the first `last` bins or none: where the lowest lies whose
+// weight rounds up to min-p's least whole units (half a unit less; two bins for what the logarithm is
+// off), and where weights vanish.
 __device__ __forceinline__ int last_bin(float min_p) {
   if (!(min_p > 0.f)) return kLastBin;
-  return (int)fminf((float)kLastBin, 2.f - __log2f(fminf(min_p, 1.f)) * ((float)kBins / kOctaves));
+  const float least = fmaxf(__builtin_ceilf(fminf(min_p, 1.f) * (float)kUnit), 1.f);
+  return (int)fminf((float)kLastBin, 2.f + (44.f - __log2f(least - 0.5f)) * ((float)kBins / kOctaves));
 }
 
 // The bin of the k-th largest of the threads' maxima: at least k values are in it or above.
