@@ -810,7 +810,7 @@ __device__ __forceinline__ QueryParts query_parts(const __bf16* from, const Scal
   top = max(top, (unsigned)__shfl_xor((int)top, 32));
   fine = top < 0x7f80u;
   // the least e with |q| <= 256 2^e, so that no high part rounds past 448
-  const int e = min(max((int)(top >> 7) - 127 - 7, -120), 119);
+  const int e = min(max((int)(top >> 7) - 127 - 7, -120), 120);
   const float factor = power_of_two(-e);
   QueryParts q;
   q.high_scale = e + 127;
