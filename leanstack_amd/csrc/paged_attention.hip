@@ -38,8 +38,11 @@
 // through a ring in LDS, filled by DMA.  K is multiplied as it is, in 8 bits with its
 // scales, on v_mfma_scale_f32_32x32x64_f8f6f4: q, of 8 significant bits, is the sum of two
 // e4m3 numbers of 4, so two products at twice the rate of bf16 give the same scores
-// without converting K (q's parts are exact down to 2^-23 of the row's largest).  V is
-// converted on its way out of LDS for v_mfma_f32_32x32x16_bf16.
+// without converting K.  The two hold a value exactly from 2^-13 of the row's largest power of two
+// on, and smaller ones to 2^-21 of its largest value.  A wave with a row of which more than a few
+// values are that small (or that holds an infinity or a NaN) multiplies bf16 by bf16 instead, K
+// converted, as few query rows do: 2 x 1500 tokens 273 us for 239, so it is not done for the few that
+// a normal row in fifty has.  V is converted on its way out of LDS for v_mfma_f32_32x32x16_bf16.
 //
 // P is rounded to bf16, at most 2^-8 of each weight, and l sums the rounded weights: the
 // result is exactly that of slightly other weights.
@@ -58,6 +61,7 @@ typedef int i32x8_t __attribute__((ext_vector_type(8)));
 typedef float f32x2_t __attribute__((ext_vector_type(2)));
 typedef float f32x4_t __attribute__((ext_vector_type(4)));
 typedef float f32x16_t __attribute__((ext_vector_type(16)));
+typedef unsigned short u16x2_t __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x4_t __attribute__((ext_vector_type(4)));
 
@@ -761,6 +765,7 @@ constexpr int kManyWaves = 4;
 constexpr int kManyRows = 32 * kManyWaves;
 constexpr int kStep = 64;                           // key rows, one block per wave
 constexpr int kRing = 4;
+constexpr int kMostLost = 2;                        // values of half a query row that its two parts may round
 constexpr int kSlot = 2 * 4 * kPagedBlockBytes;     // K, then V, of a step
 static_assert(kManyRows == kPagedManyRows && kStep == kPagedManyUnit, "as the host counts them");
 
@@ -784,31 +789,40 @@ __device__ __forceinline__ u32x4_t lds_16(lds_byte_t* at) {
   return *reinterpret_cast<__attribute__((address_space(3))) const u32x4_t*>(at);
 }
 
-// q as two e4m3 numbers per value: 32 values in units of 2^e, and what they leave in units of 2^(e - 4).
+// A lane's half of a query row: bf16 values 64 k + 32 h + 8 i .. + 7.
+struct Query {
+  u32x4_t w[2][4];
+};
+// ... as two e4m3 numbers per value: 32 values in units of 2^e, and what they leave in units of 2^(e - 4).
 struct QueryParts {
   i32x8_t high[2], low[2];  // dims 64 k + 32 h .. + 31
   int high_scale, low_scale;
 };
 
-__device__ __forceinline__ QueryParts query_parts(const __bf16* from, const Scale& sc) {
-  const int h = (threadIdx.x & 63) >> 5;
-  u32x4_t w[2][4];
-  unsigned top = 0;
-  bool fine = true;
+// The row's largest |q|, as bits (a lane's scale is not for its own 32 values alone: both halves need the same).
+__device__ __forceinline__ unsigned query_top(const Query& q) {
+  u16x2_t top = {0, 0};
 #pragma unroll
-  for (int k = 0; k < 2; ++k)
+  for (int i = 0; i < 32; ++i)
+    top = __builtin_elementwise_max(top, __builtin_bit_cast(u16x2_t, q.w[i / 16][i / 4 % 4][i % 4] & 0x7fff7fffu));
+  const int mine = max(top[0], top[1]);
+  return (unsigned)max(mine, __shfl_xor(mine, 32));
+}
+
+// Whether the parts hold all of the lane's values but kMostLost exactly: the last place of a value of 8 bits is a
+// multiple of their least step, 2^(e - 13), from 2^-13 of the row's largest power of two on.
+__device__ __forceinline__ bool query_fits(const Query& q, unsigned top) {
+  const unsigned short least = (unsigned short)max((int)(top & 0x7f80u) - (13 << 7) - 1, 0);
+  u16x2_t lost = {0, 0};
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      w[k][i] = *reinterpret_cast<const u32x4_t*>(from + 64 * k + 32 * h + 8 * i);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const unsigned lo = w[k][i][e] & 0x7fffu, hi = (w[k][i][e] >> 16) & 0x7fffu;
-        top = max(top, max(lo, hi));
-        w[k][i][e] = scaled_bits(w[k][i][e], sc);
-      }
-    }
-  top = max(top, (unsigned)__shfl_xor((int)top, 32));
-  fine = top < 0x7f80u;
+  for (int i = 0; i < 32; ++i) {
+    const u16x2_t below = __builtin_bit_cast(u16x2_t, q.w[i / 16][i / 4 % 4][i % 4] & 0x7fff7fffu) - u16x2_t{1, 1};  // (of zeros: above all)
+    lost += __builtin_elementwise_min(__builtin_elementwise_sub_sat(u16x2_t{least, least}, below), u16x2_t{1, 1});
+  }
+  return top < 0x7f80u && lost[0] + lost[1] <= kMostLost;
+}
+
+__device__ __forceinline__ QueryParts query_parts(const Query& query, unsigned top) {
   // the least e with |q| <= 256 2^e, so that no high part rounds past 448
   const int e = min(max((int)(top >> 7) - 127 - 7, -120), 120);
   const float factor = power_of_two(-e);
@@ -819,7 +833,7 @@ __device__ __forceinline__ QueryParts query_parts(const __bf16* from, const Scal
   for (int k = 0; k < 2; ++k)
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const unsigned w0 = w[k][i >> 1][2 * (i & 1)], w1 = w[k][i >> 1][2 * (i & 1) + 1];
+      const unsigned w0 = query.w[k][i >> 1][2 * (i & 1)], w1 = query.w[k][i >> 1][2 * (i & 1) + 1];
       float x[4] = {__builtin_bit_cast(float, w0 << 16), __builtin_bit_cast(float, w0 & 0xffff0000u),
                     __builtin_bit_cast(float, w1 << 16), __builtin_bit_cast(float, w1 & 0xffff0000u)};
 #pragma unroll
@@ -829,9 +843,8 @@ __device__ __forceinline__ QueryParts query_parts(const __bf16* from, const Scal
       const f32x2_t a = __builtin_amdgcn_cvt_pk_f32_fp8(high, false), b = __builtin_amdgcn_cvt_pk_f32_fp8(high, true);
       int low = __builtin_amdgcn_cvt_pk_fp8_f32((x[0] - a[0]) * 16.f, (x[1] - a[1]) * 16.f, 0, false);
       low = __builtin_amdgcn_cvt_pk_fp8_f32((x[2] - b[0]) * 16.f, (x[3] - b[1]) * 16.f, low, true);
-      // (a query with an infinity or a NaN has no finite score: NaN)
-      q.high[k][i] = fine ? high : 0x7f7f7f7f;
-      q.low[k][i] = fine ? low : 0;
+      q.high[k][i] = high;
+      q.low[k][i] = low;
     }
   return q;
 }
@@ -861,6 +874,19 @@ __device__ __forceinline__ f32x16_t many_scores(const Keys& keys, const QueryPar
     s = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(keys.k[k], q.low[k], s, 0, 0, 0, scale, 0, q.low_scale);
     s = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(keys.k[k], q.high[k], s, 0, 0, 0, scale, 0, q.high_scale);
   }
+  return s;
+}
+
+// The same with the query as it is.
+__device__ __forceinline__ f32x16_t many_scores(const Keys& keys, const Query& q, int scale) {
+  const float ks = power_of_two(scale - 127);
+  f32x16_t s = {};
+#pragma unroll
+  for (int k = 0; k < 2; ++k)
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(eight((unsigned)keys.k[k][2 * i], (unsigned)keys.k[k][2 * i + 1], ks, ks),
+                                                  __builtin_bit_cast(bf16x8_t, q.w[k][i]), s, 0, 0, 0);
   return s;
 }
 
@@ -950,7 +976,18 @@ __device__ __forceinline__ void many_rows(const PagedAttentionArgs& a, ManyShare
   // (the wave's first row sees the fewest)
   const int least = rq.visible(min(tile * kManyRows + 32 * wave, rows - 1) / a.G);
   const Scale sc = scale_of(a.scale);
-  const QueryParts q = query_parts(a.q + (size_t)b * a.q_b + (size_t)head * a.q_h + (size_t)t * a.q_t, sc);
+  Query query;
+  const __bf16* from = a.q + (size_t)b * a.q_b + (size_t)head * a.q_h + (size_t)t * a.q_t + 32 * h;
+#pragma unroll
+  for (int k = 0; k < 2; ++k)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      query.w[k][i] = *reinterpret_cast<const u32x4_t*>(from + 64 * k + 8 * i);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) query.w[k][i][e] = scaled_bits(query.w[k][i][e], sc);
+    }
+  const unsigned top = query_top(query);
+  const bool wide = __ballot(!query_fits(query, top)) != 0;
   bool any = false;
   ManyState st;
   st.sums = no_sums(sc.c2);
@@ -992,7 +1029,7 @@ __device__ __forceinline__ void many_rows(const PagedAttentionArgs& a, ManyShare
     asm volatile("s_waitcnt vmcnt(4) lgkmcnt(0)\n\ts_barrier" ::: "memory");
     load(step + 2, (step - first_step + 2) & (kRing - 1));
   };
-  if (first_step < stop) {
+  auto steps = [&](const auto& q) __attribute__((always_inline)) {
     load(first_step, 0);
     load(first_step + 1, 1);
     begin_step(first_step);
@@ -1070,6 +1107,12 @@ __device__ __forceinline__ void many_rows(const PagedAttentionArgs& a, ManyShare
         s = then;
       }
     }
+  };
+  if (first_step < stop) {
+    if (wide)
+      steps(query);
+    else
+      steps(query_parts(query, top));
   }
   asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
 
