@@ -82,7 +82,7 @@ class PagedKVCache:
         self.page_rows = page_blocks * BLOCK_ROWS
         self._holders = [0] * self.num_pages
         self._free = list(range(self.num_pages - 1, -1, -1))  # the lowest is taken first
-        self._requests: list[Request] = []
+        self._requests: dict[int, Request] = {}  # the open ones, by id()
 
     # -- pages ------------------------------------------------------------------
 
@@ -96,13 +96,13 @@ class PagedKVCache:
 
     def _known(self, requests: list[Request]) -> None:
         for r in requests:
-            if not any(r is known for known in self._requests):
+            if self._requests.get(id(r)) is not r:
                 raise ValueError("the request is not open in this cache")
 
     def open(self) -> Request:
         """A request without rows."""
         r = Request()
-        self._requests.append(r)
+        self._requests[id(r)] = r
         return r
 
     def close(self, request: Request) -> None:
@@ -110,7 +110,7 @@ class PagedKVCache:
         self._known([request])
         self._release(request.pages)
         request.pages, request.rows = [], 0
-        self._requests = [r for r in self._requests if r is not request]
+        del self._requests[id(request)]
 
     def _release(self, pages: list[int]) -> None:
         freed = False
@@ -224,7 +224,7 @@ class PagedKVCache:
         self._copy(moved, holes)
         for old, page in names.items():
             self._holders[page], self._holders[old] = self._holders[old], 0
-        for r in self._requests:
+        for r in self._requests.values():
             r.pages = [names.get(page, page) for page in r.pages]
         self._free = list(range(self.num_pages - 1, used - 1, -1))
         return used
