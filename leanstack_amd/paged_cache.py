@@ -259,12 +259,21 @@ class PagedKVCache:
 
     def export(self, request: Request, cache) -> None:
         """The request's rows appended to an ArenaKVCache (exact: stored values are bf16
-        numbers), for a request that goes on alone in a captured decode step."""
+        numbers), for a request that goes on alone in a captured decode step.  Nothing is
+        written if they do not fit."""
         from . import kernels
         self._known([request])
+        layers, _, heads, capacity, dim = cache.storage.shape
+        if (layers, heads, dim) != (self.num_layers, self.num_key_value_heads, HEAD_DIM):
+            raise ValueError(f"a cache of {self.num_layers} layers and {self.num_key_value_heads} kv heads of {HEAD_DIM} is "
+                             f"needed, got {layers} layers and {heads} heads of {dim}")
+        for layer, rows in enumerate(cache.layer_seq_lens):
+            if rows + request.rows > capacity:
+                raise ValueError(f"layer {layer}: {rows} + {request.rows} rows have no room in {capacity}")
+        if not request.rows:
+            return
         table, lens = self.batch([request])
         starts = torch.zeros_like(lens)
-        if request.rows:
-            for layer in range(self.num_layers):
-                keys, values = kernels.paged_read(self, layer, table, starts, request.rows, lens=lens)
-                cache.write_rows(layer, keys, values)
+        for layer in range(self.num_layers):
+            keys, values = kernels.paged_read(self, layer, table, starts, request.rows, lens=lens)
+            cache.write_rows(layer, keys, values)
