@@ -44,8 +44,9 @@
 // converted, as few query rows do: 2 x 1500 tokens 273 us for 239, so it is not done for the few that
 // a normal row in fifty has.  V is converted on its way out of LDS for v_mfma_f32_32x32x16_bf16.
 //
-// P is rounded to bf16, at most 2^-8 of each weight, and l sums the rounded weights: the
-// result is exactly that of slightly other weights.
+// P: up to 16 query rows (single tokens) two bf16 numbers a weight, the second what the first leaves,
+// 2^-16 of it at most; with more of them one, 2^-8 at most: a second product would be as long as the
+// first.  l sums what is multiplied, so the result is exactly that of slightly other weights.
 
 #include <hip/hip_runtime.h>
 
@@ -303,9 +304,13 @@ __device__ __forceinline__ u32x4_t load_1k(const unsigned char* blocks, int at, 
   return __builtin_bit_cast(u32x4_t, __builtin_amdgcn_raw_buffer_load_b128(block, (threadIdx.x & 63) * 16, half * 1024, kStream));
 }
 
-// The weights P of a step as the operand of the second product, and m, l, O brought to
+// The weights P of a step as operands of the second product, and m, l, O brought to
 // the new maximum.  s[m][i]: row 16 m + 4 g + i of the step, -inf where it is not seen.
-__device__ __forceinline__ bf16x8_t step_weights(const f32x4_t (&s)[2], float c2, State& st) {
+struct Weights {
+  bf16x8_t high, low;  // low: what high leaves of them
+};
+template <bool FINE>
+__device__ __forceinline__ Weights step_weights(const f32x4_t (&s)[2], float c2, State& st) {
   float top = fmaxf(s[0][0], s[0][1]);
 #pragma unroll
   for (int i = 2; i < 8; ++i) top = fmaxf(top, s[i / 4][i % 4]);
@@ -316,14 +321,19 @@ __device__ __forceinline__ bf16x8_t step_weights(const f32x4_t (&s)[2], float c2
 #pragma unroll
       for (int e = 0; e < 4; ++e) st.o[i][e] *= f;
   }
-  bf16x8_t p;
+  Weights p;
 #pragma unroll
-  for (int i = 0; i < 8; ++i)
-    p[i] = static_cast<__bf16>(__builtin_amdgcn_exp2f(__builtin_fmaf(s[i / 4][i % 4], st.sums.c2, -st.sums.m)));
+  for (int i = 0; i < 8; ++i) {
+    const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i / 4][i % 4], st.sums.c2, -st.sums.m));
+    p.high[i] = static_cast<__bf16>(w);
+    if constexpr (FINE) p.low[i] = static_cast<__bf16>(w - static_cast<float>(p.high[i]));
+  }
   const bf16x2_t ones = {static_cast<__bf16>(1.f), static_cast<__bf16>(1.f)};
 #pragma unroll
-  for (int i = 0; i < 8; i += 2)
-    st.sums.l = __builtin_amdgcn_fdot2_f32_bf16(bf16x2_t{p[i], p[i + 1]}, ones, st.sums.l, false);
+  for (int i = 0; i < 8; i += 2) {
+    st.sums.l = __builtin_amdgcn_fdot2_f32_bf16(bf16x2_t{p.high[i], p.high[i + 1]}, ones, st.sums.l, false);
+    if constexpr (FINE) st.sums.l = __builtin_amdgcn_fdot2_f32_bf16(bf16x2_t{p.low[i], p.low[i + 1]}, ones, st.sums.l, false);
+  }
   return p;
 }
 
@@ -355,6 +365,12 @@ __device__ __forceinline__ int own_thread() {
   asm volatile("" : "+v"(tid));
   return tid;
 }
+
+// The weights as two bf16 numbers, not one.  The second product of 16 query rows runs while the next rows are on their
+// way: 1 request over 900 rows 10.1 us for 9.5, 64 over 17..8001 95 for 94; of 32 rows it would not (24 x 5 tokens over
+// 5..3001 rows 29.5 us for 27.3, 8 x 8 over 8192 38.8 for 36.3).
+template <int NT>
+constexpr bool kFine = NT == 1;
 
 // Query rows of more than one tile are kept in LDS (16 registers each).
 template <int NT>
@@ -483,9 +499,9 @@ __device__ __forceinline__ void few_steps(const PagedAttentionArgs& a, Queries<N
 #pragma unroll
         for (int n = 0; n < NT; ++n) any[n] = true;
       }
-      bf16x8_t w[NT];
+      Weights w[NT];
 #pragma unroll
-      for (int n = 0; n < NT; ++n) w[n] = step_weights(s[n], sc.c2, st[n]);
+      for (int n = 0; n < NT; ++n) w[n] = step_weights<kFine<NT>>(s[n], sc.c2, st[n]);
       if (masked) {
         // A weight of zero does not take a NaN out of a product: those become zero here and
         // come back for the query rows that see them.
@@ -525,8 +541,10 @@ __device__ __forceinline__ void few_steps(const PagedAttentionArgs& a, Queries<N
       for (int d = 0; d < 8; ++d) {
         const bf16x8_t value = eight(vq[0][d & 1][d >> 1], vq[1][d & 1][d >> 1], vs[0], vs[1]);
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
-          st[n].o[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(value, w[n], st[n].o[d], 0, 0, 0);
+        for (int n = 0; n < NT; ++n) {
+          if constexpr (kFine<NT>) st[n].o[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(value, w[n].low, st[n].o[d], 0, 0, 0);
+          st[n].o[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(value, w[n].high, st[n].o[d], 0, 0, 0);
+        }
       }
       load_v(i + kAhead, vq);
     };
