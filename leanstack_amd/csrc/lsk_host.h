@@ -216,6 +216,8 @@ constexpr PagedPlan paged_plan(int B, int T, int n_q, int n_kv, int capacity) {
   p.join_passes = many && p.join_shift == 4 && p.joins * n_kv * ((p.slot_rows + 15) / 16) > kPagedJoinGroups ? kPagedJoinPasses : 1;
   return p;
 }
+static_assert(paged_plan(1, 64, 1, 1, 64).tiles == 1 && paged_plan(600, 16, 4, 1, 64).tiles == 1 && paged_plan(1, 17, 1, 1, 1 << 20).tiles == 1,
+              "up to 64 query rows are one item: the kernels for few have no tiles");
 // (m, l) and O of every slot, and where the items begin and which of 128 rows are cut.
 constexpr unsigned long long paged_begins_bytes(const PagedPlan& p) {
   const unsigned long long words = (unsigned long long)p.items + 1 + (p.rows == kPagedManyRows ? (unsigned long long)p.workers : 0);

@@ -107,19 +107,24 @@ __device__ __forceinline__ Request request_of(const PagedAttentionArgs& a, int b
   return {max(a.lens[b], 0), a.counts ? min(max(a.counts[b], 0), a.T) : a.T, 16 * a.pool.blocks};
 }
 
-// Query rows r0 .. + ROWS - 1 of request b: rows that the last one sees.
-template <int ROWS>
-__device__ __forceinline__ int item_rows(const PagedAttentionArgs& a, const Request& q, int tile) {
-  if (a.tiles == 1) return q.count > 0 ? q.visible(a.T - 1) : 0;
-  const int r0 = tile * ROWS;
-  if (q.count <= r0 / a.G) return 0;
-  return q.visible((min(r0 + ROWS, a.T * a.G) - 1) / a.G);
+// An item's request.  Up to 64 query rows are one item (paged_plan).
+template <bool MANY>
+__device__ __forceinline__ int request_at(const PagedAttentionArgs& a, int item) {
+  return !MANY || a.tiles == 1 ? item : item / a.tiles;
 }
-template <int ROWS>
+// The rows that the last query row of a tile of a request sees.
+template <bool MANY>
+__device__ __forceinline__ int item_rows(const PagedAttentionArgs& a, const Request& q, int tile) {
+  if (!MANY || a.tiles == 1) return q.count > 0 ? q.visible(a.T - 1) : 0;
+  const int r0 = tile * kPagedManyRows;
+  if (q.count <= r0 / a.G) return 0;
+  return q.visible((min(r0 + kPagedManyRows, a.T * a.G) - 1) / a.G);
+}
+template <bool MANY>
 __device__ __forceinline__ int item_units(const PagedAttentionArgs& a, int item) {
-  constexpr int kUnit = ROWS == kPagedManyRows ? kPagedManyUnit : kPagedFewUnit;
-  const int b = a.tiles == 1 ? item : item / a.tiles;
-  return max((item_rows<ROWS>(a, request_of(a, b), item - b * a.tiles) + kUnit - 1) / kUnit, 1);
+  constexpr int kUnit = MANY ? kPagedManyUnit : kPagedFewUnit;
+  const int b = request_at<MANY>(a, item);
+  return max((item_rows<MANY>(a, request_of(a, b), MANY ? item - b * a.tiles : 0) + kUnit - 1) / kUnit, 1);
 }
 
 // Inclusive sums over a wave's lanes.
@@ -180,18 +185,17 @@ struct Chunk {
   int item, first, last;
   bool whole;
 };
-template <int ROWS>
 __device__ __forceinline__ Chunk chunk_of(const PagedAttentionArgs& a, int w, bool write) {
-  auto units_of = [&](int i) { return item_units<ROWS>(a, i); };
+  auto units_of = [&](int i) { return item_units<false>(a, i); };
   const int total = __builtin_amdgcn_readlane(wave_sums(lane_items(a, units_of)), 63);
   const int most = max((total + a.places - 1) / a.places, a.least_units);  // units of a chunk
-  auto chunks_of = [&](int i) { return (item_units<ROWS>(a, i) + most - 1) / most; };
+  auto chunks_of = [&](int i) { return (item_units<false>(a, i) + most - 1) / most; };
   const int mine = lane_items(a, chunks_of), up_to = wave_sums(mine);
   const int chunks = __builtin_amdgcn_readlane(up_to, 63);
   if (write) write_begins(a, up_to - mine, chunks, chunks_of);
   if (w >= chunks) return {0, 0, 0, false};
   const Found f = item_at(a, w, mine, up_to - mine, chunks_of);
-  const int units = item_units<ROWS>(a, f.item), n = (units + most - 1) / most;
+  const int units = item_units<false>(a, f.item), n = (units + most - 1) / most;
   const int each = (units + n - 1) / n;  // (at most `most`: none of the n is empty)
   const int first = (w - f.begin) * each;
   return {f.item, first, min(first + each, units), n == 1};
@@ -207,9 +211,8 @@ struct Share {
   int item, skip, places;
   bool cuts;
 };
-template <int ROWS>
 __device__ __forceinline__ Share share_of(const PagedAttentionArgs& a, int w, bool write) {
-  auto places_of = [&](int i) { return item_units<ROWS>(a, i) + kPagedManyStart; };
+  auto places_of = [&](int i) { return item_units<true>(a, i) + kPagedManyStart; };
   const int mine = lane_items(a, places_of), up_to = wave_sums(mine);
   const int total = __builtin_amdgcn_readlane(up_to, 63);
   if (write) write_begins(a, up_to - mine, total, places_of);
@@ -367,7 +370,7 @@ __device__ __forceinline__ int own_thread() {
 }
 
 // The weights as two bf16 numbers, not one.  The second product of 16 query rows runs while the next rows are on their
-// way: 1 request over 900 rows 10.1 us for 9.5, 64 over 17..8001 95 for 94; of 32 rows it would not (24 x 5 tokens over
+// way: 1 request over 900 rows 10.0 us for 9.5, 64 over 17..8001 95 for 94; of 32 rows it would not (24 x 5 tokens over
 // 5..3001 rows 29.5 us for 27.3, 8 x 8 over 8192 38.8 for 36.3).
 template <int NT>
 constexpr bool kFine = NT == 1;
@@ -380,18 +383,18 @@ struct Queries {
   u32x4_t q[kQueriesInLds<NT> ? NT : 1][4][64];
 };
 
-// A wave's steps first_step + i NW (up to stop_step), i = 0, 1, .., for query rows 16 NT tile .. of
+// A wave's steps first_step + i NW (up to stop_step), i = 0, 1, .., for the query rows of
 // kv head j of request b.  any[n]: whether the lane has met a row that its query row sees.
 template <int NT, int NW>
-__device__ __forceinline__ void few_steps(const PagedAttentionArgs& a, Queries<NT>& lds, int j, int b, int tile, int first_step,
-                                          int stop_step, const Request& rq, State (&st)[NT], bool (&any)[NT]) {
+__device__ __forceinline__ void few_steps(const PagedAttentionArgs& a, Queries<NT>& lds, int j, int b, int first_step, int stop_step,
+                                          const Request& rq, State (&st)[NT], bool (&any)[NT]) {
   constexpr bool kInLds = kQueriesInLds<NT>;
   constexpr int kAhead = NT > 2 ? 1 : 2;  // steps on their way
   const PagedPool& p = a.pool;
   const int lane = own_thread() & 63, c = lane & 15, g = lane >> 4;
-  const int r0 = tile * 16 * NT, rows = a.T * a.G;
-  const int least = rq.count > r0 / a.G ? rq.visible(r0 / a.G) : 0;
-  const int end_block = (item_rows<16 * NT>(a, rq, tile) + 15) / 16, stop = min(stop_step, (end_block + 1) / 2);
+  const int rows = a.T * a.G;
+  const int least = rq.count > 0 ? rq.visible(0) : 0;
+  const int end_block = (item_rows<false>(a, rq, 0) + 15) / 16, stop = min(stop_step, (end_block + 1) / 2);
   // 32 steps' blocks in the lanes at a time; the first steps' rows are on their way before anything else.
   Blocks blocks;
   int here = 0;
@@ -431,7 +434,7 @@ __device__ __forceinline__ void few_steps(const PagedAttentionArgs& a, Queries<N
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
     any[n] = false;
-    const int r = min(r0 + 16 * n + c, rows - 1);
+    const int r = min(16 * n + c, rows - 1);
     const int t = r / a.G, h = j * a.G + r % a.G;
     limit[n] = rq.visible(t);
     st[n].sums = no_sums(sc.c2);
@@ -567,18 +570,18 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void few_attention_kernel(PagedA
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int j = blockIdx.x % a.pool.n_kv, w = (blockIdx.x / a.pool.n_kv) * kFewWaves + wave;
   if (w >= a.workers) return;
-  const Chunk ch = chunk_of<16 * NT>(a, w, j == 0 && w == 0);
+  const Chunk ch = chunk_of(a, w, j == 0 && w == 0);
   if (ch.first == ch.last) return;
-  const int b = a.tiles == 1 ? ch.item : ch.item / a.tiles, tile = ch.item - b * a.tiles;
+  const int b = ch.item;
   State st[NT];
   bool any[NT];
   const Request rq = request_of(a, b);
-  few_steps<NT, 1>(a, queries[wave], j, b, tile, ch.first, ch.last, rq, st, any);
+  few_steps<NT, 1>(a, queries[wave], j, b, ch.first, ch.last, rq, st, any);
   const int lane = own_thread() & 63, c = lane & 15, g = lane >> 4;
   const Part part = part_of(a, (size_t)j * a.workers + w);
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
-    const int r = 16 * n + c, row = tile * 16 * NT + r;
+    const int row = 16 * n + c;
     const float l = rows_sum(st[n].sums.l);
     const bool met = met_any(any[n], c);
     if (row >= a.T * a.G) continue;
@@ -595,15 +598,15 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void few_attention_kernel(PagedA
         *reinterpret_cast<bf16x4_t*>(out + 16 * d) = o;
       }
     } else {
-      float* out = part.o + (size_t)r * D + 4 * g;
+      float* out = part.o + (size_t)row * D + 4 * g;
 #pragma unroll
       for (int d = 0; d < 8; ++d) *reinterpret_cast<f32x4_t*>(out + 16 * d) = st[n].o[d];
-      if (g == 0) *reinterpret_cast<f32x2_t*>(part.ml + r * 2) = f32x2_t{met ? st[n].sums.m : neg_inf(), l};
+      if (g == 0) *reinterpret_cast<f32x2_t*>(part.ml + row * 2) = f32x2_t{met ? st[n].sums.m : neg_inf(), l};
     }
   }
 }
 
-// One launch, an item per workgroup whose waves take its steps by turns.  Grid: kv head (fastest), item.
+// One launch, an item per workgroup whose waves take its steps by turns.  Grid: kv head (fastest), request.
 template <int NT>
 __global__ __launch_bounds__(64 * kShortWaves, 2) void short_attention_kernel(PagedAttentionArgs a) {
   constexpr int NW = kShortWaves;
@@ -613,12 +616,11 @@ __global__ __launch_bounds__(64 * kShortWaves, 2) void short_attention_kernel(Pa
   } sh;
   __shared__ float ms[NW][16], ls[NW][16];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int j = blockIdx.x % a.pool.n_kv, item = blockIdx.x / a.pool.n_kv;
-  const int b = a.tiles == 1 ? item : item / a.tiles, tile = item - b * a.tiles;
+  const int j = blockIdx.x % a.pool.n_kv, b = blockIdx.x / a.pool.n_kv;
   State st[NT];
   bool any[NT];
   const Request rq = request_of(a, b);
-  few_steps<NT, NW>(a, sh.queries[wave], j, b, tile, wave, 1 << 26, rq, st, any);
+  few_steps<NT, NW>(a, sh.queries[wave], j, b, wave, 1 << 26, rq, st, any);
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
     __syncthreads();  // the queries, or the last tile's sums, have been read
@@ -638,7 +640,7 @@ __global__ __launch_bounds__(64 * kShortWaves, 2) void short_attention_kernel(Pa
     // 32 lanes to a query row, 4 dims each
     static_assert(NW * 64 == 16 * 32, "lanes to a query row");
     const int r = tid >> 5, d0 = (tid & 31) * 4;
-    const int row = (tile * NT + n) * 16 + r;
+    const int row = n * 16 + r;
     if (row < a.T * a.G) {
       const int t = row / a.G, h = j * a.G + row % a.G;
       float m = neg_inf(), sum = 0.f, w[NW];
@@ -692,7 +694,7 @@ __global__ __launch_bounds__(THREADS) void join_kernel(PagedAttentionArgs a, int
     from = worker_of(begin + kPagedManyStart), last = worker_of(end - 1);
   }
   if (from == last) return;
-  const int b = a.tiles == 1 ? item : item / a.tiles, tile = item - b * a.tiles;
+  const int b = request_at<MANY>(a, item), tile = MANY ? item - b * a.tiles : 0;
   const int slot = threadIdx.x >> 4, d0 = (threadIdx.x & 15) * 8;
   const int stream = slot >> a.join_shift;
   const int r0 = group * own * PASSES + (slot & (own - 1)), end_row = min(rows, a.T * a.G - tile * rows);
@@ -986,7 +988,7 @@ __device__ __forceinline__ void many_rows(const PagedAttentionArgs& a, ManyShare
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int rows = a.T * a.G, row = tile * kManyRows + 32 * wave + c;
   const Request rq = request_of(a, b);
-  const int most = item_rows<kManyRows>(a, rq, tile);
+  const int most = item_rows<true>(a, rq, tile);
   const int end_block = (most + 15) / 16;
   const int stop = min(stop_step, (end_block + 3) / 4);
   const int t = min(row, rows - 1) / a.G, head = j * a.G + min(row, rows - 1) % a.G;
@@ -1167,12 +1169,12 @@ __device__ __forceinline__ void many_rows(const PagedAttentionArgs& a, ManyShare
 __global__ __launch_bounds__(64 * kManyWaves, 2) void many_attention_kernel(PagedAttentionArgs a) {
   __shared__ __align__(1024) ManyShared sh;
   const int j = blockIdx.x % a.pool.n_kv, w = blockIdx.x / a.pool.n_kv;
-  const Share s = share_of<kManyRows>(a, w, blockIdx.x == 0 && threadIdx.x < 64);
+  const Share s = share_of(a, w, blockIdx.x == 0 && threadIdx.x < 64);
   if (j == 0 && threadIdx.x == 0) a.cuts[w] = s.cuts ? s.item : -1;
   int item = s.item, skip = s.skip, left = s.places;
   while (left > 0) {
-    const int b = a.tiles == 1 ? item : item / a.tiles;
-    const int units = item_units<kManyRows>(a, item);
+    const int b = request_at<true>(a, item);
+    const int units = item_units<true>(a, item);
     const int stop = min(skip + left, units + kPagedManyStart);
     const int first = max(skip - kPagedManyStart, 0), last = stop - kPagedManyStart;
     if (first < last)
