@@ -615,7 +615,7 @@ def _pool(cache: PagedKVCache, layer: int, table: torch.Tensor) -> tuple[_lib.Pa
                           stride), b, index
 
 
-def _head_rows(x: torch.Tensor, what: str) -> tuple[torch.Tensor, tuple[int, ...]]:
+def _head_rows(x: torch.Tensor) -> tuple[torch.Tensor, tuple[int, ...]]:
     """x [B, heads, T, d] as the paged kernels read it in place, copied if they cannot, and its strides."""
     strides = x.stride()
     if strides[3] != 1 or (strides[0] | strides[1] | strides[2]) & 7 or x.data_ptr() % 16:
@@ -648,8 +648,8 @@ def paged_append(cache: PagedKVCache, layer: int, k: torch.Tensor, v: torch.Tens
     t = k.shape[2]
     if b * t == 0:
         return
-    k, ks = _head_rows(k, "k")
-    v, vs = _head_rows(v, "v")
+    k, ks = _head_rows(k)
+    v, vs = _head_rows(v)
     with _on_index(index):
         status = _lib.load().lsk_paged_append_bf16(
             ctypes.byref(pool), k.data_ptr(), ks[0], ks[1], ks[2], v.data_ptr(), vs[0], vs[1], vs[2], b, t, lens_at,
@@ -738,7 +738,7 @@ def paged_attention(q: torch.Tensor, cache: PagedKVCache, layer: int, table: tor
         out = q.new_empty((b, t, n_q * 128))
     if b * t == 0:
         return out
-    q, qs = _head_rows(q, "q")
+    q, qs = _head_rows(q)
     nbytes = _paged_workspace_bytes(b, t, n_q, n_kv, table.shape[1] * cache.page_rows)
     workspace = q.new_empty((nbytes // 2,)) if nbytes else None
     with _on_index(index):
