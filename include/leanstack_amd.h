@@ -446,7 +446,7 @@ int lsk_constrain_logits(const void* logits, int logits_mode, int M, int V, long
                          void* out, long long* tokens, void* workspace, size_t ws_bytes, void* hip_stream);
 
 /* Device workspace of lsk_sample_logits (any contents; 0: none, or sizes that it refuses): few rows
- * without top_k and min_p are worked on by several workgroups each.  by_*: whether the
+ * are worked on by several workgroups each, with top_k or min_p only long ones.  by_*: whether the
  * argument is given. */
 size_t lsk_sample_workspace_bytes(int logits_mode, int M, int V, int by_top_k, int by_top_p, int by_min_p);
 
