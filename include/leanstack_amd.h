@@ -545,9 +545,7 @@ size_t lsk_paged_attention_workspace_bytes(int B, int T, int n_q, int n_kv, int 
  *   out[b][t][h][d] = softmax(scale * q K^T) V,  q head h reading kv head h / (n_q / n_kv);
  * scores, maxima and sums in fp32, the weights of V rounded to 16 significant bits with up to 16
  * query rows T * n_q / n_kv, to bf16 with more, and normalised by the sum of the rounded ones, bf16
- * output.  Products are of q's and the cache's values as they are, but
- * with more than 32 query rows T * n_q / n_kv up to 4 of a query's 128 values may be off by
- * 2^-21 of its largest.  Query tokens from counts[b] on, and those that see
+ * output.  Query tokens from counts[b] on, and those that see
  * no row, give zeros; one whose rows all score -inf gives NaN.  Weights reach 2^12 before they
  * are normalised: over n rows, finite values above 2^115 / n may give infinities.
  *   q          device bf16, [d] at q + b * q_batch_stride + h * q_head_stride + t *

@@ -163,8 +163,8 @@ constexpr int paged_windows(int rows) { return (int)(((long long)rows + 2 * kPag
 //   more with a row (24 x 5 tokens over 2000 rows: 24 us, with 2048 waves 26, with 512 37).
 //   Chunks of 4 units: 1 request over 8192 rows 13.5 us, of 2 15.3, of 8 15.6.
 // - More are taken 128 at a time by workgroups of which `workers` per kv head share all units,
-//   512 in all (256 were 342 us for 276 in prompts of 1500 tokens).  Also 33..64 rows: 8 x 16
-//   tokens over 8192 rows 55 us, 71 by waves of 64 rows.
+//   512 in all (256 were 313 us for 260 in 2 x 1500 tokens over 5500 rows).  Also 33..64 rows: 8 x 16
+//   tokens over 8192 rows 59 us, 71 by waves of 64 rows.
 // The second launch adds up parts, 2^join_shift query rows to a workgroup; with more parts than
 // its threads can take at once it has fewer rows (1 request over 32768 rows, 256 parts: 6.4 us, 39
 // with 16 rows); with many query rows more of them, `join_passes` times, so that fewer
@@ -175,7 +175,7 @@ constexpr int kPagedFewUnit = 32;
 constexpr int kPagedManyUnit = 64;
 constexpr int kPagedManyRows = 128;
 // Units that an item's beginning (lens, table, exponents, first rows, one behind the other) and end
-// take as long as: 4 prompts of 2000 tokens, whose first items are short, 176 us, 268 counting none.
+// take as long as: 4 prompts of 2000 tokens, whose first items are short, 184 us, 253 counting none.
 constexpr int kPagedManyStart = 6;
 constexpr int kPagedShortRows = 2048, kPagedShortFewRows = 1536, kPagedShortFewGroups = 128, kPagedShortGroups = 512;
 constexpr int kPagedJoinGroups = 2048, kPagedJoinPasses = 2;

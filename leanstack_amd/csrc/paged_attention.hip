@@ -21,7 +21,7 @@
 // 6.0 TB/s, and 4 for the second launch), where there is little to read the chain of lens,
 // table, rows, sums and the second launch (1 request over 32768 rows 17 + 6 us); prompts, the
 // chain of products, exponentials and conversions of two waves that share a SIMD (2 x 1500
-// tokens, the last of 4000 and 7001 rows: 238 us, 980 TFLOP/s, and 13 for the parts' 110 MB).
+// tokens, the last of 4000 and 7001 rows: 261 us, 897 TFLOP/s, and 13 for the parts' 110 MB).
 //
 // Few query rows (decode, verify).  A wave takes two blocks, 32 key rows, a step, for up to
 // 4 x 16 query rows:
@@ -35,14 +35,11 @@
 // Nothing goes through LDS but the waves' sums at the end.
 //
 // Many query rows (prompts).  Four waves of 32 query rows share the key rows of a step (64)
-// through a ring in LDS, filled by DMA.  K is multiplied as it is, in 8 bits with its
-// scales, on v_mfma_scale_f32_32x32x64_f8f6f4: q, of 8 significant bits, is the sum of two
-// e4m3 numbers of 4, so two products at twice the rate of bf16 give the same scores
-// without converting K.  The two hold a value exactly from 2^-13 of the row's largest power of two
-// on, and smaller ones to 2^-21 of its largest value.  A wave with a row of which more than a few
-// values are that small (or that holds an infinity or a NaN) multiplies bf16 by bf16 instead, K
-// converted, as few query rows do: 2 x 1500 tokens 273 us for 239, so it is not done for the few that
-// a normal row in fifty has.  V is converted on its way out of LDS for v_mfma_f32_32x32x16_bf16.
+// through a ring in LDS, filled by DMA.  K and V are converted on their way out of LDS, each wave for
+// itself, for v_mfma_f32_32x32x16_bf16.  (K as it is stored, against q as the sum of two e4m3 numbers on
+// v_mfma_scale_f32_32x32x64_f8f6f4, takes as long on the matrix units and saves the conversion: 239 us for the 264 of
+// 2 x 1500 tokens over 4000 and 7001 rows.  But that instruction drops of eight products what is below 2^-13 of the largest, where
+// the bf16 one keeps 24 bits: scores were off by hundredths beside a few large dims.)
 //
 // P: up to 16 query rows (single tokens) two bf16 numbers a weight, the second what the first leaves,
 // 2^-16 of it at most; with more of them one, 2^-8 at most: a second product would be as long as the
@@ -58,11 +55,9 @@ namespace lsk {
 namespace {
 
 typedef unsigned u32x4_t __attribute__((ext_vector_type(4)));
-typedef int i32x8_t __attribute__((ext_vector_type(8)));
 typedef float f32x2_t __attribute__((ext_vector_type(2)));
 typedef float f32x4_t __attribute__((ext_vector_type(4)));
 typedef float f32x16_t __attribute__((ext_vector_type(16)));
-typedef unsigned short u16x2_t __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x4_t __attribute__((ext_vector_type(4)));
 
@@ -785,7 +780,6 @@ constexpr int kManyWaves = 4;
 constexpr int kManyRows = 32 * kManyWaves;
 constexpr int kStep = 64;                           // key rows, one block per wave
 constexpr int kRing = 4;
-constexpr int kMostLost = 2;                        // values of half a query row that its two parts may round
 constexpr int kSlot = 2 * 4 * kPagedBlockBytes;     // K, then V, of a step
 static_assert(kManyRows == kPagedManyRows && kStep == kPagedManyUnit, "as the host counts them");
 
@@ -809,69 +803,14 @@ __device__ __forceinline__ u32x4_t lds_16(lds_byte_t* at) {
   return *reinterpret_cast<__attribute__((address_space(3))) const u32x4_t*>(at);
 }
 
-// A lane's half of a query row: bf16 values 64 k + 32 h + 8 i .. + 7.
+// A lane's half of a query row: values 64 k + 32 h + 8 i .. + 7.
 struct Query {
-  u32x4_t w[2][4];
+  bf16x8_t q[2][4];
 };
-// ... as two e4m3 numbers per value: 32 values in units of 2^e, and what they leave in units of 2^(e - 4).
-struct QueryParts {
-  i32x8_t high[2], low[2];  // dims 64 k + 32 h .. + 31
-  int high_scale, low_scale;
-};
-
-// The row's largest |q|, as bits (a lane's scale is not for its own 32 values alone: both halves need the same).
-__device__ __forceinline__ unsigned query_top(const Query& q) {
-  u16x2_t top = {0, 0};
-#pragma unroll
-  for (int i = 0; i < 32; ++i)
-    top = __builtin_elementwise_max(top, __builtin_bit_cast(u16x2_t, q.w[i / 16][i / 4 % 4][i % 4] & 0x7fff7fffu));
-  const int mine = max(top[0], top[1]);
-  return (unsigned)max(mine, __shfl_xor(mine, 32));
-}
-
-// Whether the parts hold all of the lane's values but kMostLost exactly: the last place of a value of 8 bits is a
-// multiple of their least step, 2^(e - 13), from 2^-13 of the row's largest power of two on.
-__device__ __forceinline__ bool query_fits(const Query& q, unsigned top) {
-  const unsigned short least = (unsigned short)max((int)(top & 0x7f80u) - (13 << 7) - 1, 0);
-  u16x2_t lost = {0, 0};
-#pragma unroll
-  for (int i = 0; i < 32; ++i) {
-    const u16x2_t below = __builtin_bit_cast(u16x2_t, q.w[i / 16][i / 4 % 4][i % 4] & 0x7fff7fffu) - u16x2_t{1, 1};  // (of zeros: above all)
-    lost += __builtin_elementwise_min(__builtin_elementwise_sub_sat(u16x2_t{least, least}, below), u16x2_t{1, 1});
-  }
-  return top < 0x7f80u && lost[0] + lost[1] <= kMostLost;
-}
-
-__device__ __forceinline__ QueryParts query_parts(const Query& query, unsigned top) {
-  // the least e with |q| <= 256 2^e, so that no high part rounds past 448
-  const int e = min(max((int)(top >> 7) - 127 - 7, -120), 120);
-  const float factor = power_of_two(-e);
-  QueryParts q;
-  q.high_scale = e + 127;
-  q.low_scale = e - 4 + 127;
-#pragma unroll
-  for (int k = 0; k < 2; ++k)
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const unsigned w0 = query.w[k][i >> 1][2 * (i & 1)], w1 = query.w[k][i >> 1][2 * (i & 1) + 1];
-      float x[4] = {__builtin_bit_cast(float, w0 << 16), __builtin_bit_cast(float, w0 & 0xffff0000u),
-                    __builtin_bit_cast(float, w1 << 16), __builtin_bit_cast(float, w1 & 0xffff0000u)};
-#pragma unroll
-      for (int u = 0; u < 4; ++u) x[u] *= factor;
-      int high = __builtin_amdgcn_cvt_pk_fp8_f32(x[0], x[1], 0, false);
-      high = __builtin_amdgcn_cvt_pk_fp8_f32(x[2], x[3], high, true);
-      const f32x2_t a = __builtin_amdgcn_cvt_pk_f32_fp8(high, false), b = __builtin_amdgcn_cvt_pk_f32_fp8(high, true);
-      int low = __builtin_amdgcn_cvt_pk_fp8_f32((x[0] - a[0]) * 16.f, (x[1] - a[1]) * 16.f, 0, false);
-      low = __builtin_amdgcn_cvt_pk_fp8_f32((x[2] - b[0]) * 16.f, (x[3] - b[1]) * 16.f, low, true);
-      q.high[k][i] = high;
-      q.low[k][i] = low;
-    }
-  return q;
-}
 
 // 32 key rows of K, blocks 2 m and 2 m + 1 of a slot, as the lanes multiply them.
 struct Keys {
-  i32x8_t k[2];
+  unsigned k[2][8];  // dims 64 k + 32 h + 4 i .. + 3
 };
 __device__ __forceinline__ Keys many_keys(lds_byte_t* slot, int m) {
   const int lane = threadIdx.x & 63, c = lane & 31, h = lane >> 5;
@@ -880,33 +819,22 @@ __device__ __forceinline__ Keys many_keys(lds_byte_t* slot, int m) {
 #pragma unroll
   for (int k = 0; k < 2; ++k) {
     const u32x4_t lo = lds_16(at + k * 1024), hi = lds_16(at + k * 1024 + 256);
-    keys.k[k] = i32x8_t{(int)lo[0], (int)lo[1], (int)lo[2], (int)lo[3], (int)hi[0], (int)hi[1], (int)hi[2], (int)hi[3]};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) keys.k[k][i] = lo[i], keys.k[k][4 + i] = hi[i];
   }
   return keys;
 }
 
 // S^T of 32 key rows: lane (h, c) holds query row c, key rows 8 (i / 4) + 4 h + i % 4.  scale:
 // exponent byte of the block that key row c is in.
-__device__ __forceinline__ f32x16_t many_scores(const Keys& keys, const QueryParts& q, int scale) {
-  f32x16_t s = {};
-#pragma unroll
-  for (int k = 0; k < 2; ++k) {
-    s = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(keys.k[k], q.low[k], s, 0, 0, 0, scale, 0, q.low_scale);
-    s = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(keys.k[k], q.high[k], s, 0, 0, 0, scale, 0, q.high_scale);
-  }
-  return s;
-}
-
-// The same with the query as it is.
-__device__ __forceinline__ f32x16_t many_scores(const Keys& keys, const Query& q, int scale) {
+__device__ __forceinline__ f32x16_t many_scores(const Keys& keys, const Query& query, int scale) {
   const float ks = power_of_two(scale - 127);
   f32x16_t s = {};
 #pragma unroll
   for (int k = 0; k < 2; ++k)
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-      s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(eight((unsigned)keys.k[k][2 * i], (unsigned)keys.k[k][2 * i + 1], ks, ks),
-                                                  __builtin_bit_cast(bf16x8_t, q.w[k][i]), s, 0, 0, 0);
+      s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(eight(keys.k[k][2 * i], keys.k[k][2 * i + 1], ks, ks), query.q[k][i], s, 0, 0, 0);
   return s;
 }
 
@@ -996,18 +924,17 @@ __device__ __forceinline__ void many_rows(const PagedAttentionArgs& a, ManyShare
   // (the wave's first row sees the fewest)
   const int least = rq.visible(min(tile * kManyRows + 32 * wave, rows - 1) / a.G);
   const Scale sc = scale_of(a.scale);
-  Query query;
+  Query q;
   const __bf16* from = a.q + (size_t)b * a.q_b + (size_t)head * a.q_h + (size_t)t * a.q_t + 32 * h;
 #pragma unroll
   for (int k = 0; k < 2; ++k)
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      query.w[k][i] = *reinterpret_cast<const u32x4_t*>(from + 64 * k + 8 * i);
+      u32x4_t w = *reinterpret_cast<const u32x4_t*>(from + 64 * k + 8 * i);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) query.w[k][i][e] = scaled_bits(query.w[k][i][e], sc);
+      for (int e = 0; e < 4; ++e) w[e] = scaled_bits(w[e], sc);
+      q.q[k][i] = __builtin_bit_cast(bf16x8_t, w);
     }
-  const unsigned top = query_top(query);
-  const bool wide = __ballot(!query_fits(query, top)) != 0;
   bool any = false;
   ManyState st;
   st.sums = no_sums(sc.c2);
@@ -1049,7 +976,7 @@ __device__ __forceinline__ void many_rows(const PagedAttentionArgs& a, ManyShare
     asm volatile("s_waitcnt vmcnt(4) lgkmcnt(0)\n\ts_barrier" ::: "memory");
     load(step + 2, (step - first_step + 2) & (kRing - 1));
   };
-  auto steps = [&](const auto& q) __attribute__((always_inline)) {
+  if (first_step < stop) {
     load(first_step, 0);
     load(first_step + 1, 1);
     begin_step(first_step);
@@ -1127,12 +1054,6 @@ __device__ __forceinline__ void many_rows(const PagedAttentionArgs& a, ManyShare
         s = then;
       }
     }
-  };
-  if (first_step < stop) {
-    if (wide)
-      steps(query);
-    else
-      steps(query_parts(query, top));
   }
   asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
 

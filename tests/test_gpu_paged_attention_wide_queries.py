@@ -3,15 +3,11 @@ definition in 64 bits."""
 
 from __future__ import annotations
 
-import math
-
 import pytest
 import torch
 
-from leanstack_amd import kernels
-
-from paged_helpers import D, Pool, attention, places
-from test_gpu_paged_attention import check, ints, queries, setup
+from paged_helpers import D, places
+from test_gpu_paged_attention import check, queries, setup
 
 pytestmark = pytest.mark.gpu
 
@@ -39,11 +35,7 @@ def test_one_large_dim_that_meets_zeros(gpu, t, power):
 @pytest.mark.parametrize("t", [3, 70])
 @pytest.mark.parametrize("dims", [1, 2, 5, 16, 64, 127])
 def test_small_dims_beside_large_ones(gpu, t, dims):
-    """`dims` dims 2^14..2^18 times smaller than the others, which the keys do not have.
-
-    More than 32 query rows: up to four values of a query may be off by 2^-21 of its largest.  Of the
-    first dims that is so for one and two of them; a score is then off by at most as many times
-    2^-21 max |q| max |k| scale, a weight beside the sum of all by the exponential of twice that."""
+    """`dims` dims 2^14..2^18 times smaller than the others, which the keys do not have."""
     lens = [150, 90]
     cache, table = setup(gpu, 2, 32, lens, seed=62)
     large = list(range(dims, D))
@@ -51,17 +43,7 @@ def test_small_dims_beside_large_ones(gpu, t, dims):
     q = queries(2, 8, t, seed=63).float()
     q[..., :dims] = q[..., :dims] * torch.exp2(-torch.arange(14, 19).float()[torch.arange(dims) % 5]) * 2.0 ** 10
     q[..., large] *= 2.0 ** 10
-    q = q.to(torch.bfloat16)
-    if t * 4 <= 32 or dims > 2:
-        check(gpu, cache, q, table, lens, 20.0)
-        return
-    pool = Pool(cache.storage[0], cache.exponents[0])
-    want, bound = attention(pool, q, table, lens, 20.0)
-    dense = [pool.dense(table[b], n)[:2] for b, n in enumerate(lens)]
-    most_k, most_v = (max(float(x[i].abs().max()) for x in dense) for i in (0, 1))
-    off = dims * 2.0 ** -21 * float(q.abs().max()) * most_k * 20.0
-    got = kernels.paged_attention(q.to(gpu), cache, 0, ints(gpu, table), ints(gpu, lens), 20.0).cpu().double().view_as(want)
-    assert bool(((got - want).abs() <= bound + math.expm1(2 * off) * most_v).all())
+    check(gpu, cache, q.to(torch.bfloat16), table, lens, 20.0)
 
 
 @pytest.mark.parametrize("t", [3, 70])
