@@ -82,7 +82,7 @@ class PagedKVCache:
         self.page_rows = page_blocks * BLOCK_ROWS
         self._holders = [0] * self.num_pages
         self._free = list(range(self.num_pages - 1, -1, -1))  # the lowest is taken first
-        self._requests: dict[int, Request] = {}  # the open ones, by id()
+        self._requests: dict[Request, None] = {}  # the open ones, in their order
 
     # -- pages ------------------------------------------------------------------
 
@@ -96,13 +96,13 @@ class PagedKVCache:
 
     def _known(self, requests: list[Request]) -> None:
         for r in requests:
-            if self._requests.get(id(r)) is not r:
+            if not isinstance(r, Request) or r not in self._requests:
                 raise ValueError("the request is not open in this cache")
 
     def open(self) -> Request:
         """A request without rows."""
         r = Request()
-        self._requests[id(r)] = r
+        self._requests[r] = None
         return r
 
     def close(self, request: Request) -> None:
@@ -110,7 +110,7 @@ class PagedKVCache:
         self._known([request])
         self._release(request.pages)
         request.pages, request.rows = [], 0
-        del self._requests[id(request)]
+        del self._requests[request]
 
     def _release(self, pages: list[int]) -> None:
         freed = False
@@ -224,7 +224,7 @@ class PagedKVCache:
         self._copy(moved, holes)
         for old, page in names.items():
             self._holders[page], self._holders[old] = self._holders[old], 0
-        for r in self._requests.values():
+        for r in self._requests:
             r.pages = [names.get(page, page) for page in r.pages]
         self._free = list(range(self.num_pages - 1, used - 1, -1))
         return used

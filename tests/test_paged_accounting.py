@@ -2,6 +2,7 @@
 
 from __future__ import annotations
 
+import copy
 import sys
 
 import pytest
@@ -25,8 +26,8 @@ def calls(work) -> int:
     return count
 
 
-def opened(n):
-    cache = PagedKVCache(1, 1, n, page_rows=16)
+def opened(n, pages=None):
+    cache = PagedKVCache(1, 1, pages or n, page_rows=16)
     return cache, [cache.open() for _ in range(n)]
 
 
@@ -74,3 +75,26 @@ def test_requests_keep_their_order_when_others_end():
     assert cache.compact() == 4
     assert sorted(requests[i].pages[0] for i in (1, 2, 4, 5)) == [0, 1, 2, 3]
     assert [len(cache.batch([requests[i]])[0][0]) for i in (1, 2, 4, 5)] == [1] * 4
+
+
+def test_a_copy_with_its_requests():
+    """A cache that is copied together with its requests knows the copies, and only them."""
+    cache, requests = opened(3, pages=9)
+    cache.reserve(requests, 5)
+    cache.advance(requests, 5)
+    other, theirs = copy.deepcopy((cache, requests))
+    other.reserve(theirs, 20)
+    other.advance(theirs[:1], 20)
+    other.close(theirs[1])
+    assert [r.rows for r in requests] == [5] * 3 and theirs[0].rows == 25
+    assert cache.free_pages == 6 and cache.batch(requests)[1].tolist() == [5] * 3
+    for r in (requests[0], theirs[1]):
+        with pytest.raises(ValueError, match="not open"):
+            other.batch([r])
+
+
+@pytest.mark.parametrize("name", [None, 0, [], "a", object()])
+def test_what_is_no_request_is_refused(name):
+    cache, _ = opened(2)
+    with pytest.raises(ValueError, match="not open"):
+        cache.batch([name])
